@@ -26,7 +26,7 @@ import numpy as np
 from . import _lib
 
 __all__ = [
-    "Algo", "CublasError", "DeviceBuffer", "GemmConfig", "Handle", "Transpose", "load_library", "version",
+    "Algo", "CublasError", "DeviceBuffer", "GemmConfig", "Half", "Handle", "Transpose", "load_library", "version",
 ]
 
 load_library = _lib.load
@@ -68,6 +68,14 @@ class Algo(enum.IntEnum):
     Vectorized = 3
     DoubleBuf = 4
     Tf32x3 = 5
+
+
+class Half(enum.IntEnum):
+    """16-bit element type of the grouped and 4-bit-weight calls (b2b_type in
+    b2blas.h); buffers hold either as uint16 bit patterns."""
+
+    F16 = 0
+    BF16 = 1
 
 
 @dataclass
@@ -461,6 +469,39 @@ class Handle:
             self._h, config.m, config.n, config.k, config.alpha, cast(pa), la, cast(pb), lb, config.beta, cast(pc),
             lc, n))
 
+    # ---- grouped HGEMM (no reference counterpart)
+    def hgemm_grouped(self, config, groups, a, b, offsets, c, trans_b=False, half=Half.F16):
+        """C[r] = alpha*A[r]*op(B_g) + beta*C[r] for the rows r in
+        [offsets[g], offsets[g+1]) of every group g (b2b_hgemm_grouped).
+        config.m counts all rows of A (m x k) and C (m x n); b holds `groups`
+        matrices of k x n, or of n x k when trans_b; offsets is an int32
+        DeviceBuffer of groups + 1 values.  a, b, c are uint16 bit patterns."""
+        m, n, k = config.m, config.n, config.k
+        if m and n and k and groups:
+            self._need(a, m * k, "A", np.uint16)
+            self._need(b, groups * k * n, "B", np.uint16)
+            self._need(offsets, groups + 1, "offsets", np.int32)
+            self._need(c, m * n, "C", np.uint16)
+        _check(self._lib.b2b_hgemm_grouped(
+            self._h, int(half), 1 if trans_b else 0, groups, m, n, k, config.alpha, ctypes.c_void_p(a.ptr),
+            ctypes.c_void_p(b.ptr), config.beta, ctypes.c_void_p(c.ptr), ctypes.c_void_p(offsets.ptr)))
+
+    def hgemm_grouped_wgrad(self, config, groups, a, b, offsets, c, half=Half.F16):
+        """C_g = alpha*A[rows of g]^T*B[rows of g] + beta*C_g
+        (b2b_hgemm_grouped_wgrad).  config.k counts all rows of A (k x m) and
+        B (k x n); c holds `groups` m x n matrices, in float32 or in the
+        operands' type (uint16), by its dtype."""
+        m, n, rows = config.m, config.n, config.k
+        f32 = c.dtype == np.dtype(np.float32)
+        if m and n and groups:
+            self._need(a, rows * m, "A", np.uint16)
+            self._need(b, rows * n, "B", np.uint16)
+            self._need(offsets, groups + 1, "offsets", np.int32)
+            self._need(c, groups * m * n, "C", np.float32 if f32 else np.uint16)
+        _check(self._lib.b2b_hgemm_grouped_wgrad(
+            self._h, int(half), 2 if f32 else int(half), groups, rows, m, n, config.alpha, ctypes.c_void_p(a.ptr),
+            ctypes.c_void_p(b.ptr), config.beta, ctypes.c_void_p(c.ptr), ctypes.c_void_p(offsets.ptr)))
+
     # ---- Level 2: SGEMV (lib.rs:230-309)
     def sgemv(self, trans, m, n, alpha, a, x, beta, y, algo=Algo.Default):
         xl, yl = (n, m) if int(trans) == 0 else (m, n)
@@ -514,6 +555,62 @@ class Handle:
             self._need(y, yl, "y", np.uint16)
         _check(self._lib.b2b_hgemv(self._h, int(trans), m, n, alpha, ctypes.c_void_p(a.ptr),
                                    ctypes.c_void_p(x.ptr), beta, ctypes.c_void_p(y.ptr)))
+
+    # ---- Level 2: 4-bit weights (no reference counterpart)
+    def _need_w4(self, matrices, m, n, group, packed, scales, zeros):
+        gs = -(-n // group) if group > 0 else 0  # the library refuses a group of 0
+        self._need(packed, matrices * m * ((n + 1) // 2), "packed", np.uint8)
+        self._need(scales, matrices * m * gs, "scales", np.uint16)
+        if zeros is not None:
+            self._need(zeros, matrices * m * gs, "zeros", np.uint8)
+        return ctypes.c_void_p(zeros.ptr if zeros is not None else 0)
+
+    def quantize_w4(self, m, n, group, w, packed, scales, zeros=None, half=Half.F16):
+        """W (m x n, uint16 bit patterns) to 4-bit values with one scale, and
+        with `zeros` one zero point, per group of columns (b2b_quantize_w4)."""
+        z = ctypes.c_void_p(zeros.ptr if zeros is not None else 0)
+        if m and n:
+            z = self._need_w4(1, m, n, group, packed, scales, zeros)
+            self._need(w, m * n, "W", np.uint16)
+        _check(self._lib.b2b_quantize_w4(self._h, int(half), m, n, group, ctypes.c_void_p(w.ptr),
+                                         ctypes.c_void_p(packed.ptr), ctypes.c_void_p(scales.ptr), z))
+
+    def dequantize_w4(self, m, n, group, packed, scales, zeros, w, half=Half.F16):
+        """4-bit values back to the 16-bit W (b2b_dequantize_w4); zeros may be None."""
+        z = ctypes.c_void_p(zeros.ptr if zeros is not None else 0)
+        if m and n:
+            z = self._need_w4(1, m, n, group, packed, scales, zeros)
+            self._need(w, m * n, "W", np.uint16)
+        _check(self._lib.b2b_dequantize_w4(self._h, int(half), m, n, group, ctypes.c_void_p(packed.ptr),
+                                           ctypes.c_void_p(scales.ptr), z, ctypes.c_void_p(w.ptr)))
+
+    def hgemv_w4(self, m, n, group, alpha, packed, scales, zeros, x, beta, y, count=1, half=Half.F16):
+        """y_i = alpha*W*x_i + beta*y_i for `count` vectors with the 4-bit W
+        (b2b_hgemv_w4); zeros may be None."""
+        z = ctypes.c_void_p(zeros.ptr if zeros is not None else 0)
+        if m and n and count:
+            z = self._need_w4(1, m, n, group, packed, scales, zeros)
+            self._need(x, count * n, "x", np.uint16)
+            self._need(y, count * m, "y", np.uint16)
+        _check(self._lib.b2b_hgemv_w4(self._h, int(half), m, n, group, alpha, ctypes.c_void_p(packed.ptr),
+                                      ctypes.c_void_p(scales.ptr), z, ctypes.c_void_p(x.ptr), count, beta,
+                                      ctypes.c_void_p(y.ptr)))
+
+    def hgemv_w4_grouped(self, groups, m, n, group, alpha, packed, scales, zeros, x, index, beta, y, count, fan=1,
+                         half=Half.F16):
+        """y_i = alpha*W_e*x_{i // fan} + beta*y_i with e = index[i] of `groups`
+        4-bit matrices (b2b_hgemv_w4_grouped); index is an int32 DeviceBuffer,
+        and one outside [0, groups) names no expert."""
+        z = ctypes.c_void_p(zeros.ptr if zeros is not None else 0)
+        if m and n and count and groups:
+            z = self._need_w4(groups, m, n, group, packed, scales, zeros)
+            if fan > 0:  # the library refuses a fan of 0
+                self._need(x, -(-count // fan) * n, "x", np.uint16)
+            self._need(index, count, "index", np.int32)
+            self._need(y, count * m, "y", np.uint16)
+        _check(self._lib.b2b_hgemv_w4_grouped(
+            self._h, int(half), groups, m, n, group, alpha, ctypes.c_void_p(packed.ptr), ctypes.c_void_p(scales.ptr),
+            z, ctypes.c_void_p(x.ptr), count, fan, ctypes.c_void_p(index.ptr), beta, ctypes.c_void_p(y.ptr)))
 
     # ---- Level 1: SAXPY (lib.rs:110-129)
     def saxpy(self, n, alpha, x, y):

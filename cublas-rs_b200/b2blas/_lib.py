@@ -53,6 +53,8 @@ SIGNATURES = {
     "b2b_sgemm_strided_batched_simple": (
         _i, [_vp, _sz, _sz, _sz, _f, _vp, _sz, _sz, _vp, _sz, _sz, _f, _vp, _sz, _sz, _sz]),
     "b2b_sgemm_batched_simple": (_i, [_vp, _sz, _sz, _sz, _f, _vpp, _szp, _vpp, _szp, _f, _vpp, _szp, _sz]),
+    "b2b_hgemm_grouped": (_i, [_vp, _i, _i, _sz, _sz, _sz, _sz, _f, _vp, _vp, _f, _vp, _vp]),
+    "b2b_hgemm_grouped_wgrad": (_i, [_vp, _i, _i, _sz, _sz, _sz, _sz, _f, _vp, _vp, _f, _vp, _vp]),
     "b2b_sgemv": (_i, [_vp, _i, _i, _sz, _sz, _f, _vp, _vp, _f, _vp]),
     "b2b_sgemv_simple": (_i, [_vp, _i, _i, _sz, _sz, _f, _vp, _sz, _vp, _sz, _f, _vp, _sz]),
     "b2b_sgemv_noalloc": (_i, [_vp, _i, _sz, _sz, _f, _vp, _vp, _f, _vp]),
@@ -60,6 +62,11 @@ SIGNATURES = {
     "b2b_dgemv_simple": (_i, [_vp, _i, _sz, _sz, _d, _vp, _sz, _vp, _sz, _d, _vp, _sz]),
     "b2b_hgemv": (_i, [_vp, _i, _sz, _sz, _f, _vp, _vp, _f, _vp]),
     "b2b_hgemv_simple": (_i, [_vp, _i, _sz, _sz, _f, _vp, _sz, _vp, _sz, _f, _vp, _sz]),
+    "b2b_quantize_w4": (_i, [_vp, _i, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
+    "b2b_dequantize_w4": (_i, [_vp, _i, _sz, _sz, _sz, _vp, _vp, _vp, _vp]),
+    "b2b_hgemv_w4": (_i, [_vp, _i, _sz, _sz, _sz, _f, _vp, _vp, _vp, _vp, _sz, _f, _vp]),
+    "b2b_hgemv_w4_grouped": (
+        _i, [_vp, _i, _sz, _sz, _sz, _sz, _f, _vp, _vp, _vp, _vp, _sz, _sz, _vp, _f, _vp]),
     "b2b_sdot": (_i, [_vp, _sz, _vp, _vp, _fp]),
     "b2b_sdot_simple": (_i, [_vp, _sz, _vp, _sz, _vp, _sz, _fp]),
     "b2b_snrm2": (_i, [_vp, _sz, _vp, _fp]),

@@ -37,6 +37,47 @@ int check_algo(int algo, const char *fn, bool allow_3xtf32) {
     return B2B_OK;
 }
 
+int check_half(int type, const char *fn) {
+    if (type != B2B_TYPE_F16 && type != B2B_TYPE_BF16)
+        return fail(B2B_ERR_INVALID_ARG, std::string(fn) + ": type must be B2B_TYPE_F16 or B2B_TYPE_BF16");
+    return B2B_OK;
+}
+
+// Limits of the grouped calls: 32-bit rows, columns and offsets, and a group
+// table that fits shared memory; byte sizes of `groups` a x b matrices.
+int check_grouped(const char *fn, size_t groups, size_t rows, size_t a, size_t b) {
+    const size_t top = static_cast<size_t>(INT32_MAX);
+    if (groups > 1024 || rows > top || a > top || b > top)
+        return fail(B2B_ERR_NOT_SUPPORTED, std::string(fn) + ": more than 1024 groups, or a size of 2^31 or more");
+    size_t t;
+    if (!mul_ok(a, b, &t) || !bytes_ok(groups, t, 4) || !bytes_ok(rows, a, 2) || !bytes_ok(rows, b, 2))
+        return fail(B2B_ERR_INVALID_ARG, std::string(fn) + ": sizes overflow");
+    return B2B_OK;
+}
+
+// Limits of the 4-bit-weight calls, for `matrices` matrices of m x n.
+int check_w4(const char *fn, int type, size_t matrices, size_t m, size_t n, size_t group) {
+    if (int rc = check_half(type, fn)) return rc;
+    const size_t top = static_cast<size_t>(INT32_MAX);
+    if (group == 0 || group % 32 != 0)
+        return fail(B2B_ERR_INVALID_ARG, std::string(fn) + ": group must be a positive multiple of 32");
+    if (group > top || m > top || n > top || matrices > top)
+        return fail(B2B_ERR_NOT_SUPPORTED, std::string(fn) + ": a size of 2^31 or more");
+    size_t t;
+    if (!mul_ok(m, n, &t) || !bytes_ok(matrices, t, 2))
+        return fail(B2B_ERR_INVALID_ARG, std::string(fn) + ": sizes overflow");
+    return B2B_OK;
+}
+
+// ... and of x (xs vectors of n) and y (count vectors of m).
+int check_w4_vectors(const char *fn, size_t xs, size_t n, size_t count, size_t m) {
+    if (count > static_cast<size_t>(INT32_MAX))
+        return fail(B2B_ERR_NOT_SUPPORTED, std::string(fn) + ": 2^31 products or more");
+    if (!bytes_ok(xs, n, 2) || !bytes_ok(count, m, 2))
+        return fail(B2B_ERR_INVALID_ARG, std::string(fn) + ": sizes overflow");
+    return B2B_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -123,6 +164,82 @@ int b2b_sgemm_strided_batched(b2b_handle *h, size_t m, size_t n, size_t k, float
         return fail(B2B_ERR_INVALID_ARG, "b2b_sgemm_strided_batched: sizes overflow");
     DeviceGuard g(h);
     return launch_sgemm_strided_batched(h, m, n, k, alpha, A, stride_a, B, stride_b, beta, C, stride_c, batch);
+}
+
+int b2b_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, size_t rows, size_t n, size_t k,
+                      float alpha, const uint16_t *A, const uint16_t *B, float beta, uint16_t *C,
+                      const int32_t *offsets) {
+    if (!h) return fail(B2B_ERR_INVALID_ARG, "b2b_hgemm_grouped: NULL handle");
+    if (int rc = check_half(type, "b2b_hgemm_grouped")) return rc;
+    if (trans_b != B2B_OP_N && trans_b != B2B_OP_T)
+        return fail(B2B_ERR_INVALID_ARG, "b2b_hgemm_grouped: trans_b must be B2B_OP_N or B2B_OP_T");
+    if (groups == 0 || rows == 0 || n == 0 || k == 0) return B2B_OK;
+    if (!A || !B || !C || !offsets) return fail(B2B_ERR_INVALID_ARG, "b2b_hgemm_grouped: NULL operand");
+    if (int rc = check_grouped("b2b_hgemm_grouped", groups, rows, n, k)) return rc;
+    DeviceGuard g(h);
+    return launch_hgemm_grouped(h, type, trans_b, groups, rows, n, k, alpha, A, B, beta, C, offsets);
+}
+
+int b2b_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t groups, size_t rows, size_t m, size_t n,
+                            float alpha, const uint16_t *A, const uint16_t *B, float beta, void *C,
+                            const int32_t *offsets) {
+    if (!h) return fail(B2B_ERR_INVALID_ARG, "b2b_hgemm_grouped_wgrad: NULL handle");
+    if (int rc = check_half(type, "b2b_hgemm_grouped_wgrad")) return rc;
+    if (c_type != type && c_type != B2B_TYPE_F32)
+        return fail(B2B_ERR_INVALID_ARG, "b2b_hgemm_grouped_wgrad: c_type must be type or B2B_TYPE_F32");
+    if (groups == 0 || m == 0 || n == 0) return B2B_OK;
+    if ((rows != 0 && (!A || !B)) || !C || !offsets)
+        return fail(B2B_ERR_INVALID_ARG, "b2b_hgemm_grouped_wgrad: NULL operand");
+    if (int rc = check_grouped("b2b_hgemm_grouped_wgrad", groups, rows, m, n)) return rc;
+    DeviceGuard g(h);
+    return launch_hgemm_grouped_wgrad(h, type, c_type, groups, rows, m, n, alpha, A, B, beta, C, offsets);
+}
+
+int b2b_quantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, const uint16_t *W, uint8_t *packed,
+                    uint16_t *scales, uint8_t *zeros) {
+    if (!h) return fail(B2B_ERR_INVALID_ARG, "b2b_quantize_w4: NULL handle");
+    if (int rc = check_w4("b2b_quantize_w4", type, 1, m, n, group)) return rc;
+    if (m == 0 || n == 0) return B2B_OK;
+    if (!W || !packed || !scales) return fail(B2B_ERR_INVALID_ARG, "b2b_quantize_w4: NULL operand");
+    DeviceGuard g(h);
+    return launch_quantize_w4(h, type, m, n, group, W, packed, scales, zeros);
+}
+
+int b2b_dequantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, const uint8_t *packed,
+                      const uint16_t *scales, const uint8_t *zeros, uint16_t *W) {
+    if (!h) return fail(B2B_ERR_INVALID_ARG, "b2b_dequantize_w4: NULL handle");
+    if (int rc = check_w4("b2b_dequantize_w4", type, 1, m, n, group)) return rc;
+    if (m == 0 || n == 0) return B2B_OK;
+    if (!W || !packed || !scales) return fail(B2B_ERR_INVALID_ARG, "b2b_dequantize_w4: NULL operand");
+    DeviceGuard g(h);
+    return launch_dequantize_w4(h, type, m, n, group, packed, scales, zeros, W);
+}
+
+int b2b_hgemv_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, float alpha, const uint8_t *packed,
+                 const uint16_t *scales, const uint8_t *zeros, const uint16_t *x, size_t count, float beta,
+                 uint16_t *y) {
+    if (!h) return fail(B2B_ERR_INVALID_ARG, "b2b_hgemv_w4: NULL handle");
+    if (int rc = check_w4("b2b_hgemv_w4", type, 1, m, n, group)) return rc;
+    if (m == 0 || n == 0 || count == 0) return B2B_OK;
+    if (!packed || !scales || !x || !y) return fail(B2B_ERR_INVALID_ARG, "b2b_hgemv_w4: NULL operand");
+    if (int rc = check_w4_vectors("b2b_hgemv_w4", count, n, count, m)) return rc;
+    DeviceGuard g(h);
+    return launch_hgemv_w4(h, type, 1, m, n, group, alpha, packed, scales, zeros, x, count, 1, nullptr, beta, y);
+}
+
+int b2b_hgemv_w4_grouped(b2b_handle *h, int type, size_t groups, size_t m, size_t n, size_t group, float alpha,
+                         const uint8_t *packed, const uint16_t *scales, const uint8_t *zeros, const uint16_t *x,
+                         size_t count, size_t fan, const int32_t *index, float beta, uint16_t *y) {
+    if (!h) return fail(B2B_ERR_INVALID_ARG, "b2b_hgemv_w4_grouped: NULL handle");
+    if (int rc = check_w4("b2b_hgemv_w4_grouped", type, groups, m, n, group)) return rc;
+    if (fan == 0) return fail(B2B_ERR_INVALID_ARG, "b2b_hgemv_w4_grouped: fan must be at least 1");
+    if (groups == 0 || m == 0 || n == 0 || count == 0) return B2B_OK;
+    if (!packed || !scales || !x || !y || !index)
+        return fail(B2B_ERR_INVALID_ARG, "b2b_hgemv_w4_grouped: NULL operand");
+    if (int rc = check_w4_vectors("b2b_hgemv_w4_grouped", count / fan + (count % fan != 0), n, count, m)) return rc;
+    DeviceGuard g(h);
+    return launch_hgemv_w4(h, type, groups, m, n, group, alpha, packed, scales, zeros, x, count,
+                           fan < count ? fan : count, index, beta, y);
 }
 
 int b2b_sgemv(b2b_handle *h, int algo, int trans, size_t m, size_t n, float alpha, const float *A, const float *x,

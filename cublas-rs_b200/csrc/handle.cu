@@ -262,6 +262,9 @@ int b2b_synchronize(b2b_handle *h) {
     if (e != cudaSuccess) return fail_cuda(e, "reading device status");
     if (st != 0) {
         cudaMemset(h->d_status, 0, sizeof(int));
+        if (st == B2B_DEVSTAT_OFFSETS)
+            return fail(B2B_ERR_INVALID_ARG,
+                        "a grouped call's offsets do not ascend within [0, rows]; its C was left as it was");
         char buf[96];
         snprintf(buf, sizeof buf, "a bounded device wait gave up (status 0x%x)", st);
         return fail(B2B_ERR_DEVICE_TIMEOUT, buf);

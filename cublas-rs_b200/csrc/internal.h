@@ -13,8 +13,11 @@
 // Device status word values written by kernels whose waits are bounded.
 // The low byte names the wait that gave up.
 #define B2B_DEVSTAT_TIMEOUT 0x100
+// A grouped call found offsets that do not ascend within its rows and wrote
+// nothing.
+#define B2B_DEVSTAT_OFFSETS 0x200
 // Layout of the handle's 256-byte device status block (zeroed at creation):
-//   byte   0: int status word (bounded-wait timeouts)
+//   byte   0: int status word (bounded-wait timeouts, refused group offsets)
 //   byte  64: unsigned reduction ticket counter (back to 0 after each reduction)
 //   byte 128: 8-byte result slot of the blocking reductions
 #define B2B_STATUS_REDUCE_COUNTER 64
@@ -161,6 +164,20 @@ int launch_dgemv(b2b_handle *h, int trans, size_t m, size_t n, double alpha, con
                  double beta, double *y);
 int launch_hgemv(b2b_handle *h, int trans, size_t m, size_t n, float alpha, const uint16_t *A, const uint16_t *x,
                  float beta, uint16_t *y);
+int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, size_t rows, size_t n, size_t k,
+                         float alpha, const uint16_t *A, const uint16_t *B, float beta, uint16_t *C,
+                         const int32_t *offsets);
+int launch_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t groups, size_t rows, size_t m, size_t n,
+                               float alpha, const uint16_t *A, const uint16_t *B, float beta, void *C,
+                               const int32_t *offsets);
+int launch_quantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, const uint16_t *W, uint8_t *packed,
+                       uint16_t *scales, uint8_t *zeros);
+int launch_dequantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, const uint8_t *packed,
+                         const uint16_t *scales, const uint8_t *zeros, uint16_t *W);
+// index == nullptr: every product uses the one matrix.
+int launch_hgemv_w4(b2b_handle *h, int type, size_t groups, size_t m, size_t n, size_t group, float alpha,
+                    const uint8_t *packed, const uint16_t *scales, const uint8_t *zeros, const uint16_t *x,
+                    size_t count, size_t fan, const int32_t *index, float beta, uint16_t *y);
 int launch_saxpy(b2b_handle *h, size_t n, float alpha, const float *x, float *y);
 int launch_panels_to_rowmajor(b2b_handle *h, size_t elem_bytes, size_t m, size_t g, const size_t *widths,
                               const void *panels, void *C);

@@ -31,6 +31,9 @@ pub const B2B_ALGO_TILED: c_int = 2;
 pub const B2B_ALGO_VECTORIZED: c_int = 3;
 pub const B2B_ALGO_DOUBLE_BUF: c_int = 4;
 pub const B2B_ALGO_3XTF32: c_int = 5;
+pub const B2B_TYPE_F16: c_int = 0;
+pub const B2B_TYPE_BF16: c_int = 1;
+pub const B2B_TYPE_F32: c_int = 2;
 pub const B2B_REDUCE_DOT: c_int = 0;
 pub const B2B_REDUCE_NRM2: c_int = 1;
 pub const B2B_REDUCE_ASUM: c_int = 2;
@@ -87,6 +90,12 @@ extern "C" {
                                     a: *const *const f32, a_lens: *const usize, b: *const *const f32,
                                     b_lens: *const usize, beta: f32, c: *const *mut f32,
                                     c_lens: *const usize, batch: usize) -> c_int;
+    pub fn b2b_hgemm_grouped(h: *mut b2b_handle, ty: c_int, trans_b: c_int, groups: usize, rows: usize,
+                             n: usize, k: usize, alpha: f32, a: *const u16, b: *const u16, beta: f32,
+                             c: *mut u16, offsets: *const i32) -> c_int;
+    pub fn b2b_hgemm_grouped_wgrad(h: *mut b2b_handle, ty: c_int, c_type: c_int, groups: usize, rows: usize,
+                                   m: usize, n: usize, alpha: f32, a: *const u16, b: *const u16, beta: f32,
+                                   c: *mut c_void, offsets: *const i32) -> c_int;
     pub fn b2b_sgemv(h: *mut b2b_handle, algo: c_int, trans: c_int, m: usize, n: usize, alpha: f32,
                      a: *const f32, x: *const f32, beta: f32, y: *mut f32) -> c_int;
     pub fn b2b_sgemv_simple(h: *mut b2b_handle, algo: c_int, trans: c_int, m: usize, n: usize, alpha: f32,
@@ -104,6 +113,17 @@ extern "C" {
     pub fn b2b_hgemv_simple(h: *mut b2b_handle, trans: c_int, m: usize, n: usize, alpha: f32, a: *const u16,
                             a_len: usize, x: *const u16, x_len: usize, beta: f32, y: *mut u16,
                             y_len: usize) -> c_int;
+    pub fn b2b_quantize_w4(h: *mut b2b_handle, ty: c_int, m: usize, n: usize, group: usize, w: *const u16,
+                           packed: *mut u8, scales: *mut u16, zeros: *mut u8) -> c_int;
+    pub fn b2b_dequantize_w4(h: *mut b2b_handle, ty: c_int, m: usize, n: usize, group: usize,
+                             packed: *const u8, scales: *const u16, zeros: *const u8, w: *mut u16) -> c_int;
+    pub fn b2b_hgemv_w4(h: *mut b2b_handle, ty: c_int, m: usize, n: usize, group: usize, alpha: f32,
+                        packed: *const u8, scales: *const u16, zeros: *const u8, x: *const u16, count: usize,
+                        beta: f32, y: *mut u16) -> c_int;
+    pub fn b2b_hgemv_w4_grouped(h: *mut b2b_handle, ty: c_int, groups: usize, m: usize, n: usize,
+                                group: usize, alpha: f32, packed: *const u8, scales: *const u16,
+                                zeros: *const u8, x: *const u16, count: usize, fan: usize, index: *const i32,
+                                beta: f32, y: *mut u16) -> c_int;
     pub fn b2b_saxpy(h: *mut b2b_handle, n: usize, alpha: f32, x: *const f32, y: *mut f32) -> c_int;
     pub fn b2b_saxpy_simple(h: *mut b2b_handle, n: usize, alpha: f32, x: *const f32, x_len: usize,
                             y: *mut f32, y_len: usize) -> c_int;

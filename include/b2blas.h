@@ -69,6 +69,11 @@ typedef enum {
     B2B_ALGO_3XTF32 = 5
 } b2b_algo;
 
+/* Element types of the calls that take more than one (no reference
+ * counterpart; its half type is f16 only).  16-bit operands are passed as
+ * their bit patterns. */
+typedef enum { B2B_TYPE_F16 = 0, B2B_TYPE_BF16 = 1, B2B_TYPE_F32 = 2 } b2b_type;
+
 typedef struct b2b_handle b2b_handle;
 
 /* ------------------------------------------------------------ lifecycle */
@@ -93,7 +98,8 @@ B2B_API int b2b_get_stream(b2b_handle *h, void **stream);
 B2B_API int b2b_set_stream(b2b_handle *h, void *stream);
 /* Handle::synchronize (lib.rs:79-82): blocks on the stream, then reports a
  * device-side bounded-wait timeout, if one was recorded, as
- * B2B_ERR_DEVICE_TIMEOUT (and clears it). */
+ * B2B_ERR_DEVICE_TIMEOUT, or group offsets that a grouped call refused on
+ * the device, as B2B_ERR_INVALID_ARG (and clears it). */
 B2B_API int b2b_synchronize(b2b_handle *h);
 /* Device ordinal, SM count and clock, for the facade and the bench. */
 B2B_API int b2b_device_info(b2b_handle *h, int *device, int *sm_count, int *sm_clock_khz);
@@ -207,6 +213,40 @@ B2B_API int b2b_sgemm_batched_simple(b2b_handle *h, size_t m, size_t n, size_t k
                                      const size_t *b_lens, float beta, float *const *C, const size_t *c_lens,
                                      size_t batch);
 
+/* ------------------------------------------- Level 3: grouped HGEMM
+ * No reference counterpart; the ragged sibling of the batched family above,
+ * with 16-bit operands and f32 accumulation as in b2b_hgemm: the products of
+ * an expert layer, whose tokens are sorted by expert.
+ *   - offsets is a device array of groups + 1 int32 values, read by the
+ *     kernel: group g owns rows [offsets[g], offsets[g+1]).  They must ascend
+ *     within [0, rows]; empty groups are fine, and offsets[0] need not be 0.
+ *     Offsets that break this write nothing: the call leaves C as it was and
+ *     the next b2b_synchronize returns B2B_ERR_INVALID_ARG.
+ *   - type is B2B_TYPE_F16 or B2B_TYPE_BF16 and holds for A and B; results
+ *     are rounded to nearest even once, after alpha and beta.
+ *   - At most 1024 groups, and sizes below 2^31 (else B2B_ERR_NOT_SUPPORTED).
+ *   - C must not overlap A, B or the offsets.
+ *   - No workspace is used: calls through one handle may be captured in
+ *     several graphs and replayed at once. */
+
+/* C[r] <- alpha*A[r]*op(B_g) + beta*C[r] for every row r of every group g.
+ * A is rows x k, C rows x n; B holds groups matrices back to back, k x n
+ * each (trans_b = B2B_OP_N) or n x k each (B2B_OP_T: the gradient with
+ * respect to A, given the weights as the forward call takes them).  Rows
+ * that no group owns are neither read into a result nor written. */
+B2B_API int b2b_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, size_t rows, size_t n, size_t k,
+                              float alpha, const uint16_t *A, const uint16_t *B, float beta, uint16_t *C,
+                              const int32_t *offsets);
+/* C_g <- alpha*A[rows of g]^T*B[rows of g] + beta*C_g for every group g: the
+ * gradient with respect to the weights.  A is rows x m, B rows x n, C holds
+ * groups m x n matrices of c_type, which is type or B2B_TYPE_F32.  A group
+ * without rows is an empty sum, so its C_g becomes beta*C_g (zeros when beta
+ * is 0); so does every C_g when rows is 0 (A and B may then be NULL).
+ * Values in rows that no group owns reach no result, NaN included. */
+B2B_API int b2b_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t groups, size_t rows, size_t m,
+                                    size_t n, float alpha, const uint16_t *A, const uint16_t *B, float beta, void *C,
+                                    const int32_t *offsets);
+
 /* -------------------------------------------------------- Level 2: SGEMV */
 
 /* Handle::sgemv / sgemv_tiled (lib.rs:230-283) -> cublas_l2::sgemv_dev /
@@ -268,6 +308,54 @@ B2B_API int b2b_hgemv(b2b_handle *h, int trans, size_t m, size_t n, float alpha,
 B2B_API int b2b_hgemv_simple(b2b_handle *h, int trans, size_t m, size_t n, float alpha, const uint16_t *A,
                              size_t a_len, const uint16_t *x, size_t x_len, float beta, uint16_t *y,
                              size_t y_len);
+
+/* ------------------------------------------------ Level 2: 4-bit weights
+ * No reference counterpart; the siblings of b2b_hgemv for matrices held in 4
+ * bits, as single-token products with large weights take them.  A matrix W
+ * of m x n is held as
+ *   packed  m rows of (n + 1) / 2 bytes: two values 0..15 to a byte, the even
+ *           column in the low four bits (the last high four bits of an odd
+ *           row have no meaning),
+ *   scales  m x ceil(n / group) values of `type` (16 bits), and
+ *   zeros   m x ceil(n / group) bytes, of which the low four bits count, or
+ *           NULL, which stands for 8 everywhere:
+ *   W[i][j] = scales[i][j / group] * (packed[i][j] - zeros[i][j / group]).
+ * group is a multiple of 32; the last group of a row may be short.  type is
+ * B2B_TYPE_F16 or B2B_TYPE_BF16 and holds for W, x, y and the scales.  Sizes
+ * are below 2^31.  No workspace is used. */
+
+/* W -> packed, scales and (when zeros is not NULL) zeros.  Without zeros the
+ * scale is max|w| / 7 of the group; with them it is (hi - lo) / 15 and the
+ * zero point -lo / scale, lo and hi being the group's extremes with 0 among
+ * them.  Scales are rounded to `type` first, values and zero points to
+ * nearest even in f32 arithmetic on the rounded scale, then clamped to 0..15.
+ * A group whose scale rounds to 0 holds zeros; one that has an infinity or a
+ * NaN gets a NaN scale, so that it shows in every product. */
+B2B_API int b2b_quantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, const uint16_t *W,
+                            uint8_t *packed, uint16_t *scales, uint8_t *zeros);
+/* packed, scales, zeros -> W in `type`, each value rounded once to nearest
+ * even (one that a finite scale takes beyond the type becomes its largest
+ * finite value): the 16-bit operand that the matrix products take. */
+B2B_API int b2b_dequantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, const uint8_t *packed,
+                              const uint16_t *scales, const uint8_t *zeros, uint16_t *W);
+/* y_i <- alpha*W*x_i + beta*y_i for `count` vectors: x is count x n, y is
+ * count x m.  Products are exact, sums f32, y is rounded to nearest even
+ * once.  The weights are read once for every 8 vectors.  y must not overlap
+ * the other operands. */
+B2B_API int b2b_hgemv_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, float alpha,
+                         const uint8_t *packed, const uint16_t *scales, const uint8_t *zeros, const uint16_t *x,
+                         size_t count, float beta, uint16_t *y);
+/* y_i <- alpha*W_e*x_{i / fan} + beta*y_i with e = index[i], for `count`
+ * products: packed, scales and zeros hold `groups` matrices of m x n back to
+ * back, x has ceil(count / fan) vectors, y is count x m, index is a device
+ * array of count int32 values.  A token's `fan` experts share its vector
+ * (fan = 1: a vector for each product).  An index outside [0, groups) names
+ * no expert: an empty product, which leaves beta*y_i (zeros when beta is 0).
+ * Products that name the same expert share its weights. */
+B2B_API int b2b_hgemv_w4_grouped(b2b_handle *h, int type, size_t groups, size_t m, size_t n, size_t group,
+                                 float alpha, const uint8_t *packed, const uint16_t *scales, const uint8_t *zeros,
+                                 const uint16_t *x, size_t count, size_t fan, const int32_t *index, float beta,
+                                 uint16_t *y);
 
 /* -------------------------------------------------------- Level 1: SAXPY */
 
