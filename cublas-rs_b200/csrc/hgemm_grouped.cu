@@ -7,11 +7,15 @@
 //   wgrad     C_g = alpha * A[rows of g]^T B[rows of g] + beta * C_g
 //
 // 16-bit operands (f16 or bf16), f32 sums.
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "half_types.cuh"
 #include "internal.h"
+#include "sm100.cuh"
 
 namespace {
 
@@ -141,6 +145,547 @@ __global__ void __launch_bounds__(256) grouped_simt_kernel(GroupedArgs p) {
     }
 }
 
+
+// ---------------------------------------------------------------------------
+// Tensor-core kernel: tcgen05.mma on 128 x BN tiles of one CTA, or 256 x 256
+// tiles of a CTA pair, persistent over the tiles of all groups.
+//
+//   kNN  C[r] = A[r] B_g     A K-major, B (k x n rows) MN-major
+//   kNT  C[r] = A[r] B_g^T   A K-major, B (n x k rows) K-major
+//   kTN  C_g = A_g^T B_g     both MN-major; the ragged rows are the k axis
+//
+// No operand is transposed or copied: the three products differ in the shared
+// memory layouts that the MMA descriptors name.  B of kNN / kNT is a 3-D
+// tensor map (columns, rows, group), so a box never reads across a matrix and
+// ragged edges arrive as zeros.  Boxes of A start at any row: those past a
+// group's end belong to the next group and, rows being independent, only
+// reach accumulator rows that are not stored.  In kTN they would reach every
+// sum, so the last k block of a group is wiped: a warp of its own zeroes the
+// rows past the end, in A and B both (0 times a neighbour's NaN is a NaN),
+// up to the next multiple of 16, and the MMA issues only those k steps.
+//
+// Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer, 2..5 epilogue, 6
+// (kTN) the wiper.  Two accumulators: the epilogue of a tile runs under the
+// MMAs of the next.  The epilogue goes through shared memory to whole 128-byte
+// row segments, since a TMA store would write past the group's last row.
+enum Mode { kNN = 0, kNT = 1, kTN = 2 };
+
+template <int MODE, bool PAIR, int BN_>
+struct Cfg {
+    static constexpr int BN = BN_;                     // columns of a tile
+    static constexpr int BM = PAIR ? 256 : 128;        // rows of a tile, 128 to a CTA
+    static constexpr int BN_CTA = PAIR ? BN / 2 : BN;  // columns of B that a CTA loads
+    static constexpr int A_BYTES = 128 * 64 * 2;
+    static constexpr int B_BYTES = BN_CTA * 64 * 2;
+    static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+    static constexpr int STAGES = 196608 / STAGE_BYTES;
+    static constexpr int EPI_BYTES = 4 * 4096;  // 32 rows of 128 bytes for each epilogue warp
+    static constexpr int TMEM_COLS = 2 * BN;
+    static constexpr int THREADS = MODE == kTN ? 224 : 192;
+    static constexpr int TABLE_BYTES = 4352;  // kMaxGroups + 1 ints, rounded up
+    static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + TABLE_BYTES + 1024 + 512;
+    static_assert(SMEM_BYTES <= 232448 && TABLE_BYTES >= 4 * (kMaxGroups + 1), "shared memory per CTA");
+};
+constexpr int kBoxBytes = 64 * 64 * 2;  // 64 columns x 64 rows of an MN-major operand
+constexpr int kGroupM = 16;             // raster: tile rows that sweep a group's columns together
+
+struct TcArgs {
+    void *C;
+    const int32_t *offsets;
+    int *status;
+    uint64_t wait_ns;
+    int groups, rows, M, N, K;  // M: kTN only; K: kNN and kNT
+    float alpha, beta;
+    uint32_t idesc;
+    int bf16, f32;  // element types: of the operands, of C
+    int vec;        // rows of C start on 16-byte boundaries
+};
+
+struct Tile {
+    int g;
+    int row0;       // first row of A (kTN: of A and B)
+    int m0, n0;     // first row (kTN) and column within the group's C
+    int valid;      // rows of the tile that exist
+    int kblocks, klast;  // k blocks of 64, and what the last one holds
+};
+
+// The t-th tile, t ascending from call to call (g is kept between them).
+template <int MODE, typename Cf>
+__device__ __forceinline__ Tile tile_at(const TcArgs &p, const int *start, int64_t t, int &g) {
+    const int nt = (p.N + Cf::BN - 1) / Cf::BN;
+    int mt;
+    int64_t local;
+    Tile o;
+    if constexpr (MODE == kTN) {
+        mt = (p.M + Cf::BM - 1) / Cf::BM;
+        const int64_t per = static_cast<int64_t>(mt) * nt;
+        g = static_cast<int>(t / per);
+        local = t - g * per;
+    } else {
+        while (t >= static_cast<int64_t>(start[g + 1]) * nt) ++g;
+        mt = start[g + 1] - start[g];
+        local = t - static_cast<int64_t>(start[g]) * nt;
+    }
+    const int64_t span = static_cast<int64_t>(kGroupM) * nt;
+    const int first = static_cast<int>(local / span) * kGroupM;
+    const int gm = min(mt - first, kGroupM);
+    const int r = static_cast<int>(local % span);
+    const int tm = first + r % gm;
+    o.g = g;
+    o.n0 = r / gm * Cf::BN;
+    o.m0 = tm * Cf::BM;
+    const int lo = p.offsets[g], hi = p.offsets[g + 1];
+    const int depth = MODE == kTN ? hi - lo : p.K;
+    o.row0 = MODE == kTN ? lo : lo + o.m0;
+    o.valid = min(Cf::BM, (MODE == kTN ? p.M : hi - lo) - o.m0);
+    o.kblocks = (depth + 63) / 64;
+    o.klast = depth - (o.kblocks - 1) * 64;
+    return o;
+}
+
+// Rows of A that CTA `rank` of a kNN / kNT tile loads: all 128 in one box, or
+// boxes of 16 when half of them or fewer exist (a decoding step has a few
+// rows an expert: 16 of 128 loaded rows leave the L2 to the weights).
+__device__ __forceinline__ int a_boxes16(int valid, int rank) {
+    const int v = valid - 128 * rank;
+    return v > 64 ? 8 : v > 0 ? (v + 15) / 16 : 0;
+}
+
+template <int MODE, bool PAIR, int BN>
+__global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
+    grouped_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA16,
+                      const __grid_constant__ CUtensorMap tmB, TcArgs p) {
+    using namespace sm100;
+    using Cf = Cfg<MODE, PAIR, BN>;
+    constexpr int S = Cf::STAGES;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t *sA = smem;
+    uint8_t *sB = smem + S * Cf::A_BYTES;
+    uint8_t *epi = smem + S * Cf::STAGE_BYTES;
+    int *start = reinterpret_cast<int *>(epi + Cf::EPI_BYTES);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(epi + Cf::EPI_BYTES + Cf::TABLE_BYTES);
+    uint64_t *full = bars, *empty = bars + S, *landed = bars + 2 * S;  // landed: kTN, last k block of a group
+    uint64_t *tfull = bars + 3 * S, *tempty = bars + 3 * S + 2, *drain = bars + 3 * S + 4;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 3 * S + 5);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    int *valid_flag = reinterpret_cast<int *>(tmem_slot + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
+    const bool leader = rank == 0;
+    const int64_t first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            // a pair's kTN stage is full when both CTAs say so: their
+            // producers, or for a group's last k block their wipers
+            mbar_init(&full[s], PAIR && MODE == kTN ? 2 : 1);
+            mbar_init(&empty[s], 1);
+            mbar_init(&landed[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&tfull[a], 1);
+            mbar_init(&tempty[a], PAIR ? 8 : 4);
+        }
+        mbar_init(drain, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        prefetch_tensormap(&tmA);
+        prefetch_tensormap(&tmB);
+    }
+    if (warp == 1) {
+        if constexpr (PAIR) {
+            tmem_alloc_pair(tmem_slot, Cf::TMEM_COLS);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(tmem_slot, Cf::TMEM_COLS);
+            tmem_relinquish();
+        }
+    }
+    if (warp == 2) {
+        const bool ok = scan_groups(p.offsets, p.groups, p.rows, Cf::BM, start);
+        if (lane == 0) {
+            *valid_flag = ok;
+            if (!ok) atomicCAS(p.status, 0, B2B_DEVSTAT_OFFSETS);
+        }
+    }
+    tc_fence_before();
+    if constexpr (PAIR)
+        cluster_sync();
+    else
+        __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int nt = (p.N + BN - 1) / BN;
+    int64_t tiles = 0;
+    if (*valid_flag)
+        tiles = (MODE == kTN ? static_cast<int64_t>(p.groups) * ((p.M + Cf::BM - 1) / Cf::BM)
+                             : static_cast<int64_t>(start[p.groups])) * nt;
+
+    if (warp == 0) {
+        // ------------------------------------------------ TMA producer
+        if (lane == 0) {
+            int stage = 0, g = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int64_t t = first; t < tiles && ok; t += step) {
+                const Tile o = tile_at<MODE, Cf>(p, start, t, g);
+                const int mine = MODE == kTN ? 8 : a_boxes16(o.valid, rank);
+                const int both = !PAIR ? mine : MODE == kTN ? 16 : a_boxes16(o.valid, 0) + a_boxes16(o.valid, 1);
+                for (int kb = 0; kb < o.kblocks; ++kb) {
+                    if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x21,
+                                   p.wait_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    uint8_t *a_dst = sA + stage * Cf::A_BYTES, *b_dst = sB + stage * Cf::B_BYTES;
+                    const int bn0 = o.n0 + rank * Cf::BN_CTA;
+                    const bool tail = MODE == kTN && kb == o.kblocks - 1 && o.klast < 64;
+                    if (tail) {
+                        // both operands land on this CTA's own barrier, for its wiper
+                        mbar_arrive_expect_tx(&landed[stage], Cf::STAGE_BYTES);
+                        for (int j = 0; j < 2; ++j)
+                            tma_load_2d(a_dst + j * kBoxBytes, &tmA, &landed[stage], o.m0 + rank * 128 + 64 * j,
+                                        o.row0 + kb * 64);
+                        for (int j = 0; j < Cf::BN_CTA / 64; ++j)
+                            tma_load_2d(b_dst + j * kBoxBytes, &tmB, &landed[stage], bn0 + 64 * j, o.row0 + kb * 64);
+                    } else if constexpr (PAIR) {
+                        const uint32_t bar = mapa_shared(smem_u32(&full[stage]), 0);
+                        if (leader)
+                            mbar_arrive_expect_tx(&full[stage], both * 2048 + 2 * Cf::B_BYTES);
+                        else if (MODE == kTN)
+                            mbar_arrive_cluster(bar);
+                        if constexpr (MODE == kTN) {
+                            for (int j = 0; j < 2; ++j)
+                                tma_load_2d_pair(a_dst + j * kBoxBytes, &tmA, bar, o.m0 + rank * 128 + 64 * j,
+                                                 o.row0 + kb * 64);
+                            for (int j = 0; j < Cf::BN_CTA / 64; ++j)
+                                tma_load_2d_pair(b_dst + j * kBoxBytes, &tmB, bar, bn0 + 64 * j, o.row0 + kb * 64);
+                        } else {
+                            const int r0 = o.row0 + rank * 128;
+                            if (mine == 8)
+                                tma_load_2d_pair(a_dst, &tmA, bar, kb * 64, r0);
+                            else
+                                for (int j = 0; j < mine; ++j)
+                                    tma_load_2d_pair(a_dst + j * 2048, &tmA16, bar, kb * 64, r0 + 16 * j);
+                            if constexpr (MODE == kNN)
+                                for (int j = 0; j < Cf::BN_CTA / 64; ++j)
+                                    tma_load_3d_pair(b_dst + j * kBoxBytes, &tmB, bar, bn0 + 64 * j, kb * 64, o.g);
+                            else
+                                tma_load_3d_pair(b_dst, &tmB, bar, kb * 64, bn0, o.g);
+                        }
+                    } else {
+                        uint64_t *bar = &full[stage];
+                        mbar_arrive_expect_tx(bar, mine * 2048 + Cf::B_BYTES);
+                        if constexpr (MODE == kTN) {
+                            for (int j = 0; j < 2; ++j)
+                                tma_load_2d(a_dst + j * kBoxBytes, &tmA, bar, o.m0 + 64 * j, o.row0 + kb * 64);
+                            for (int j = 0; j < Cf::BN_CTA / 64; ++j)
+                                tma_load_2d(b_dst + j * kBoxBytes, &tmB, bar, bn0 + 64 * j, o.row0 + kb * 64);
+                        } else {
+                            if (mine == 8)
+                                tma_load_2d(a_dst, &tmA, bar, kb * 64, o.row0);
+                            else
+                                for (int j = 0; j < mine; ++j)
+                                    tma_load_2d(a_dst + j * 2048, &tmA16, bar, kb * 64, o.row0 + 16 * j);
+                            if constexpr (MODE == kNN)
+                                for (int j = 0; j < Cf::BN_CTA / 64; ++j)
+                                    tma_load_3d(b_dst + j * kBoxBytes, &tmB, bar, bn0 + 64 * j, kb * 64, o.g);
+                            else
+                                tma_load_3d(b_dst, &tmB, bar, kb * 64, bn0, o.g);
+                        }
+                    }
+                    if (++stage == S) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+            }
+            if (!ok) {
+                // loads in flight complete on barriers of three kinds, a
+                // partner's among them: give them a bounded grace period
+                const uint64_t t0 = globaltimer_ns();
+                while (globaltimer_ns() - t0 < 2000000ull) {
+                }
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------ MMA issuer (a pair's leader)
+        if (leader && lane == 0) {
+            int stage = 0, acc = 0, g = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true, issued = false;
+            for (int64_t t = first; t < tiles && ok; t += step) {
+                const Tile o = tile_at<MODE, Cf>(p, start, t, g);
+                if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x22,
+                               p.wait_ns)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+                for (int kb = 0; kb < o.kblocks; ++kb) {
+                    if (!mbar_wait(&full[stage], phase, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x23, p.wait_ns)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(sA + stage * Cf::A_BYTES), b = smem_u32(sB + stage * Cf::B_BYTES);
+                    const int steps = kb == o.kblocks - 1 ? (o.klast + 15) / 16 : 4;
+                    for (int kk = 0; kk < steps; ++kk) {
+                        // K-major: 8-row atoms 1024 bytes apart, a k step of 16
+                        // moves 32 bytes inside the swizzled row.  MN-major:
+                        // 64-wide boxes, 8-row k groups 1024 bytes apart, a k
+                        // step moves 16 rows.
+                        const uint64_t ad = MODE == kTN ? sdesc_sw128(a + kk * 2048, kBoxBytes, 1024)
+                                                        : sdesc_sw128(a + kk * 32, 16, 1024);
+                        const uint64_t bd = MODE == kNT ? sdesc_sw128(b + kk * 32, 16, 1024)
+                                                        : sdesc_sw128(b + kk * 2048, kBoxBytes, 1024);
+                        if constexpr (PAIR)
+                            umma_f16_pair(d, ad, bd, p.idesc, (kb | kk) != 0 ? 1u : 0u);
+                        else
+                            umma_f16(d, ad, bd, p.idesc, (kb | kk) != 0 ? 1u : 0u);
+                    }
+                    if constexpr (PAIR)
+                        umma_commit_pair(&empty[stage], 0x3);
+                    else
+                        umma_commit(&empty[stage]);
+                    issued = true;
+                    if (++stage == S) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                }
+                if (!ok) break;
+                if constexpr (PAIR)
+                    umma_commit_pair(&tfull[acc], 0x3);
+                else
+                    umma_commit(&tfull[acc]);
+                if (++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1u;
+                }
+            }
+            if (!ok && issued) {
+                if constexpr (PAIR)
+                    umma_commit_pair(drain, 0x1);
+                else
+                    umma_commit(drain);
+                mbar_wait_drain(drain, 0, 1000000000ull);
+            }
+        }
+        __syncwarp();
+    } else if (MODE == kTN && warp == 6) {
+        // ------------------------------------------------ wiper (kTN)
+        int stage = 0, g = 0;
+        uint32_t phases = 0;  // bit s: parity of landed[s]
+        for (int64_t t = first; t < tiles; t += step) {
+            const Tile o = tile_at<MODE, Cf>(p, start, t, g);
+            if (o.kblocks == 0) continue;
+            const int s = (stage + o.kblocks - 1) % S;
+            stage = (stage + o.kblocks) % S;
+            if (o.klast == 64) continue;
+            const bool ok = mbar_wait_sleepy(&landed[s], phases >> s & 1u, abort_flag, p.status,
+                                             B2B_DEVSTAT_TIMEOUT | 0x25, p.wait_ns);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            phases ^= 1u << s;
+            // row r of a box is its 128 bytes at r * 128, whatever the swizzle
+            const int chunks = ((o.klast + 15) / 16 * 16 - o.klast) * 8;
+            for (int box = 0; box < 2 + Cf::BN_CTA / 64; ++box) {
+                uint8_t *at = (box < 2 ? sA + s * Cf::A_BYTES + box * kBoxBytes
+                                       : sB + s * Cf::B_BYTES + (box - 2) * kBoxBytes) + o.klast * 128;
+                for (int i = lane; i < chunks; i += 32) *reinterpret_cast<uint4 *>(at + i * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (leader)
+                    mbar_arrive(&full[s]);
+                else
+                    mbar_arrive_cluster(mapa_shared(smem_u32(&full[s]), 0));
+            }
+        }
+    } else {
+        // ------------------------------------------------ epilogue
+        const int q = warp & 3;  // TMEM lanes 32q .. 32q + 31
+        uint8_t *buf = epi + (warp - 2) * 4096;
+        const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
+        const int cols = p.f32 ? 32 : 64;  // columns of a chunk: 128 bytes of C
+        const int csize = p.f32 ? 4 : 2, per16 = 16 / csize;
+        int acc = 0, g = 0;
+        uint32_t acc_phase = 0;
+        for (int64_t t = first; t < tiles; t += step) {
+            const Tile o = tile_at<MODE, Cf>(p, start, t, g);
+            const bool ok = mbar_wait_sleepy(&tfull[acc], acc_phase, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x24,
+                                             p.wait_ns);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_fence_after();
+            const int r0 = rank * 128 + q * 32;  // the warp's first row in the tile
+            const int rows = min(32, o.valid - r0);
+            uint8_t *C = static_cast<uint8_t *>(p.C) +
+                         ((MODE == kTN ? static_cast<int64_t>(o.g) * p.M + o.m0 : static_cast<int64_t>(o.row0)) + r0) *
+                             p.N * csize;
+            const int64_t pitch = static_cast<int64_t>(p.N) * csize;
+#pragma unroll 1
+            for (int c = 0; c < BN; c += cols) {
+                uint32_t r[64];
+                __syncwarp();
+                const uint32_t taddr = tmem_base + lane_off + static_cast<uint32_t>(acc * BN + c);
+                tmem_ld_32x32b_x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r));
+                if (!p.f32) tmem_ld_32x32b_x32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
+                tmem_ld_wait();
+                if (c + cols >= BN) {  // the whole accumulator is in registers
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (leader)
+                            mbar_arrive(&tempty[acc]);
+                        else
+                            mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
+                    }
+                }
+                const int col0 = o.n0 + c;
+                if (rows <= 0 || col0 >= p.N) continue;  // the same for all lanes
+                const int ncols = min(cols, p.N - col0);
+                const bool empty_sum = MODE == kTN && o.kblocks == 0;
+                uint8_t *crow = C + lane * pitch + static_cast<int64_t>(col0) * csize;  // this lane's row
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {  // 16-byte chunks of the row
+                    uint4 v;
+                    uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+                    const int base = j * per16;
+                    const bool old = p.beta != 0.0f && lane < rows && base < ncols;
+                    if (p.f32) {
+                        float x[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            x[e] = empty_sum ? 0.0f : p.alpha * __uint_as_float(r[4 * j + e]);
+                            if (old && base + e < ncols)
+                                x[e] = fmaf(p.beta, reinterpret_cast<const float *>(crow)[base + e], x[e]);
+                            w[e] = __float_as_uint(x[e]);
+                        }
+                    } else {
+                        float x[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x[e] = empty_sum ? 0.0f : p.alpha * __uint_as_float(r[8 * j + e]);
+                        if (old) {
+                            const uint16_t *c16 = reinterpret_cast<const uint16_t *>(crow) + base;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                if (base + e < ncols)
+                                    x[e] = fmaf(p.beta, p.bf16 ? b2b::Half16<true>::get(c16[e])
+                                                               : b2b::Half16<false>::get(c16[e]), x[e]);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = p.bf16 ? b2b::Half16<true>::put2(x[2 * e], x[2 * e + 1])
+                                          : b2b::Half16<false>::put2(x[2 * e], x[2 * e + 1]);
+                    }
+                    // chunk j of row i sits at chunk j ^ (i % 8): conflict-free both ways
+                    *reinterpret_cast<uint4 *>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
+                }
+                __syncwarp();
+                uint8_t *cbase = C + static_cast<int64_t>(col0) * csize;
+                if (p.vec) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {  // four whole row segments an instruction
+                        const int row = i * 4 + (lane >> 3), j = lane & 7;
+                        if (row < rows && j * per16 < ncols)
+                            *reinterpret_cast<uint4 *>(cbase + row * pitch + j * 16) =
+                                *reinterpret_cast<const uint4 *>(buf + row * 128 + ((j ^ (row & 7)) << 4));
+                    }
+                } else {
+                    for (int row = 0; row < rows; ++row)
+                        for (int col = lane; col < ncols; col += 32) {
+                            const uint8_t *from = buf + row * 128 + (((col / per16) ^ (row & 7)) << 4) + col % per16 * csize;
+                            if (p.f32)
+                                *reinterpret_cast<float *>(cbase + row * pitch + col * 4) =
+                                    *reinterpret_cast<const float *>(from);
+                            else
+                                *reinterpret_cast<uint16_t *>(cbase + row * pitch + col * 2) =
+                                    *reinterpret_cast<const uint16_t *>(from);
+                        }
+                }
+            }
+            if (++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1u;
+            }
+        }
+    }
+
+    tc_fence_before();
+    if constexpr (PAIR)
+        cluster_sync();
+    else
+        __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        if constexpr (PAIR)
+            tmem_dealloc_pair(tmem_base, Cf::TMEM_COLS);
+        else
+            tmem_dealloc(tmem_base, Cf::TMEM_COLS);
+    }
+}
+
+// Launch state of one kernel instance on each device: the shared-memory
+// attribute is set, and how many CTAs (or pairs) are resident at once.
+struct Launch {
+    int ready[64] = {};
+    int resident[64] = {};
+};
+std::mutex g_mu;
+
+template <int MODE, bool PAIR, int BN>
+int launch_tc(b2b_handle *h, const CUtensorMap &tmA, const CUtensorMap &tmA16, const CUtensorMap &tmB,
+              const TcArgs &p, int64_t most_tiles) {
+    using Cf = Cfg<MODE, PAIR, BN>;
+    static Launch state;
+    auto kernel = grouped_tc_kernel<MODE, PAIR, BN>;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(Cf::THREADS);
+    cfg.dynamicSmemBytes = Cf::SMEM_BYTES;
+    cfg.stream = h->stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const int dev = h->device & 63;
+    int resident;
+    {
+        std::lock_guard<std::mutex> lock(g_mu);
+        if (!state.ready[dev]) {
+            cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::SMEM_BYTES);
+            if (e != cudaSuccess) return b2b::fail_cuda(e, "grouped HGEMM shared memory");
+            int clusters = h->sm_count;
+            if (PAIR) {
+                cfg.gridDim = dim3(2 * (h->sm_count / 2));
+                e = cudaOccupancyMaxActiveClusters(&clusters, reinterpret_cast<const void *>(kernel), &cfg);
+                if (e != cudaSuccess) return b2b::fail_cuda(e, "cudaOccupancyMaxActiveClusters");
+                if (clusters < 1) clusters = h->sm_count / 2;
+            }
+            state.resident[dev] = clusters;
+            state.ready[dev] = 1;
+        }
+        resident = state.resident[dev];
+    }
+    const int units = static_cast<int>(most_tiles < resident ? most_tiles : resident);
+    cfg.gridDim = dim3((PAIR ? 2 : 1) * units);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmA, tmA16, tmB, p);
+    return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, "grouped HGEMM tcgen05 launch");
+}
+
+// Tensor maps describe rows of a multiple of 16 bytes at 16-byte aligned
+// bases, and matrices less than 2^40 bytes apart.
+bool tma_can(const void *A, const void *B, int64_t ld_a, int64_t rows_b, int64_t ld_b) {
+    return b2b::aligned16(A) && b2b::aligned16(B) && ld_a % 8 == 0 && ld_b % 8 == 0 && rows_b * ld_b < (1ll << 39);
+}
+
 template <bool WGRAD, bool F32>
 int launch_simt(b2b_handle *h, int type, const GroupedArgs &p) {
     auto kernel = type == B2B_TYPE_BF16 ? grouped_simt_kernel<true, WGRAD, F32> : grouped_simt_kernel<false, WGRAD, F32>;
@@ -157,19 +702,73 @@ namespace b2b {
 int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, size_t rows, size_t n, size_t k,
                          float alpha, const uint16_t *A, const uint16_t *B, float beta, uint16_t *C,
                          const int32_t *offsets) {
-    const int64_t N = static_cast<int64_t>(n), K = static_cast<int64_t>(k);
-    const GroupedArgs p{A, B, C, offsets, h->d_status, static_cast<int>(groups), static_cast<int64_t>(rows), 0, N, K,
-                        K, 1, trans_b ? 1 : N, trans_b ? K : 1, alpha, beta};
-    return launch_simt<false, false>(h, type, p);
+    const int64_t N = static_cast<int64_t>(n), K = static_cast<int64_t>(k), R = static_cast<int64_t>(rows);
+    const int G = static_cast<int>(groups);
+    const bool bf16 = type == B2B_TYPE_BF16;
+    if (!tma_can(A, B, K, trans_b ? N : K, trans_b ? K : N)) {
+        const GroupedArgs p{A, B, C, offsets, h->d_status, G, R, 0, N, K, K, 1, trans_b ? 1 : N, trans_b ? K : 1,
+                            alpha, beta};
+        return launch_simt<false, false>(h, type, p);
+    }
+    // pairs where groups are long enough on average to fill their 256 rows
+    const bool pair = R >= 192 * static_cast<int64_t>(G) && N > 128;
+    int bn = 256;
+    if (!pair) {
+        const int64_t tiles_m = R / 128 + (R < G ? R : G);
+        while (bn > 64 && (tiles_m * ((N + bn - 1) / bn) < h->sm_count || N <= bn / 2)) bn /= 2;
+    }
+    const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap tmA, tmA16, tmB;
+    if (int rc = encode_tma_2d(&tmA, dt, 2, A, rows, k, 64, 128)) return rc;
+    if (int rc = encode_tma_2d(&tmA16, dt, 2, A, rows, k, 64, 16)) return rc;
+    const uint32_t ncta = pair ? 128 : bn;
+    const uint64_t cols = trans_b ? k : n, brows = trans_b ? n : k;
+    if (int rc = encode_tma_3d(&tmB, dt, 2, B, cols, brows, groups, cols * 2, cols * brows * 2, 64, trans_b ? ncta : 64,
+                               CU_TENSOR_MAP_SWIZZLE_128B))
+        return rc;
+    const uint32_t idesc = sm100::idesc_f32acc(bf16, 0, trans_b ? 0 : 1, pair ? 256 : 128, pair ? 256 : bn);
+    const TcArgs p{C, offsets, h->d_status, h->wait_limit_ns, G, static_cast<int>(rows), 0, static_cast<int>(n),
+                   static_cast<int>(k), alpha, beta, idesc, bf16, 0, n % 8 == 0 && aligned16(C)};
+    const int bm = pair ? 256 : 128;
+    const int64_t most = (R / bm + (R < G ? R : G)) * ((N + bn - 1) / bn);
+    if (trans_b) {
+        if (pair) return launch_tc<kNT, true, 256>(h, tmA, tmA16, tmB, p, most);
+        if (bn == 256) return launch_tc<kNT, false, 256>(h, tmA, tmA16, tmB, p, most);
+        if (bn == 128) return launch_tc<kNT, false, 128>(h, tmA, tmA16, tmB, p, most);
+        return launch_tc<kNT, false, 64>(h, tmA, tmA16, tmB, p, most);
+    }
+    if (pair) return launch_tc<kNN, true, 256>(h, tmA, tmA16, tmB, p, most);
+    if (bn == 256) return launch_tc<kNN, false, 256>(h, tmA, tmA16, tmB, p, most);
+    if (bn == 128) return launch_tc<kNN, false, 128>(h, tmA, tmA16, tmB, p, most);
+    return launch_tc<kNN, false, 64>(h, tmA, tmA16, tmB, p, most);
 }
 
 int launch_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t groups, size_t rows, size_t m, size_t n,
                                float alpha, const uint16_t *A, const uint16_t *B, float beta, void *C,
                                const int32_t *offsets) {
-    const int64_t M = static_cast<int64_t>(m), N = static_cast<int64_t>(n);
-    const GroupedArgs p{A, B, C, offsets, h->d_status, static_cast<int>(groups), static_cast<int64_t>(rows), M, N, 0,
-                        1, M, N, 1, alpha, beta};
-    return c_type == B2B_TYPE_F32 ? launch_simt<true, true>(h, type, p) : launch_simt<true, false>(h, type, p);
+    const int64_t M = static_cast<int64_t>(m), N = static_cast<int64_t>(n), R = static_cast<int64_t>(rows);
+    const int G = static_cast<int>(groups);
+    const bool bf16 = type == B2B_TYPE_BF16, f32 = c_type == B2B_TYPE_F32;
+    if (rows == 0 || !tma_can(A, B, M, 1, N)) {
+        const GroupedArgs p{A, B, C, offsets, h->d_status, G, R, M, N, 0, 1, M, N, 1, alpha, beta};
+        return f32 ? launch_simt<true, true>(h, type, p) : launch_simt<true, false>(h, type, p);
+    }
+    const bool pair = M > 128 && N > 128;
+    int bn = 256;
+    while (!pair && bn > 64 && (G * ((M + 127) / 128) * ((N + bn - 1) / bn) < h->sm_count || N <= bn / 2)) bn /= 2;
+    const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUtensorMap tmA, tmB;
+    if (int rc = encode_tma_2d(&tmA, dt, 2, A, rows, m, 64, 64)) return rc;
+    if (int rc = encode_tma_2d(&tmB, dt, 2, B, rows, n, 64, 64)) return rc;
+    const uint32_t idesc = sm100::idesc_f32acc(bf16, 1, 1, pair ? 256 : 128, pair ? 256 : bn);
+    const TcArgs p{C, offsets, h->d_status, h->wait_limit_ns, G, static_cast<int>(rows), static_cast<int>(m),
+                   static_cast<int>(n), 0, alpha, beta, idesc, bf16, f32, n % (f32 ? 4 : 8) == 0 && aligned16(C)};
+    const int bm = pair ? 256 : 128;
+    const int64_t most = G * ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+    if (pair) return launch_tc<kTN, true, 256>(h, tmA, tmA, tmB, p, most);
+    if (bn == 256) return launch_tc<kTN, false, 256>(h, tmA, tmA, tmB, p, most);
+    if (bn == 128) return launch_tc<kTN, false, 128>(h, tmA, tmA, tmB, p, most);
+    return launch_tc<kTN, false, 64>(h, tmA, tmA, tmB, p, most);
 }
 
 }  // namespace b2b
