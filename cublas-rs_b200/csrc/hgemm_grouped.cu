@@ -36,9 +36,11 @@ struct GroupedArgs {
 };
 
 // Tiles of `bm` rows that groups 0..g-1 hold, for g = 0..groups, in
-// start[0..groups]; false when the offsets do not ascend within [0, rows].
+// start[0..groups], and the offsets themselves in off[0..groups] (when given);
+// false when the offsets do not ascend within [0, rows].
 // One warp; every lane returns the verdict.
-__device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, int bm, int *start) {
+__device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, int bm, int *start,
+                            int *off = nullptr) {
     const int lane = threadIdx.x & 31;
     bool ok = true;
     int carry = 0;
@@ -47,6 +49,10 @@ __device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, in
         int tiles = 0;
         if (g < groups) {
             const int64_t lo = offsets[g], hi = offsets[g + 1];
+            if (off) {
+                off[g] = static_cast<int>(lo);
+                if (g == groups - 1) off[groups] = static_cast<int>(hi);
+            }
             if (lo < 0 || hi < lo || hi > rows)
                 ok = false;
             else
@@ -182,9 +188,9 @@ struct Cfg {
     static constexpr int EPI_BYTES = 4 * 4096;  // 32 rows of 128 bytes for each epilogue warp
     static constexpr int TMEM_COLS = 2 * BN;
     static constexpr int THREADS = MODE == kTN ? 224 : 192;
-    static constexpr int TABLE_BYTES = 4352;  // kMaxGroups + 1 ints, rounded up
+    static constexpr int TABLE_BYTES = 2 * 4224;  // tile starts and offsets: kMaxGroups + 1 ints each, rounded up
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + TABLE_BYTES + 1024 + 512;
-    static_assert(SMEM_BYTES <= 232448 && TABLE_BYTES >= 4 * (kMaxGroups + 1), "shared memory per CTA");
+    static_assert(SMEM_BYTES <= 232448 && TABLE_BYTES / 2 >= 4 * (kMaxGroups + 1), "shared memory per CTA");
 };
 constexpr int kBoxBytes = 64 * 64 * 2;  // 64 columns x 64 rows of an MN-major operand
 constexpr int kGroupM = 16;             // raster: tile rows that sweep a group's columns together
@@ -206,39 +212,37 @@ struct Tile {
     int row0;       // first row of A (kTN: of A and B)
     int m0, n0;     // first row (kTN) and column within the group's C
     int valid;      // rows of the tile that exist
+    int depth;           // of the sum
     int kblocks, klast;  // k blocks of 64, and what the last one holds
 };
 
 // The t-th tile, t ascending from call to call (g is kept between them).
 template <int MODE, typename Cf>
-__device__ __forceinline__ Tile tile_at(const TcArgs &p, const int *start, int64_t t, int &g) {
-    const int nt = (p.N + Cf::BN - 1) / Cf::BN;
-    int mt;
-    int64_t local;
+__device__ __forceinline__ Tile tile_at(const TcArgs &p, const int *start, const int *off, uint32_t t, int &g) {
+    const uint32_t nt = static_cast<uint32_t>(p.N + Cf::BN - 1) / Cf::BN;
+    uint32_t mt, local;
     Tile o;
     if constexpr (MODE == kTN) {
-        mt = (p.M + Cf::BM - 1) / Cf::BM;
-        const int64_t per = static_cast<int64_t>(mt) * nt;
-        g = static_cast<int>(t / per);
-        local = t - g * per;
+        mt = static_cast<uint32_t>(p.M + Cf::BM - 1) / Cf::BM;
+        g = static_cast<int>(t / (mt * nt));
+        local = t % (mt * nt);
     } else {
-        while (t >= static_cast<int64_t>(start[g + 1]) * nt) ++g;
+        while (t >= static_cast<uint32_t>(start[g + 1]) * nt) ++g;
         mt = start[g + 1] - start[g];
-        local = t - static_cast<int64_t>(start[g]) * nt;
+        local = t - static_cast<uint32_t>(start[g]) * nt;
     }
-    const int64_t span = static_cast<int64_t>(kGroupM) * nt;
-    const int first = static_cast<int>(local / span) * kGroupM;
-    const int gm = min(mt - first, kGroupM);
-    const int r = static_cast<int>(local % span);
-    const int tm = first + r % gm;
+    const uint32_t span = kGroupM * nt;
+    const uint32_t first = local / span * kGroupM;
+    const uint32_t gm = min(mt - first, static_cast<uint32_t>(kGroupM));
+    const uint32_t r = local % span;
     o.g = g;
-    o.n0 = r / gm * Cf::BN;
-    o.m0 = tm * Cf::BM;
-    const int lo = p.offsets[g], hi = p.offsets[g + 1];
-    const int depth = MODE == kTN ? hi - lo : p.K;
+    o.n0 = static_cast<int>(r / gm) * Cf::BN;
+    o.m0 = static_cast<int>(first + r % gm) * Cf::BM;
+    const int lo = off[g], hi = off[g + 1];
+    const int depth = o.depth = MODE == kTN ? hi - lo : p.K;
     o.row0 = MODE == kTN ? lo : lo + o.m0;
     o.valid = min(Cf::BM, (MODE == kTN ? p.M : hi - lo) - o.m0);
-    o.kblocks = (depth + 63) / 64;
+    o.kblocks = static_cast<int>(static_cast<uint32_t>(depth + 63) / 64);
     o.klast = depth - (o.kblocks - 1) * 64;
     return o;
 }
@@ -264,6 +268,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
     uint8_t *sB = smem + S * Cf::A_BYTES;
     uint8_t *epi = smem + S * Cf::STAGE_BYTES;
     int *start = reinterpret_cast<int *>(epi + Cf::EPI_BYTES);
+    int *off = start + Cf::TABLE_BYTES / 8;
     uint64_t *bars = reinterpret_cast<uint64_t *>(epi + Cf::EPI_BYTES + Cf::TABLE_BYTES);
     uint64_t *full = bars, *empty = bars + S, *landed = bars + 2 * S;  // landed: kTN, last k block of a group
     uint64_t *tfull = bars + 3 * S, *tempty = bars + 3 * S + 2, *drain = bars + 3 * S + 4;
@@ -274,7 +279,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
     const bool leader = rank == 0;
-    const int64_t first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    const uint32_t first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
@@ -304,7 +309,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
         }
     }
     if (warp == 2) {
-        const bool ok = scan_groups(p.offsets, p.groups, p.rows, Cf::BM, start);
+        const bool ok = scan_groups(p.offsets, p.groups, p.rows, Cf::BM, start, off);
         if (lane == 0) {
             *valid_flag = ok;
             if (!ok) atomicCAS(p.status, 0, B2B_DEVSTAT_OFFSETS);
@@ -317,11 +322,11 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
         __syncthreads();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const int nt = (p.N + BN - 1) / BN;
-    int64_t tiles = 0;
+    uint32_t tiles = 0;  // the launcher has seen to it that they stay below 2^31
     if (*valid_flag)
-        tiles = (MODE == kTN ? static_cast<int64_t>(p.groups) * ((p.M + Cf::BM - 1) / Cf::BM)
-                             : static_cast<int64_t>(start[p.groups])) * nt;
+        tiles = static_cast<uint32_t>(MODE == kTN ? p.groups * (static_cast<uint32_t>(p.M + Cf::BM - 1) / Cf::BM)
+                                                  : start[p.groups]) *
+                (static_cast<uint32_t>(p.N + BN - 1) / BN);
 
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
@@ -329,8 +334,8 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
             int stage = 0, g = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int64_t t = first; t < tiles && ok; t += step) {
-                const Tile o = tile_at<MODE, Cf>(p, start, t, g);
+            for (uint32_t t = first; t < tiles && ok; t += step) {
+                const Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
                 const int mine = MODE == kTN ? 8 : a_boxes16(o.valid, rank);
                 const int both = !PAIR ? mine : MODE == kTN ? 16 : a_boxes16(o.valid, 0) + a_boxes16(o.valid, 1);
                 for (int kb = 0; kb < o.kblocks; ++kb) {
@@ -355,7 +360,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
                         if (leader)
                             mbar_arrive_expect_tx(&full[stage], both * 2048 + 2 * Cf::B_BYTES);
                         else if (MODE == kTN)
-                            mbar_arrive_cluster(bar);
+                            mbar_arrive_cluster_relaxed(bar);
                         if constexpr (MODE == kTN) {
                             for (int j = 0; j < 2; ++j)
                                 tma_load_2d_pair(a_dst + j * kBoxBytes, &tmA, bar, o.m0 + rank * 128 + 64 * j,
@@ -417,8 +422,10 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
             int stage = 0, acc = 0, g = 0;
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true, issued = false;
-            for (int64_t t = first; t < tiles && ok; t += step) {
-                const Tile o = tile_at<MODE, Cf>(p, start, t, g);
+            for (uint32_t t = first; t < tiles && ok; t += step) {
+                int depth = p.K;
+                if constexpr (MODE == kTN) depth = tile_at<MODE, Cf>(p, start, off, t, g).depth;
+                const int kblocks = static_cast<int>(static_cast<uint32_t>(depth + 63) / 64);
                 if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x22,
                                p.wait_ns)) {
                     ok = false;
@@ -426,19 +433,18 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
                 }
                 tc_fence_after();
                 const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
-                for (int kb = 0; kb < o.kblocks; ++kb) {
+                for (int kb = 0; kb < kblocks; ++kb) {
                     if (!mbar_wait(&full[stage], phase, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x23, p.wait_ns)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
                     const uint32_t a = smem_u32(sA + stage * Cf::A_BYTES), b = smem_u32(sB + stage * Cf::B_BYTES);
-                    const int steps = kb == o.kblocks - 1 ? (o.klast + 15) / 16 : 4;
-                    for (int kk = 0; kk < steps; ++kk) {
-                        // K-major: 8-row atoms 1024 bytes apart, a k step of 16
-                        // moves 32 bytes inside the swizzled row.  MN-major:
-                        // 64-wide boxes, 8-row k groups 1024 bytes apart, a k
-                        // step moves 16 rows.
+                    // K-major: 8-row atoms 1024 bytes apart, a k step of 16
+                    // moves 32 bytes inside the swizzled row.  MN-major:
+                    // 64-wide boxes, 8-row k groups 1024 bytes apart, a k
+                    // step moves 16 rows.
+                    auto k_step = [&](int kk) {
                         const uint64_t ad = MODE == kTN ? sdesc_sw128(a + kk * 2048, kBoxBytes, 1024)
                                                         : sdesc_sw128(a + kk * 32, 16, 1024);
                         const uint64_t bd = MODE == kNT ? sdesc_sw128(b + kk * 32, 16, 1024)
@@ -447,6 +453,13 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
                             umma_f16_pair(d, ad, bd, p.idesc, (kb | kk) != 0 ? 1u : 0u);
                         else
                             umma_f16(d, ad, bd, p.idesc, (kb | kk) != 0 ? 1u : 0u);
+                    };
+                    const int left = depth - kb * 64;
+                    if (left >= 64) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk) k_step(kk);
+                    } else {
+                        for (int kk = 0; kk * 16 < left; ++kk) k_step(kk);
                     }
                     if constexpr (PAIR)
                         umma_commit_pair(&empty[stage], 0x3);
@@ -481,8 +494,8 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
         // ------------------------------------------------ wiper (kTN)
         int stage = 0, g = 0;
         uint32_t phases = 0;  // bit s: parity of landed[s]
-        for (int64_t t = first; t < tiles; t += step) {
-            const Tile o = tile_at<MODE, Cf>(p, start, t, g);
+        for (uint32_t t = first; t < tiles; t += step) {
+            const Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
             if (o.kblocks == 0) continue;
             const int s = (stage + o.kblocks - 1) % S;
             stage = (stage + o.kblocks) % S;
@@ -516,8 +529,8 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
         const int csize = p.f32 ? 4 : 2, per16 = 16 / csize;
         int acc = 0, g = 0;
         uint32_t acc_phase = 0;
-        for (int64_t t = first; t < tiles; t += step) {
-            const Tile o = tile_at<MODE, Cf>(p, start, t, g);
+        for (uint32_t t = first; t < tiles; t += step) {
+            const Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
             const bool ok = mbar_wait_sleepy(&tfull[acc], acc_phase, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x24,
                                              p.wait_ns);
             if (!__all_sync(0xffffffffu, ok)) break;
@@ -705,7 +718,7 @@ int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, si
     const int64_t N = static_cast<int64_t>(n), K = static_cast<int64_t>(k), R = static_cast<int64_t>(rows);
     const int G = static_cast<int>(groups);
     const bool bf16 = type == B2B_TYPE_BF16;
-    if (!tma_can(A, B, K, trans_b ? N : K, trans_b ? K : N)) {
+    if (!tma_can(A, B, K, trans_b ? N : K, trans_b ? K : N) || (R / 128 + (R < G ? R : G)) * (N / 64 + 1) >= 1ll << 31) {
         const GroupedArgs p{A, B, C, offsets, h->d_status, G, R, 0, N, K, K, 1, trans_b ? 1 : N, trans_b ? K : 1,
                             alpha, beta};
         return launch_simt<false, false>(h, type, p);
@@ -749,7 +762,7 @@ int launch_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t group
     const int64_t M = static_cast<int64_t>(m), N = static_cast<int64_t>(n), R = static_cast<int64_t>(rows);
     const int G = static_cast<int>(groups);
     const bool bf16 = type == B2B_TYPE_BF16, f32 = c_type == B2B_TYPE_F32;
-    if (rows == 0 || !tma_can(A, B, M, 1, N)) {
+    if (rows == 0 || !tma_can(A, B, M, 1, N) || G * (M / 128 + 1) * (N / 64 + 1) >= 1ll << 31) {
         const GroupedArgs p{A, B, C, offsets, h->d_status, G, R, M, N, 0, 1, M, N, 1, alpha, beta};
         return f32 ? launch_simt<true, true>(h, type, p) : launch_simt<true, false>(h, type, p);
     }

@@ -256,6 +256,12 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t remote_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_addr) : "memory");
 }
 
+// The same without ordering this thread's memory accesses before it: for an
+// arrival that hands over no data of its own.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t remote_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_addr) : "memory");
+}
+
 // Full cluster barrier (every thread of every CTA in the cluster).
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
