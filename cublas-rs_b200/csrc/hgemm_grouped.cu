@@ -170,10 +170,11 @@ __global__ void __launch_bounds__(256) grouped_simt_kernel(GroupedArgs p) {
 // rows past the end, in A and B both (0 times a neighbour's NaN is a NaN),
 // up to the next multiple of 16, and the MMA issues only those k steps.
 //
-// Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer, 2..5 epilogue, 6
+// Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer, 2..9 epilogue, 10
 // (kTN) the wiper.  Two accumulators: the epilogue of a tile runs under the
-// MMAs of the next.  The epilogue goes through shared memory to whole 128-byte
-// row segments, since a TMA store would write past the group's last row.
+// MMAs of the next.  The epilogue goes through shared memory to 64-byte row
+// segments, since a TMA store would write past the group's last row; it is a
+// chain of short latencies, so two warps share each quarter of the TMEM lanes.
 enum Mode { kNN = 0, kNT = 1, kTN = 2 };
 
 template <int MODE, bool PAIR, int BN_>
@@ -185,9 +186,9 @@ struct Cfg {
     static constexpr int B_BYTES = BN_CTA * 64 * 2;
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int STAGES = 196608 / STAGE_BYTES;
-    static constexpr int EPI_BYTES = 4 * 4096;  // 32 rows of 128 bytes for each epilogue warp
+    static constexpr int EPI_BYTES = 8 * 2048;  // 32 rows of 64 bytes for each epilogue warp
     static constexpr int TMEM_COLS = 2 * BN;
-    static constexpr int THREADS = MODE == kTN ? 224 : 192;
+    static constexpr int THREADS = MODE == kTN ? 352 : 320;
     static constexpr int TABLE_BYTES = 2 * 4224;  // tile starts and offsets: kMaxGroups + 1 ints each, rounded up
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + TABLE_BYTES + 1024 + 512;
     static_assert(SMEM_BYTES <= 232448 && TABLE_BYTES / 2 >= 4 * (kMaxGroups + 1), "shared memory per CTA");
@@ -255,6 +256,75 @@ __device__ __forceinline__ int a_boxes16(int valid, int rank) {
     return v > 64 ? 8 : v > 0 ? (v + 15) / 16 : 0;
 }
 
+// Where 16-byte chunk j (0..3) of row i sits in an epilogue warp's 32 x 64
+// byte buffer: rows i and i + 1 share 128 bytes, chunks turn with i / 2, so
+// that writes by row and reads by segment both meet every bank once.
+__device__ __forceinline__ int seg_chunk(int i, int j) { return i * 64 + ((j ^ ((i >> 1) & 3)) << 4); }
+
+// The buffer's rows to C: `ncols` columns (at most a segment's) of `rows` rows.
+template <typename T>
+__device__ __forceinline__ void store_segment(uint8_t *c, int64_t pitch, const uint8_t *buf, int rows, int ncols,
+                                              int vec, int lane) {
+    constexpr int per16 = 16 / sizeof(T);
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + (lane >> 2), j = lane & 3;
+            if (row < rows && j * per16 < ncols)
+                *reinterpret_cast<uint4 *>(c + row * pitch + j * 16) =
+                    *reinterpret_cast<const uint4 *>(buf + seg_chunk(row, j));
+        }
+    } else {
+        const int col = lane % (4 * per16);
+        if (col < ncols)
+            for (int row = lane / (4 * per16); row < rows; row += 32 / (4 * per16))
+                *reinterpret_cast<T *>(c + row * pitch + col * sizeof(T)) =
+                    *reinterpret_cast<const T *>(buf + seg_chunk(row, col / per16) + col % per16 * sizeof(T));
+    }
+}
+
+// x += beta * (the row's old values).
+__device__ __forceinline__ void add_old(float (&x)[32], const uint8_t *row, int ncols, const TcArgs &p) {
+    if (p.f32) {
+        const float *c = reinterpret_cast<const float *>(row);
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+            if (p.vec) {
+                if (e >= ncols) continue;
+                const float4 v = *reinterpret_cast<const float4 *>(c + e);
+                x[e] = fmaf(p.beta, v.x, x[e]);
+                x[e + 1] = fmaf(p.beta, v.y, x[e + 1]);
+                x[e + 2] = fmaf(p.beta, v.z, x[e + 2]);
+                x[e + 3] = fmaf(p.beta, v.w, x[e + 3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (e + i < ncols) x[e + i] = fmaf(p.beta, c[e + i], x[e + i]);
+            }
+        }
+    } else {
+        const uint16_t *c = reinterpret_cast<const uint16_t *>(row);
+#pragma unroll
+        for (int e = 0; e < 32; e += 8) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+            if (p.vec) {
+                if (e < ncols) v = *reinterpret_cast<const uint4 *>(c + e);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (e + i < ncols) w[i / 2] |= static_cast<uint32_t>(c[e + i]) << (i % 2 * 16);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = p.bf16 ? b2b::Half16<true>::get2(w[i]) : b2b::Half16<false>::get2(w[i]);
+                x[e + 2 * i] = fmaf(p.beta, f.x, x[e + 2 * i]);
+                x[e + 2 * i + 1] = fmaf(p.beta, f.y, x[e + 2 * i + 1]);
+            }
+        }
+    }
+}
+
 template <int MODE, bool PAIR, int BN>
 __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA16,
@@ -291,7 +361,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&tfull[a], 1);
-            mbar_init(&tempty[a], PAIR ? 8 : 4);
+            mbar_init(&tempty[a], PAIR ? 16 : 8);
         }
         mbar_init(drain, 1);
         *abort_flag = 0;
@@ -490,7 +560,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
             }
         }
         __syncwarp();
-    } else if (MODE == kTN && warp == 6) {
+    } else if (MODE == kTN && warp == 10) {
         // ------------------------------------------------ wiper (kTN)
         int stage = 0, g = 0;
         uint32_t phases = 0;  // bit s: parity of landed[s]
@@ -523,10 +593,10 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
     } else {
         // ------------------------------------------------ epilogue
         const int q = warp & 3;  // TMEM lanes 32q .. 32q + 31
-        uint8_t *buf = epi + (warp - 2) * 4096;
-        const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
-        const int cols = p.f32 ? 32 : 64;  // columns of a chunk: 128 bytes of C
-        const int csize = p.f32 ? 4 : 2, per16 = 16 / csize;
+        const int c_first = (warp - 2) / 4 * (BN / 2), c_end = c_first + BN / 2;  // the warp's columns
+        uint8_t *buf = epi + (warp - 2) * 2048;
+        const int csize = p.f32 ? 4 : 2;
+        const int64_t pitch = static_cast<int64_t>(p.N) * csize;
         int acc = 0, g = 0;
         uint32_t acc_phase = 0;
         for (uint32_t t = first; t < tiles; t += step) {
@@ -537,19 +607,18 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
             tc_fence_after();
             const int r0 = rank * 128 + q * 32;  // the warp's first row in the tile
             const int rows = min(32, o.valid - r0);
+            const bool empty_sum = MODE == kTN && o.kblocks == 0;
             uint8_t *C = static_cast<uint8_t *>(p.C) +
                          ((MODE == kTN ? static_cast<int64_t>(o.g) * p.M + o.m0 : static_cast<int64_t>(o.row0)) + r0) *
-                             p.N * csize;
-            const int64_t pitch = static_cast<int64_t>(p.N) * csize;
+                             pitch;
 #pragma unroll 1
-            for (int c = 0; c < BN; c += cols) {
-                uint32_t r[64];
+            for (int c = c_first; c < c_end; c += 32) {
+                uint32_t r[32];
                 __syncwarp();
-                const uint32_t taddr = tmem_base + lane_off + static_cast<uint32_t>(acc * BN + c);
-                tmem_ld_32x32b_x32(taddr, *reinterpret_cast<uint32_t(*)[32]>(r));
-                if (!p.f32) tmem_ld_32x32b_x32(taddr + 32, *reinterpret_cast<uint32_t(*)[32]>(r + 32));
+                tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
+                                       static_cast<uint32_t>(acc * BN + c), r);
                 tmem_ld_wait();
-                if (c + cols >= BN) {  // the whole accumulator is in registers
+                if (c + 32 == c_end) {  // the warp's share of the accumulator is in registers
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
@@ -561,65 +630,46 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
                 }
                 const int col0 = o.n0 + c;
                 if (rows <= 0 || col0 >= p.N) continue;  // the same for all lanes
-                const int ncols = min(cols, p.N - col0);
-                const bool empty_sum = MODE == kTN && o.kblocks == 0;
-                uint8_t *crow = C + lane * pitch + static_cast<int64_t>(col0) * csize;  // this lane's row
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {  // 16-byte chunks of the row
-                    uint4 v;
-                    uint32_t *w = reinterpret_cast<uint32_t *>(&v);
-                    const int base = j * per16;
-                    const bool old = p.beta != 0.0f && lane < rows && base < ncols;
-                    if (p.f32) {
-                        float x[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            x[e] = empty_sum ? 0.0f : p.alpha * __uint_as_float(r[4 * j + e]);
-                            if (old && base + e < ncols)
-                                x[e] = fmaf(p.beta, reinterpret_cast<const float *>(crow)[base + e], x[e]);
-                            w[e] = __float_as_uint(x[e]);
-                        }
-                    } else {
-                        float x[8];
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = empty_sum ? 0.0f : p.alpha * __uint_as_float(r[8 * j + e]);
-                        if (old) {
-                            const uint16_t *c16 = reinterpret_cast<const uint16_t *>(crow) + base;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                if (base + e < ncols)
-                                    x[e] = fmaf(p.beta, p.bf16 ? b2b::Half16<true>::get(c16[e])
-                                                               : b2b::Half16<false>::get(c16[e]), x[e]);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            w[e] = p.bf16 ? b2b::Half16<true>::put2(x[2 * e], x[2 * e + 1])
-                                          : b2b::Half16<false>::put2(x[2 * e], x[2 * e + 1]);
-                    }
-                    // chunk j of row i sits at chunk j ^ (i % 8): conflict-free both ways
-                    *reinterpret_cast<uint4 *>(buf + lane * 128 + ((j ^ (lane & 7)) << 4)) = v;
-                }
-                __syncwarp();
+                const int ncols = min(32, p.N - col0);
                 uint8_t *cbase = C + static_cast<int64_t>(col0) * csize;
-                if (p.vec) {
+                float x[32];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {  // four whole row segments an instruction
-                        const int row = i * 4 + (lane >> 3), j = lane & 7;
-                        if (row < rows && j * per16 < ncols)
-                            *reinterpret_cast<uint4 *>(cbase + row * pitch + j * 16) =
-                                *reinterpret_cast<const uint4 *>(buf + row * 128 + ((j ^ (row & 7)) << 4));
+                for (int e = 0; e < 32; ++e) x[e] = p.alpha * __uint_as_float(r[e]);
+                if (empty_sum) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[e] = 0.0f;
+                }
+                if (p.beta != 0.0f && lane < rows) add_old(x, cbase + lane * pitch, ncols, p);
+                if (p.f32) {
+                    // two segments of 16 columns through the one buffer
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        if (s) __syncwarp();
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            *reinterpret_cast<float4 *>(buf + seg_chunk(lane, j)) = make_float4(
+                                x[16 * s + 4 * j], x[16 * s + 4 * j + 1], x[16 * s + 4 * j + 2], x[16 * s + 4 * j + 3]);
+                        __syncwarp();
+                        store_segment<float>(cbase + s * 64, pitch, buf, rows, ncols - 16 * s, p.vec, lane);
                     }
                 } else {
-                    for (int row = 0; row < rows; ++row)
-                        for (int col = lane; col < ncols; col += 32) {
-                            const uint8_t *from = buf + row * 128 + (((col / per16) ^ (row & 7)) << 4) + col % per16 * csize;
-                            if (p.f32)
-                                *reinterpret_cast<float *>(cbase + row * pitch + col * 4) =
-                                    *reinterpret_cast<const float *>(from);
-                            else
-                                *reinterpret_cast<uint16_t *>(cbase + row * pitch + col * 2) =
-                                    *reinterpret_cast<const uint16_t *>(from);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint4 v;
+                        uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+                        if (p.bf16) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                w[e] = b2b::Half16<true>::put2(x[8 * j + 2 * e], x[8 * j + 2 * e + 1]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                w[e] = b2b::Half16<false>::put2(x[8 * j + 2 * e], x[8 * j + 2 * e + 1]);
                         }
+                        *reinterpret_cast<uint4 *>(buf + seg_chunk(lane, j)) = v;
+                    }
+                    __syncwarp();
+                    store_segment<uint16_t>(cbase, pitch, buf, rows, ncols, p.vec, lane);
                 }
             }
             if (++acc == 2) {
@@ -727,8 +777,11 @@ int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, si
     const bool pair = R >= 192 * static_cast<int64_t>(G) && N > 128;
     int bn = 256;
     if (!pair) {
+        // the width whose waves of CTAs compute the fewest columns in turn
         const int64_t tiles_m = R / 128 + (R < G ? R : G);
-        while (bn > 64 && (tiles_m * ((N + bn - 1) / bn) < h->sm_count || N <= bn / 2)) bn /= 2;
+        auto turn = [&](int w) { return (tiles_m * ((N + w - 1) / w) + h->sm_count - 1) / h->sm_count * w; };
+        for (int w = 128; w >= 64; w /= 2)
+            if (turn(w) < turn(bn)) bn = w;
     }
     const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap tmA, tmA16, tmB;
