@@ -605,31 +605,36 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
                                              p.wait_ns);
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
+            // the warp has read its share of the accumulator
+            auto release = [&] {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (leader)
+                        mbar_arrive(&tempty[acc]);
+                    else
+                        mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
+                }
+            };
             const int r0 = rank * 128 + q * 32;  // the warp's first row in the tile
             const int rows = min(32, o.valid - r0);
             const bool empty_sum = MODE == kTN && o.kblocks == 0;
             uint8_t *C = static_cast<uint8_t *>(p.C) +
                          ((MODE == kTN ? static_cast<int64_t>(o.g) * p.M + o.m0 : static_cast<int64_t>(o.row0)) + r0) *
                              pitch;
+            // the warp's columns that exist, in steps of 32; none where no row does
+            const int left = p.N - o.n0 - c_first;
+            const int c_stop = rows > 0 && left > 0 ? min(c_end, c_first + (left + 31) / 32 * 32) : c_first;
+            if (c_stop == c_first) release();
 #pragma unroll 1
-            for (int c = c_first; c < c_end; c += 32) {
+            for (int c = c_first; c < c_stop; c += 32) {
                 uint32_t r[32];
                 __syncwarp();
                 tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
                                        static_cast<uint32_t>(acc * BN + c), r);
                 tmem_ld_wait();
-                if (c + 32 == c_end) {  // the warp's share of the accumulator is in registers
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) {
-                        if (leader)
-                            mbar_arrive(&tempty[acc]);
-                        else
-                            mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
-                    }
-                }
+                if (c + 32 == c_stop) release();
                 const int col0 = o.n0 + c;
-                if (rows <= 0 || col0 >= p.N) continue;  // the same for all lanes
                 const int ncols = min(32, p.N - col0);
                 uint8_t *cbase = C + static_cast<int64_t>(col0) * csize;
                 float x[32];
@@ -777,11 +782,14 @@ int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, si
     const bool pair = R >= 192 * static_cast<int64_t>(G) && N > 128;
     int bn = 256;
     if (!pair) {
-        // the width whose waves of CTAs compute the fewest columns in turn
+        // The width whose turns of CTAs take least.  A k block of 64 costs a
+        // CTA about 340 ns at 64 columns, 375 at 128 and 680 at 256 (its MMAs
+        // take as long at any width, its share of HBM does not).
         const int64_t tiles_m = R / 128 + (R < G ? R : G);
-        auto turn = [&](int w) { return (tiles_m * ((N + w - 1) / w) + h->sm_count - 1) / h->sm_count * w; };
-        for (int w = 128; w >= 64; w /= 2)
-            if (turn(w) < turn(bn)) bn = w;
+        auto turns = [&](int w) { return (tiles_m * ((N + w - 1) / w) + h->sm_count - 1) / h->sm_count; };
+        const double t256 = 2.0 * turns(256), t128 = 1.1 * turns(128), t64 = 1.0 * turns(64);
+        if (t128 < t256 || N <= 128) bn = 128;
+        if (t64 < (bn == 128 ? t128 : t256) || N <= 64) bn = 64;
     }
     const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap tmA, tmA16, tmB;

@@ -244,6 +244,13 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
     return r;
 }
 
+// CTAs of this cluster.
+__device__ __forceinline__ uint32_t cluster_nctarank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+
 // Address of the same shared-memory offset in CTA `rank` of this cluster.
 __device__ __forceinline__ uint32_t mapa_shared(uint32_t saddr, uint32_t rank) {
     uint32_t r;
@@ -265,6 +272,15 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t remote_addr
 // Full cluster barrier (every thread of every CTA in the cluster).
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The two halves of cluster_sync, for work between them.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Store to shared memory of a CTA of the cluster (address from mapa).
+__device__ __forceinline__ void st_shared_cluster(uint32_t addr, float v) {
+    asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
 // 2-D tiled load into this CTA's shared memory whose completion is counted

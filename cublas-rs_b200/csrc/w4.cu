@@ -5,11 +5,16 @@
 //
 //   W[i][j] = scale[i][j / group] * (q[i][j] - zero[i][j / group])
 //   y_i = alpha * W x_i + beta * y_i
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <mutex>
+#include <vector>
+
 #include "half_types.cuh"
 #include "internal.h"
+#include "sm100.cuh"
 
 namespace {
 
@@ -92,29 +97,420 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(W4Args p, uint16_t *
     }
 }
 
-// One warp a row and product.
+// ---------------------------------------------------------------------------
+// Products with vectors: y_i = alpha W x_i + beta y_i for up to 8 vectors that
+// share W.  HBM-bound: the packed values are read once, so the work for each
+// must stay under the ~2.5 instructions that 148 SMs can issue in the time a
+// value takes to arrive.  Multiplying on the tensor cores with the 8 columns
+// of mma.m16n8k16 does that for 1 vector as for 8: a word of 8 values becomes
+// four register pairs of exact (q - zero) in 9 instructions (f16: or the bits
+// into 1024 + q or 1024 + 16 q, then one packed subtraction or fma), and 16
+// words of a warp are one MMA operand.  Sums are f32, a group's sum is scaled
+// in f32 and added to the row's; no product or sum is rounded to 16 bits.
+//
+//   * A unit is 32 rows of W for one set of vectors; its n columns are cut
+//     into chunks of 256 (128 bytes of a row).  Chunk c belongs to CTA c % KS
+//     of a cluster, and there to warp (c / KS) % 8.
+//   * Each warp keeps its own ring of chunks (32 rows x 128 bytes, 128-byte
+//     swizzle) filled by TMA ahead of its use, across units, so nothing
+//     drains at a unit's end; 2 CTAs of 8 warps x 2 chunks hold 128 KiB of W
+//     in flight on an SM.
+//   * The vectors are staged once for each set, each 8 columns reordered to
+//     the pairs (0,4) (1,5) (2,6) (3,7) that the words unpack to.
+//   * Warps join their sums through shared memory, CTAs of a cluster through
+//     the first CTA's shared memory, one unit later so that no one waits;
+//     both in a fixed order.
+// Rows that TMA cannot describe (n not a multiple of 32, packed not 16-byte
+// aligned) are read by the same kernel with plain loads.
+constexpr int kWarps = 8;
+constexpr int kTileRows = 32;
+constexpr int kChunk = 256;                       // columns
+constexpr int kChunkBytes = kTileRows * kChunk / 2;
+constexpr int kMaxIndexed = 256;                  // products of one launch that choose their matrix
+
+struct GemvArgs {
+    W4Args w;
+    const uint16_t *x;
+    const int32_t *index;  // nullptr: every product uses matrix 0
+    uint16_t *y;
+    int *status;
+    uint64_t wait_ns;
+    int matrices, count, fan, first;  // first: number of this launch's first product
+    int width;    // vectors of a set: 8, or fewer where longer rows leave room for fewer
+    int stages;   // chunks of a warp's ring
+    int x_bytes;  // of the staged vectors
+    float alpha, beta;
+    int64_t total;  // bytes of packed
+};
+
+// Products that share a matrix, at most 8; counted from the launch's first.
+struct Item {
+    int matrix;  // -1: none
+    int count;
+    uint8_t member[8];
+};
+// What a launch that chooses matrices keeps of its products.
+struct Table {
+    Item item[kMaxIndexed];
+    int index[kMaxIndexed];
+    uint8_t lead[kMaxIndexed];
+    int items;
+};
+
+// The 4 bytes at packed + at, wherever that is aligned; bytes past the end
+// are 0 (they meet zeros of x).
+__device__ __forceinline__ uint32_t word_at(const GemvArgs &p, int64_t at) {
+    const uint8_t *src = p.w.packed + at;
+    const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(src) & 3);
+    if (at - shift >= 0 && at - shift + 8 <= p.total) {
+        const uint32_t *word = reinterpret_cast<const uint32_t *>(src - shift);
+        return shift ? __funnelshift_r(__ldg(word), __ldg(word + 1), 8 * shift) : __ldg(word);
+    }
+    uint32_t v = 0;
+    for (int i = 0; i < 4; ++i)
+        if (at + i < p.total) v |= static_cast<uint32_t>(src[i]) << (8 * i);
+    return v;
+}
+
 template <bool BF16>
-__global__ void __launch_bounds__(256)
-    w4_gemv_kernel(W4Args p, int64_t matrices, const uint16_t *x, int64_t count, int64_t fan, const int32_t *index,
-                   float alpha, float beta, uint16_t *y) {
-    using H = b2b::Half16<BF16>;
-    const int lane = threadIdx.x & 31;
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
-    for (int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); at < count * p.m; at += warps) {
-        const int64_t i = at / p.m, e = index ? index[i] : 0;
-        float sum = 0.0f;
-        if (e >= 0 && e < matrices) {
-            const int64_t row = e * p.m + at % p.m;
-            for (int64_t j = lane; j < p.n; j += 32)
-                sum = fmaf(H::get(p.scales[row * p.gs + j / p.group]) * static_cast<float>(w4_value(p, row, j)),
-                           H::get(x[i / fan * p.n + j]), sum);
-        }
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    if constexpr (BF16)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <uint32_t MASK, uint32_t BITS>
+__device__ __forceinline__ uint32_t and_or(uint32_t v) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "n"(MASK), "n"(BITS));  // (v & MASK) | BITS
+    return r;
+}
+
+// The pairs (0,4) (1,5) (2,6) (3,7) of a word's values, less `zero`, exact in
+// 16 bits.
+template <bool BF16>
+struct Unpack;
+template <>
+struct Unpack<false> {
+    __half2 low, high;  // 1024 + zero; -(64 + zero)
+    __device__ __forceinline__ explicit Unpack(int zero) {
+        low = __half2half2(__int2half_rn(1024 + zero));
+        high = __half2half2(__int2half_rn(-64 - zero));
+    }
+    __device__ __forceinline__ void operator()(uint32_t w, uint32_t (&v)[4]) const {
+        const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
 #pragma unroll
-        for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (lane == 0) {
-            float v = e >= 0 && e < matrices ? alpha * sum : 0.0f;
-            if (beta != 0.0f) v = fmaf(beta, H::get(y[at]), v);
-            y[at] = H::put(v);
+        for (int i = 0; i < 2; ++i, w >>= 8) {
+            const uint32_t a = and_or<0x000f000fu, 0x64006400u>(w), b = and_or<0x00f000f0u, 0x64006400u>(w);
+            const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), low);
+            const __half2 y = __hfma2(*reinterpret_cast<const __half2 *>(&b), sixteenth, high);
+            v[2 * i] = *reinterpret_cast<const uint32_t *>(&x);
+            v[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&y);
+        }
+    }
+};
+template <>
+struct Unpack<true> {
+    __nv_bfloat162 low;  // 128 + zero
+    __device__ __forceinline__ explicit Unpack(int zero) { low = __bfloat162bfloat162(__int2bfloat16_rn(128 + zero)); }
+    __device__ __forceinline__ void operator()(uint32_t w, uint32_t (&v)[4]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t a = and_or<0x000f000fu, 0x43004300u>(w >> (4 * i));
+            const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), low);
+            v[i] = *reinterpret_cast<const uint32_t *>(&x);
+        }
+    }
+};
+
+template <bool BF16, bool ZEROS, bool TMA>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+    w4_gemv_kernel(const __grid_constant__ CUtensorMap tmW, GemvArgs p) {
+    using namespace sm100;
+    using H = b2b::Half16<BF16>;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ int abort_flag;
+    uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int g = lane >> 2, q = lane & 3;
+    const int KS = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
+    uint8_t *ring = smem;
+    uint8_t *sx = smem + (TMA ? kWarps * p.stages * kChunkBytes : 0);
+    float *part = reinterpret_cast<float *>(sx + p.x_bytes);  // [2][kWarps][32 rows][width]
+    const int sums = kTileRows * p.width;                     // of a unit
+    float *red = part + 2 * kWarps * sums;                    // [2][KS][32 rows][width]
+    uint64_t *full = reinterpret_cast<uint64_t *>(red + 2 * KS * sums) + warp * p.stages;
+    Table *table = reinterpret_cast<Table *>(reinterpret_cast<uint64_t *>(red + 2 * KS * sums) + kWarps * p.stages);
+    const Item *items = table->item;
+
+    // ---- the sets of products
+    if (tid == 0) abort_flag = 0;
+    if (TMA && lane == 0) {
+        for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+        fence_barrier_init();
+    }
+    if (p.index) {
+        const int mine = tid < p.count ? p.index[p.first + tid] : 0;
+        const int e = mine >= 0 && mine < p.matrices ? mine : -1;
+        table->index[tid] = e;
+        __syncthreads();
+        int seen = 0, lead = tid;  // products before this one of its matrix; the first of its set
+        for (int i = 0; i < tid && tid < p.count; ++i)
+            if (table->index[i] == e) {
+                if (seen % p.width == 0) lead = i;
+                ++seen;
+            }
+        if (seen % p.width == 0) lead = tid;
+        table->lead[tid] = tid < p.count && lead == tid;
+        __syncthreads();
+        int number = 0;  // of this product's set
+        if (tid < p.count)
+            for (int i = 0; i < lead; ++i) number += table->lead[i];
+        if (tid < p.count && lead == tid) {
+            table->item[number].matrix = e;
+            table->item[number].count = 0;
+        }
+        if (tid == p.count - 1) {
+            int all = 0;
+            for (int i = 0; i < p.count; ++i) all += table->lead[i];
+            table->items = all;
+        }
+        __syncthreads();
+        if (tid < p.count) {
+            table->item[number].member[seen % p.width] = static_cast<uint8_t>(tid);
+            atomicAdd(&table->item[number].count, 1);
+        }
+    }
+    __syncthreads();
+    if (KS > 1) cluster_sync();  // every CTA has started before one writes to another
+    const int64_t sets = p.index ? table->items : (p.count + p.width - 1) / p.width;
+    const int64_t tiles = (p.w.m + kTileRows - 1) / kTileRows;
+    const int chunks = static_cast<int>((p.w.n + kChunk - 1) / kChunk);
+    const int local = chunks > rank ? (chunks - rank + KS - 1) / KS : 0;         // this CTA's chunks of a unit
+    const int own = local > warp ? (local - warp + kWarps - 1) / kWarps : 0;     // this warp's
+    const int64_t clusters = gridDim.x / KS, cluster = blockIdx.x / KS;
+    // consecutive units to a cluster, so that it changes its vectors rarely
+    const int64_t u_begin = sets * tiles * cluster / clusters, u_end = sets * tiles * (cluster + 1) / clusters;
+
+    auto matrix_of = [&](int64_t u) { return p.index ? items[u / tiles].matrix : 0; };
+    // first row of unit u in the stack of matrices, and the rows that it has
+    auto row_of = [&](int64_t u) { return matrix_of(u) * p.w.m + u % tiles * kTileRows; };
+
+    bool dead = false;
+    // The loads run p.stages chunks ahead of their use.
+    int64_t iu = u_begin;
+    int ic = 0, istage = 0;
+    auto issue = [&] {
+        if constexpr (TMA) {
+            while (iu < u_end && (own == 0 || matrix_of(iu) < 0)) ++iu;
+            if (iu >= u_end || dead) return;
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&full[istage], kChunkBytes);
+                tma_load_2d(ring + (warp * p.stages + istage) * kChunkBytes, &tmW, &full[istage],
+                            ((warp + ic * kWarps) * KS + rank) * (kChunk / 2), static_cast<int>(row_of(iu)));
+            }
+            if (++istage == p.stages) istage = 0;
+            if (++ic == own) {
+                ic = 0;
+                ++iu;
+            }
+        }
+    };
+    for (int s = 0; s < p.stages; ++s) issue();
+
+    // Sums of unit u leave the cluster: thread tid < 32 nb has row tid / nb of
+    // the unit and vector tid % nb of its set.
+    auto vectors_of = [&](int64_t u) {
+        return p.index ? items[u / tiles].count
+                       : static_cast<int>(min(static_cast<int64_t>(p.width), p.count - u / tiles * p.width));
+    };
+    auto put = [&](int64_t u, const float *from, int step, int terms) {
+        const int nb = vectors_of(u);
+        const int64_t row = u % tiles * kTileRows + tid / nb;
+        const int v = tid % nb;
+        if (tid >= kTileRows * nb || row >= p.w.m) return;
+        float sum = 0.0f;
+        for (int i = 0; i < terms; ++i) sum += from[i * step + tid];
+        const int64_t i = p.index ? p.first + items[u / tiles].member[v] : u / tiles * p.width + v;
+        uint16_t *y = p.y + i * p.w.m + row;
+        float r = matrix_of(u) >= 0 ? p.alpha * sum : 0.0f;
+        if (p.beta != 0.0f) r = fmaf(p.beta, H::get(*y), r);
+        *y = H::put(r);
+    };
+
+    const int64_t spg = p.w.group / 32;  // steps of 32 columns in a group
+    int stage = 0, flip = 0, nb = 0;
+    uint32_t phase = 0;
+    int64_t staged = -1;
+    for (int64_t u = u_begin; u < u_end; ++u, flip ^= 1) {
+        const int64_t set = u / tiles;
+        const bool some = matrix_of(u) >= 0;
+        if (set != staged) {
+            staged = set;
+            nb = vectors_of(u);
+            __syncthreads();  // everyone is done with the old vectors
+            if (some) {
+                // 8 columns of one vector a turn; local chunk l is chunk l * KS + rank
+                const int per = kChunk / 8 * nb;
+                for (int i = tid; i < local * per; i += kWarps * 32) {
+                    const int l = i / per, r = i % per;
+                    const int b = r / (kChunk / 8), oct = r % (kChunk / 8);  // lanes along a vector
+                    const int64_t j = (static_cast<int64_t>(l) * KS + rank) * kChunk + oct * 8;
+                    const int64_t v = (p.index ? p.first + items[set].member[b] : set * p.width + b) / p.fan;
+                    const uint16_t *src = p.x + v * p.w.n + j;
+                    uint16_t h[8];
+                    if (j + 8 <= p.w.n && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+                        *reinterpret_cast<uint4 *>(h) = __ldg(reinterpret_cast<const uint4 *>(src));
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) h[k] = j + k < p.w.n ? src[k] : uint16_t(0);
+                    }
+                    uint4 o;
+                    o.x = h[0] | static_cast<uint32_t>(h[4]) << 16;
+                    o.y = h[1] | static_cast<uint32_t>(h[5]) << 16;
+                    o.z = h[2] | static_cast<uint32_t>(h[6]) << 16;
+                    o.w = h[3] | static_cast<uint32_t>(h[7]) << 16;
+                    // step (oct / 4), vector b, quarter oct % 4
+                    *reinterpret_cast<uint4 *>(sx + ((l * 8 + (oct >> 2)) * nb + b) * 64 + (oct & 3) * 16) = o;
+                }
+            }
+            __syncthreads();
+        }
+
+        float total[2][4] = {};
+        if (some) {
+            const int64_t row0 = row_of(u);
+            const int rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), p.w.m - u % tiles * kTileRows));
+            const uint16_t *scale0 = p.w.scales + (row0 + g) * p.w.gs;
+            const uint8_t *zero0 = ZEROS ? p.w.zeros + (row0 + g) * p.w.gs : nullptr;
+            uint16_t sn[4];
+            int zn[4];
+            auto fetch = [&](int64_t grp) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool live = g + 8 * i < rows && grp < p.w.gs;
+                    sn[i] = live ? __ldg(scale0 + 8 * i * p.w.gs + grp) : uint16_t(0);
+                    zn[i] = ZEROS ? (live ? __ldg(zero0 + 8 * i * p.w.gs + grp) & 15 : 0) : 8;
+                }
+            };
+            if (own > 0) fetch((static_cast<int64_t>(warp) * KS + rank) * 8 / spg);
+            for (int c = 0; c < own; ++c) {
+                const int l = warp + c * kWarps;
+                const int64_t chunk = static_cast<int64_t>(l) * KS + rank;
+                const int steps = static_cast<int>(min(static_cast<int64_t>(8), (p.w.n - chunk * kChunk + 31) / 32));
+                if (TMA && !dead) {
+                    const bool ok = mbar_wait(&full[stage], phase, &abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x31,
+                                              p.wait_ns);
+                    dead = !__all_sync(0xffffffffu, ok);
+                }
+                const uint8_t *w = ring + (warp * p.stages + stage) * kChunkBytes + g * 128 + q * 4;
+                const uint8_t *xs = sx + l * 8 * nb * 64 + lane * 16;
+                const int64_t byte0 = (row0 + g) * p.w.pitch + chunk * (kChunk / 2) + q * 4;
+                int64_t grp = chunk * 8 / spg;
+                int64_t left = spg - chunk * 8 % spg;  // steps of the group from here on
+                float scale[4], sum[2][4] = {};
+                Unpack<BF16> un0(8), un1(8), un2(8), un3(8);
+                auto turn = [&](int done) {  // the next group's scales and zero points, after `done` steps
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) scale[i] = H::get(sn[i]);
+                    if (ZEROS) {
+                        un0 = Unpack<BF16>(zn[0]);
+                        un1 = Unpack<BF16>(zn[1]);
+                        un2 = Unpack<BF16>(zn[2]);
+                        un3 = Unpack<BF16>(zn[3]);
+                    }
+                    // what follows: the next group here, or the next chunk's first
+                    if (done + left < steps) fetch(grp + 1);
+                    else if (c + 1 < own) fetch((chunk + static_cast<int64_t>(kWarps) * KS) * 8 / spg);
+                };
+                turn(0);
+#pragma unroll
+                for (int st = 0; st < 8; ++st) {
+                    if (st < steps) {
+                        uint4 xb = make_uint4(0, 0, 0, 0);
+                        if (g < nb) xb = *reinterpret_cast<const uint4 *>(xs + st * nb * 64);
+                        uint32_t words[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            words[i] = TMA ? *reinterpret_cast<const uint32_t *>(w + i * 1024 + ((st ^ g) << 4))
+                                       : g + 8 * i < rows ? word_at(p, byte0 + 8 * i * p.w.pitch + st * 16)
+                                                          : 0u;
+                        uint32_t a[4], b[4];
+                        un0(words[0], a);
+                        un1(words[1], b);
+                        mma16816<BF16>(sum[0], a[0], b[0], a[1], b[1], xb.x, xb.y);
+                        mma16816<BF16>(sum[0], a[2], b[2], a[3], b[3], xb.z, xb.w);
+                        un2(words[2], a);
+                        un3(words[3], b);
+                        mma16816<BF16>(sum[1], a[0], b[0], a[1], b[1], xb.x, xb.y);
+                        mma16816<BF16>(sum[1], a[2], b[2], a[3], b[3], xb.z, xb.w);
+                        if (--left == 0 || st == steps - 1) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                total[0][i] = fmaf(scale[i >> 1], sum[0][i], total[0][i]);
+                                total[1][i] = fmaf(scale[2 + (i >> 1)], sum[1][i], total[1][i]);
+                                sum[0][i] = sum[1][i] = 0.0f;
+                            }
+                            if (left == 0 && st < steps - 1) {
+                                ++grp;
+                                left = spg;
+                                turn(st + 1);
+                            }
+                        }
+                    }
+                }
+                if constexpr (TMA) {
+                    __syncwarp();
+                    if (++stage == p.stages) {
+                        stage = 0;
+                        phase ^= 1u;
+                    }
+                    issue();
+                }
+            }
+        }
+
+        // ---- join: warps, then the cluster's CTAs
+        float *mine = part + (flip * kWarps + warp) * sums;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {  // row g + 8 (i / 2), vector 2 q + i % 2
+            const int v = 2 * q + (i & 1);
+            if (v < nb) mine[(g + 8 * (i >> 1)) * nb + v] = total[i >> 2][i & 3];
+        }
+        __syncthreads();
+        if (KS == 1) {
+            put(u, part + flip * kWarps * sums, sums, kWarps);
+        } else {
+            if (u > u_begin) {  // the previous unit's sums have arrived
+                cluster_wait();
+                if (rank == 0) put(u - 1, red + (flip ^ 1) * KS * sums, sums, KS);
+            }
+            if (tid < kTileRows * nb) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) sum += part[(flip * kWarps + w) * sums + tid];
+                st_shared_cluster(mapa_shared(smem_u32(red + (flip * KS + rank) * sums + tid), 0), sum);
+            }
+            __syncwarp();
+            cluster_arrive();
+        }
+    }
+    if (KS > 1 && u_end > u_begin) {
+        __syncwarp();
+        cluster_wait();
+        if (rank == 0) put(u_end - 1, red + (flip ^ 1) * KS * sums, sums, KS);
+    }
+    if (TMA && dead && lane == 0) {  // loads in flight land before the CTA leaves
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 2000000ull) {
         }
     }
 }
@@ -132,6 +528,112 @@ unsigned ctas_for(b2b_handle *h, const void *kernel, int64_t blocks) {
 int launched(const char *what) {
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, what);
+}
+
+constexpr int kMaxSmem = 227 * 1024 - 1024;   // dynamic shared memory of the GEMV kernel, static beside it
+constexpr int kHalfSmem = 113 * 1024 - 1024;  // of one of two CTAs on an SM
+constexpr int64_t kMaxXBytes = 104 * 1024;    // of its staged vectors
+
+// Its shared memory for KS CTAs a unit; sets the ring's stages and the
+// vectors' bytes.  Two chunks a warp where two CTAs fit an SM, else up to four.
+template <bool TMA>
+size_t gemv_smem(GemvArgs &p, int KS, int64_t local) {
+    p.x_bytes = static_cast<int>(local * kChunk * p.width * 2);
+    const size_t fixed = p.x_bytes + 2 * (kWarps + KS) * kTileRows * p.width * 4 + (p.index ? sizeof(Table) : 0) + 1024;
+    if (!TMA) {
+        p.stages = 0;
+        return fixed;
+    }
+    const size_t stage = kWarps * (kChunkBytes + 8);
+    p.stages = 2;
+    if (fixed + 2 * stage > kHalfSmem)
+        while (p.stages < 4 && fixed + (p.stages + 1) * stage <= kMaxSmem) ++p.stages;
+    return fixed + p.stages * stage;
+}
+
+// Resident clusters of KS CTAs of a kernel with that much shared memory,
+// asked once for each device.
+int resident_clusters(b2b_handle *h, const void *kernel, cudaLaunchConfig_t &cfg, int KS) {
+    struct Entry {
+        const void *kernel;
+        int device, ks, clusters;
+        size_t smem;
+    };
+    static std::mutex mu;
+    static std::vector<Entry> cache;
+    std::lock_guard<std::mutex> lock(mu);
+    for (const Entry &e : cache)
+        if (e.kernel == kernel && e.device == h->device && e.ks == KS && e.smem == cfg.dynamicSmemBytes)
+            return e.clusters;
+    int clusters = 0;
+    cfg.gridDim = dim3(KS);
+    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
+        cudaGetLastError();
+        clusters = h->sm_count / KS;
+    }
+    cache.push_back(Entry{kernel, h->device, KS, clusters, cfg.dynamicSmemBytes});
+    return clusters;
+}
+
+template <bool TMA>
+int launch_gemv(b2b_handle *h, bool bf16, bool zeros, const CUtensorMap &tmW, GemvArgs &p) {
+    auto kernel = bf16 ? (zeros ? w4_gemv_kernel<true, true, TMA> : w4_gemv_kernel<true, false, TMA>)
+                       : (zeros ? w4_gemv_kernel<false, true, TMA> : w4_gemv_kernel<false, false, TMA>);
+    const void *fn = reinterpret_cast<const void *>(kernel);
+    const int64_t chunks = (p.w.n + kChunk - 1) / kChunk, tiles = (p.w.m + kTileRows - 1) / kTileRows;
+    p.width = p.count < 8 ? p.count : 8;
+    while (p.width > 1 && (chunks + 7) / 8 * kChunk * p.width * 2 > kMaxXBytes) --p.width;
+    // with an index: the sets that it makes where it names each matrix equally often
+    const int64_t each = p.index ? (p.count + p.matrices - 1) / p.matrices : p.count;
+    const int64_t sets = (p.count + each - 1) / each * ((each + p.width - 1) / p.width);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.stream = h->stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    // Split a unit's columns over the CTAs of a cluster where that takes the
+    // fewest turns: chunks that a warp computes one after another, and about
+    // one more for each unit's start and joining.
+    int best = 0, best_grid = 0;
+    double best_time = 0;
+    for (int KS = 1; KS <= 8 && (KS == 1 || KS < 2 * chunks); KS *= 2) {
+        const int64_t local = (chunks + KS - 1) / KS;
+        if (local * kChunk * p.width * 2 > kMaxXBytes) continue;
+        const size_t smem = gemv_smem<TMA>(p, KS, local);
+        attr[0].val.clusterDim.x = KS;
+        cfg.dynamicSmemBytes = smem;
+        {
+            static std::mutex mu;
+            static bool ready[2][2][64];
+            std::lock_guard<std::mutex> lock(mu);
+            bool &done = ready[bf16][zeros][h->device & 63];
+            if (!done) {
+                const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+                if (e != cudaSuccess) return b2b::fail_cuda(e, "4-bit GEMV shared memory");
+                done = true;
+            }
+        }
+        const int64_t clusters = resident_clusters(h, fn, cfg, KS);
+        const int64_t units = sets * tiles;
+        const double time = static_cast<double>((units + clusters - 1) / clusters) *
+                            (static_cast<double>((local + kWarps - 1) / kWarps) + 1.0);
+        if (!best || time < best_time) {
+            best = KS;
+            best_time = time;
+            best_grid = static_cast<int>(units < clusters ? units : clusters);
+        }
+    }
+    if (!best) return b2b::fail(B2B_ERR_NOT_SUPPORTED, "4-bit GEMV: rows longer than 425984 columns");
+    const int64_t local = (chunks + best - 1) / best;
+    attr[0].val.clusterDim.x = best;
+    cfg.dynamicSmemBytes = gemv_smem<TMA>(p, best, local);
+    cfg.gridDim = dim3(best * best_grid);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmW, p);
+    return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, "4-bit GEMV launch");
 }
 
 }  // namespace
@@ -158,13 +660,36 @@ int launch_dequantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t gro
 int launch_hgemv_w4(b2b_handle *h, int type, size_t groups, size_t m, size_t n, size_t group, float alpha,
                     const uint8_t *packed, const uint16_t *scales, const uint8_t *zeros, const uint16_t *x,
                     size_t count, size_t fan, const int32_t *index, float beta, uint16_t *y) {
-    const W4Args p = w4_args(m, n, group, packed, scales, zeros);
-    const int64_t products = static_cast<int64_t>(count);
-    auto kernel = type == B2B_TYPE_BF16 ? w4_gemv_kernel<true> : w4_gemv_kernel<false>;
-    const unsigned ctas = ctas_for(h, reinterpret_cast<const void *>(kernel), (p.m * products + 7) / 8);
-    kernel<<<ctas, 256, 0, h->stream>>>(p, static_cast<int64_t>(groups), x, products, static_cast<int64_t>(fan),
-                                        index, alpha, beta, y);
-    return launched("4-bit GEMV launch");
+    GemvArgs p{};
+    p.w = w4_args(m, n, group, packed, scales, zeros);
+    p.x = x;
+    p.index = index;
+    p.y = y;
+    p.status = h->d_status;
+    p.wait_ns = h->wait_limit_ns;
+    p.matrices = static_cast<int>(groups);
+    p.fan = static_cast<int>(fan);
+    p.alpha = alpha;
+    p.beta = beta;
+    const int64_t rows = static_cast<int64_t>(groups) * p.w.m;
+    p.total = rows * p.w.pitch;
+    const bool bf16 = type == B2B_TYPE_BF16;
+    const bool tma = n % 32 == 0 && aligned16(packed) && rows < (1ll << 31);
+    CUtensorMap tmW{};
+    if (tma) {
+        if (int rc = encode_tma_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, packed, rows, p.w.pitch, kChunk / 2,
+                                   kTileRows))
+            return rc;
+    }
+    const int64_t all = static_cast<int64_t>(count);
+    for (int64_t first = 0; first < all; first += index ? kMaxIndexed : all) {
+        p.first = static_cast<int>(first);
+        p.count = static_cast<int>(index && all - first > kMaxIndexed ? kMaxIndexed : all - first);
+        if (int rc = tma ? launch_gemv<true>(h, bf16, zeros != nullptr, tmW, p)
+                         : launch_gemv<false>(h, bf16, zeros != nullptr, tmW, p))
+            return rc;
+    }
+    return B2B_OK;
 }
 
 }  // namespace b2b
