@@ -100,31 +100,35 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(W4Args p, uint16_t *
 // ---------------------------------------------------------------------------
 // Products with vectors: y_i = alpha W x_i + beta y_i for up to 8 vectors that
 // share W.  HBM-bound: the packed values are read once, so the work for each
-// must stay under the ~2.5 instructions that 148 SMs can issue in the time a
-// value takes to arrive.  Multiplying on the tensor cores with the 8 columns
-// of mma.m16n8k16 does that for 1 vector as for 8: a word of 8 values becomes
-// four register pairs of exact (q - zero) in 9 instructions (f16: or the bits
-// into 1024 + q or 1024 + 16 q, then one packed subtraction or fma), and 16
-// words of a warp are one MMA operand.  Sums are f32, a group's sum is scaled
-// in f32 and added to the row's; no product or sum is rounded to 16 bits.
+// must stay well under the ~2.5 instructions that 148 SMs can issue in the
+// time a value takes to arrive.  Multiplying on the tensor cores with the 8
+// columns of mma.m16n8k16 does that for 1 vector as for 8: a word of 8 values
+// becomes four register pairs of exact (q - zero) in 9 instructions (f16: or
+// the bits into 1024 + q or 1024 + 16 q, then one packed subtraction or fma),
+// and 16 words of a warp are one MMA operand.  Sums are f32; a group's sum is
+// scaled in f32 and added to the row's.  No product or sum is rounded to 16
+// bits.
 //
-//   * A unit is 32 rows of W for one set of vectors; its n columns are cut
-//     into chunks of 256 (128 bytes of a row).  Chunk c belongs to CTA c % KS
-//     of a cluster, and there to warp (c / KS) % 8.
+//   * A tile is 32 rows of W for one set of vectors; its n columns are cut
+//     into chunks of 256 (128 bytes of a row), which the CTAs of a cluster
+//     and kw of a CTA's 16 warps take in turn; the 16 / kw parts of a CTA have
+//     a tile each.  A unit is those tiles.
 //   * Each warp keeps its own ring of chunks (32 rows x 128 bytes, 128-byte
 //     swizzle) filled by TMA ahead of its use, across units, so nothing
-//     drains at a unit's end; 2 CTAs of 8 warps x 2 chunks hold 128 KiB of W
-//     in flight on an SM.
+//     drains at a unit's end; 16 warps x 2 chunks are 128 KiB of W in flight.
 //   * The vectors are staged once for each set, each 8 columns reordered to
 //     the pairs (0,4) (1,5) (2,6) (3,7) that the words unpack to.
 //   * Warps join their sums through shared memory, CTAs of a cluster through
 //     the first CTA's shared memory, one unit later so that no one waits;
 //     both in a fixed order.
 // Rows that TMA cannot describe (n not a multiple of 32, packed not 16-byte
-// aligned) are read by the same kernel with plain loads.
-constexpr int kWarps = 8;
+// aligned) and groups that do not fit a chunk evenly are read by the same
+// kernel with plain loads (SPG = 0).
+constexpr int kWarps = 16;
+constexpr int kThreads = kWarps * 32;
 constexpr int kTileRows = 32;
 constexpr int kChunk = 256;                       // columns
+constexpr int kSteps = kChunk / 32;               // of 32 columns
 constexpr int kChunkBytes = kTileRows * kChunk / 2;
 constexpr int kMaxIndexed = 256;                  // products of one launch that choose their matrix
 
@@ -137,8 +141,10 @@ struct GemvArgs {
     uint64_t wait_ns;
     int matrices, count, fan, first;  // first: number of this launch's first product
     int width;    // vectors of a set: 8, or fewer where longer rows leave room for fewer
+    int kw;       // warps that share a tile
     int stages;   // chunks of a warp's ring
     int x_bytes;  // of the staged vectors
+    int vec;      // a chunk's scales and zero points of a row are one aligned word each
     float alpha, beta;
     int64_t total;  // bytes of packed
 };
@@ -172,87 +178,159 @@ __device__ __forceinline__ uint32_t word_at(const GemvArgs &p, int64_t at) {
     return v;
 }
 
-template <bool BF16>
+// c += a b, or c = a b where FRESH.
+template <bool BF16, bool FRESH>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
+    const float c0 = FRESH ? 0.0f : c[0], c1 = FRESH ? 0.0f : c[1], c2 = FRESH ? 0.0f : c[2], c3 = FRESH ? 0.0f : c[3];
     if constexpr (BF16)
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+            "{%10, %11, %12, %13};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
     else
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-            "{%0, %1, %2, %3};"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+            "{%10, %11, %12, %13};"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 
-template <uint32_t MASK, uint32_t BITS>
-__device__ __forceinline__ uint32_t and_or(uint32_t v) {
+// (v & mask) | bits
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t bits) {
     uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "n"(MASK), "n"(BITS));  // (v & MASK) | BITS
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "r"(mask), "r"(bits));
     return r;
 }
 
-// The pairs (0,4) (1,5) (2,6) (3,7) of a word's values, less `zero`, exact in
-// 16 bits.
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2 *>(&v); }
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162 *>(&v); }
+template <typename T>
+__device__ __forceinline__ uint32_t as_word(T v) { return *reinterpret_cast<const uint32_t *>(&v); }
+
+// The pairs (0,4) (1,5) (2,6) (3,7) of a word's values, less `zero` (0..15),
+// exact in 16 bits.
 template <bool BF16>
 struct Unpack;
 template <>
 struct Unpack<false> {
-    __half2 low, high;  // 1024 + zero; -(64 + zero)
-    __device__ __forceinline__ explicit Unpack(int zero) {
-        low = __half2half2(__int2half_rn(1024 + zero));
-        high = __half2half2(__int2half_rn(-64 - zero));
+    uint32_t low, high;  // pairs of 1024 + zero and of -(64 + zero)
+    __device__ __forceinline__ explicit Unpack(uint32_t zero) {
+        low = (0x6400u + zero) * 0x10001u;
+        high = (0xd400u + (zero << 4)) * 0x10001u;
     }
     __device__ __forceinline__ void operator()(uint32_t w, uint32_t (&v)[4]) const {
-        const __half2 sixteenth = __half2half2(__ushort_as_half(0x2c00));
 #pragma unroll
         for (int i = 0; i < 2; ++i, w >>= 8) {
-            const uint32_t a = and_or<0x000f000fu, 0x64006400u>(w), b = and_or<0x00f000f0u, 0x64006400u>(w);
-            const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&a), low);
-            const __half2 y = __hfma2(*reinterpret_cast<const __half2 *>(&b), sixteenth, high);
-            v[2 * i] = *reinterpret_cast<const uint32_t *>(&x);
-            v[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&y);
+            v[2 * i] = as_word(__hsub2(as_half2(and_or(w, 0x000f000fu, 0x64006400u)), as_half2(low)));
+            v[2 * i + 1] = as_word(__hfma2(as_half2(and_or(w, 0x00f000f0u, 0x64006400u)), as_half2(0x2c002c00u),
+                                           as_half2(high)));
         }
     }
 };
 template <>
 struct Unpack<true> {
-    __nv_bfloat162 low;  // 128 + zero
-    __device__ __forceinline__ explicit Unpack(int zero) { low = __bfloat162bfloat162(__int2bfloat16_rn(128 + zero)); }
+    uint32_t low;  // pair of 128 + zero
+    __device__ __forceinline__ explicit Unpack(uint32_t zero) { low = (0x4300u + zero) * 0x10001u; }
     __device__ __forceinline__ void operator()(uint32_t w, uint32_t (&v)[4]) const {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t a = and_or<0x000f000fu, 0x43004300u>(w >> (4 * i));
-            const __nv_bfloat162 x = __hsub2(*reinterpret_cast<const __nv_bfloat162 *>(&a), low);
-            v[i] = *reinterpret_cast<const uint32_t *>(&x);
-        }
+        for (int i = 0; i < 4; ++i, w >>= 4)
+            v[i] = as_word(__hsub2(as_bf162(and_or(w, 0x000f000fu, 0x43004300u)), as_bf162(low)));
     }
 };
 
-template <bool BF16, bool ZEROS, bool TMA>
-__global__ void __launch_bounds__(kWarps * 32, 2)
-    w4_gemv_kernel(const __grid_constant__ CUtensorMap tmW, GemvArgs p) {
+// Two tiles of 16 rows times 32 columns: words of rows g, g + 8, g + 16, g + 24.
+template <bool BF16, bool FRESH>
+__device__ __forceinline__ void step32(float (&sum)[2][4], const uint32_t (&words)[4], const Unpack<BF16> (&un)[4],
+                                       const uint4 &x) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint32_t a[4], b[4];
+        un[2 * h](words[2 * h], a);
+        un[2 * h + 1](words[2 * h + 1], b);
+        mma16816<BF16, FRESH>(sum[h], a[0], b[0], a[1], b[1], x.x, x.y);
+        mma16816<BF16, false>(sum[h], a[2], b[2], a[3], b[3], x.z, x.w);
+    }
+}
+
+__device__ __forceinline__ void add_scaled(float (&total)[2][4], const float (&sum)[2][4], const float (&scale)[4]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        total[i >> 2][i & 3] = fmaf(scale[i >> 1], sum[i >> 2][i & 3], total[i >> 2][i & 3]);
+}
+
+// Scales and zero points of one row's groups in a chunk (at most 8).
+template <int SPG, bool ZEROS>
+struct RowScales {
+    static constexpr int N = SPG ? kSteps / SPG : 1;
+    uint32_t s[(N + 1) / 2];
+    uint32_t z[(N + 3) / 4];
+    __device__ __forceinline__ void load(const W4Args &w, const uint16_t *scales, const uint8_t *zeros, int grp, int vec,
+                                         bool live) {
+#pragma unroll
+        for (int i = 0; i < (N + 1) / 2; ++i) s[i] = 0;
+#pragma unroll
+        for (int i = 0; i < (N + 3) / 4; ++i) z[i] = 0;
+        if (!live) return;
+        scales += grp;
+        zeros += grp;
+        if (vec && N > 1) {
+            if constexpr (N == 8) {
+                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(scales));
+                s[0] = v.x, s[1] = v.y, s[2] = v.z, s[3] = v.w;
+                if constexpr (ZEROS) {
+                    const uint2 u = __ldg(reinterpret_cast<const uint2 *>(zeros));
+                    z[0] = u.x, z[1] = u.y;
+                }
+            } else if constexpr (N == 4) {
+                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(scales));
+                s[0] = v.x, s[1] = v.y;
+                if constexpr (ZEROS) z[0] = __ldg(reinterpret_cast<const uint32_t *>(zeros));
+            } else {
+                s[0] = __ldg(reinterpret_cast<const uint32_t *>(scales));
+                if constexpr (ZEROS) z[0] = __ldg(reinterpret_cast<const uint16_t *>(zeros));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (grp + i < w.gs) {
+                    s[i / 2] |= static_cast<uint32_t>(__ldg(scales + i)) << (16 * (i & 1));
+                    if constexpr (ZEROS) z[i / 4] |= static_cast<uint32_t>(__ldg(zeros + i)) << (8 * (i & 3));
+                }
+        }
+    }
+    __device__ __forceinline__ uint16_t scale(int i) const { return static_cast<uint16_t>(s[i / 2] >> (16 * (i & 1))); }
+    __device__ __forceinline__ uint32_t zero(int i) const { return ZEROS ? z[i / 4] >> (8 * (i & 3)) & 15u : 8u; }
+};
+
+// SPG: steps of 32 columns in a group, 8 standing for its multiples; 0: plain
+// loads, any group.
+template <bool BF16, bool ZEROS, int SPG>
+__global__ void __launch_bounds__(kThreads, 1)
+    w4_gemv_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ GemvArgs p) {
     using namespace sm100;
     using H = b2b::Half16<BF16>;
+    constexpr bool TMA = SPG != 0;
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag;
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, q = lane & 3;
     const int KS = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-    uint8_t *ring = smem;
+    const int kw = p.kw, parts = kWarps / kw, part_no = warp / kw, kwarp = warp % kw;
+    uint8_t *ring = smem + (TMA ? warp * p.stages * kChunkBytes : 0);
     uint8_t *sx = smem + (TMA ? kWarps * p.stages * kChunkBytes : 0);
-    float *part = reinterpret_cast<float *>(sx + p.x_bytes);  // [2][kWarps][32 rows][width]
-    const int sums = kTileRows * p.width;                     // of a unit
-    float *red = part + 2 * kWarps * sums;                    // [2][KS][32 rows][width]
-    uint64_t *full = reinterpret_cast<uint64_t *>(red + 2 * KS * sums) + warp * p.stages;
-    Table *table = reinterpret_cast<Table *>(reinterpret_cast<uint64_t *>(red + 2 * KS * sums) + kWarps * p.stages);
+    const int sums = kTileRows * p.width;                     // of a tile
+    float *part = reinterpret_cast<float *>(sx + p.x_bytes);  // [kWarps][32 rows][width]
+    float *red = part + kWarps * sums;                        // [2][KS][32 rows][width]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(red + 2 * KS * sums);
+    uint64_t *full = bars + warp * p.stages;
+    uint8_t *nothing = reinterpret_cast<uint8_t *>(bars + kWarps * p.stages);  // 16 bytes of 0
+    Table *table = reinterpret_cast<Table *>(nothing + 16);
     const Item *items = table->item;
 
     // ---- the sets of products
     if (tid == 0) abort_flag = 0;
+    if (tid < 4) reinterpret_cast<uint32_t *>(nothing)[tid] = 0;
     if (TMA && lane == 0) {
         for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
         fence_barrier_init();
@@ -260,28 +338,31 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     if (p.index) {
         const int mine = tid < p.count ? p.index[p.first + tid] : 0;
         const int e = mine >= 0 && mine < p.matrices ? mine : -1;
-        table->index[tid] = e;
+        if (tid < p.count) table->index[tid] = e;
         __syncthreads();
         int seen = 0, lead = tid;  // products before this one of its matrix; the first of its set
-        for (int i = 0; i < tid && tid < p.count; ++i)
-            if (table->index[i] == e) {
-                if (seen % p.width == 0) lead = i;
-                ++seen;
-            }
-        if (seen % p.width == 0) lead = tid;
-        table->lead[tid] = tid < p.count && lead == tid;
+        if (tid < p.count) {
+            for (int i = 0; i < tid; ++i)
+                if (table->index[i] == e) {
+                    if (seen % p.width == 0) lead = i;
+                    ++seen;
+                }
+            if (seen % p.width == 0) lead = tid;
+            table->lead[tid] = lead == tid;
+        }
         __syncthreads();
         int number = 0;  // of this product's set
-        if (tid < p.count)
+        if (tid < p.count) {
             for (int i = 0; i < lead; ++i) number += table->lead[i];
-        if (tid < p.count && lead == tid) {
-            table->item[number].matrix = e;
-            table->item[number].count = 0;
-        }
-        if (tid == p.count - 1) {
-            int all = 0;
-            for (int i = 0; i < p.count; ++i) all += table->lead[i];
-            table->items = all;
+            if (lead == tid) {
+                table->item[number].matrix = e;
+                table->item[number].count = 0;
+            }
+            if (tid == p.count - 1) {
+                int all = 0;
+                for (int i = 0; i < p.count; ++i) all += table->lead[i];
+                table->items = all;
+            }
         }
         __syncthreads();
         if (tid < p.count) {
@@ -291,80 +372,98 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     }
     __syncthreads();
     if (KS > 1) cluster_sync();  // every CTA has started before one writes to another
-    const int64_t sets = p.index ? table->items : (p.count + p.width - 1) / p.width;
-    const int64_t tiles = (p.w.m + kTileRows - 1) / kTileRows;
+    const uint32_t tiles = static_cast<uint32_t>((p.w.m + kTileRows - 1) / kTileRows);
+    const uint32_t upers = (tiles + parts - 1) / parts;  // units of a set
+    const uint32_t sets = p.index ? table->items : (p.count + p.width - 1) / p.width;
     const int chunks = static_cast<int>((p.w.n + kChunk - 1) / kChunk);
-    const int local = chunks > rank ? (chunks - rank + KS - 1) / KS : 0;         // this CTA's chunks of a unit
-    const int own = local > warp ? (local - warp + kWarps - 1) / kWarps : 0;     // this warp's
-    const int64_t clusters = gridDim.x / KS, cluster = blockIdx.x / KS;
+    const int local = chunks > rank ? (chunks - rank + KS - 1) / KS : 0;   // this CTA's chunks of a tile
+    const int own = local > kwarp ? (local - kwarp + kw - 1) / kw : 0;     // this warp's
+    const uint32_t clusters = gridDim.x / KS, cluster = blockIdx.x / KS;
     // consecutive units to a cluster, so that it changes its vectors rarely
-    const int64_t u_begin = sets * tiles * cluster / clusters, u_end = sets * tiles * (cluster + 1) / clusters;
+    const uint64_t units = static_cast<uint64_t>(sets) * upers;
+    const uint32_t u_begin = static_cast<uint32_t>(units * cluster / clusters);
+    const uint32_t u_end = static_cast<uint32_t>(units * (cluster + 1) / clusters);
 
-    auto matrix_of = [&](int64_t u) { return p.index ? items[u / tiles].matrix : 0; };
-    // first row of unit u in the stack of matrices, and the rows that it has
-    auto row_of = [&](int64_t u) { return matrix_of(u) * p.w.m + u % tiles * kTileRows; };
+    auto matrix_of = [&](uint32_t set) { return p.index ? items[set].matrix : 0; };
 
     bool dead = false;
     // The loads run p.stages chunks ahead of their use.
-    int64_t iu = u_begin;
+    uint32_t iset = u_begin / upers, iunit = u_begin % upers, ileft = u_end - u_begin;
     int ic = 0, istage = 0;
     auto issue = [&] {
         if constexpr (TMA) {
-            while (iu < u_end && (own == 0 || matrix_of(iu) < 0)) ++iu;
-            if (iu >= u_end || dead) return;
+            while (ileft && ic == 0 &&
+                   (own == 0 || matrix_of(iset) < 0 || iunit * parts + part_no >= tiles)) {  // nothing to load
+                --ileft;
+                if (++iunit == upers) {
+                    iunit = 0;
+                    ++iset;
+                }
+            }
+            if (!ileft || dead) return;
             if (lane == 0) {
+                const int row = static_cast<int>(matrix_of(iset) * p.w.m + (iunit * parts + part_no) * kTileRows);
                 mbar_arrive_expect_tx(&full[istage], kChunkBytes);
-                tma_load_2d(ring + (warp * p.stages + istage) * kChunkBytes, &tmW, &full[istage],
-                            ((warp + ic * kWarps) * KS + rank) * (kChunk / 2), static_cast<int>(row_of(iu)));
+                tma_load_2d(ring + istage * kChunkBytes, &tmW, &full[istage],
+                            ((kwarp + ic * kw) * KS + rank) * (kChunk / 2), row);
             }
             if (++istage == p.stages) istage = 0;
             if (++ic == own) {
                 ic = 0;
-                ++iu;
+                --ileft;
+                if (++iunit == upers) {
+                    iunit = 0;
+                    ++iset;
+                }
             }
         }
     };
     for (int s = 0; s < p.stages; ++s) issue();
 
-    // Sums of unit u leave the cluster: thread tid < 32 nb has row tid / nb of
-    // the unit and vector tid % nb of its set.
-    auto vectors_of = [&](int64_t u) {
-        return p.index ? items[u / tiles].count
-                       : static_cast<int>(min(static_cast<int64_t>(p.width), p.count - u / tiles * p.width));
+    auto vectors_of = [&](uint32_t set) {
+        return p.index ? items[set].count
+                       : static_cast<int>(min(static_cast<int64_t>(p.width), p.count - static_cast<int64_t>(set) * p.width));
     };
-    auto put = [&](int64_t u, const float *from, int step, int terms) {
-        const int nb = vectors_of(u);
-        const int64_t row = u % tiles * kTileRows + tid / nb;
-        const int v = tid % nb;
-        if (tid >= kTileRows * nb || row >= p.w.m) return;
-        float sum = 0.0f;
-        for (int i = 0; i < terms; ++i) sum += from[i * step + tid];
-        const int64_t i = p.index ? p.first + items[u / tiles].member[v] : u / tiles * p.width + v;
-        uint16_t *y = p.y + i * p.w.m + row;
-        float r = matrix_of(u) >= 0 ? p.alpha * sum : 0.0f;
-        if (p.beta != 0.0f) r = fmaf(p.beta, H::get(*y), r);
-        *y = H::put(r);
+    // Sums leave the cluster: `terms` arrays of `step` sums for each of
+    // `ntiles` tiles, [tile][term][row][vector].
+    auto put = [&](uint32_t u, const float *from, int ntiles, int step, int terms) {
+        const uint32_t set = u / upers, tile0 = u % upers * parts;
+        const int nb = vectors_of(set);
+        const bool some = matrix_of(set) >= 0;
+        for (int o = tid; o < ntiles * kTileRows * nb; o += kThreads) {
+            const int t = o / (kTileRows * nb), r = o % (kTileRows * nb);
+            const int64_t row = static_cast<int64_t>(tile0 + t) * kTileRows + r / nb;
+            if (row >= p.w.m) continue;
+            float sum = 0.0f;
+            for (int i = 0; i < terms; ++i) sum += from[(t * terms + i) * step + r];
+            const int v = r % nb;
+            const int64_t i = p.index ? p.first + items[set].member[v] : static_cast<int64_t>(set) * p.width + v;
+            uint16_t *y = p.y + i * p.w.m + row;
+            float res = some ? p.alpha * sum : 0.0f;
+            if (p.beta != 0.0f) res = fmaf(p.beta, H::get(*y), res);
+            *y = H::put(res);
+        }
     };
 
-    const int64_t spg = p.w.group / 32;  // steps of 32 columns in a group
+    const int spg = static_cast<int>(p.w.group / 32);
     int stage = 0, flip = 0, nb = 0;
-    uint32_t phase = 0;
-    int64_t staged = -1;
-    for (int64_t u = u_begin; u < u_end; ++u, flip ^= 1) {
-        const int64_t set = u / tiles;
-        const bool some = matrix_of(u) >= 0;
+    uint32_t phase = 0, staged = 0xffffffffu;
+    for (uint32_t u = u_begin; u < u_end; ++u, flip ^= 1) {
+        const uint32_t set = u / upers, tile = u % upers * parts + part_no;
+        const bool some = matrix_of(set) >= 0;
         if (set != staged) {
             staged = set;
-            nb = vectors_of(u);
+            nb = vectors_of(set);
             __syncthreads();  // everyone is done with the old vectors
             if (some) {
                 // 8 columns of one vector a turn; local chunk l is chunk l * KS + rank
                 const int per = kChunk / 8 * nb;
-                for (int i = tid; i < local * per; i += kWarps * 32) {
+                for (int i = tid; i < local * per; i += kThreads) {
                     const int l = i / per, r = i % per;
                     const int b = r / (kChunk / 8), oct = r % (kChunk / 8);  // lanes along a vector
                     const int64_t j = (static_cast<int64_t>(l) * KS + rank) * kChunk + oct * 8;
-                    const int64_t v = (p.index ? p.first + items[set].member[b] : set * p.width + b) / p.fan;
+                    const int64_t v = (p.index ? p.first + items[set].member[b]
+                                               : static_cast<int64_t>(set) * p.width + b) / p.fan;
                     const uint16_t *src = p.x + v * p.w.n + j;
                     uint16_t h[8];
                     if (j + 8 <= p.w.n && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
@@ -379,95 +478,69 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
                     o.z = h[2] | static_cast<uint32_t>(h[6]) << 16;
                     o.w = h[3] | static_cast<uint32_t>(h[7]) << 16;
                     // step (oct / 4), vector b, quarter oct % 4
-                    *reinterpret_cast<uint4 *>(sx + ((l * 8 + (oct >> 2)) * nb + b) * 64 + (oct & 3) * 16) = o;
+                    *reinterpret_cast<uint4 *>(sx + ((l * kSteps + (oct >> 2)) * nb + b) * 64 + (oct & 3) * 16) = o;
                 }
             }
             __syncthreads();
         }
 
         float total[2][4] = {};
-        if (some) {
-            const int64_t row0 = row_of(u);
-            const int rows = static_cast<int>(min(static_cast<int64_t>(kTileRows), p.w.m - u % tiles * kTileRows));
-            const uint16_t *scale0 = p.w.scales + (row0 + g) * p.w.gs;
-            const uint8_t *zero0 = ZEROS ? p.w.zeros + (row0 + g) * p.w.gs : nullptr;
-            uint16_t sn[4];
-            int zn[4];
-            auto fetch = [&](int64_t grp) {
+        if (some && tile < tiles) {
+            const int64_t row0 = matrix_of(set) * p.w.m + static_cast<int64_t>(tile) * kTileRows + g;
+            const int rows = static_cast<int>(p.w.m - static_cast<int64_t>(tile) * kTileRows) - g;  // > 8 i: row g + 8 i exists
+            // lanes of vectors that the set does not have read zeros
+            const int xstep = g < nb ? nb * 64 : 0;
+            if constexpr (TMA) {
+                RowScales<SPG, ZEROS> next[4];
+                auto fetch = [&](int chunk) {
+                    const int grp = SPG == 8 ? chunk / (spg / 8) : chunk * (kSteps / SPG);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool live = g + 8 * i < rows && grp < p.w.gs;
-                    sn[i] = live ? __ldg(scale0 + 8 * i * p.w.gs + grp) : uint16_t(0);
-                    zn[i] = ZEROS ? (live ? __ldg(zero0 + 8 * i * p.w.gs + grp) & 15 : 0) : 8;
-                }
-            };
-            if (own > 0) fetch((static_cast<int64_t>(warp) * KS + rank) * 8 / spg);
-            for (int c = 0; c < own; ++c) {
-                const int l = warp + c * kWarps;
-                const int64_t chunk = static_cast<int64_t>(l) * KS + rank;
-                const int steps = static_cast<int>(min(static_cast<int64_t>(8), (p.w.n - chunk * kChunk + 31) / 32));
-                if (TMA && !dead) {
-                    const bool ok = mbar_wait(&full[stage], phase, &abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x31,
-                                              p.wait_ns);
-                    dead = !__all_sync(0xffffffffu, ok);
-                }
-                const uint8_t *w = ring + (warp * p.stages + stage) * kChunkBytes + g * 128 + q * 4;
-                const uint8_t *xs = sx + l * 8 * nb * 64 + lane * 16;
-                const int64_t byte0 = (row0 + g) * p.w.pitch + chunk * (kChunk / 2) + q * 4;
-                int64_t grp = chunk * 8 / spg;
-                int64_t left = spg - chunk * 8 % spg;  // steps of the group from here on
-                float scale[4], sum[2][4] = {};
-                Unpack<BF16> un0(8), un1(8), un2(8), un3(8);
-                auto turn = [&](int done) {  // the next group's scales and zero points, after `done` steps
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) scale[i] = H::get(sn[i]);
-                    if (ZEROS) {
-                        un0 = Unpack<BF16>(zn[0]);
-                        un1 = Unpack<BF16>(zn[1]);
-                        un2 = Unpack<BF16>(zn[2]);
-                        un3 = Unpack<BF16>(zn[3]);
-                    }
-                    // what follows: the next group here, or the next chunk's first
-                    if (done + left < steps) fetch(grp + 1);
-                    else if (c + 1 < own) fetch((chunk + static_cast<int64_t>(kWarps) * KS) * 8 / spg);
+                    for (int i = 0; i < 4; ++i)
+                        next[i].load(p.w, p.w.scales + (row0 + 8 * i) * p.w.gs, p.w.zeros + (row0 + 8 * i) * p.w.gs, grp,
+                                     p.vec, 8 * i < rows);
                 };
-                turn(0);
+                if (own > 0) fetch(kwarp * KS + rank);
+                for (int c = 0; c < own; ++c) {
+                    const int l = kwarp + c * kw, chunk = l * KS + rank;
+                    const int steps = min(kSteps, static_cast<int>(p.w.n / 32) - chunk * kSteps);
+                    RowScales<SPG, ZEROS> here[4];
 #pragma unroll
-                for (int st = 0; st < 8; ++st) {
-                    if (st < steps) {
-                        uint4 xb = make_uint4(0, 0, 0, 0);
-                        if (g < nb) xb = *reinterpret_cast<const uint4 *>(xs + st * nb * 64);
-                        uint32_t words[4];
+                    for (int i = 0; i < 4; ++i) here[i] = next[i];
+                    if (c + 1 < own) fetch(chunk + kw * KS);
+                    if (!dead) {
+                        const bool ok = mbar_wait(&full[stage], phase, &abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x31,
+                                                  p.wait_ns);
+                        dead = !__all_sync(0xffffffffu, ok);
+                    }
+                    const uint8_t *w = ring + stage * kChunkBytes + g * 128 + q * 4;
+                    const uint8_t *xs = g < nb ? sx + l * kSteps * nb * 64 + lane * 16 : nothing;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            words[i] = TMA ? *reinterpret_cast<const uint32_t *>(w + i * 1024 + ((st ^ g) << 4))
-                                       : g + 8 * i < rows ? word_at(p, byte0 + 8 * i * p.w.pitch + st * 16)
-                                                          : 0u;
-                        uint32_t a[4], b[4];
-                        un0(words[0], a);
-                        un1(words[1], b);
-                        mma16816<BF16>(sum[0], a[0], b[0], a[1], b[1], xb.x, xb.y);
-                        mma16816<BF16>(sum[0], a[2], b[2], a[3], b[3], xb.z, xb.w);
-                        un2(words[2], a);
-                        un3(words[3], b);
-                        mma16816<BF16>(sum[1], a[0], b[0], a[1], b[1], xb.x, xb.y);
-                        mma16816<BF16>(sum[1], a[2], b[2], a[3], b[3], xb.z, xb.w);
-                        if (--left == 0 || st == steps - 1) {
+                    for (int gi = 0; gi < kSteps / SPG; ++gi) {
+                        if (gi * SPG < steps) {
+                            const Unpack<BF16> un[4] = {Unpack<BF16>(here[0].zero(gi)), Unpack<BF16>(here[1].zero(gi)),
+                                                        Unpack<BF16>(here[2].zero(gi)), Unpack<BF16>(here[3].zero(gi))};
+                            const float scale[4] = {H::get(here[0].scale(gi)), H::get(here[1].scale(gi)),
+                                                    H::get(here[2].scale(gi)), H::get(here[3].scale(gi))};
+                            float sum[2][4];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                total[0][i] = fmaf(scale[i >> 1], sum[0][i], total[0][i]);
-                                total[1][i] = fmaf(scale[2 + (i >> 1)], sum[1][i], total[1][i]);
-                                sum[0][i] = sum[1][i] = 0.0f;
+                            for (int si = 0; si < SPG; ++si) {
+                                const int st = gi * SPG + si;
+                                if (si == 0 || st < steps) {
+                                    const uint4 x = *reinterpret_cast<const uint4 *>(xs);
+                                    xs += xstep;
+                                    uint32_t words[4];
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        words[i] = *reinterpret_cast<const uint32_t *>(w + i * 1024 + ((st ^ g) << 4));
+                                    if (si == 0)
+                                        step32<BF16, true>(sum, words, un, x);
+                                    else
+                                        step32<BF16, false>(sum, words, un, x);
+                                }
                             }
-                            if (left == 0 && st < steps - 1) {
-                                ++grp;
-                                left = spg;
-                                turn(st + 1);
-                            }
+                            add_scaled(total, sum, scale);
                         }
                     }
-                }
-                if constexpr (TMA) {
                     __syncwarp();
                     if (++stage == p.stages) {
                         stage = 0;
@@ -475,11 +548,48 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
                     }
                     issue();
                 }
+            } else {
+                for (int c = 0; c < own; ++c) {
+                    const int l = kwarp + c * kw, chunk = l * KS + rank;
+                    const int steps = static_cast<int>(min(static_cast<int64_t>(kSteps),
+                                                           (p.w.n - static_cast<int64_t>(chunk) * kChunk + 31) / 32));
+                    uint32_t words[kSteps][4];
+#pragma unroll
+                    for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            words[st][i] = st < steps && 8 * i < rows
+                                               ? word_at(p, (row0 + 8 * i) * p.w.pitch +
+                                                                static_cast<int64_t>(chunk) * (kChunk / 2) + st * 16 + q * 4)
+                                               : 0u;
+                    const uint8_t *xs = g < nb ? sx + l * kSteps * nb * 64 + lane * 16 : nothing;
+#pragma unroll
+                    for (int st = 0; st < kSteps; ++st) {
+                        if (st < steps) {
+                            const int grp = (chunk * kSteps + st) / spg;
+                            RowScales<0, ZEROS> here[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                here[i].load(p.w, p.w.scales + (row0 + 8 * i) * p.w.gs,
+                                             p.w.zeros + (row0 + 8 * i) * p.w.gs, grp, 0, 8 * i < rows);
+                            const Unpack<BF16> un[4] = {Unpack<BF16>(here[0].zero(0)), Unpack<BF16>(here[1].zero(0)),
+                                                        Unpack<BF16>(here[2].zero(0)), Unpack<BF16>(here[3].zero(0))};
+                            const float scale[4] = {H::get(here[0].scale(0)), H::get(here[1].scale(0)),
+                                                    H::get(here[2].scale(0)), H::get(here[3].scale(0))};
+                            const uint4 x = *reinterpret_cast<const uint4 *>(xs);
+                            xs += xstep;
+                            float sum[2][4];
+                            step32<BF16, true>(sum, words[st], un, x);
+                            add_scaled(total, sum, scale);
+                        }
+                    }
+                }
             }
         }
 
         // ---- join: warps, then the cluster's CTAs
-        float *mine = part + (flip * kWarps + warp) * sums;
+        __syncthreads();  // everyone has read the previous unit's sums
+        float *mine = part + warp * sums;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {  // row g + 8 (i / 2), vector 2 q + i % 2
             const int v = 2 * q + (i & 1);
@@ -487,16 +597,16 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         }
         __syncthreads();
         if (KS == 1) {
-            put(u, part + flip * kWarps * sums, sums, kWarps);
-        } else {
+            put(u, part, parts, sums, kw);
+        } else {  // one tile
             if (u > u_begin) {  // the previous unit's sums have arrived
                 cluster_wait();
-                if (rank == 0) put(u - 1, red + (flip ^ 1) * KS * sums, sums, KS);
+                if (rank == 0) put(u - 1, red + (flip ^ 1) * KS * sums, 1, sums, KS);
             }
             if (tid < kTileRows * nb) {
                 float sum = 0.0f;
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) sum += part[(flip * kWarps + w) * sums + tid];
+                for (int w = 0; w < kWarps; ++w) sum += part[w * sums + tid];
                 st_shared_cluster(mapa_shared(smem_u32(red + (flip * KS + rank) * sums + tid), 0), sum);
             }
             __syncwarp();
@@ -506,7 +616,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     if (KS > 1 && u_end > u_begin) {
         __syncwarp();
         cluster_wait();
-        if (rank == 0) put(u_end - 1, red + (flip ^ 1) * KS * sums, sums, KS);
+        if (rank == 0) put(u_end - 1, red + (flip ^ 1) * KS * sums, 1, sums, KS);
     }
     if (TMA && dead && lane == 0) {  // loads in flight land before the CTA leaves
         const uint64_t t0 = globaltimer_ns();
@@ -530,25 +640,16 @@ int launched(const char *what) {
     return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, what);
 }
 
-constexpr int kMaxSmem = 227 * 1024 - 1024;   // dynamic shared memory of the GEMV kernel, static beside it
-constexpr int kHalfSmem = 113 * 1024 - 1024;  // of one of two CTAs on an SM
-constexpr int64_t kMaxXBytes = 104 * 1024;    // of its staged vectors
+constexpr int kMaxSmem = 227 * 1024 - 1024;  // dynamic shared memory of the GEMV kernel, static beside it
+constexpr int64_t kMaxXBytes = 56 * 1024;    // of its staged vectors
 
-// Its shared memory for KS CTAs a unit; sets the ring's stages and the
-// vectors' bytes.  Two chunks a warp where two CTAs fit an SM, else up to four.
-template <bool TMA>
-size_t gemv_smem(GemvArgs &p, int KS, int64_t local) {
+// Its shared memory for KS CTAs a tile; sets the ring's stages and the
+// vectors' bytes.
+size_t gemv_smem(GemvArgs &p, bool tma, int KS, int64_t local) {
     p.x_bytes = static_cast<int>(local * kChunk * p.width * 2);
-    const size_t fixed = p.x_bytes + 2 * (kWarps + KS) * kTileRows * p.width * 4 + (p.index ? sizeof(Table) : 0) + 1024;
-    if (!TMA) {
-        p.stages = 0;
-        return fixed;
-    }
-    const size_t stage = kWarps * (kChunkBytes + 8);
-    p.stages = 2;
-    if (fixed + 2 * stage > kHalfSmem)
-        while (p.stages < 4 && fixed + (p.stages + 1) * stage <= kMaxSmem) ++p.stages;
-    return fixed + p.stages * stage;
+    p.stages = tma ? 2 : 0;
+    return p.x_bytes + (kWarps + 2 * KS) * kTileRows * p.width * 4 + p.stages * kWarps * (kChunkBytes + 8) + 16 +
+           (p.index ? sizeof(Table) : 0) + 1024;
 }
 
 // Resident clusters of KS CTAs of a kernel with that much shared memory,
@@ -575,10 +676,23 @@ int resident_clusters(b2b_handle *h, const void *kernel, cudaLaunchConfig_t &cfg
     return clusters;
 }
 
-template <bool TMA>
-int launch_gemv(b2b_handle *h, bool bf16, bool zeros, const CUtensorMap &tmW, GemvArgs &p) {
-    auto kernel = bf16 ? (zeros ? w4_gemv_kernel<true, true, TMA> : w4_gemv_kernel<true, false, TMA>)
-                       : (zeros ? w4_gemv_kernel<false, true, TMA> : w4_gemv_kernel<false, false, TMA>);
+using GemvKernel = void (*)(CUtensorMap, GemvArgs);
+
+template <bool BF16, bool ZEROS>
+GemvKernel gemv_kernel(int spg) {
+    switch (spg) {
+        case 1: return w4_gemv_kernel<BF16, ZEROS, 1>;
+        case 2: return w4_gemv_kernel<BF16, ZEROS, 2>;
+        case 4: return w4_gemv_kernel<BF16, ZEROS, 4>;
+        case 8: return w4_gemv_kernel<BF16, ZEROS, 8>;
+        default: return w4_gemv_kernel<BF16, ZEROS, 0>;
+    }
+}
+
+int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvArgs &p) {
+    const bool zeros = p.w.zeros != nullptr;
+    const GemvKernel kernel = bf16 ? (zeros ? gemv_kernel<true, true>(spg) : gemv_kernel<true, false>(spg))
+                                   : (zeros ? gemv_kernel<false, true>(spg) : gemv_kernel<false, false>(spg));
     const void *fn = reinterpret_cast<const void *>(kernel);
     const int64_t chunks = (p.w.n + kChunk - 1) / kChunk, tiles = (p.w.m + kTileRows - 1) / kTileRows;
     p.width = p.count < 8 ? p.count : 8;
@@ -591,46 +705,49 @@ int launch_gemv(b2b_handle *h, bool bf16, bool zeros, const CUtensorMap &tmW, Ge
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.blockDim = dim3(kWarps * 32);
+    cfg.blockDim = dim3(kThreads);
     cfg.stream = h->stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    // Split a unit's columns over the CTAs of a cluster where that takes the
+    {
+        static std::mutex mu;
+        static bool ready[2][2][9][64];
+        std::lock_guard<std::mutex> lock(mu);
+        bool &done = ready[bf16][zeros][spg][h->device & 63];
+        if (!done) {
+            const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
+            if (e != cudaSuccess) return b2b::fail_cuda(e, "4-bit GEMV shared memory");
+            done = true;
+        }
+    }
+    // Split a tile's columns over the CTAs of a cluster where that takes the
     // fewest turns: chunks that a warp computes one after another, and about
     // one more for each unit's start and joining.
-    int best = 0, best_grid = 0;
+    int best = 0, best_grid = 0, best_kw = 0;
     double best_time = 0;
     for (int KS = 1; KS <= 8 && (KS == 1 || KS < 2 * chunks); KS *= 2) {
         const int64_t local = (chunks + KS - 1) / KS;
         if (local * kChunk * p.width * 2 > kMaxXBytes) continue;
-        const size_t smem = gemv_smem<TMA>(p, KS, local);
+        int kw = kWarps;
+        while (KS == 1 && kw / 2 >= local) kw /= 2;
         attr[0].val.clusterDim.x = KS;
-        cfg.dynamicSmemBytes = smem;
-        {
-            static std::mutex mu;
-            static bool ready[2][2][64];
-            std::lock_guard<std::mutex> lock(mu);
-            bool &done = ready[bf16][zeros][h->device & 63];
-            if (!done) {
-                const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
-                if (e != cudaSuccess) return b2b::fail_cuda(e, "4-bit GEMV shared memory");
-                done = true;
-            }
-        }
+        cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, KS, local);
         const int64_t clusters = resident_clusters(h, fn, cfg, KS);
-        const int64_t units = sets * tiles;
+        const int64_t units = sets * ((tiles + kWarps / kw - 1) / (kWarps / kw));
         const double time = static_cast<double>((units + clusters - 1) / clusters) *
-                            (static_cast<double>((local + kWarps - 1) / kWarps) + 1.0);
+                            (static_cast<double>((local + kw - 1) / kw) + 1.0);
         if (!best || time < best_time) {
             best = KS;
+            best_kw = kw;
             best_time = time;
             best_grid = static_cast<int>(units < clusters ? units : clusters);
         }
     }
-    if (!best) return b2b::fail(B2B_ERR_NOT_SUPPORTED, "4-bit GEMV: rows longer than 425984 columns");
+    if (!best) return b2b::fail(B2B_ERR_NOT_SUPPORTED, "4-bit GEMV: rows longer than 229376 columns");
     const int64_t local = (chunks + best - 1) / best;
+    p.kw = best_kw;
     attr[0].val.clusterDim.x = best;
-    cfg.dynamicSmemBytes = gemv_smem<TMA>(p, best, local);
+    cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, best, local);
     cfg.gridDim = dim3(best * best_grid);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmW, p);
     return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, "4-bit GEMV launch");
@@ -674,20 +791,24 @@ int launch_hgemv_w4(b2b_handle *h, int type, size_t groups, size_t m, size_t n, 
     const int64_t rows = static_cast<int64_t>(groups) * p.w.m;
     p.total = rows * p.w.pitch;
     const bool bf16 = type == B2B_TYPE_BF16;
-    const bool tma = n % 32 == 0 && aligned16(packed) && rows < (1ll << 31);
+    // steps of a group that the TMA-fed kernel is made for
+    int spg = static_cast<int>(group / 32);
+    if (spg % 8 == 0) spg = 8;
+    const bool tma = n % 32 == 0 && aligned16(packed) && rows < (1ll << 31) && (spg == 1 || spg == 2 || spg == 4 || spg == 8);
+    if (!tma) spg = 0;
     CUtensorMap tmW{};
     if (tma) {
         if (int rc = encode_tma_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, packed, rows, p.w.pitch, kChunk / 2,
                                    kTileRows))
             return rc;
+        const int64_t per = 8 / spg;  // groups of a chunk
+        p.vec = p.w.gs % per == 0 && aligned16(scales) && aligned16(zeros);
     }
     const int64_t all = static_cast<int64_t>(count);
     for (int64_t first = 0; first < all; first += index ? kMaxIndexed : all) {
         p.first = static_cast<int>(first);
         p.count = static_cast<int>(index && all - first > kMaxIndexed ? kMaxIndexed : all - first);
-        if (int rc = tma ? launch_gemv<true>(h, bf16, zeros != nullptr, tmW, p)
-                         : launch_gemv<false>(h, bf16, zeros != nullptr, tmW, p))
-            return rc;
+        if (int rc = launch_gemv(h, bf16, spg, tmW, p)) return rc;
     }
     return B2B_OK;
 }
