@@ -202,6 +202,17 @@ __device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t b
     return r;
 }
 
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+    return v;
+}
+
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2 *>(&v); }
 __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t v) { return *reinterpret_cast<const __nv_bfloat162 *>(&v); }
 template <typename T>
@@ -302,6 +313,38 @@ struct RowScales {
     __device__ __forceinline__ uint32_t zero(int i) const { return ZEROS ? z[i / 4] >> (8 * (i & 3)) & 15u : 8u; }
 };
 
+// A chunk's products, its words at shared address w, the vectors' pieces of
+// its first step at x.  FULL: it has all its steps.
+template <bool BF16, bool ZEROS, int SPG, bool FULL>
+__device__ __forceinline__ void chunk_products(float (&total)[2][4], uint32_t w, uint32_t x, int xstep,
+                                               const RowScales<SPG, ZEROS> (&here)[4], int steps) {
+    using H = b2b::Half16<BF16>;
+#pragma unroll
+    for (int gi = 0; gi < kSteps / SPG; ++gi) {
+        if (!FULL && gi * SPG >= steps) break;
+        const Unpack<BF16> un[4] = {Unpack<BF16>(here[0].zero(gi)), Unpack<BF16>(here[1].zero(gi)),
+                                    Unpack<BF16>(here[2].zero(gi)), Unpack<BF16>(here[3].zero(gi))};
+        const float scale[4] = {H::get(here[0].scale(gi)), H::get(here[1].scale(gi)), H::get(here[2].scale(gi)),
+                                H::get(here[3].scale(gi))};
+        float sum[2][4];
+#pragma unroll
+        for (int si = 0; si < SPG; ++si) {
+            const int st = gi * SPG + si;
+            if (!FULL && si > 0 && st >= steps) break;
+            const uint4 xv = lds128(x);
+            x += xstep;
+            uint32_t words[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) words[i] = lds32((w ^ (st << 4)) + i * 1024);
+            if (si == 0)
+                step32<BF16, true>(sum, words, un, xv);
+            else
+                step32<BF16, false>(sum, words, un, xv);
+        }
+        add_scaled(total, sum, scale);
+    }
+}
+
 // SPG: steps of 32 columns in a group, 8 standing for its multiples; 0: plain
 // loads, any group.
 template <bool BF16, bool ZEROS, int SPG>
@@ -321,8 +364,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *sx = smem + (TMA ? kWarps * p.stages * kChunkBytes : 0);
     const int sums = kTileRows * p.width;                     // of a tile
     float *part = reinterpret_cast<float *>(sx + p.x_bytes);  // [kWarps][32 rows][width]
-    float *red = part + kWarps * sums;                        // [2][KS][32 rows][width]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(red + 2 * KS * sums);
+    float *red = part + kWarps * sums;                        // [2][KS][parts][32 rows][width]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(red + 2 * KS * parts * sums);
     uint64_t *full = bars + warp * p.stages;
     uint8_t *nothing = reinterpret_cast<uint8_t *>(bars + kWarps * p.stages);  // 16 bytes of 0
     Table *table = reinterpret_cast<Table *>(nothing + 16);
@@ -424,18 +467,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         return p.index ? items[set].count
                        : static_cast<int>(min(static_cast<int64_t>(p.width), p.count - static_cast<int64_t>(set) * p.width));
     };
-    // Sums leave the cluster: `terms` arrays of `step` sums for each of
-    // `ntiles` tiles, [tile][term][row][vector].
-    auto put = [&](uint32_t u, const float *from, int ntiles, int step, int terms) {
+    // Sums of a unit's tiles leave the cluster: sum i of the `terms` to add is
+    // `step` behind the one before, a tile `tile_step` behind the one before.
+    auto put = [&](uint32_t u, const float *from, int tile_step, int step, int terms) {
         const uint32_t set = u / upers, tile0 = u % upers * parts;
         const int nb = vectors_of(set);
         const bool some = matrix_of(set) >= 0;
-        for (int o = tid; o < ntiles * kTileRows * nb; o += kThreads) {
+        for (int o = tid; o < parts * kTileRows * nb; o += kThreads) {
             const int t = o / (kTileRows * nb), r = o % (kTileRows * nb);
             const int64_t row = static_cast<int64_t>(tile0 + t) * kTileRows + r / nb;
             if (row >= p.w.m) continue;
             float sum = 0.0f;
-            for (int i = 0; i < terms; ++i) sum += from[(t * terms + i) * step + r];
+            for (int i = 0; i < terms; ++i) sum += from[t * tile_step + i * step + r];
             const int v = r % nb;
             const int64_t i = p.index ? p.first + items[set].member[v] : static_cast<int64_t>(set) * p.width + v;
             uint16_t *y = p.y + i * p.w.m + row;
@@ -512,35 +555,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                   p.wait_ns);
                         dead = !__all_sync(0xffffffffu, ok);
                     }
-                    const uint8_t *w = ring + stage * kChunkBytes + g * 128 + q * 4;
-                    const uint8_t *xs = g < nb ? sx + l * kSteps * nb * 64 + lane * 16 : nothing;
-#pragma unroll
-                    for (int gi = 0; gi < kSteps / SPG; ++gi) {
-                        if (gi * SPG < steps) {
-                            const Unpack<BF16> un[4] = {Unpack<BF16>(here[0].zero(gi)), Unpack<BF16>(here[1].zero(gi)),
-                                                        Unpack<BF16>(here[2].zero(gi)), Unpack<BF16>(here[3].zero(gi))};
-                            const float scale[4] = {H::get(here[0].scale(gi)), H::get(here[1].scale(gi)),
-                                                    H::get(here[2].scale(gi)), H::get(here[3].scale(gi))};
-                            float sum[2][4];
-#pragma unroll
-                            for (int si = 0; si < SPG; ++si) {
-                                const int st = gi * SPG + si;
-                                if (si == 0 || st < steps) {
-                                    const uint4 x = *reinterpret_cast<const uint4 *>(xs);
-                                    xs += xstep;
-                                    uint32_t words[4];
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i)
-                                        words[i] = *reinterpret_cast<const uint32_t *>(w + i * 1024 + ((st ^ g) << 4));
-                                    if (si == 0)
-                                        step32<BF16, true>(sum, words, un, x);
-                                    else
-                                        step32<BF16, false>(sum, words, un, x);
-                                }
-                            }
-                            add_scaled(total, sum, scale);
-                        }
-                    }
+                    // 16-byte piece st of row r sits at piece st ^ (r % 8)
+                    const uint32_t w = smem_u32(ring) + stage * kChunkBytes + g * 128 + (g << 4) + q * 4;
+                    const uint32_t xs = g < nb ? smem_u32(sx) + l * kSteps * nb * 64 + lane * 16 : smem_u32(nothing);
+                    if (steps == kSteps)
+                        chunk_products<BF16, ZEROS, SPG, true>(total, w, xs, xstep, here, steps);
+                    else
+                        chunk_products<BF16, ZEROS, SPG, false>(total, w, xs, xstep, here, steps);
                     __syncwarp();
                     if (++stage == p.stages) {
                         stage = 0;
@@ -597,17 +618,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncthreads();
         if (KS == 1) {
-            put(u, part, parts, sums, kw);
-        } else {  // one tile
+            put(u, part, kw * sums, sums, kw);
+        } else {
             if (u > u_begin) {  // the previous unit's sums have arrived
                 cluster_wait();
-                if (rank == 0) put(u - 1, red + (flip ^ 1) * KS * sums, 1, sums, KS);
+                if (rank == 0) put(u - 1, red + (flip ^ 1) * KS * parts * sums, sums, parts * sums, KS);
             }
-            if (tid < kTileRows * nb) {
+            for (int o = tid; o < parts * kTileRows * nb; o += kThreads) {
+                const int t = o / (kTileRows * nb), r = o % (kTileRows * nb);
                 float sum = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kWarps; ++w) sum += part[w * sums + tid];
-                st_shared_cluster(mapa_shared(smem_u32(red + (flip * KS + rank) * sums + tid), 0), sum);
+                for (int w = 0; w < kw; ++w) sum += part[(t * kw + w) * sums + r];
+                st_shared_cluster(mapa_shared(smem_u32(red + ((flip * KS + rank) * parts + t) * sums + r), 0), sum);
             }
             __syncwarp();
             cluster_arrive();
@@ -616,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (KS > 1 && u_end > u_begin) {
         __syncwarp();
         cluster_wait();
-        if (rank == 0) put(u_end - 1, red + (flip ^ 1) * KS * sums, 1, sums, KS);
+        if (rank == 0) put(u_end - 1, red + (flip ^ 1) * KS * parts * sums, sums, parts * sums, KS);
     }
     if (TMA && dead && lane == 0) {  // loads in flight land before the CTA leaves
         const uint64_t t0 = globaltimer_ns();
@@ -645,10 +666,10 @@ constexpr int64_t kMaxXBytes = 56 * 1024;    // of its staged vectors
 
 // Its shared memory for KS CTAs a tile; sets the ring's stages and the
 // vectors' bytes.
-size_t gemv_smem(GemvArgs &p, bool tma, int KS, int64_t local) {
+size_t gemv_smem(GemvArgs &p, bool tma, int KS, int kw, int64_t local) {
     p.x_bytes = static_cast<int>(local * kChunk * p.width * 2);
     p.stages = tma ? 2 : 0;
-    return p.x_bytes + (kWarps + 2 * KS) * kTileRows * p.width * 4 + p.stages * kWarps * (kChunkBytes + 8) + 16 +
+    return p.x_bytes + (kWarps + 2 * KS * (kWarps / kw)) * kTileRows * p.width * 4 + p.stages * kWarps * (kChunkBytes + 8) + 16 +
            (p.index ? sizeof(Table) : 0) + 1024;
 }
 
@@ -729,9 +750,10 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
         const int64_t local = (chunks + KS - 1) / KS;
         if (local * kChunk * p.width * 2 > kMaxXBytes) continue;
         int kw = kWarps;
-        while (KS == 1 && kw / 2 >= local) kw /= 2;
+        while (kw / 2 >= local) kw /= 2;
         attr[0].val.clusterDim.x = KS;
-        cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, KS, local);
+        cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, KS, kw, local);
+        if (cfg.dynamicSmemBytes > static_cast<size_t>(kMaxSmem)) continue;
         const int64_t clusters = resident_clusters(h, fn, cfg, KS);
         const int64_t units = sets * ((tiles + kWarps / kw - 1) / (kWarps / kw));
         const double time = static_cast<double>((units + clusters - 1) / clusters) *
@@ -747,7 +769,7 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
     const int64_t local = (chunks + best - 1) / best;
     p.kw = best_kw;
     attr[0].val.clusterDim.x = best;
-    cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, best, local);
+    cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, best, best_kw, local);
     cfg.gridDim = dim3(best * best_grid);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmW, p);
     return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, "4-bit GEMV launch");
