@@ -130,6 +130,7 @@ constexpr int kTileRows = 32;
 constexpr int kChunk = 256;                       // columns
 constexpr int kSteps = kChunk / 32;               // of 32 columns
 constexpr int kChunkBytes = kTileRows * kChunk / 2;
+constexpr int kStages = 2;                        // chunks of a warp's ring
 constexpr int kMaxIndexed = 256;                  // products of one launch that choose their matrix
 
 struct GemvArgs {
@@ -142,7 +143,6 @@ struct GemvArgs {
     int matrices, count, fan, first;  // first: number of this launch's first product
     int width;    // vectors of a set: 8, or fewer where longer rows leave room for fewer
     int kw;       // warps that share a tile
-    int stages;   // chunks of a warp's ring
     int x_bytes;  // of the staged vectors
     int vec;      // a chunk's scales and zero points of a row are one aligned word each
     float alpha, beta;
@@ -275,16 +275,12 @@ struct RowScales {
     static constexpr int N = SPG ? kSteps / SPG : 1;
     uint32_t s[(N + 1) / 2];
     uint32_t z[(N + 3) / 4];
-    __device__ __forceinline__ void load(const W4Args &w, const uint16_t *scales, const uint8_t *zeros, int grp, int vec,
-                                         bool live) {
-#pragma unroll
-        for (int i = 0; i < (N + 1) / 2; ++i) s[i] = 0;
-#pragma unroll
-        for (int i = 0; i < (N + 3) / 4; ++i) z[i] = 0;
-        if (!live) return;
-        scales += grp;
-        zeros += grp;
-        if (vec && N > 1) {
+    // `left`: groups that the row has from here on
+    __device__ __forceinline__ void load(const uint16_t *scales, const uint8_t *zeros, int left, int vec) {
+        if (N == 1) {
+            s[0] = __ldg(scales);
+            if constexpr (ZEROS) z[0] = __ldg(zeros);
+        } else if (vec) {
             if constexpr (N == 8) {
                 const uint4 v = __ldg(reinterpret_cast<const uint4 *>(scales));
                 s[0] = v.x, s[1] = v.y, s[2] = v.z, s[3] = v.w;
@@ -302,8 +298,12 @@ struct RowScales {
             }
         } else {
 #pragma unroll
+            for (int i = 0; i < (N + 1) / 2; ++i) s[i] = 0;
+#pragma unroll
+            for (int i = 0; i < (N + 3) / 4; ++i) z[i] = 0;
+#pragma unroll
             for (int i = 0; i < N; ++i)
-                if (grp + i < w.gs) {
+                if (i < left) {
                     s[i / 2] |= static_cast<uint32_t>(__ldg(scales + i)) << (16 * (i & 1));
                     if constexpr (ZEROS) z[i / 4] |= static_cast<uint32_t>(__ldg(zeros + i)) << (8 * (i & 3));
                 }
@@ -360,14 +360,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int g = lane >> 2, q = lane & 3;
     const int KS = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
     const int kw = p.kw, parts = kWarps / kw, part_no = warp / kw, kwarp = warp % kw;
-    uint8_t *ring = smem + (TMA ? warp * p.stages * kChunkBytes : 0);
-    uint8_t *sx = smem + (TMA ? kWarps * p.stages * kChunkBytes : 0);
+    uint8_t *ring = smem + (TMA ? warp * kStages * kChunkBytes : 0);
+    uint8_t *sx = smem + (TMA ? kWarps * kStages * kChunkBytes : 0);
     const int sums = kTileRows * p.width;                     // of a tile
     float *part = reinterpret_cast<float *>(sx + p.x_bytes);  // [kWarps][32 rows][width]
     float *red = part + kWarps * sums;                        // [2][KS][parts][32 rows][width]
     uint64_t *bars = reinterpret_cast<uint64_t *>(red + 2 * KS * parts * sums);
-    uint64_t *full = bars + warp * p.stages;
-    uint8_t *nothing = reinterpret_cast<uint8_t *>(bars + kWarps * p.stages);  // 16 bytes of 0
+    uint64_t *full = bars + warp * kStages;
+    uint8_t *nothing = reinterpret_cast<uint8_t *>(bars + kWarps * kStages);  // 16 bytes of 0
     Table *table = reinterpret_cast<Table *>(nothing + 16);
     const Item *items = table->item;
 
@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) abort_flag = 0;
     if (tid < 4) reinterpret_cast<uint32_t *>(nothing)[tid] = 0;
     if (TMA && lane == 0) {
-        for (int s = 0; s < p.stages; ++s) mbar_init(&full[s], 1);
+        for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
         fence_barrier_init();
     }
     if (p.index) {
@@ -430,38 +430,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto matrix_of = [&](uint32_t set) { return p.index ? items[set].matrix : 0; };
 
     bool dead = false;
-    // The loads run p.stages chunks ahead of their use.
-    uint32_t iset = u_begin / upers, iunit = u_begin % upers, ileft = u_end - u_begin;
-    int ic = 0, istage = 0;
-    auto issue = [&] {
-        if constexpr (TMA) {
-            while (ileft && ic == 0 &&
-                   (own == 0 || matrix_of(iset) < 0 || iunit * parts + part_no >= tiles)) {  // nothing to load
-                --ileft;
-                if (++iunit == upers) {
-                    iunit = 0;
-                    ++iset;
-                }
-            }
-            if (!ileft || dead) return;
-            if (lane == 0) {
-                const int row = static_cast<int>(matrix_of(iset) * p.w.m + (iunit * parts + part_no) * kTileRows);
-                mbar_arrive_expect_tx(&full[istage], kChunkBytes);
-                tma_load_2d(ring + istage * kChunkBytes, &tmW, &full[istage],
-                            ((kwarp + ic * kw) * KS + rank) * (kChunk / 2), row);
-            }
-            if (++istage == p.stages) istage = 0;
-            if (++ic == own) {
-                ic = 0;
-                --ileft;
-                if (++iunit == upers) {
-                    iunit = 0;
-                    ++iset;
-                }
-            }
+    // The loads run kStages chunks ahead of their use: iu and ic are the unit
+    // and the chunk (of this warp's) to load next, at byte icol of row irow.
+    uint32_t iu = u_begin;
+    int ic = 0, irow = 0, icol = 0, istage = 0;
+    auto seek = [&] {  // the first unit from iu on in which this warp has chunks
+        for (; iu < u_end; ++iu) {
+            const uint32_t set = iu / upers, tile = iu % upers * parts + part_no;
+            const int e = matrix_of(set);
+            if (own == 0 || e < 0 || tile >= tiles) continue;
+            irow = static_cast<int>(e * p.w.m + tile * kTileRows);
+            icol = (kwarp * KS + rank) * (kChunk / 2);
+            return;
         }
     };
-    for (int s = 0; s < p.stages; ++s) issue();
+    auto issue = [&] {
+        if (iu >= u_end || dead) return;
+        if (lane == 0) {
+            mbar_arrive_expect_tx(&full[istage], kChunkBytes);
+            tma_load_2d(ring + istage * kChunkBytes, &tmW, &full[istage], icol, irow);
+        }
+        istage ^= 1;
+        icol += kw * KS * (kChunk / 2);
+        if (++ic == own) {
+            ic = 0;
+            ++iu;
+            seek();
+        }
+    };
+    if constexpr (TMA) {
+        seek();
+        for (int s = 0; s < kStages; ++s) issue();
+    }
 
     auto vectors_of = [&](uint32_t set) {
         return p.index ? items[set].count
@@ -489,6 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     const int spg = static_cast<int>(p.w.group / 32);
+    const int nsteps = static_cast<int>(p.w.n / 32);
     int stage = 0, flip = 0, nb = 0;
     uint32_t phase = 0, staged = 0xffffffffu;
     for (uint32_t u = u_begin; u < u_end; ++u, flip ^= 1) {
@@ -534,18 +535,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             // lanes of vectors that the set does not have read zeros
             const int xstep = g < nb ? nb * 64 : 0;
             if constexpr (TMA) {
+                // this lane's rows, or the last one for those that are not there
+                const int last = rows - 1;  // of this matrix, less g
+                const uint32_t gs = static_cast<uint32_t>(p.w.gs);
+                const int64_t at0 = (row0 + min(last, 0)) * p.w.gs;
+                uint32_t at[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) at[i] = static_cast<uint32_t>(max(min(8 * i, last), 0)) * gs;
                 RowScales<SPG, ZEROS> next[4];
                 auto fetch = [&](int chunk) {
                     const int grp = SPG == 8 ? chunk / (spg / 8) : chunk * (kSteps / SPG);
+                    const uint16_t *scales = p.w.scales + at0 + grp;
+                    const uint8_t *zeros = p.w.zeros + at0 + grp;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        next[i].load(p.w, p.w.scales + (row0 + 8 * i) * p.w.gs, p.w.zeros + (row0 + 8 * i) * p.w.gs, grp,
-                                     p.vec, 8 * i < rows);
+                        next[i].load(scales + at[i], zeros + at[i], static_cast<int>(gs) - grp, p.vec);
                 };
                 if (own > 0) fetch(kwarp * KS + rank);
                 for (int c = 0; c < own; ++c) {
                     const int l = kwarp + c * kw, chunk = l * KS + rank;
-                    const int steps = min(kSteps, static_cast<int>(p.w.n / 32) - chunk * kSteps);
+                    const int steps = min(kSteps, nsteps - chunk * kSteps);
                     RowScales<SPG, ZEROS> here[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) here[i] = next[i];
@@ -563,13 +572,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     else
                         chunk_products<BF16, ZEROS, SPG, false>(total, w, xs, xstep, here, steps);
                     __syncwarp();
-                    if (++stage == p.stages) {
-                        stage = 0;
-                        phase ^= 1u;
-                    }
+                    phase ^= stage;
+                    stage ^= 1;
                     issue();
                 }
             } else {
+                // a row of this lane, or the last one for one that is not there
+                auto row_at = [&](int i) { return row0 + min(i, rows - 1); };
                 for (int c = 0; c < own; ++c) {
                     const int l = kwarp + c * kw, chunk = l * KS + rank;
                     const int steps = static_cast<int>(min(static_cast<int64_t>(kSteps),
@@ -591,8 +600,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                             RowScales<0, ZEROS> here[4];
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                here[i].load(p.w, p.w.scales + (row0 + 8 * i) * p.w.gs,
-                                             p.w.zeros + (row0 + 8 * i) * p.w.gs, grp, 0, 8 * i < rows);
+                                here[i].load(p.w.scales + row_at(8 * i) * p.w.gs + grp,
+                                             p.w.zeros + row_at(8 * i) * p.w.gs + grp, 1, 0);
                             const Unpack<BF16> un[4] = {Unpack<BF16>(here[0].zero(0)), Unpack<BF16>(here[1].zero(0)),
                                                         Unpack<BF16>(here[2].zero(0)), Unpack<BF16>(here[3].zero(0))};
                             const float scale[4] = {H::get(here[0].scale(0)), H::get(here[1].scale(0)),
@@ -664,12 +673,11 @@ int launched(const char *what) {
 constexpr int kMaxSmem = 227 * 1024 - 1024;  // dynamic shared memory of the GEMV kernel, static beside it
 constexpr int64_t kMaxXBytes = 56 * 1024;    // of its staged vectors
 
-// Its shared memory for KS CTAs a tile; sets the ring's stages and the
+// Its shared memory for KS CTAs and kw warps of each a tile; sets the
 // vectors' bytes.
 size_t gemv_smem(GemvArgs &p, bool tma, int KS, int kw, int64_t local) {
     p.x_bytes = static_cast<int>(local * kChunk * p.width * 2);
-    p.stages = tma ? 2 : 0;
-    return p.x_bytes + (kWarps + 2 * KS * (kWarps / kw)) * kTileRows * p.width * 4 + p.stages * kWarps * (kChunkBytes + 8) + 16 +
+    return p.x_bytes + (kWarps + 2 * KS * (kWarps / kw)) * kTileRows * p.width * 4 + kWarps * kStages * ((tma ? kChunkBytes : 0) + 8) + 16 +
            (p.index ? sizeof(Table) : 0) + 1024;
 }
 
