@@ -110,27 +110,30 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(W4Args p, uint16_t *
 // bits.
 //
 //   * A tile is 32 rows of W for one set of vectors; its n columns are cut
-//     into chunks of 256 (128 bytes of a row), which the CTAs of a cluster
-//     and kw of a CTA's 16 warps take in turn; the 16 / kw parts of a CTA have
+//     into chunks of 512 (256 bytes of a row), which the CTAs of a cluster
+//     and kw of a CTA's 8 warps take in turn; the 8 / kw parts of a CTA have
 //     a tile each.  A unit is those tiles.
-//   * Each warp keeps its own ring of chunks (32 rows x 128 bytes, 128-byte
-//     swizzle) filled by TMA ahead of its use, across units, so nothing
-//     drains at a unit's end; 16 warps x 2 chunks are 128 KiB of W in flight.
+//   * Each warp keeps its own ring of chunks (two boxes of 32 rows x 128
+//     bytes, 128-byte swizzle) filled by TMA ahead of its use, across units, so
+//     nothing drains at a unit's end; 8 warps x 2 chunks are 128 KiB in flight.
 //   * The vectors are staged once for each set, each 8 columns reordered to
 //     the pairs (0,4) (1,5) (2,6) (3,7) that the words unpack to.
-//   * Warps join their sums through shared memory, CTAs of a cluster through
-//     the first CTA's shared memory, one unit later so that no one waits;
-//     both in a fixed order.
+//   * The last of a tile's warps to arrive adds their sums up while the others
+//     go on; the CTAs of a cluster read one another's sums once for 8 units.
+//     Both in a fixed order, whoever adds.
 // Rows that TMA cannot describe (n not a multiple of 32, packed not 16-byte
 // aligned) and groups that do not fit a chunk evenly are read by the same
 // kernel with plain loads (SPG = 0).
-constexpr int kWarps = 16;
+constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTileRows = 32;
-constexpr int kChunk = 256;                       // columns
+constexpr int kChunk = 512;                       // columns, as two boxes
 constexpr int kSteps = kChunk / 32;               // of 32 columns
 constexpr int kChunkBytes = kTileRows * kChunk / 2;
+constexpr int kBoxCols = 256;                     // 128 bytes of a row
+constexpr int kBoxBytes = kTileRows * kBoxCols / 2;
 constexpr int kStages = 2;                        // chunks of a warp's ring
+constexpr int kBatch = 8;                         // units that the CTAs of a cluster join at once
 constexpr int kMaxIndexed = 256;                  // products of one launch that choose their matrix
 
 struct GemvArgs {
@@ -269,33 +272,36 @@ __device__ __forceinline__ void add_scaled(float (&total)[2][4], const float (&s
         total[i >> 2][i & 3] = fmaf(scale[i >> 1], sum[i >> 2][i & 3], total[i >> 2][i & 3]);
 }
 
-// Scales and zero points of one row's groups in a chunk (at most 8).
+// Scales and zero points of one row's groups in a chunk (at most 16).
 template <int SPG, bool ZEROS>
 struct RowScales {
     static constexpr int N = SPG ? kSteps / SPG : 1;
     uint32_t s[(N + 1) / 2];
     uint32_t z[(N + 3) / 4];
+    template <int WORDS>
+    __device__ __forceinline__ static void words(uint32_t *to, const void *from) {
+        if constexpr (WORDS >= 4) {
+#pragma unroll
+            for (int i = 0; i < WORDS / 4; ++i) {
+                const uint4 v = __ldg(static_cast<const uint4 *>(from) + i);
+                to[4 * i] = v.x, to[4 * i + 1] = v.y, to[4 * i + 2] = v.z, to[4 * i + 3] = v.w;
+            }
+        } else if constexpr (WORDS == 2) {
+            const uint2 v = __ldg(static_cast<const uint2 *>(from));
+            to[0] = v.x, to[1] = v.y;
+        } else {
+            to[0] = __ldg(static_cast<const uint32_t *>(from));
+        }
+    }
     // `left`: groups that the row has from here on
     __device__ __forceinline__ void load(const uint16_t *scales, const uint8_t *zeros, int left, int vec) {
         if (N == 1) {
             s[0] = __ldg(scales);
             if constexpr (ZEROS) z[0] = __ldg(zeros);
         } else if (vec) {
-            if constexpr (N == 8) {
-                const uint4 v = __ldg(reinterpret_cast<const uint4 *>(scales));
-                s[0] = v.x, s[1] = v.y, s[2] = v.z, s[3] = v.w;
-                if constexpr (ZEROS) {
-                    const uint2 u = __ldg(reinterpret_cast<const uint2 *>(zeros));
-                    z[0] = u.x, z[1] = u.y;
-                }
-            } else if constexpr (N == 4) {
-                const uint2 v = __ldg(reinterpret_cast<const uint2 *>(scales));
-                s[0] = v.x, s[1] = v.y;
-                if constexpr (ZEROS) z[0] = __ldg(reinterpret_cast<const uint32_t *>(zeros));
-            } else {
-                s[0] = __ldg(reinterpret_cast<const uint32_t *>(scales));
-                if constexpr (ZEROS) z[0] = __ldg(reinterpret_cast<const uint16_t *>(zeros));
-            }
+            words<(N + 1) / 2>(s, scales);
+            if constexpr (ZEROS && N >= 4) words<(N + 3) / 4>(z, zeros);
+            if constexpr (ZEROS && N == 2) z[0] = __ldg(reinterpret_cast<const uint16_t *>(zeros));
         } else {
 #pragma unroll
             for (int i = 0; i < (N + 1) / 2; ++i) s[i] = 0;
@@ -335,7 +341,7 @@ __device__ __forceinline__ void chunk_products(float (&total)[2][4], uint32_t w,
             x += xstep;
             uint32_t words[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) words[i] = lds32((w ^ (st << 4)) + i * 1024);
+            for (int i = 0; i < 4; ++i) words[i] = lds32((w ^ ((st & 7) << 4)) + (st >> 3) * kBoxBytes + i * 1024);
             if (si == 0)
                 step32<BF16, true>(sum, words, un, xv);
             else
@@ -345,7 +351,26 @@ __device__ __forceinline__ void chunk_products(float (&total)[2][4], uint32_t w,
     }
 }
 
-// SPG: steps of 32 columns in a group, 8 standing for its multiples; 0: plain
+// Waits until *count reaches `want`; bounded like every wait (the warps that
+// raise it wait for their own loads, each at most wait_ns).
+__device__ __forceinline__ bool wait_finished(const volatile int *count, int want, volatile int *abort, const GemvArgs &p,
+                                              int lane) {
+    int ok = 1;
+    if (lane == 0 && *count < want) {
+        const uint64_t t0 = sm100::globaltimer_ns();
+        while (*count < want) {
+            if (*abort || sm100::globaltimer_ns() - t0 > 2 * p.wait_ns) {
+                *abort = 1;
+                atomicCAS(p.status, 0, B2B_DEVSTAT_TIMEOUT | 0x32);
+                ok = 0;
+                break;
+            }
+        }
+    }
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
+// SPG: steps of 32 columns in a group, 16 standing for its multiples; 0: plain
 // loads, any group.
 template <bool BF16, bool ZEROS, int SPG>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -355,6 +380,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr bool TMA = SPG != 0;
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag;
+    __shared__ int arrived[2][kWarps];            // warps whose sums of a tile are in `part`
+    __shared__ volatile int finished[2][kWarps];  // tiles joined from there so far
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, q = lane & 3;
@@ -363,9 +390,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t *ring = smem + (TMA ? warp * kStages * kChunkBytes : 0);
     uint8_t *sx = smem + (TMA ? kWarps * kStages * kChunkBytes : 0);
     const int sums = kTileRows * p.width;                     // of a tile
-    float *part = reinterpret_cast<float *>(sx + p.x_bytes);  // [kWarps][32 rows][width]
-    float *red = part + kWarps * sums;                        // [2][KS][parts][32 rows][width]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(red + 2 * KS * parts * sums);
+    float *part = reinterpret_cast<float *>(sx + p.x_bytes);  // [2][kWarps][32 rows][width]
+    float *slots = part + 2 * kWarps * sums;                  // KS > 1: [2][kBatch][parts][32 rows][width]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(slots + (KS > 1 ? 2 * kBatch * parts * sums : 0));
     uint64_t *full = bars + warp * kStages;
     uint8_t *nothing = reinterpret_cast<uint8_t *>(bars + kWarps * kStages);  // 16 bytes of 0
     Table *table = reinterpret_cast<Table *>(nothing + 16);
@@ -374,6 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ---- the sets of products
     if (tid == 0) abort_flag = 0;
     if (tid < 4) reinterpret_cast<uint32_t *>(nothing)[tid] = 0;
+    if (tid < 2 * kWarps) arrived[tid / kWarps][tid % kWarps] = finished[tid / kWarps][tid % kWarps] = 0;
     if (TMA && lane == 0) {
         for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
         fence_barrier_init();
@@ -414,7 +442,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     }
     __syncthreads();
-    if (KS > 1) cluster_sync();  // every CTA has started before one writes to another
     const uint32_t tiles = static_cast<uint32_t>((p.w.m + kTileRows - 1) / kTileRows);
     const uint32_t upers = (tiles + parts - 1) / parts;  // units of a set
     const uint32_t sets = p.index ? table->items : (p.count + p.width - 1) / p.width;
@@ -449,6 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) {
             mbar_arrive_expect_tx(&full[istage], kChunkBytes);
             tma_load_2d(ring + istage * kChunkBytes, &tmW, &full[istage], icol, irow);
+            tma_load_2d(ring + istage * kChunkBytes + kBoxBytes, &tmW, &full[istage], icol + kBoxCols / 2, irow);
         }
         istage ^= 1;
         icol += kw * KS * (kChunk / 2);
@@ -467,32 +495,62 @@ __global__ void __launch_bounds__(kThreads, 1)
         return p.index ? items[set].count
                        : static_cast<int>(min(static_cast<int64_t>(p.width), p.count - static_cast<int64_t>(set) * p.width));
     };
-    // Sums of a unit's tiles leave the cluster: sum i of the `terms` to add is
-    // `step` behind the one before, a tile `tile_step` behind the one before.
-    auto put = [&](uint32_t u, const float *from, int tile_step, int step, int terms) {
-        const uint32_t set = u / upers, tile0 = u % upers * parts;
-        const int nb = vectors_of(set);
-        const bool some = matrix_of(set) >= 0;
-        for (int o = tid; o < parts * kTileRows * nb; o += kThreads) {
-            const int t = o / (kTileRows * nb), r = o % (kTileRows * nb);
-            const int64_t row = static_cast<int64_t>(tile0 + t) * kTileRows + r / nb;
-            if (row >= p.w.m) continue;
-            float sum = 0.0f;
-            for (int i = 0; i < terms; ++i) sum += from[t * tile_step + i * step + r];
-            const int v = r % nb;
-            const int64_t i = p.index ? p.first + items[set].member[v] : static_cast<int64_t>(set) * p.width + v;
-            uint16_t *y = p.y + i * p.w.m + row;
-            float res = some ? p.alpha * sum : 0.0f;
-            if (p.beta != 0.0f) res = fmaf(p.beta, H::get(*y), res);
-            *y = H::put(res);
-        }
+    // Sum o (row o / nb, vector o % nb) of a tile leaves.
+    auto put = [&](uint32_t set, uint32_t tile, int nb, int o, float sum) {
+        const int64_t row = static_cast<int64_t>(tile) * kTileRows + o / nb;
+        if (row >= p.w.m) return;
+        const int64_t i = p.index ? p.first + items[set].member[o % nb] : static_cast<int64_t>(set) * p.width + o % nb;
+        uint16_t *y = p.y + i * p.w.m + row;
+        float res = matrix_of(set) >= 0 ? p.alpha * sum : 0.0f;
+        if (p.beta != 0.0f) res = fmaf(p.beta, H::get(*y), res);
+        *y = H::put(res);
     };
 
     const int spg = static_cast<int>(p.w.group / 32);
     const int nsteps = static_cast<int>(p.w.n / 32);
-    int stage = 0, flip = 0, nb = 0;
+    int stage = 0, nb = 0;
     uint32_t phase = 0, staged = 0xffffffffu;
-    for (uint32_t u = u_begin; u < u_end; ++u, flip ^= 1) {
+
+    // Scales and zero points are read a chunk ahead of their use, across units
+    // too: fu and fc are the unit and the chunk to read them for next.
+    RowScales<SPG, ZEROS> next[4];
+    uint32_t fu = u_begin, fat[4];  // fat: this lane's four rows (the last one for rows that are not there)
+    int64_t fbase = 0;
+    int fc = 0, fchunk = 0;
+    auto fetch_seek = [&] {
+        for (; fu < u_end; ++fu) {
+            const uint32_t set = fu / upers, tile = fu % upers * parts + part_no;
+            const int e = matrix_of(set);
+            if (own == 0 || e < 0 || tile >= tiles) continue;
+            const int64_t left = p.w.m - 1 - static_cast<int64_t>(tile) * kTileRows;  // rows behind the tile's first
+            const int last = static_cast<int>(min(left, static_cast<int64_t>(kTileRows - 1)));
+            fbase = (e * p.w.m + static_cast<int64_t>(tile) * kTileRows) * p.w.gs;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fat[i] = static_cast<uint32_t>(min(g + 8 * i, last)) * static_cast<uint32_t>(p.w.gs);
+            fchunk = kwarp * KS + rank;
+            return;
+        }
+    };
+    auto fetch = [&] {
+        if (fu >= u_end) return;
+        const int grp = SPG == kSteps ? fchunk / (spg / kSteps) : fchunk * (kSteps / (SPG ? SPG : 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            next[i].load(p.w.scales + fbase + (fat[i] + grp), p.w.zeros + fbase + (fat[i] + grp),
+                         static_cast<int>(p.w.gs) - grp, p.vec);
+        fchunk += kw * KS;
+        if (++fc == own) {
+            fc = 0;
+            ++fu;
+            fetch_seek();
+        }
+    };
+    if constexpr (TMA) {
+        fetch_seek();
+        fetch();
+    }
+
+    for (uint32_t u = u_begin; u < u_end; ++u) {
         const uint32_t set = u / upers, tile = u % upers * parts + part_no;
         const bool some = matrix_of(set) >= 0;
         if (set != staged) {
@@ -535,30 +593,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             // lanes of vectors that the set does not have read zeros
             const int xstep = g < nb ? nb * 64 : 0;
             if constexpr (TMA) {
-                // this lane's rows, or the last one for those that are not there
-                const int last = rows - 1;  // of this matrix, less g
-                const uint32_t gs = static_cast<uint32_t>(p.w.gs);
-                const int64_t at0 = (row0 + min(last, 0)) * p.w.gs;
-                uint32_t at[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) at[i] = static_cast<uint32_t>(max(min(8 * i, last), 0)) * gs;
-                RowScales<SPG, ZEROS> next[4];
-                auto fetch = [&](int chunk) {
-                    const int grp = SPG == 8 ? chunk / (spg / 8) : chunk * (kSteps / SPG);
-                    const uint16_t *scales = p.w.scales + at0 + grp;
-                    const uint8_t *zeros = p.w.zeros + at0 + grp;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        next[i].load(scales + at[i], zeros + at[i], static_cast<int>(gs) - grp, p.vec);
-                };
-                if (own > 0) fetch(kwarp * KS + rank);
                 for (int c = 0; c < own; ++c) {
                     const int l = kwarp + c * kw, chunk = l * KS + rank;
                     const int steps = min(kSteps, nsteps - chunk * kSteps);
                     RowScales<SPG, ZEROS> here[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) here[i] = next[i];
-                    if (c + 1 < own) fetch(chunk + kw * KS);
+                    fetch();
                     if (!dead) {
                         const bool ok = mbar_wait(&full[stage], phase, &abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x31,
                                                   p.wait_ns);
@@ -583,70 +624,97 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int l = kwarp + c * kw, chunk = l * KS + rank;
                     const int steps = static_cast<int>(min(static_cast<int64_t>(kSteps),
                                                            (p.w.n - static_cast<int64_t>(chunk) * kChunk + 31) / 32));
-                    uint32_t words[kSteps][4];
-#pragma unroll
-                    for (int st = 0; st < kSteps; ++st)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            words[st][i] = st < steps && 8 * i < rows
-                                               ? word_at(p, (row0 + 8 * i) * p.w.pitch +
-                                                                static_cast<int64_t>(chunk) * (kChunk / 2) + st * 16 + q * 4)
-                                               : 0u;
                     const uint8_t *xs = g < nb ? sx + l * kSteps * nb * 64 + lane * 16 : nothing;
+                    // all loads of 8 steps before their use
+                    for (int s0 = 0; s0 < steps; s0 += 8) {
+                        uint32_t words[8][4];
 #pragma unroll
-                    for (int st = 0; st < kSteps; ++st) {
-                        if (st < steps) {
-                            const int grp = (chunk * kSteps + st) / spg;
-                            RowScales<0, ZEROS> here[4];
+                        for (int st = 0; st < 8; ++st)
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                here[i].load(p.w.scales + row_at(8 * i) * p.w.gs + grp,
-                                             p.w.zeros + row_at(8 * i) * p.w.gs + grp, 1, 0);
-                            const Unpack<BF16> un[4] = {Unpack<BF16>(here[0].zero(0)), Unpack<BF16>(here[1].zero(0)),
-                                                        Unpack<BF16>(here[2].zero(0)), Unpack<BF16>(here[3].zero(0))};
-                            const float scale[4] = {H::get(here[0].scale(0)), H::get(here[1].scale(0)),
-                                                    H::get(here[2].scale(0)), H::get(here[3].scale(0))};
-                            const uint4 x = *reinterpret_cast<const uint4 *>(xs);
-                            xs += xstep;
-                            float sum[2][4];
-                            step32<BF16, true>(sum, words[st], un, x);
-                            add_scaled(total, sum, scale);
+                                words[st][i] = s0 + st < steps && 8 * i < rows
+                                                   ? word_at(p, (row0 + 8 * i) * p.w.pitch + static_cast<int64_t>(chunk) * (kChunk / 2) +
+                                                                    (s0 + st) * 16 + q * 4)
+                                                   : 0u;
+#pragma unroll
+                        for (int st = 0; st < 8; ++st) {
+                            if (s0 + st < steps) {
+                                const int grp = (chunk * kSteps + s0 + st) / spg;
+                                RowScales<0, ZEROS> here[4];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    here[i].load(p.w.scales + row_at(8 * i) * p.w.gs + grp,
+                                                 p.w.zeros + row_at(8 * i) * p.w.gs + grp, 1, 0);
+                                const Unpack<BF16> un[4] = {Unpack<BF16>(here[0].zero(0)), Unpack<BF16>(here[1].zero(0)),
+                                                            Unpack<BF16>(here[2].zero(0)), Unpack<BF16>(here[3].zero(0))};
+                                const float scale[4] = {H::get(here[0].scale(0)), H::get(here[1].scale(0)),
+                                                        H::get(here[2].scale(0)), H::get(here[3].scale(0))};
+                                const uint4 x = *reinterpret_cast<const uint4 *>(xs);
+                                xs += xstep;
+                                float sum[2][4];
+                                step32<BF16, true>(sum, words[st], un, x);
+                                add_scaled(total, sum, scale);
+                            }
                         }
                     }
                 }
             }
         }
 
-        // ---- join: warps, then the cluster's CTAs
-        __syncthreads();  // everyone has read the previous unit's sums
-        float *mine = part + warp * sums;
+        // ---- join: the last of a tile's warps to get here adds their sums up;
+        // none waits, but to reuse a buffer that is not joined yet
+        const int v = static_cast<int>(u - u_begin), flip = v & 1;
+        if (v >= 2 && !wait_finished(&finished[flip][part_no], v >> 1, &abort_flag, p, lane)) dead = true;
+        float *mine = part + (flip * kWarps + warp) * sums;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {  // row g + 8 (i / 2), vector 2 q + i % 2
-            const int v = 2 * q + (i & 1);
-            if (v < nb) mine[(g + 8 * (i >> 1)) * nb + v] = total[i >> 2][i & 3];
+            const int col = 2 * q + (i & 1);
+            if (col < nb) mine[(g + 8 * (i >> 1)) * nb + col] = total[i >> 2][i & 3];
         }
-        __syncthreads();
-        if (KS == 1) {
-            put(u, part, kw * sums, sums, kw);
-        } else {
-            if (u > u_begin) {  // the previous unit's sums have arrived
-                cluster_wait();
-                if (rank == 0) put(u - 1, red + (flip ^ 1) * KS * parts * sums, sums, parts * sums, KS);
-            }
-            for (int o = tid; o < parts * kTileRows * nb; o += kThreads) {
-                const int t = o / (kTileRows * nb), r = o % (kTileRows * nb);
+        __threadfence_block();
+        __syncwarp();
+        int last = 0;
+        if (lane == 0) last = atomicAdd(&arrived[flip][part_no], 1) == kw - 1;
+        if (__shfl_sync(0xffffffffu, last, 0)) {
+            __threadfence_block();
+            if (lane == 0) arrived[flip][part_no] = 0;
+            const float *from = part + (flip * kWarps + part_no * kw) * sums;
+            float *slot = slots + ((v / kBatch % 2 * kBatch + v % kBatch) * parts + part_no) * sums;
+            for (int o = lane; o < kTileRows * nb; o += 32) {
                 float sum = 0.0f;
-                for (int w = 0; w < kw; ++w) sum += part[(t * kw + w) * sums + r];
-                st_shared_cluster(mapa_shared(smem_u32(red + ((flip * KS + rank) * parts + t) * sums + r), 0), sum);
+#pragma unroll 4
+                for (int w = 0; w < kw; ++w) sum += from[w * sums + o];
+                if (KS == 1)
+                    put(set, tile, nb, o, sum);
+                else
+                    slot[o] = sum;
             }
+            __threadfence_block();
             __syncwarp();
-            cluster_arrive();
+            if (lane == 0) finished[flip][part_no] = (v >> 1) + 1;
+        }
+        if (KS > 1 && (v % kBatch == kBatch - 1 || u + 1 == u_end)) {
+            // the batch's sums are in the CTAs of the cluster: each adds up its
+            // share of the units, and the next batch goes to the other slots
+            __syncwarp();
+            cluster_sync();
+            const int v0 = v / kBatch * kBatch;
+            for (int i = rank; i <= v - v0; i += KS) {
+                const uint32_t bu = u_begin + v0 + i, bset = bu / upers;
+                const int bnb = vectors_of(bset), per = kTileRows * bnb;
+                for (int o = tid; o < parts * per; o += kThreads) {
+                    const int t = o / per;
+                    const uint32_t at = smem_u32(slots + ((v / kBatch % 2 * kBatch + i) * parts + t) * sums + o % per);
+                    float sum = 0.0f;
+                    for (int r = 0; r < KS; ++r) sum += ld_shared_cluster(mapa_shared(at, r));
+                    put(bset, bu % upers * parts + t, bnb, o % per, sum);
+                }
+            }
         }
     }
-    if (KS > 1 && u_end > u_begin) {
+    if (KS > 1) {  // no CTA leaves while another reads its sums
         __syncwarp();
-        cluster_wait();
-        if (rank == 0) put(u_end - 1, red + (flip ^ 1) * KS * parts * sums, sums, parts * sums, KS);
+        cluster_sync();
     }
     if (TMA && dead && lane == 0) {  // loads in flight land before the CTA leaves
         const uint64_t t0 = globaltimer_ns();
@@ -671,13 +739,13 @@ int launched(const char *what) {
 }
 
 constexpr int kMaxSmem = 227 * 1024 - 1024;  // dynamic shared memory of the GEMV kernel, static beside it
-constexpr int64_t kMaxXBytes = 56 * 1024;    // of its staged vectors
+constexpr int64_t kMaxXBytes = 40 * 1024;    // of its staged vectors
 
 // Its shared memory for KS CTAs and kw warps of each a tile; sets the
 // vectors' bytes.
 size_t gemv_smem(GemvArgs &p, bool tma, int KS, int kw, int64_t local) {
     p.x_bytes = static_cast<int>(local * kChunk * p.width * 2);
-    return p.x_bytes + (kWarps + 2 * KS * (kWarps / kw)) * kTileRows * p.width * 4 + kWarps * kStages * ((tma ? kChunkBytes : 0) + 8) + 16 +
+    return p.x_bytes + 2 * (kWarps + (KS > 1 ? kBatch * (kWarps / kw) : 0)) * kTileRows * p.width * 4 + kWarps * kStages * ((tma ? kChunkBytes : 0) + 8) + 16 +
            (p.index ? sizeof(Table) : 0) + 1024;
 }
 
@@ -714,6 +782,7 @@ GemvKernel gemv_kernel(int spg) {
         case 2: return w4_gemv_kernel<BF16, ZEROS, 2>;
         case 4: return w4_gemv_kernel<BF16, ZEROS, 4>;
         case 8: return w4_gemv_kernel<BF16, ZEROS, 8>;
+        case 16: return w4_gemv_kernel<BF16, ZEROS, 16>;
         default: return w4_gemv_kernel<BF16, ZEROS, 0>;
     }
 }
@@ -740,7 +809,7 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
     cfg.numAttrs = 1;
     {
         static std::mutex mu;
-        static bool ready[2][2][9][64];
+        static bool ready[2][2][17][64];
         std::lock_guard<std::mutex> lock(mu);
         bool &done = ready[bf16][zeros][spg][h->device & 63];
         if (!done) {
@@ -749,31 +818,32 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
             done = true;
         }
     }
-    // Split a tile's columns over the CTAs of a cluster where that takes the
-    // fewest turns: chunks that a warp computes one after another, and about
-    // one more for each unit's start and joining.
+    // Share a tile's columns among KS CTAs of a cluster and kw warps of each so
+    // that the turns take least: the chunks that a warp computes one after
+    // another, and about as much as one for each tile's joining.
     int best = 0, best_grid = 0, best_kw = 0;
     double best_time = 0;
     for (int KS = 1; KS <= 8 && (KS == 1 || KS < 2 * chunks); KS *= 2) {
         const int64_t local = (chunks + KS - 1) / KS;
         if (local * kChunk * p.width * 2 > kMaxXBytes) continue;
-        int kw = kWarps;
-        while (kw / 2 >= local) kw /= 2;
-        attr[0].val.clusterDim.x = KS;
-        cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, KS, kw, local);
-        if (cfg.dynamicSmemBytes > static_cast<size_t>(kMaxSmem)) continue;
-        const int64_t clusters = resident_clusters(h, fn, cfg, KS);
-        const int64_t units = sets * ((tiles + kWarps / kw - 1) / (kWarps / kw));
-        const double time = static_cast<double>((units + clusters - 1) / clusters) *
-                            (static_cast<double>((local + kw - 1) / kw) + 1.0);
-        if (!best || time < best_time) {
-            best = KS;
-            best_kw = kw;
-            best_time = time;
-            best_grid = static_cast<int>(units < clusters ? units : clusters);
+        for (int kw = kWarps; kw >= 1; kw /= 2) {
+            if (kw / 2 >= local) continue;
+            attr[0].val.clusterDim.x = KS;
+            cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, KS, kw, local);
+            if (cfg.dynamicSmemBytes > static_cast<size_t>(kMaxSmem)) continue;
+            const int64_t clusters = resident_clusters(h, fn, cfg, KS);
+            const int64_t units = sets * ((tiles + kWarps / kw - 1) / (kWarps / kw));
+            const double time = static_cast<double>((units + clusters - 1) / clusters) *
+                                (static_cast<double>((local + kw - 1) / kw) + 1.0);
+            if (!best || time < best_time) {
+                best = KS;
+                best_kw = kw;
+                best_time = time;
+                best_grid = static_cast<int>(units < clusters ? units : clusters);
+            }
         }
     }
-    if (!best) return b2b::fail(B2B_ERR_NOT_SUPPORTED, "4-bit GEMV: rows longer than 229376 columns");
+    if (!best) return b2b::fail(B2B_ERR_NOT_SUPPORTED, "4-bit GEMV: rows longer than 163840 columns");
     const int64_t local = (chunks + best - 1) / best;
     p.kw = best_kw;
     attr[0].val.clusterDim.x = best;
@@ -823,15 +893,15 @@ int launch_hgemv_w4(b2b_handle *h, int type, size_t groups, size_t m, size_t n, 
     const bool bf16 = type == B2B_TYPE_BF16;
     // steps of a group that the TMA-fed kernel is made for
     int spg = static_cast<int>(group / 32);
-    if (spg % 8 == 0) spg = 8;
-    const bool tma = n % 32 == 0 && aligned16(packed) && rows < (1ll << 31) && (spg == 1 || spg == 2 || spg == 4 || spg == 8);
+    if (spg % kSteps == 0) spg = kSteps;
+    const bool tma = n % 32 == 0 && aligned16(packed) && rows < (1ll << 31) && kSteps % spg == 0;
     if (!tma) spg = 0;
     CUtensorMap tmW{};
     if (tma) {
-        if (int rc = encode_tma_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, packed, rows, p.w.pitch, kChunk / 2,
+        if (int rc = encode_tma_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, packed, rows, p.w.pitch, kBoxCols / 2,
                                    kTileRows))
             return rc;
-        const int64_t per = 8 / spg;  // groups of a chunk
+        const int64_t per = kSteps / spg;  // groups of a chunk
         p.vec = p.w.gs % per == 0 && aligned16(scales) && aligned16(zeros);
     }
     const int64_t all = static_cast<int64_t>(count);
