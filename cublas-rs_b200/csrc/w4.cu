@@ -110,12 +110,13 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(W4Args p, uint16_t *
 // bits.
 //
 //   * A tile is 32 rows of W for one set of vectors; its n columns are cut
-//     into chunks of 512 (256 bytes of a row), which the CTAs of a cluster
-//     and kw of a CTA's 8 warps take in turn; the 8 / kw parts of a CTA have
+//     into chunks of 256 or 512 (a box or two), which the CTAs of a cluster
+//     and kw of a CTA's 16 warps take in turn; the 16 / kw parts of a CTA have
 //     a tile each.  A unit is those tiles.
-//   * Each warp keeps its own ring of chunks (two boxes of 32 rows x 128
-//     bytes, 128-byte swizzle) filled by TMA ahead of its use, across units, so
-//     nothing drains at a unit's end; 8 warps x 2 chunks are 128 KiB in flight.
+//   * Each warp holds one chunk (boxes of 32 rows x 128 bytes, 128-byte
+//     swizzle); TMA refills a box with the next chunk's as soon as it is used
+//     up, across units, so nothing drains at a unit's end.  16 warps hold
+//     128 KiB of W, in flight or in use.
 //   * The vectors are staged once for each set, each 8 columns reordered to
 //     the pairs (0,4) (1,5) (2,6) (3,7) that the words unpack to.
 //   * The last of a tile's warps to arrive adds their sums up while the others
@@ -124,15 +125,12 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(W4Args p, uint16_t *
 // Rows that TMA cannot describe (n not a multiple of 32, packed not 16-byte
 // aligned) and groups that do not fit a chunk evenly are read by the same
 // kernel with plain loads (SPG = 0).
-constexpr int kWarps = 8;
+constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTileRows = 32;
-constexpr int kChunk = 512;                       // columns, as two boxes
-constexpr int kSteps = kChunk / 32;               // of 32 columns
-constexpr int kChunkBytes = kTileRows * kChunk / 2;
 constexpr int kBoxCols = 256;                     // 128 bytes of a row
+constexpr int kBoxSteps = kBoxCols / 32;          // of 32 columns
 constexpr int kBoxBytes = kTileRows * kBoxCols / 2;
-constexpr int kStages = 2;                        // chunks of a warp's ring
 constexpr int kBatch = 8;                         // units that the CTAs of a cluster join at once
 constexpr int kMaxIndexed = 256;                  // products of one launch that choose their matrix
 
@@ -146,8 +144,9 @@ struct GemvArgs {
     int matrices, count, fan, first;  // first: number of this launch's first product
     int width;    // vectors of a set: 8, or fewer where longer rows leave room for fewer
     int kw;       // warps that share a tile
+    int boxes;    // of a chunk: 1 or 2
     int x_bytes;  // of the staged vectors
-    int vec;      // a chunk's scales and zero points of a row are one aligned word each
+    int vec;      // a box's scales and zero points of a row are one aligned word each
     float alpha, beta;
     int64_t total;  // bytes of packed
 };
@@ -272,10 +271,10 @@ __device__ __forceinline__ void add_scaled(float (&total)[2][4], const float (&s
         total[i >> 2][i & 3] = fmaf(scale[i >> 1], sum[i >> 2][i & 3], total[i >> 2][i & 3]);
 }
 
-// Scales and zero points of one row's groups in a chunk (at most 16).
+// Scales and zero points of one row's groups in a box (at most 8).
 template <int SPG, bool ZEROS>
 struct RowScales {
-    static constexpr int N = SPG ? kSteps / SPG : 1;
+    static constexpr int N = SPG ? kBoxSteps / SPG : 1;
     uint32_t s[(N + 1) / 2];
     uint32_t z[(N + 3) / 4];
     template <int WORDS>
@@ -319,19 +318,19 @@ struct RowScales {
     __device__ __forceinline__ uint32_t zero(int i) const { return ZEROS ? z[i / 4] >> (8 * (i & 3)) & 15u : 8u; }
 };
 
-// A chunk's products, its words at shared address w, the vectors' pieces of
-// its first step at x.  FULL: it has all its steps.
+// A box's products, its words at shared address w, the vectors' pieces of its
+// first step at x.  FULL: it has all its steps.
 template <bool BF16, bool ZEROS, int SPG, bool FULL>
-__device__ __forceinline__ void chunk_products(float (&total)[2][4], uint32_t w, uint32_t x, int xstep,
-                                               const RowScales<SPG, ZEROS> (&here)[4], int steps) {
+__device__ __forceinline__ void box_products(float (&total)[2][4], uint32_t w, uint32_t x, int xstep,
+                                             const RowScales<SPG, ZEROS> (&rows)[4], int steps) {
     using H = b2b::Half16<BF16>;
 #pragma unroll
-    for (int gi = 0; gi < kSteps / SPG; ++gi) {
+    for (int gi = 0; gi < kBoxSteps / SPG; ++gi) {
         if (!FULL && gi * SPG >= steps) break;
-        const Unpack<BF16> un[4] = {Unpack<BF16>(here[0].zero(gi)), Unpack<BF16>(here[1].zero(gi)),
-                                    Unpack<BF16>(here[2].zero(gi)), Unpack<BF16>(here[3].zero(gi))};
-        const float scale[4] = {H::get(here[0].scale(gi)), H::get(here[1].scale(gi)), H::get(here[2].scale(gi)),
-                                H::get(here[3].scale(gi))};
+        const Unpack<BF16> un[4] = {Unpack<BF16>(rows[0].zero(gi)), Unpack<BF16>(rows[1].zero(gi)),
+                                    Unpack<BF16>(rows[2].zero(gi)), Unpack<BF16>(rows[3].zero(gi))};
+        const float scale[4] = {H::get(rows[0].scale(gi)), H::get(rows[1].scale(gi)), H::get(rows[2].scale(gi)),
+                                H::get(rows[3].scale(gi))};
         float sum[2][4];
 #pragma unroll
         for (int si = 0; si < SPG; ++si) {
@@ -341,7 +340,7 @@ __device__ __forceinline__ void chunk_products(float (&total)[2][4], uint32_t w,
             x += xstep;
             uint32_t words[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) words[i] = lds32((w ^ ((st & 7) << 4)) + (st >> 3) * kBoxBytes + i * 1024);
+            for (int i = 0; i < 4; ++i) words[i] = lds32((w ^ (st << 4)) + i * 1024);
             if (si == 0)
                 step32<BF16, true>(sum, words, un, xv);
             else
@@ -370,7 +369,7 @@ __device__ __forceinline__ bool wait_finished(const volatile int *count, int wan
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
-// SPG: steps of 32 columns in a group, 16 standing for its multiples; 0: plain
+// SPG: steps of 32 columns in a group, 8 standing for its multiples; 0: plain
 // loads, any group.
 template <bool BF16, bool ZEROS, int SPG>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -387,14 +386,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int g = lane >> 2, q = lane & 3;
     const int KS = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
     const int kw = p.kw, parts = kWarps / kw, part_no = warp / kw, kwarp = warp % kw;
-    uint8_t *ring = smem + (TMA ? warp * kStages * kChunkBytes : 0);
-    uint8_t *sx = smem + (TMA ? kWarps * kStages * kChunkBytes : 0);
+    uint8_t *ring = smem + (TMA ? warp * 2 * kBoxBytes : 0);
+    uint8_t *sx = smem + (TMA ? kWarps * 2 * kBoxBytes : 0);
     const int sums = kTileRows * p.width;                     // of a tile
     float *part = reinterpret_cast<float *>(sx + p.x_bytes);  // [2][kWarps][32 rows][width]
     float *slots = part + 2 * kWarps * sums;                  // KS > 1: [2][kBatch][parts][32 rows][width]
     uint64_t *bars = reinterpret_cast<uint64_t *>(slots + (KS > 1 ? 2 * kBatch * parts * sums : 0));
-    uint64_t *full = bars + warp * kStages;
-    uint8_t *nothing = reinterpret_cast<uint8_t *>(bars + kWarps * kStages);  // 16 bytes of 0
+    uint64_t *full = bars + warp * 2;  // of its chunk's two boxes
+    uint8_t *nothing = reinterpret_cast<uint8_t *>(bars + kWarps * 2);  // 16 bytes of 0
     Table *table = reinterpret_cast<Table *>(nothing + 16);
     const Item *items = table->item;
 
@@ -403,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid < 4) reinterpret_cast<uint32_t *>(nothing)[tid] = 0;
     if (tid < 2 * kWarps) arrived[tid / kWarps][tid % kWarps] = finished[tid / kWarps][tid % kWarps] = 0;
     if (TMA && lane == 0) {
-        for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1);
+        for (int b = 0; b < 2; ++b) mbar_init(&full[b], 1);
         fence_barrier_init();
     }
     if (p.index) {
@@ -445,7 +444,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tiles = static_cast<uint32_t>((p.w.m + kTileRows - 1) / kTileRows);
     const uint32_t upers = (tiles + parts - 1) / parts;  // units of a set
     const uint32_t sets = p.index ? table->items : (p.count + p.width - 1) / p.width;
-    const int chunks = static_cast<int>((p.w.n + kChunk - 1) / kChunk);
+    const int steps_of = p.boxes * kBoxSteps, cols_of = p.boxes * kBoxCols;  // of a chunk
+    const int chunks = static_cast<int>((p.w.n + cols_of - 1) / cols_of);
     const int local = chunks > rank ? (chunks - rank + KS - 1) / KS : 0;   // this CTA's chunks of a tile
     const int own = local > kwarp ? (local - kwarp + kw - 1) / kw : 0;     // this warp's
     const uint32_t clusters = gridDim.x / KS, cluster = blockIdx.x / KS;
@@ -457,40 +457,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto matrix_of = [&](uint32_t set) { return p.index ? items[set].matrix : 0; };
 
     bool dead = false;
-    // The loads run kStages chunks ahead of their use: iu and ic are the unit
-    // and the chunk (of this warp's) to load next, at byte icol of row irow.
-    uint32_t iu = u_begin;
-    int ic = 0, irow = 0, icol = 0, istage = 0;
-    auto seek = [&] {  // the first unit from iu on in which this warp has chunks
-        for (; iu < u_end; ++iu) {
-            const uint32_t set = iu / upers, tile = iu % upers * parts + part_no;
-            const int e = matrix_of(set);
-            if (own == 0 || e < 0 || tile >= tiles) continue;
-            irow = static_cast<int>(e * p.w.m + tile * kTileRows);
-            icol = (kwarp * KS + rank) * (kChunk / 2);
-            return;
-        }
-    };
-    auto issue = [&] {
-        if (iu >= u_end || dead) return;
-        if (lane == 0) {
-            mbar_arrive_expect_tx(&full[istage], kChunkBytes);
-            tma_load_2d(ring + istage * kChunkBytes, &tmW, &full[istage], icol, irow);
-            tma_load_2d(ring + istage * kChunkBytes + kBoxBytes, &tmW, &full[istage], icol + kBoxCols / 2, irow);
-        }
-        istage ^= 1;
-        icol += kw * KS * (kChunk / 2);
-        if (++ic == own) {
-            ic = 0;
-            ++iu;
-            seek();
-        }
-    };
-    if constexpr (TMA) {
-        seek();
-        for (int s = 0; s < kStages; ++s) issue();
-    }
-
     auto vectors_of = [&](uint32_t set) {
         return p.index ? items[set].count
                        : static_cast<int>(min(static_cast<int64_t>(p.width), p.count - static_cast<int64_t>(set) * p.width));
@@ -508,46 +474,60 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     const int spg = static_cast<int>(p.w.group / 32);
     const int nsteps = static_cast<int>(p.w.n / 32);
-    int stage = 0, nb = 0;
+    int nb = 0;
     uint32_t phase = 0, staged = 0xffffffffu;
 
-    // Scales and zero points are read a chunk ahead of their use, across units
-    // too: fu and fc are the unit and the chunk to read them for next.
-    RowScales<SPG, ZEROS> next[4];
-    uint32_t fu = u_begin, fat[4];  // fat: this lane's four rows (the last one for rows that are not there)
-    int64_t fbase = 0;
-    int fc = 0, fchunk = 0;
-    auto fetch_seek = [&] {
-        for (; fu < u_end; ++fu) {
-            const uint32_t set = fu / upers, tile = fu % upers * parts + part_no;
+    // The warp's next chunk, in this unit or a later one: as soon as a box of
+    // the present chunk is used up, the next chunk's takes its place, and the
+    // scales and zero points that belong to it are read.
+    RowScales<SPG, ZEROS> scales[2][4];
+    uint32_t nu = u_begin, nat[4];  // nat: this lane's four rows (the last one for rows that are not there)
+    int64_t nbase = 0;
+    int nc = 0, nchunk = 0, nrow = 0;
+    auto seek = [&] {
+        for (; nu < u_end; ++nu) {
+            const uint32_t set = nu / upers, tile = nu % upers * parts + part_no;
             const int e = matrix_of(set);
             if (own == 0 || e < 0 || tile >= tiles) continue;
+            const int64_t row = e * p.w.m + static_cast<int64_t>(tile) * kTileRows;
             const int64_t left = p.w.m - 1 - static_cast<int64_t>(tile) * kTileRows;  // rows behind the tile's first
             const int last = static_cast<int>(min(left, static_cast<int64_t>(kTileRows - 1)));
-            fbase = (e * p.w.m + static_cast<int64_t>(tile) * kTileRows) * p.w.gs;
+            nrow = static_cast<int>(row);
+            nbase = row * p.w.gs;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fat[i] = static_cast<uint32_t>(min(g + 8 * i, last)) * static_cast<uint32_t>(p.w.gs);
-            fchunk = kwarp * KS + rank;
+            for (int i = 0; i < 4; ++i) nat[i] = static_cast<uint32_t>(min(g + 8 * i, last)) * static_cast<uint32_t>(p.w.gs);
+            nchunk = kwarp * KS + rank;
             return;
         }
     };
-    auto fetch = [&] {
-        if (fu >= u_end) return;
-        const int grp = SPG == kSteps ? fchunk / (spg / kSteps) : fchunk * (kSteps / (SPG ? SPG : 1));
+    auto load = [&](int b) {
+        if (nu >= u_end || dead) return;
+        if (lane == 0) {
+            mbar_arrive_expect_tx(&full[b], kBoxBytes);
+            tma_load_2d(ring + b * kBoxBytes, &tmW, &full[b], nchunk * (cols_of / 2) + b * (kBoxCols / 2), nrow);
+        }
+        // a box behind the row's end loads zeros and has no groups
+        const int step = nchunk * steps_of + b * kBoxSteps;
+        if (step >= nsteps) return;
+        const int grp = SPG == kBoxSteps ? step / spg : step / (SPG ? SPG : 1);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            next[i].load(p.w.scales + fbase + (fat[i] + grp), p.w.zeros + fbase + (fat[i] + grp),
-                         static_cast<int>(p.w.gs) - grp, p.vec);
-        fchunk += kw * KS;
-        if (++fc == own) {
-            fc = 0;
-            ++fu;
-            fetch_seek();
+            scales[b][i].load(p.w.scales + nbase + (nat[i] + grp), p.w.zeros + nbase + (nat[i] + grp),
+                              static_cast<int>(p.w.gs) - grp, p.vec);
+    };
+    auto advance = [&] {
+        nchunk += kw * KS;
+        if (++nc == own) {
+            nc = 0;
+            ++nu;
+            seek();
         }
     };
     if constexpr (TMA) {
-        fetch_seek();
-        fetch();
+        seek();
+        load(0);
+        if (p.boxes == 2) load(1);
+        advance();
     }
 
     for (uint32_t u = u_begin; u < u_end; ++u) {
@@ -559,11 +539,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncthreads();  // everyone is done with the old vectors
             if (some) {
                 // 8 columns of one vector a turn; local chunk l is chunk l * KS + rank
-                const int per = kChunk / 8 * nb;
+                const int octs = cols_of / 8, per = octs * nb;
                 for (int i = tid; i < local * per; i += kThreads) {
                     const int l = i / per, r = i % per;
-                    const int b = r / (kChunk / 8), oct = r % (kChunk / 8);  // lanes along a vector
-                    const int64_t j = (static_cast<int64_t>(l) * KS + rank) * kChunk + oct * 8;
+                    const int b = r / octs, oct = r % octs;  // lanes along a vector
+                    const int64_t j = (static_cast<int64_t>(l) * KS + rank) * cols_of + oct * 8;
                     const int64_t v = (p.index ? p.first + items[set].member[b]
                                                : static_cast<int64_t>(set) * p.width + b) / p.fan;
                     const uint16_t *src = p.x + v * p.w.n + j;
@@ -580,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     o.z = h[2] | static_cast<uint32_t>(h[6]) << 16;
                     o.w = h[3] | static_cast<uint32_t>(h[7]) << 16;
                     // step (oct / 4), vector b, quarter oct % 4
-                    *reinterpret_cast<uint4 *>(sx + ((l * kSteps + (oct >> 2)) * nb + b) * 64 + (oct & 3) * 16) = o;
+                    *reinterpret_cast<uint4 *>(sx + ((l * steps_of + (oct >> 2)) * nb + b) * 64 + (oct & 3) * 16) = o;
                 }
             }
             __syncthreads();
@@ -595,36 +575,36 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (TMA) {
                 for (int c = 0; c < own; ++c) {
                     const int l = kwarp + c * kw, chunk = l * KS + rank;
-                    const int steps = min(kSteps, nsteps - chunk * kSteps);
-                    RowScales<SPG, ZEROS> here[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) here[i] = next[i];
-                    fetch();
-                    if (!dead) {
-                        const bool ok = mbar_wait(&full[stage], phase, &abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x31,
-                                                  p.wait_ns);
-                        dead = !__all_sync(0xffffffffu, ok);
+                    for (int b = 0; b < 2; ++b) {
+                        if (b && p.boxes == 1) break;
+                        const int steps = nsteps - chunk * steps_of - b * kBoxSteps;
+                        if (!dead) {
+                            const bool ok = mbar_wait(&full[b], phase, &abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x31,
+                                                      p.wait_ns);
+                            dead = !__all_sync(0xffffffffu, ok);
+                        }
+                        // 16-byte piece st of row r sits at piece st ^ (r % 8)
+                        const uint32_t w = smem_u32(ring) + b * kBoxBytes + g * 128 + (g << 4) + q * 4;
+                        const uint32_t xs = g < nb ? smem_u32(sx) + (l * steps_of + b * kBoxSteps) * nb * 64 + lane * 16
+                                                   : smem_u32(nothing);
+                        if (steps >= kBoxSteps)
+                            box_products<BF16, ZEROS, SPG, true>(total, w, xs, xstep, scales[b], steps);
+                        else if (steps > 0)
+                            box_products<BF16, ZEROS, SPG, false>(total, w, xs, xstep, scales[b], steps);
+                        __syncwarp();
+                        load(b);
                     }
-                    // 16-byte piece st of row r sits at piece st ^ (r % 8)
-                    const uint32_t w = smem_u32(ring) + stage * kChunkBytes + g * 128 + (g << 4) + q * 4;
-                    const uint32_t xs = g < nb ? smem_u32(sx) + l * kSteps * nb * 64 + lane * 16 : smem_u32(nothing);
-                    if (steps == kSteps)
-                        chunk_products<BF16, ZEROS, SPG, true>(total, w, xs, xstep, here, steps);
-                    else
-                        chunk_products<BF16, ZEROS, SPG, false>(total, w, xs, xstep, here, steps);
-                    __syncwarp();
-                    phase ^= stage;
-                    stage ^= 1;
-                    issue();
+                    phase ^= 1u;
+                    advance();
                 }
             } else {
                 // a row of this lane, or the last one for one that is not there
                 auto row_at = [&](int i) { return row0 + min(i, rows - 1); };
                 for (int c = 0; c < own; ++c) {
                     const int l = kwarp + c * kw, chunk = l * KS + rank;
-                    const int steps = static_cast<int>(min(static_cast<int64_t>(kSteps),
-                                                           (p.w.n - static_cast<int64_t>(chunk) * kChunk + 31) / 32));
-                    const uint8_t *xs = g < nb ? sx + l * kSteps * nb * 64 + lane * 16 : nothing;
+                    const int steps = min(steps_of, static_cast<int>((p.w.n + 31) / 32) - chunk * steps_of);
+                    const uint8_t *xs = g < nb ? sx + l * steps_of * nb * 64 + lane * 16 : nothing;
                     // all loads of 8 steps before their use
                     for (int s0 = 0; s0 < steps; s0 += 8) {
                         uint32_t words[8][4];
@@ -633,13 +613,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
                                 words[st][i] = s0 + st < steps && 8 * i < rows
-                                                   ? word_at(p, (row0 + 8 * i) * p.w.pitch + static_cast<int64_t>(chunk) * (kChunk / 2) +
+                                                   ? word_at(p, (row0 + 8 * i) * p.w.pitch + static_cast<int64_t>(chunk) * (cols_of / 2) +
                                                                     (s0 + st) * 16 + q * 4)
                                                    : 0u;
 #pragma unroll
                         for (int st = 0; st < 8; ++st) {
                             if (s0 + st < steps) {
-                                const int grp = (chunk * kSteps + s0 + st) / spg;
+                                const int grp = (chunk * steps_of + s0 + st) / spg;
                                 RowScales<0, ZEROS> here[4];
 #pragma unroll
                                 for (int i = 0; i < 4; ++i)
@@ -744,8 +724,8 @@ constexpr int64_t kMaxXBytes = 40 * 1024;    // of its staged vectors
 // Its shared memory for KS CTAs and kw warps of each a tile; sets the
 // vectors' bytes.
 size_t gemv_smem(GemvArgs &p, bool tma, int KS, int kw, int64_t local) {
-    p.x_bytes = static_cast<int>(local * kChunk * p.width * 2);
-    return p.x_bytes + 2 * (kWarps + (KS > 1 ? kBatch * (kWarps / kw) : 0)) * kTileRows * p.width * 4 + kWarps * kStages * ((tma ? kChunkBytes : 0) + 8) + 16 +
+    p.x_bytes = static_cast<int>(local * p.boxes * kBoxCols * p.width * 2);
+    return p.x_bytes + 2 * (kWarps + (KS > 1 ? kBatch * (kWarps / kw) : 0)) * kTileRows * p.width * 4 + kWarps * ((tma ? 2 * kBoxBytes : 0) + 16) + 16 +
            (p.index ? sizeof(Table) : 0) + 1024;
 }
 
@@ -782,7 +762,6 @@ GemvKernel gemv_kernel(int spg) {
         case 2: return w4_gemv_kernel<BF16, ZEROS, 2>;
         case 4: return w4_gemv_kernel<BF16, ZEROS, 4>;
         case 8: return w4_gemv_kernel<BF16, ZEROS, 8>;
-        case 16: return w4_gemv_kernel<BF16, ZEROS, 16>;
         default: return w4_gemv_kernel<BF16, ZEROS, 0>;
     }
 }
@@ -792,9 +771,9 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
     const GemvKernel kernel = bf16 ? (zeros ? gemv_kernel<true, true>(spg) : gemv_kernel<true, false>(spg))
                                    : (zeros ? gemv_kernel<false, true>(spg) : gemv_kernel<false, false>(spg));
     const void *fn = reinterpret_cast<const void *>(kernel);
-    const int64_t chunks = (p.w.n + kChunk - 1) / kChunk, tiles = (p.w.m + kTileRows - 1) / kTileRows;
+    const int64_t cols = (p.w.n + kBoxCols - 1) / kBoxCols, tiles = (p.w.m + kTileRows - 1) / kTileRows;
     p.width = p.count < 8 ? p.count : 8;
-    while (p.width > 1 && (chunks + 7) / 8 * kChunk * p.width * 2 > kMaxXBytes) --p.width;
+    while (p.width > 1 && (cols + 7) / 8 * kBoxCols * p.width * 2 > kMaxXBytes) --p.width;
     // with an index: the sets that it makes where it names each matrix equally often
     const int64_t each = p.index ? (p.count + p.matrices - 1) / p.matrices : p.count;
     const int64_t sets = (p.count + each - 1) / each * ((each + p.width - 1) / p.width);
@@ -809,7 +788,7 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
     cfg.numAttrs = 1;
     {
         static std::mutex mu;
-        static bool ready[2][2][17][64];
+        static bool ready[2][2][9][64];
         std::lock_guard<std::mutex> lock(mu);
         bool &done = ready[bf16][zeros][spg][h->device & 63];
         if (!done) {
@@ -818,34 +797,39 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
             done = true;
         }
     }
-    // Share a tile's columns among KS CTAs of a cluster and kw warps of each so
-    // that the turns take least: the chunks that a warp computes one after
-    // another, and about as much as one for each tile's joining.
-    int best = 0, best_grid = 0, best_kw = 0;
+    // Share a tile's columns among KS CTAs of a cluster and kw warps of each, in
+    // chunks of one box or two, so that the turns take least: the boxes that a
+    // warp computes one after another, a third of one for each chunk's
+    // bookkeeping and one for each tile's joining.
+    int best = 0, best_grid = 0, best_kw = 0, best_boxes = 0;
     double best_time = 0;
-    for (int KS = 1; KS <= 8 && (KS == 1 || KS < 2 * chunks); KS *= 2) {
-        const int64_t local = (chunks + KS - 1) / KS;
-        if (local * kChunk * p.width * 2 > kMaxXBytes) continue;
-        for (int kw = kWarps; kw >= 1; kw /= 2) {
-            if (kw / 2 >= local) continue;
-            attr[0].val.clusterDim.x = KS;
-            cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, KS, kw, local);
-            if (cfg.dynamicSmemBytes > static_cast<size_t>(kMaxSmem)) continue;
-            const int64_t clusters = resident_clusters(h, fn, cfg, KS);
-            const int64_t units = sets * ((tiles + kWarps / kw - 1) / (kWarps / kw));
-            const double time = static_cast<double>((units + clusters - 1) / clusters) *
-                                (static_cast<double>((local + kw - 1) / kw) + 1.0);
-            if (!best || time < best_time) {
-                best = KS;
-                best_kw = kw;
-                best_time = time;
-                best_grid = static_cast<int>(units < clusters ? units : clusters);
+    for (p.boxes = 1; p.boxes <= 2; ++p.boxes) {
+        const int64_t chunks = (cols + p.boxes - 1) / p.boxes;
+        for (int KS = 1; KS <= 8 && (KS == 1 || KS < 2 * chunks); KS *= 2) {
+            const int64_t local = (chunks + KS - 1) / KS;
+            if (local * p.boxes * kBoxCols * p.width * 2 > kMaxXBytes) continue;
+            for (int kw = kWarps; kw >= 1; kw /= 2) {
+                attr[0].val.clusterDim.x = KS;
+                cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, KS, kw, local);
+                if (cfg.dynamicSmemBytes > static_cast<size_t>(kMaxSmem)) continue;
+                const int64_t clusters = resident_clusters(h, fn, cfg, KS);
+                const int64_t units = sets * ((tiles + kWarps / kw - 1) / (kWarps / kw));
+                const double time = static_cast<double>((units + clusters - 1) / clusters) *
+                                    (static_cast<double>((local + kw - 1) / kw) * (p.boxes + 0.33) + 1.0);
+                if (!best || time < best_time) {
+                    best = KS;
+                    best_kw = kw;
+                    best_boxes = p.boxes;
+                    best_time = time;
+                    best_grid = static_cast<int>(units < clusters ? units : clusters);
+                }
             }
         }
     }
     if (!best) return b2b::fail(B2B_ERR_NOT_SUPPORTED, "4-bit GEMV: rows longer than 163840 columns");
-    const int64_t local = (chunks + best - 1) / best;
+    p.boxes = best_boxes;
     p.kw = best_kw;
+    const int64_t chunks = (cols + p.boxes - 1) / p.boxes, local = (chunks + best - 1) / best;
     attr[0].val.clusterDim.x = best;
     cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, best, best_kw, local);
     cfg.gridDim = dim3(best * best_grid);
@@ -893,15 +877,15 @@ int launch_hgemv_w4(b2b_handle *h, int type, size_t groups, size_t m, size_t n, 
     const bool bf16 = type == B2B_TYPE_BF16;
     // steps of a group that the TMA-fed kernel is made for
     int spg = static_cast<int>(group / 32);
-    if (spg % kSteps == 0) spg = kSteps;
-    const bool tma = n % 32 == 0 && aligned16(packed) && rows < (1ll << 31) && kSteps % spg == 0;
+    if (spg % kBoxSteps == 0) spg = kBoxSteps;
+    const bool tma = n % 32 == 0 && aligned16(packed) && rows < (1ll << 31) && kBoxSteps % spg == 0;
     if (!tma) spg = 0;
     CUtensorMap tmW{};
     if (tma) {
         if (int rc = encode_tma_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, packed, rows, p.w.pitch, kBoxCols / 2,
                                    kTileRows))
             return rc;
-        const int64_t per = kSteps / spg;  // groups of a chunk
+        const int64_t per = kBoxSteps / spg;  // groups of a box
         p.vec = p.w.gs % per == 0 && aligned16(scales) && aligned16(zeros);
     }
     const int64_t all = static_cast<int64_t>(count);
