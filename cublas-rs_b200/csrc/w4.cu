@@ -322,15 +322,22 @@ struct RowScales {
 // first step at x.  FULL: it has all its steps.
 template <bool BF16, bool ZEROS, int SPG, bool FULL>
 __device__ __forceinline__ void box_products(float (&total)[2][4], uint32_t w, uint32_t x, int xstep,
-                                             const RowScales<SPG, ZEROS> (&rows)[4], int steps) {
+                                             const RowScales<SPG, ZEROS> &row, int g, int steps) {
     using H = b2b::Half16<BF16>;
+    uint32_t sw[4], zw[4];  // of rows g, g + 8, g + 16, g + 24: two groups' scales, four groups' zero points
 #pragma unroll
     for (int gi = 0; gi < kBoxSteps / SPG; ++gi) {
         if (!FULL && gi * SPG >= steps) break;
-        const Unpack<BF16> un[4] = {Unpack<BF16>(rows[0].zero(gi)), Unpack<BF16>(rows[1].zero(gi)),
-                                    Unpack<BF16>(rows[2].zero(gi)), Unpack<BF16>(rows[3].zero(gi))};
-        const float scale[4] = {H::get(rows[0].scale(gi)), H::get(rows[1].scale(gi)), H::get(rows[2].scale(gi)),
-                                H::get(rows[3].scale(gi))};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (gi % 2 == 0) sw[i] = __shfl_sync(0xffffffffu, row.s[gi / 2], g + 8 * i);
+            if (ZEROS && gi % 4 == 0) zw[i] = __shfl_sync(0xffffffffu, row.z[gi / 4], g + 8 * i);
+        }
+        auto scale_of = [&](int i) { return H::get(static_cast<uint16_t>(gi % 2 ? sw[i] >> 16 : sw[i])); };
+        auto zero_of = [&](int i) { return ZEROS ? zw[i] >> (8 * (gi % 4)) & 15u : 8u; };
+        const Unpack<BF16> un[4] = {Unpack<BF16>(zero_of(0)), Unpack<BF16>(zero_of(1)), Unpack<BF16>(zero_of(2)),
+                                    Unpack<BF16>(zero_of(3))};
+        const float scale[4] = {scale_of(0), scale_of(1), scale_of(2), scale_of(3)};
         float sum[2][4];
 #pragma unroll
         for (int si = 0; si < SPG; ++si) {
@@ -479,11 +486,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // The warp's next chunk, in this unit or a later one: as soon as a box of
     // the present chunk is used up, the next chunk's takes its place, and the
-    // scales and zero points that belong to it are read.
-    RowScales<SPG, ZEROS> scales[2][4];
-    uint32_t nu = u_begin, nat[4];  // nat: this lane's four rows (the last one for rows that are not there)
-    int64_t nbase = 0;
+    // scales and zero points that belong to it are read, row `lane`'s by each
+    // lane (the tile's last one by lanes whose row is not there).
+    RowScales<SPG, ZEROS> scales[2];
+    uint32_t nu = u_begin;
     int nc = 0, nchunk = 0, nrow = 0;
+    const uint16_t *nscales = nullptr;
+    const uint8_t *nzeros = nullptr;
     auto seek = [&] {
         for (; nu < u_end; ++nu) {
             const uint32_t set = nu / upers, tile = nu % upers * parts + part_no;
@@ -491,11 +500,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (own == 0 || e < 0 || tile >= tiles) continue;
             const int64_t row = e * p.w.m + static_cast<int64_t>(tile) * kTileRows;
             const int64_t left = p.w.m - 1 - static_cast<int64_t>(tile) * kTileRows;  // rows behind the tile's first
-            const int last = static_cast<int>(min(left, static_cast<int64_t>(kTileRows - 1)));
+            const int64_t at = (row + min(left, static_cast<int64_t>(lane))) * p.w.gs;
             nrow = static_cast<int>(row);
-            nbase = row * p.w.gs;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) nat[i] = static_cast<uint32_t>(min(g + 8 * i, last)) * static_cast<uint32_t>(p.w.gs);
+            nscales = p.w.scales + at;
+            if (ZEROS) nzeros = p.w.zeros + at;
             nchunk = kwarp * KS + rank;
             return;
         }
@@ -510,10 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int step = nchunk * steps_of + b * kBoxSteps;
         if (step >= nsteps) return;
         const int grp = SPG == kBoxSteps ? step / spg : step / (SPG ? SPG : 1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            scales[b][i].load(p.w.scales + nbase + (nat[i] + grp), p.w.zeros + nbase + (nat[i] + grp),
-                              static_cast<int>(p.w.gs) - grp, p.vec);
+        scales[b].load(nscales + grp, nzeros + grp, static_cast<int>(p.w.gs) - grp, p.vec);
     };
     auto advance = [&] {
         nchunk += kw * KS;
@@ -589,9 +594,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const uint32_t xs = g < nb ? smem_u32(sx) + (l * steps_of + b * kBoxSteps) * nb * 64 + lane * 16
                                                    : smem_u32(nothing);
                         if (steps >= kBoxSteps)
-                            box_products<BF16, ZEROS, SPG, true>(total, w, xs, xstep, scales[b], steps);
+                            box_products<BF16, ZEROS, SPG, true>(total, w, xs, xstep, scales[b], g, steps);
                         else if (steps > 0)
-                            box_products<BF16, ZEROS, SPG, false>(total, w, xs, xstep, scales[b], steps);
+                            box_products<BF16, ZEROS, SPG, false>(total, w, xs, xstep, scales[b], g, steps);
                         __syncwarp();
                         load(b);
                     }
