@@ -318,10 +318,10 @@ struct RowScales {
     __device__ __forceinline__ uint32_t zero(int i) const { return ZEROS ? z[i / 4] >> (8 * (i & 3)) & 15u : 8u; }
 };
 
-// A box's products, its words at shared address w, the vectors' pieces of its
-// first step at x.  FULL: it has all its steps.
+// A box's products: this lane's words of its steps, the vectors' pieces of its
+// first step at shared address x.  FULL: it has all its steps.
 template <bool BF16, bool ZEROS, int SPG, bool FULL>
-__device__ __forceinline__ void box_products(float (&total)[2][4], uint32_t w, uint32_t x, int xstep,
+__device__ __forceinline__ void box_products(float (&total)[2][4], const uint32_t (&words)[kBoxSteps][4], uint32_t x, int xstep,
                                              const RowScales<SPG, ZEROS> &row, int g, int steps) {
     using H = b2b::Half16<BF16>;
     uint32_t sw[4], zw[4];  // of rows g, g + 8, g + 16, g + 24: two groups' scales, four groups' zero points
@@ -345,13 +345,10 @@ __device__ __forceinline__ void box_products(float (&total)[2][4], uint32_t w, u
             if (!FULL && si > 0 && st >= steps) break;
             const uint4 xv = lds128(x);
             x += xstep;
-            uint32_t words[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) words[i] = lds32((w ^ (st << 4)) + i * 1024);
             if (si == 0)
-                step32<BF16, true>(sum, words, un, xv);
+                step32<BF16, true>(sum, words[st], un, xv);
             else
-                step32<BF16, false>(sum, words, un, xv);
+                step32<BF16, false>(sum, words[st], un, xv);
         }
         add_scaled(total, sum, scale);
     }
@@ -589,16 +586,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                       p.wait_ns);
                             dead = !__all_sync(0xffffffffu, ok);
                         }
-                        // 16-byte piece st of row r sits at piece st ^ (r % 8)
+                        // The words go to registers at once, so that the box is in
+                        // flight again while they are multiplied.
+                        // 16-byte piece st of row r sits at piece st ^ (r % 8).
                         const uint32_t w = smem_u32(ring) + b * kBoxBytes + g * 128 + (g << 4) + q * 4;
+                        uint32_t words[kBoxSteps][4];
+#pragma unroll
+                        for (int st = 0; st < kBoxSteps; ++st)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) words[st][i] = lds32((w ^ (st << 4)) + i * 1024);
+                        const RowScales<SPG, ZEROS> here = scales[b];
+                        __syncwarp();
+                        load(b);
                         const uint32_t xs = g < nb ? smem_u32(sx) + (l * steps_of + b * kBoxSteps) * nb * 64 + lane * 16
                                                    : smem_u32(nothing);
                         if (steps >= kBoxSteps)
-                            box_products<BF16, ZEROS, SPG, true>(total, w, xs, xstep, scales[b], g, steps);
+                            box_products<BF16, ZEROS, SPG, true>(total, words, xs, xstep, here, g, steps);
                         else if (steps > 0)
-                            box_products<BF16, ZEROS, SPG, false>(total, w, xs, xstep, scales[b], g, steps);
-                        __syncwarp();
-                        load(b);
+                            box_products<BF16, ZEROS, SPG, false>(total, words, xs, xstep, here, g, steps);
                     }
                     phase ^= 1u;
                     advance();
