@@ -10,6 +10,7 @@
 #include <stdint.h>
 
 #include <mutex>
+#include <type_traits>
 #include <vector>
 
 #include "half_types.cuh"
@@ -25,75 +26,148 @@ struct W4Args {
     int64_t m, n, group, pitch, gs;  // pitch = bytes of a packed row, gs = groups of a row
 };
 
-__device__ __forceinline__ int w4_value(const W4Args &p, int64_t row, int64_t j) {
-    const int byte = p.packed[row * p.pitch + j / 2];
-    const int zero = p.zeros ? p.zeros[row * p.gs + j / p.group] & 15 : 8;
-    return ((j & 1) ? byte >> 4 : byte & 15) - zero;
+// ---------------------------------------------------------------------------
+// Quantisation.  All arithmetic that decides a value is f32 on the scale
+// rounded to 16 bits.  The quotient w / s that rounds to a value is of two
+// numbers with at most 11 significant bits: unless it lies exactly on the
+// border between two values it is at least 2^-12 away from it.  So w times the
+// reciprocal decides as the quotient would wherever it is not within 2^-12 of
+// a border, and the quotient itself is computed only there (about one value in
+// two thousand).
+
+// The scale of a group from its extremes (0 among them); NaN unless all its
+// values are finite.
+template <bool BF16>
+__device__ __forceinline__ uint16_t w4_scale(float lo, float hi, bool finite, bool zeros) {
+    // halves, so that hi - lo of bf16 extremes stays finite
+    const float s = zeros ? __fdiv_rn(0.5f * hi - 0.5f * lo, 7.5f) : __fdiv_rn(fmaxf(hi, -lo), 7.0f);
+    return b2b::Half16<BF16>::put(finite ? s : __int_as_float(0x7fffffff));
 }
 
-// One warp a group of a row.  All arithmetic that decides a value is f32 on
-// the scale rounded to 16 bits.  The quotient w / s that rounds to a value is
-// of two numbers with at most 11 significant bits: unless it lies exactly on
-// the border between two values it is at least 2^-12 away from it, so f32's
-// rounding decides as exact arithmetic would.
-template <bool BF16>
+// Values of a group whose scale is s.
+struct Quantizer {
+    float s, inverse, zero;
+    bool live;   // s > 0: false for a zero and a NaN scale, whose groups hold their zero point
+    bool exact;  // the reciprocal cannot be used: it would overflow
+    __device__ __forceinline__ Quantizer(float scale, float lo, bool zeros) : s(scale) {
+        live = s > 0.0f;
+        inverse = live ? __fdiv_rn(1.0f, s) : 0.0f;
+        exact = inverse > 1e38f;
+        zero = 8.0f;
+        if (zeros) zero = live ? fminf(rintf(__fdiv_rn(-lo, s)), 15.0f) : 0.0f;
+    }
+    // A value 0..15, as a float.
+    __device__ __forceinline__ float operator()(float w) const {
+        if (!live) return zero;
+        float r = w * inverse;
+        if (exact || fabsf(r - rintf(r)) > 0.499755859375f) r = __fdiv_rn(w, s);
+        return fminf(fmaxf(rintf(r) + zero, 0.0f), 15.0f);
+    }
+};
+
+// Whole 16-byte loads: n a multiple of 8, groups of 8 LPG columns, one to LPG
+// lanes (LPG = 4..32).  A lane reads 8 values once and writes their word; 32
+// lanes' worth is a task.  HBM-bound: about 50 instructions for the 20 bytes
+// that a lane moves.
+template <bool BF16, int LPG>
 __global__ void __launch_bounds__(256) w4_quantize_kernel(const uint16_t *W, uint8_t *packed, uint16_t *scales,
-                                                          uint8_t *zeros, int64_t m, int64_t n, int64_t group,
-                                                          int64_t pitch, int64_t gs) {
+                                                          uint8_t *zeros, int64_t m, int64_t n, int64_t gs) {
     using H = b2b::Half16<BF16>;
     const int lane = threadIdx.x & 31;
-    const int64_t warps = static_cast<int64_t>(gridDim.x) * 8;
-    for (int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); at < m * gs; at += warps) {
-        const int64_t row = at / gs, j0 = at % gs * group;
-        const int64_t j1 = j0 + group < n ? j0 + group : n;
+    const int64_t per = (gs * LPG + 31) / 32;  // tasks of a row
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
+    for (int64_t task = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); task < m * per; task += step) {
+        const int64_t row = task / per, oct = task % per * 32 + lane;
+        const bool have = oct * 8 < n;
+        uint4 in = make_uint4(0, 0, 0, 0);
+        if (have) in = __ldg(reinterpret_cast<const uint4 *>(W + row * n) + oct);
+        const uint32_t words[4] = {in.x, in.y, in.z, in.w};
+        float v[8];
         float lo = 0.0f, hi = 0.0f;
         bool finite = true;
-        for (int64_t j = j0 + lane; j < j1; j += 32) {
-            const float w = H::get(W[row * n + j]);
-            finite = finite && isfinite(w);
-            lo = fminf(lo, w);
-            hi = fmaxf(hi, w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = H::get2(words[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            finite = finite && isfinite(v[i]);
+            lo = fminf(lo, v[i]);
+            hi = fmaxf(hi, v[i]);
+        }
+        if (!finite) hi = __int_as_float(0x7f800000);  // reaches the group's other lanes as one
+#pragma unroll
+        for (int d = LPG / 2; d; d >>= 1) {
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+        }
+        const uint16_t s16 = w4_scale<BF16>(lo, hi, hi < __int_as_float(0x7f800000), zeros != nullptr);
+        const Quantizer q(H::get(s16), lo, zeros != nullptr);
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) word |= static_cast<uint32_t>(q(v[i])) << (4 * i);
+        if (have) {
+            reinterpret_cast<uint32_t *>(packed)[row * (n / 8) + oct] = word;
+            if (lane % LPG == 0) {
+                const int64_t at = row * gs + oct / LPG;
+                scales[at] = s16;
+                if (zeros) zeros[at] = static_cast<uint8_t>(q.zero);
+            }
+        }
+    }
+}
+
+// Any n, group and alignment: one warp a group, two neighbouring values a
+// lane; the first 256 values stay in registers between the two passes.
+template <bool BF16>
+__global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W, uint8_t *packed, uint16_t *scales,
+                                                              uint8_t *zeros, int64_t m, int64_t n, int64_t group,
+                                                              int64_t pitch, int64_t gs) {
+    using H = b2b::Half16<BF16>;
+    const int lane = threadIdx.x & 31;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
+    for (int64_t at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); at < m * gs; at += step) {
+        const int64_t row = at / gs, j0 = at % gs * group;
+        const int64_t j1 = j0 + group < n ? j0 + group : n;
+        const uint16_t *w = W + row * n;
+        float kept[8];
+        float lo = 0.0f, hi = 0.0f;
+        bool finite = true;
+        auto see = [&](float v) {
+            finite = finite && isfinite(v);
+            lo = fminf(lo, v);
+            hi = fmaxf(hi, v);
+        };
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int64_t j = j0 + 2 * lane + i / 2 * 64 + i % 2;
+            kept[i] = j < j1 ? H::get(w[j]) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) see(kept[i]);
+        for (int64_t j = j0 + 256 + lane; j < j1; j += 32) see(H::get(w[j]));
 #pragma unroll
         for (int d = 16; d; d >>= 1) {
             lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
         }
         finite = __all_sync(0xffffffffu, finite);
-        // halves, so that hi - lo of bf16 extremes stays finite
-        float s = zeros ? __fdiv_rn(0.5f * hi - 0.5f * lo, 7.5f) : __fdiv_rn(fmaxf(hi, -lo), 7.0f);
-        const uint16_t s16 = H::put(finite ? s : __int_as_float(0x7fffffff));
-        s = H::get(s16);
-        const bool live = s > 0.0f;  // false for a NaN scale too
-        float zero = 8.0f;
-        if (zeros) zero = live ? fminf(rintf(__fdiv_rn(-lo, s)), 15.0f) : 0.0f;
+        const uint16_t s16 = w4_scale<BF16>(lo, hi, finite, zeros != nullptr);
+        const Quantizer q(H::get(s16), lo, zeros != nullptr);
         if (lane == 0) {
             scales[at] = s16;
-            if (zeros) zeros[at] = static_cast<uint8_t>(zero);
+            if (zeros) zeros[at] = static_cast<uint8_t>(q.zero);
         }
-        for (int64_t j = j0 + 2 * lane; j < j1; j += 64) {
-            uint32_t byte = 0;
+        auto put = [&](int64_t j, float a, float b) {  // columns j, even, and j + 1
+            if (j >= j1) return;
+            const uint32_t low = static_cast<uint32_t>(q(a)), high = j + 1 < j1 ? static_cast<uint32_t>(q(b)) : 0u;
+            packed[row * pitch + j / 2] = static_cast<uint8_t>(low | high << 4);
+        };
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                if (j + e >= j1) continue;
-                float q = zero;
-                if (live) q = fminf(fmaxf(rintf(__fdiv_rn(H::get(W[row * n + j + e]), s)) + zero, 0.0f), 15.0f);
-                byte |= static_cast<uint32_t>(q) << (4 * e);
-            }
-            packed[row * pitch + j / 2] = static_cast<uint8_t>(byte);
-        }
-    }
-}
-
-template <bool BF16>
-__global__ void __launch_bounds__(256) w4_dequantize_kernel(W4Args p, uint16_t *W) {
-    using H = b2b::Half16<BF16>;
-    const int64_t total = p.m * p.n, step = static_cast<int64_t>(gridDim.x) * 256;
-    for (int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; at < total; at += step) {
-        const int64_t row = at / p.n, j = at % p.n;
-        // 11 bits times 5: exact in f32, rounded once
-        const float v = H::get(p.scales[row * p.gs + j / p.group]) * static_cast<float>(w4_value(p, row, j));
-        W[at] = H::put(v > H::kMax ? H::kMax : v < -H::kMax ? -H::kMax : v);
+        for (int i = 0; i < 4; ++i) put(j0 + 2 * lane + 64 * i, kept[2 * i], kept[2 * i + 1]);
+        for (int64_t j = j0 + 256 + 2 * lane; j < j1; j += 64) put(j, H::get(w[j]), j + 1 < j1 ? H::get(w[j + 1]) : 0.0f);
     }
 }
 
@@ -596,6 +670,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) words[st][i] = lds32((w ^ (st << 4)) + i * 1024);
                         const RowScales<SPG, ZEROS> here = scales[b];
+                        // every lane's reads come before the box's next contents
+                        fence_proxy_async_smem();
                         __syncwarp();
                         load(b);
                         const uint32_t xs = g < nb ? smem_u32(sx) + (l * steps_of + b * kBoxSteps) * nb * 64 + lane * 16
@@ -710,6 +786,85 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t t0 = globaltimer_ns();
         while (globaltimer_ns() - t0 < 2000000ull) {
         }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Back to 16 bits.  scale * (q - zero) is 11 bits times 5: its product in 16
+// bits is the exact one rounded once.
+template <bool BF16>
+__device__ __forceinline__ uint16_t w4_back(float scale, int q) {
+    using H = b2b::Half16<BF16>;
+    const float v = scale * static_cast<float>(q);
+    return H::put(v > H::kMax ? H::kMax : v < -H::kMax ? -H::kMax : v);
+}
+
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b, __half) { return as_word(__hmul2(as_half2(a), as_half2(b))); }
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b, __nv_bfloat16) {
+    return as_word(__hmul2(as_bf162(a), as_bf162(b)));
+}
+
+// Whole words and 16-byte stores: n a multiple of 8.  HBM-bound: about 25
+// instructions for the 20 bytes and more that a lane moves.
+template <bool BF16>
+__global__ void __launch_bounds__(256) w4_dequantize_kernel(W4Args p, uint16_t *W) {
+    using H = b2b::Half16<BF16>;
+    using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+    const int lane = threadIdx.x & 31;
+    const int64_t octs = p.n / 8, per = (octs + 31) / 32, og = p.group / 8;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
+    for (int64_t task = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); task < p.m * per; task += step) {
+        const int64_t row = task / per;
+        const uint32_t oct = static_cast<uint32_t>(task % per) * 32 + lane;
+        if (oct >= octs) continue;
+        const uint32_t word = __ldg(reinterpret_cast<const uint32_t *>(p.packed) + row * octs + oct);
+        const int64_t at = row * p.gs + oct / static_cast<uint32_t>(og);
+        const uint16_t s16 = __ldg(p.scales + at);
+        const uint32_t zero = p.zeros ? __ldg(p.zeros + at) & 15u : 8u;
+        const float s = H::get(s16);
+        uint32_t o[4];
+        if (fabsf(s) <= H::kMax / 16.0f) {
+            uint32_t v[4];
+            Unpack<BF16>{zero}(word, v);
+            const uint32_t ss = s16 * 0x10001u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], ss, T{});
+            // pairs (0,4) (1,5) (2,6) (3,7) to (0,1) (2,3) (4,5) (6,7)
+            o[0] = __byte_perm(v[0], v[1], 0x5410);
+            o[1] = __byte_perm(v[2], v[3], 0x5410);
+            o[2] = __byte_perm(v[0], v[1], 0x7632);
+            o[3] = __byte_perm(v[2], v[3], 0x7632);
+        } else {  // a product may pass the largest value, or the scale is a NaN
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int a = static_cast<int>(word >> (8 * i) & 15u), b = static_cast<int>(word >> (8 * i + 4) & 15u);
+                const int z = static_cast<int>(zero);
+                o[i] = w4_back<BF16>(s, a - z) | static_cast<uint32_t>(w4_back<BF16>(s, b - z)) << 16;
+            }
+        }
+        *(reinterpret_cast<uint4 *>(W + row * p.n) + oct) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+
+// Any n and alignment: a byte a lane.
+template <bool BF16>
+__global__ void __launch_bounds__(256) w4_dequantize_any_kernel(W4Args p, uint16_t *W) {
+    using H = b2b::Half16<BF16>;
+    const int lane = threadIdx.x & 31;
+    const int64_t per = (p.pitch + 31) / 32;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
+    const uint32_t half_group = static_cast<uint32_t>(p.group / 2);
+    for (int64_t task = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); task < p.m * per; task += step) {
+        const int64_t row = task / per;
+        const uint32_t at = static_cast<uint32_t>(task % per) * 32 + lane;  // byte of the row
+        if (at >= p.pitch) continue;
+        const int byte = p.packed[row * p.pitch + at];
+        const int64_t grp = row * p.gs + at / half_group;
+        const int zero = p.zeros ? p.zeros[grp] & 15 : 8;
+        const float s = H::get(p.scales[grp]);
+        uint16_t *w = W + row * p.n + 2 * static_cast<int64_t>(at);
+        w[0] = w4_back<BF16>(s, (byte & 15) - zero);
+        if (2 * static_cast<int64_t>(at) + 1 < p.n) w[1] = w4_back<BF16>(s, (byte >> 4) - zero);
     }
 }
 
@@ -854,17 +1009,37 @@ namespace b2b {
 int launch_quantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, const uint16_t *W, uint8_t *packed,
                        uint16_t *scales, uint8_t *zeros) {
     const W4Args p = w4_args(m, n, group, packed, scales, zeros);
-    auto kernel = type == B2B_TYPE_BF16 ? w4_quantize_kernel<true> : w4_quantize_kernel<false>;
-    const unsigned ctas = ctas_for(h, reinterpret_cast<const void *>(kernel), (p.m * p.gs + 7) / 8);
-    kernel<<<ctas, 256, 0, h->stream>>>(W, packed, scales, zeros, p.m, p.n, p.group, p.pitch, p.gs);
+    const bool bf16 = type == B2B_TYPE_BF16;
+    if (n % 8 == 0 && aligned16(W) && (reinterpret_cast<uintptr_t>(packed) & 3) == 0 &&
+        (group == 32 || group == 64 || group == 128 || group == 256)) {
+        auto kernel = bf16 ? (group == 32    ? w4_quantize_kernel<true, 4>
+                              : group == 64  ? w4_quantize_kernel<true, 8>
+                              : group == 128 ? w4_quantize_kernel<true, 16>
+                                             : w4_quantize_kernel<true, 32>)
+                           : (group == 32    ? w4_quantize_kernel<false, 4>
+                              : group == 64  ? w4_quantize_kernel<false, 8>
+                              : group == 128 ? w4_quantize_kernel<false, 16>
+                                             : w4_quantize_kernel<false, 32>);
+        const int64_t tasks = p.m * ((p.gs * static_cast<int64_t>(group / 8) + 31) / 32);
+        const unsigned ctas = ctas_for(h, reinterpret_cast<const void *>(kernel), (tasks + 7) / 8);
+        kernel<<<ctas, 256, 0, h->stream>>>(W, packed, scales, zeros, p.m, p.n, p.gs);
+    } else {
+        auto kernel = bf16 ? w4_quantize_any_kernel<true> : w4_quantize_any_kernel<false>;
+        const unsigned ctas = ctas_for(h, reinterpret_cast<const void *>(kernel), (p.m * p.gs + 7) / 8);
+        kernel<<<ctas, 256, 0, h->stream>>>(W, packed, scales, zeros, p.m, p.n, p.group, p.pitch, p.gs);
+    }
     return launched("4-bit quantisation launch");
 }
 
 int launch_dequantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, const uint8_t *packed,
                          const uint16_t *scales, const uint8_t *zeros, uint16_t *W) {
     const W4Args p = w4_args(m, n, group, packed, scales, zeros);
-    auto kernel = type == B2B_TYPE_BF16 ? w4_dequantize_kernel<true> : w4_dequantize_kernel<false>;
-    kernel<<<ctas_for(h, reinterpret_cast<const void *>(kernel), (p.m * p.n + 255) / 256), 256, 0, h->stream>>>(p, W);
+    const bool bf16 = type == B2B_TYPE_BF16;
+    const bool whole = n % 8 == 0 && aligned16(W) && (reinterpret_cast<uintptr_t>(packed) & 3) == 0;
+    auto kernel = whole ? (bf16 ? w4_dequantize_kernel<true> : w4_dequantize_kernel<false>)
+                        : (bf16 ? w4_dequantize_any_kernel<true> : w4_dequantize_any_kernel<false>);
+    const int64_t tasks = p.m * (((whole ? p.n / 8 : p.pitch) + 31) / 32);
+    kernel<<<ctas_for(h, reinterpret_cast<const void *>(kernel), (tasks + 7) / 8), 256, 0, h->stream>>>(p, W);
     return launched("4-bit dequantisation launch");
 }
 

@@ -326,3 +326,42 @@ def test_graph_and_other_stream():
     finally:
         h.set_stream(None)
         h.close()
+
+
+@pytest.mark.parametrize("e,m,n,group,count,t,with_zeros", [
+    (1, 16384, 16384, 128, 1, "f16", False), (1, 8192, 16384, 32, 8, "bf16", True), (5, 4096, 2048, 64, 40, "f16", True),
+    (1, 4096, 4104, 64, 3, "f16", True), (2, 20000, 20480, 256, 3, "bf16", False)])
+def test_gemv_gives_the_same_exact_bits_each_time(handle, e, m, n, group, count, t, with_zeros):
+    """Many rounds of every warp's buffers, 20 times over, against exact sums
+    of whole numbers."""
+    import torch
+
+    import b2blas
+
+    h, dt = handle, R.HALF[t]
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(6)
+    gs, pitch = -(-n // group), (n + 1) // 2
+    rand = lambda lo, hi, *s: torch.randint(lo, hi, s, generator=gen, device="cuda")  # noqa: E731
+    packed, zeros = rand(0, 256, e * m, pitch).to(torch.uint8), rand(0, 16, e * m, gs).to(torch.uint8) if with_zeros else None
+    scales, x = torch.ones(e * m, gs, device="cuda").to(dt), rand(-1, 2, count, n).to(dt)
+    index = rand(0, e, count).to(torch.int32)
+    want = torch.zeros(count, m, device="cuda").to(dt)
+    for i in range(e):
+        q = torch.stack((packed[i * m:(i + 1) * m] & 15, packed[i * m:(i + 1) * m] >> 4), -1).flatten(1)[:, :n].float()
+        q -= 8 if zeros is None else zeros[i * m:(i + 1) * m].float().repeat_interleave(group, 1)[:, :n]
+        want[index == i] = (x[index == i].double() @ q.double().t() / 64).to(dt)
+        del q
+    view = lambda v, d=np.uint16: None if v is None else b2blas.DeviceBuffer.from_ptr(h, v.data_ptr(), v.numel(), d, v)  # noqa: E731
+    for _ in range(20):
+        y = torch.full_like(want, float("nan"))
+        torch.cuda.synchronize()
+        args = (view(packed, np.uint8), view(scales), view(zeros, np.uint8), view(x))
+        if e == 1:
+            h.hgemv_w4(m, n, group, 2.0 ** -6, *args, 0.0, view(y), count=count, half=half_of(t))
+        else:
+            h.hgemv_w4_grouped(e, m, n, group, 2.0 ** -6, *args, view(index, np.int32), 0.0, view(y), count=count, half=half_of(t))
+        h.synchronize()
+        assert torch.equal(y, want)
+    del packed, want
+    torch.cuda.empty_cache()
