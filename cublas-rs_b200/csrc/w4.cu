@@ -31,9 +31,8 @@ struct W4Args {
 // rounded to 16 bits.  The quotient w / s that rounds to a value is of two
 // numbers with at most 11 significant bits: unless it lies exactly on the
 // border between two values it is at least 2^-12 away from it.  So w times the
-// reciprocal decides as the quotient would wherever it is not within 2^-12 of
-// a border, and the quotient itself is computed only there (about one value in
-// two thousand).
+// reciprocal, at most 2^-18 off, decides as the quotient would, and where it is
+// that near to a border the quotient is on the border: the even value it is.
 
 // The scale of a group from its extremes (0 among them); NaN unless all its
 // values are finite.
@@ -46,81 +45,137 @@ __device__ __forceinline__ uint16_t w4_scale(float lo, float hi, bool finite, bo
 
 // Values of a group whose scale is s.
 struct Quantizer {
+    static constexpr float kRound = 12582912.0f;  // 1.5 * 2^23: adding it rounds to a whole number, ties to even
     float s, inverse, zero;
-    bool live;   // s > 0: false for a zero and a NaN scale, whose groups hold their zero point
-    bool exact;  // the reciprocal cannot be used: it would overflow
+    static constexpr float kBorder = 0.499996185302734375f;  // 1/2 - 2^-18
+    bool live;    // s > 0: false for a zero and a NaN scale, whose groups hold their zero point
+    bool divide;  // the reciprocal overflows
     __device__ __forceinline__ Quantizer(float scale, float lo, bool zeros) : s(scale) {
         live = s > 0.0f;
-        inverse = live ? __fdiv_rn(1.0f, s) : 0.0f;
-        exact = inverse > 1e38f;
+        inverse = __fdividef(1.0f, s);
+        divide = !(inverse < 1e38f);
         zero = 8.0f;
         if (zeros) zero = live ? fminf(rintf(__fdiv_rn(-lo, s)), 15.0f) : 0.0f;
     }
-    // A value 0..15, as a float.
-    __device__ __forceinline__ float operator()(float w) const {
-        if (!live) return zero;
-        float r = w * inverse;
-        if (exact || fabsf(r - rintf(r)) > 0.499755859375f) r = __fdiv_rn(w, s);
-        return fminf(fmaxf(rintf(r) + zero, 0.0f), 15.0f);
+    __device__ __forceinline__ float clamp(float r) const { return fminf(fmaxf(r + zero, 0.0f), 15.0f); }
+    __device__ __forceinline__ float exact(float w) const { return live ? clamp(rintf(__fdiv_rn(w, s))) : zero; }
+    // N values 0..15, as floats.
+    template <int N>
+    __device__ __forceinline__ void operator()(const float (&w)[N], float (&out)[N]) const {
+        if (divide) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) out[i] = exact(w[i]);
+            return;
+        }
+        float far = 0.0f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            out[i] = fmaf(w[i], inverse, kRound) - kRound;
+            far = fmaxf(far, fabsf(fmaf(w[i], inverse, -out[i])));
+        }
+        if (far > kBorder) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float off = fmaf(w[i], inverse, -out[i]);
+                const bool odd = __float_as_uint(out[i] + kRound) & 1u;
+                if (fabsf(off) > kBorder && odd) out[i] += copysignf(1.0f, off);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = clamp(out[i]);
     }
 };
 
-// Whole 16-byte loads: n a multiple of 8, groups of 8 LPG columns, one to LPG
-// lanes (LPG = 4..32).  A lane reads 8 values once and writes their word; 32
-// lanes' worth is a task.  HBM-bound: about 50 instructions for the 20 bytes
-// that a lane moves.
-template <bool BF16, int LPG>
+// Eight values to a word: the nibbles of two halves are added up in f32, where
+// they are exact.
+__device__ __forceinline__ uint32_t pack8(const float *q) {
+    const float low = fmaf(4096.0f, q[3], fmaf(256.0f, q[2], fmaf(16.0f, q[1], q[0])));
+    const float high = fmaf(4096.0f, q[7], fmaf(256.0f, q[6], fmaf(16.0f, q[5], q[4])));
+    return static_cast<uint32_t>(low) | static_cast<uint32_t>(high) << 16;
+}
+
+// Groups of 16 LANES columns, 16 of them to a lane, which reads them once.
+// WHOLE: n is a multiple of 8 and W and packed allow 16-byte loads and 4-byte
+// stores; else values and bytes one at a time.  HBM-bound where WHOLE: about
+// 250 instructions for the 40 bytes that a lane moves, most of them the
+// rounding and clamping of its values.
+template <bool BF16, int LANES, bool WHOLE>
 __global__ void __launch_bounds__(256) w4_quantize_kernel(const uint16_t *W, uint8_t *packed, uint16_t *scales,
-                                                          uint8_t *zeros, int64_t m, int64_t n, int64_t gs) {
+                                                          uint8_t *zeros, int64_t m, int64_t n, int64_t pitch, int64_t gs) {
     using H = b2b::Half16<BF16>;
     const int lane = threadIdx.x & 31;
-    const int64_t per = (gs * LPG + 31) / 32;  // tasks of a row
+    const int64_t per = (gs * LANES + 31) / 32;  // tasks of a row: a warp's 512 columns
     const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
     for (int64_t task = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); task < m * per; task += step) {
-        const int64_t row = task / per, oct = task % per * 32 + lane;
-        const bool have = oct * 8 < n;
-        uint4 in = make_uint4(0, 0, 0, 0);
-        if (have) in = __ldg(reinterpret_cast<const uint4 *>(W + row * n) + oct);
-        const uint32_t words[4] = {in.x, in.y, in.z, in.w};
-        float v[8];
-        float lo = 0.0f, hi = 0.0f;
-        bool finite = true;
+        const int64_t row = task / per;
+        const int64_t unit = task % per * 32 + lane, j0 = unit * 16;
+        const uint16_t *w = W + row * n + j0;
+        float v[16];
+        if constexpr (WHOLE) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = H::get2(words[i]);
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
+            for (int h = 0; h < 2; ++h) {
+                uint4 in = make_uint4(0, 0, 0, 0);
+                if (j0 + 8 * h < n) in = __ldg(reinterpret_cast<const uint4 *>(w) + h);
+                const uint32_t words[4] = {in.x, in.y, in.z, in.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = H::get2(words[i]);
+                    v[8 * h + 2 * i] = f.x;
+                    v[8 * h + 2 * i + 1] = f.y;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = j0 + i < n ? H::get(w[i]) : 0.0f;
         }
+        float lo = 0.0f, hi = 0.0f, nan = 0.0f;  // nan: 0, or a NaN once an infinity or a NaN is met
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            finite = finite && isfinite(v[i]);
+        for (int i = 0; i < 16; ++i) {
+            nan = fmaf(v[i], 0.0f, nan);
             lo = fminf(lo, v[i]);
             hi = fmaxf(hi, v[i]);
         }
-        if (!finite) hi = __int_as_float(0x7f800000);  // reaches the group's other lanes as one
+        if (nan != 0.0f) hi = __int_as_float(0x7f800000);  // reaches the group's other lanes as an infinity
 #pragma unroll
-        for (int d = LPG / 2; d; d >>= 1) {
+        for (int d = LANES / 2; d; d >>= 1) {
             lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
         }
         const uint16_t s16 = w4_scale<BF16>(lo, hi, hi < __int_as_float(0x7f800000), zeros != nullptr);
         const Quantizer q(H::get(s16), lo, zeros != nullptr);
-        uint32_t word = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) word |= static_cast<uint32_t>(q(v[i])) << (4 * i);
-        if (have) {
-            reinterpret_cast<uint32_t *>(packed)[row * (n / 8) + oct] = word;
-            if (lane % LPG == 0) {
-                const int64_t at = row * gs + oct / LPG;
-                scales[at] = s16;
-                if (zeros) zeros[at] = static_cast<uint8_t>(q.zero);
+        float out[16];
+        q(v, out);
+        const uint32_t word0 = pack8(out), word1 = pack8(out + 8);
+        uint8_t *to = packed + row * pitch + unit * 8;
+        if constexpr (WHOLE) {
+            if (j0 + 8 < n) {
+                if ((reinterpret_cast<uintptr_t>(to) & 7) == 0) {
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(word0, word1);
+                } else {
+                    reinterpret_cast<uint32_t *>(to)[0] = word0;
+                    reinterpret_cast<uint32_t *>(to)[1] = word1;
+                }
+            } else if (j0 < n) {
+                *reinterpret_cast<uint32_t *>(to) = word0;
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (j0 + 2 * i < n) {
+                    uint32_t byte = (i < 4 ? word0 : word1) >> (i % 4 * 8) & 0xffu;
+                    if (j0 + 2 * i + 1 == n) byte &= 15u;
+                    to[i] = static_cast<uint8_t>(byte);
+                }
+        }
+        if (lane % LANES == 0 && j0 < n) {
+            const int64_t at = row * gs + unit / LANES;
+            scales[at] = s16;
+            if (zeros) zeros[at] = static_cast<uint8_t>(q.zero);
         }
     }
 }
 
-// Any n, group and alignment: one warp a group, two neighbouring values a
-// lane; the first 256 values stay in registers between the two passes.
+// Other groups: one warp a group, two neighbouring values a lane.
 template <bool BF16>
 __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W, uint8_t *packed, uint16_t *scales,
                                                               uint8_t *zeros, int64_t m, int64_t n, int64_t group,
@@ -132,42 +187,30 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
         const int64_t row = at / gs, j0 = at % gs * group;
         const int64_t j1 = j0 + group < n ? j0 + group : n;
         const uint16_t *w = W + row * n;
-        float kept[8];
-        float lo = 0.0f, hi = 0.0f;
-        bool finite = true;
-        auto see = [&](float v) {
-            finite = finite && isfinite(v);
+        float lo = 0.0f, hi = 0.0f, nan = 0.0f;
+        for (int64_t j = j0 + lane; j < j1; j += 32) {
+            const float v = H::get(w[j]);
+            nan = fmaf(v, 0.0f, nan);
             lo = fminf(lo, v);
             hi = fmaxf(hi, v);
-        };
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int64_t j = j0 + 2 * lane + i / 2 * 64 + i % 2;
-            kept[i] = j < j1 ? H::get(w[j]) : 0.0f;
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) see(kept[i]);
-        for (int64_t j = j0 + 256 + lane; j < j1; j += 32) see(H::get(w[j]));
 #pragma unroll
         for (int d = 16; d; d >>= 1) {
             lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
         }
-        finite = __all_sync(0xffffffffu, finite);
+        const bool finite = __all_sync(0xffffffffu, nan == 0.0f);
         const uint16_t s16 = w4_scale<BF16>(lo, hi, finite, zeros != nullptr);
         const Quantizer q(H::get(s16), lo, zeros != nullptr);
         if (lane == 0) {
             scales[at] = s16;
             if (zeros) zeros[at] = static_cast<uint8_t>(q.zero);
         }
-        auto put = [&](int64_t j, float a, float b) {  // columns j, even, and j + 1
-            if (j >= j1) return;
-            const uint32_t low = static_cast<uint32_t>(q(a)), high = j + 1 < j1 ? static_cast<uint32_t>(q(b)) : 0u;
-            packed[row * pitch + j / 2] = static_cast<uint8_t>(low | high << 4);
-        };
-#pragma unroll
-        for (int i = 0; i < 4; ++i) put(j0 + 2 * lane + 64 * i, kept[2 * i], kept[2 * i + 1]);
-        for (int64_t j = j0 + 256 + 2 * lane; j < j1; j += 64) put(j, H::get(w[j]), j + 1 < j1 ? H::get(w[j + 1]) : 0.0f);
+        for (int64_t j = j0 + 2 * lane; j < j1; j += 64) {
+            uint32_t byte = static_cast<uint32_t>(q.exact(H::get(w[j])));
+            if (j + 1 < j1) byte |= static_cast<uint32_t>(q.exact(H::get(w[j + 1]))) << 4;
+            packed[row * pitch + j / 2] = static_cast<uint8_t>(byte);
+        }
     }
 }
 
@@ -811,60 +854,79 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(W4Args p, uint16_t *
     using H = b2b::Half16<BF16>;
     using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
     const int lane = threadIdx.x & 31;
-    const int64_t octs = p.n / 8, per = (octs + 31) / 32, og = p.group / 8;
+    const int64_t octs = p.n / 8, per = (octs + 63) / 64;
+    const uint32_t og = static_cast<uint32_t>(p.group / 8);
     const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
     for (int64_t task = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); task < p.m * per; task += step) {
         const int64_t row = task / per;
-        const uint32_t oct = static_cast<uint32_t>(task % per) * 32 + lane;
-        if (oct >= octs) continue;
-        const uint32_t word = __ldg(reinterpret_cast<const uint32_t *>(p.packed) + row * octs + oct);
-        const int64_t at = row * p.gs + oct / static_cast<uint32_t>(og);
-        const uint16_t s16 = __ldg(p.scales + at);
-        const uint32_t zero = p.zeros ? __ldg(p.zeros + at) & 15u : 8u;
-        const float s = H::get(s16);
-        uint32_t o[4];
-        if (fabsf(s) <= H::kMax / 16.0f) {
-            uint32_t v[4];
-            Unpack<BF16>{zero}(word, v);
-            const uint32_t ss = s16 * 0x10001u;
+        const uint32_t oct0 = static_cast<uint32_t>(task % per) * 64 + lane;
+        uint32_t word[2], zero[2];
+        uint16_t scale[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], ss, T{});
-            // pairs (0,4) (1,5) (2,6) (3,7) to (0,1) (2,3) (4,5) (6,7)
-            o[0] = __byte_perm(v[0], v[1], 0x5410);
-            o[1] = __byte_perm(v[2], v[3], 0x5410);
-            o[2] = __byte_perm(v[0], v[1], 0x7632);
-            o[3] = __byte_perm(v[2], v[3], 0x7632);
-        } else {  // a product may pass the largest value, or the scale is a NaN
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int a = static_cast<int>(word >> (8 * i) & 15u), b = static_cast<int>(word >> (8 * i + 4) & 15u);
-                const int z = static_cast<int>(zero);
-                o[i] = w4_back<BF16>(s, a - z) | static_cast<uint32_t>(w4_back<BF16>(s, b - z)) << 16;
-            }
+        for (int h = 0; h < 2; ++h) {  // all loads before their use
+            const uint32_t oct = min(oct0 + 32 * h, static_cast<uint32_t>(octs - 1));
+            const int64_t at = row * p.gs + oct / og;
+            word[h] = __ldg(reinterpret_cast<const uint32_t *>(p.packed) + row * octs + oct);
+            scale[h] = __ldg(p.scales + at);
+            zero[h] = p.zeros ? __ldg(p.zeros + at) & 15u : 8u;
         }
-        *(reinterpret_cast<uint4 *>(W + row * p.n) + oct) = make_uint4(o[0], o[1], o[2], o[3]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (oct0 + 32 * h >= octs) continue;
+            const float s = H::get(scale[h]);
+            uint32_t o[4];
+            if (fabsf(s) <= H::kMax / 16.0f) {
+                uint32_t v[4];
+                Unpack<BF16>{zero[h]}(word[h], v);
+                const uint32_t ss = scale[h] * 0x10001u;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = mul2(v[i], ss, T{});
+                // pairs (0,4) (1,5) (2,6) (3,7) to (0,1) (2,3) (4,5) (6,7)
+                o[0] = __byte_perm(v[0], v[1], 0x5410);
+                o[1] = __byte_perm(v[2], v[3], 0x5410);
+                o[2] = __byte_perm(v[0], v[1], 0x7632);
+                o[3] = __byte_perm(v[2], v[3], 0x7632);
+            } else {  // a product may pass the largest value, or the scale is a NaN
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int a = static_cast<int>(word[h] >> (8 * i) & 15u), b = static_cast<int>(word[h] >> (8 * i + 4) & 15u);
+                    const int z = static_cast<int>(zero[h]);
+                    o[i] = w4_back<BF16>(s, a - z) | static_cast<uint32_t>(w4_back<BF16>(s, b - z)) << 16;
+                }
+            }
+            *(reinterpret_cast<uint4 *>(W + row * p.n) + oct0 + 32 * h) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
     }
 }
 
-// Any n and alignment: a byte a lane.
+// Any n and alignment: bytes 32 apart to a lane, four of them in flight.
 template <bool BF16>
 __global__ void __launch_bounds__(256) w4_dequantize_any_kernel(W4Args p, uint16_t *W) {
     using H = b2b::Half16<BF16>;
     const int lane = threadIdx.x & 31;
-    const int64_t per = (p.pitch + 31) / 32;
+    const int64_t per = (p.pitch + 127) / 128;
     const int64_t step = static_cast<int64_t>(gridDim.x) * 8;
     const uint32_t half_group = static_cast<uint32_t>(p.group / 2);
     for (int64_t task = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); task < p.m * per; task += step) {
         const int64_t row = task / per;
-        const uint32_t at = static_cast<uint32_t>(task % per) * 32 + lane;  // byte of the row
-        if (at >= p.pitch) continue;
-        const int byte = p.packed[row * p.pitch + at];
-        const int64_t grp = row * p.gs + at / half_group;
-        const int zero = p.zeros ? p.zeros[grp] & 15 : 8;
-        const float s = H::get(p.scales[grp]);
-        uint16_t *w = W + row * p.n + 2 * static_cast<int64_t>(at);
-        w[0] = w4_back<BF16>(s, (byte & 15) - zero);
-        if (2 * static_cast<int64_t>(at) + 1 < p.n) w[1] = w4_back<BF16>(s, (byte >> 4) - zero);
+        const uint32_t at0 = static_cast<uint32_t>(task % per) * 128 + lane;  // byte of the row
+        int byte[4], zero[4];
+        float s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t at = min(at0 + 32 * i, static_cast<uint32_t>(p.pitch - 1));
+            const int64_t grp = row * p.gs + at / half_group;
+            byte[i] = __ldg(p.packed + row * p.pitch + at);
+            zero[i] = p.zeros ? __ldg(p.zeros + grp) & 15 : 8;
+            s[i] = H::get(__ldg(p.scales + grp));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t at = at0 + 32 * i;
+            uint16_t *w = W + row * p.n + 2 * at;
+            if (2 * at < p.n) w[0] = w4_back<BF16>(s[i], (byte[i] & 15) - zero[i]);
+            if (2 * at + 1 < p.n) w[1] = w4_back<BF16>(s[i], (byte[i] >> 4) - zero[i]);
+        }
     }
 }
 
@@ -916,6 +978,18 @@ int resident_clusters(b2b_handle *h, const void *kernel, cudaLaunchConfig_t &cfg
     }
     cache.push_back(Entry{kernel, h->device, KS, clusters, cfg.dynamicSmemBytes});
     return clusters;
+}
+
+using QuantizeKernel = void (*)(const uint16_t *, uint8_t *, uint16_t *, uint8_t *, int64_t, int64_t, int64_t, int64_t);
+
+template <bool BF16, bool WHOLE>
+QuantizeKernel quantize_kernel(size_t group) {
+    switch (group) {
+        case 32: return w4_quantize_kernel<BF16, 2, WHOLE>;
+        case 64: return w4_quantize_kernel<BF16, 4, WHOLE>;
+        case 128: return w4_quantize_kernel<BF16, 8, WHOLE>;
+        default: return w4_quantize_kernel<BF16, 16, WHOLE>;
+    }
 }
 
 using GemvKernel = void (*)(CUtensorMap, GemvArgs);
@@ -1010,19 +1084,13 @@ int launch_quantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group
                        uint16_t *scales, uint8_t *zeros) {
     const W4Args p = w4_args(m, n, group, packed, scales, zeros);
     const bool bf16 = type == B2B_TYPE_BF16;
-    if (n % 8 == 0 && aligned16(W) && (reinterpret_cast<uintptr_t>(packed) & 3) == 0 &&
-        (group == 32 || group == 64 || group == 128 || group == 256)) {
-        auto kernel = bf16 ? (group == 32    ? w4_quantize_kernel<true, 4>
-                              : group == 64  ? w4_quantize_kernel<true, 8>
-                              : group == 128 ? w4_quantize_kernel<true, 16>
-                                             : w4_quantize_kernel<true, 32>)
-                           : (group == 32    ? w4_quantize_kernel<false, 4>
-                              : group == 64  ? w4_quantize_kernel<false, 8>
-                              : group == 128 ? w4_quantize_kernel<false, 16>
-                                             : w4_quantize_kernel<false, 32>);
-        const int64_t tasks = p.m * ((p.gs * static_cast<int64_t>(group / 8) + 31) / 32);
+    const bool whole = n % 8 == 0 && aligned16(W) && (reinterpret_cast<uintptr_t>(packed) & 3) == 0;
+    if (group == 32 || group == 64 || group == 128 || group == 256) {
+        const QuantizeKernel kernel = bf16 ? (whole ? quantize_kernel<true, true>(group) : quantize_kernel<true, false>(group))
+                                           : (whole ? quantize_kernel<false, true>(group) : quantize_kernel<false, false>(group));
+        const int64_t tasks = p.m * ((p.gs * static_cast<int64_t>(group / 16) + 31) / 32);
         const unsigned ctas = ctas_for(h, reinterpret_cast<const void *>(kernel), (tasks + 7) / 8);
-        kernel<<<ctas, 256, 0, h->stream>>>(W, packed, scales, zeros, p.m, p.n, p.gs);
+        kernel<<<ctas, 256, 0, h->stream>>>(W, packed, scales, zeros, p.m, p.n, p.pitch, p.gs);
     } else {
         auto kernel = bf16 ? w4_quantize_any_kernel<true> : w4_quantize_any_kernel<false>;
         const unsigned ctas = ctas_for(h, reinterpret_cast<const void *>(kernel), (p.m * p.gs + 7) / 8);
@@ -1038,7 +1106,7 @@ int launch_dequantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t gro
     const bool whole = n % 8 == 0 && aligned16(W) && (reinterpret_cast<uintptr_t>(packed) & 3) == 0;
     auto kernel = whole ? (bf16 ? w4_dequantize_kernel<true> : w4_dequantize_kernel<false>)
                         : (bf16 ? w4_dequantize_any_kernel<true> : w4_dequantize_any_kernel<false>);
-    const int64_t tasks = p.m * (((whole ? p.n / 8 : p.pitch) + 31) / 32);
+    const int64_t tasks = p.m * (whole ? (p.n / 8 + 63) / 64 : (p.pitch + 127) / 128);
     kernel<<<ctas_for(h, reinterpret_cast<const void *>(kernel), (tasks + 7) / 8), 256, 0, h->stream>>>(p, W);
     return launched("4-bit dequantisation launch");
 }

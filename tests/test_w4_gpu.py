@@ -89,6 +89,28 @@ def test_quantize_extremes(handle, t, with_zeros):
     assert np.isfinite(back[:9]).all()
 
 
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("with_zeros", [False, True])
+@pytest.mark.parametrize("n", [96, 97])
+def test_quantize_ties_go_to_even(handle, t, with_zeros, n):
+    """Values halfway between two steps, at scales that are not powers of two."""
+    rows = []
+    for s in (1.0, 1.25, 0.6875, 2.0 ** -9, 3 * 2.0 ** 8):
+        for z in (0, 3, 7, 12):
+            steps = np.arange(-2 * z, 31 - 2 * z) / 2 if with_zeros else np.arange(-14, 15) / 2
+            r = np.zeros(n)
+            r[:len(steps)] = steps * s
+            r[32:32 + len(steps)] = -steps * s
+            r[64:64 + len(steps)] = np.roll(steps, 5) * s
+            rows.append(r)
+    w = R.value(R.bits(np.stack(rows), t), t)
+    for group in (32, 96):
+        packed, scales, zeros = quantize(handle, t, w, group, with_zeros)
+        wp, ws, wz = R.quantize(w, group, with_zeros, t)
+        assert np.array_equal(scales, ws) and np.array_equal(packed, wp)
+        assert wz is None or np.array_equal(zeros, wz)
+
+
 def make(rng, t, matrices, m, n, group, with_zeros, exact=True):
     gs = -(-n // group)
     packed = rng.integers(0, 256, (matrices * m, (n + 1) // 2)).astype(np.uint8)
