@@ -160,6 +160,13 @@ __global__ void __launch_bounds__(256) grouped_simt_kernel(GroupedArgs p) {
 //   kNT  C[r] = A[r] B_g^T   A K-major, B (n x k rows) K-major
 //   kTN  C_g = A_g^T B_g     both MN-major; the ragged rows are the k axis
 //
+// The accumulators' f32 additions drop low bits instead of rounding them, about
+// 2^-24 of the sum for each 16 deep step and always toward zero: 2.9e-6 of a
+// sum of 2048 terms, where rounded f32 sums have 0.5e-6.  16-bit results do not
+// see it.  An f32 C_g is therefore summed in pieces of 512: the epilogue's
+// threads hold the tile in registers and add each piece, rounded, while the
+// MMAs fill the other accumulator.
+//
 // No operand is transposed or copied: the three products differ in the shared
 // memory layouts that the MMA descriptors name.  B of kNN / kNT is a 3-D
 // tensor map (columns, rows, group), so a box never reads across a matrix and
@@ -177,8 +184,10 @@ __global__ void __launch_bounds__(256) grouped_simt_kernel(GroupedArgs p) {
 // chain of short latencies, so two warps share each quarter of the TMEM lanes.
 enum Mode { kNN = 0, kNT = 1, kTN = 2 };
 
-template <int MODE, bool PAIR, int BN_>
+template <int MODE, bool PAIR, int BN_, bool F32_>
 struct Cfg {
+    static constexpr bool F32 = F32_;                  // C is f32 (kTN)
+    static constexpr int PIECE = F32 ? 8 : 1 << 30;    // k blocks that an accumulator sums up
     static constexpr int BN = BN_;                     // columns of a tile
     static constexpr int BM = PAIR ? 256 : 128;        // rows of a tile, 128 to a CTA
     static constexpr int BN_CTA = PAIR ? BN / 2 : BN;  // columns of B that a CTA loads
@@ -204,7 +213,7 @@ struct TcArgs {
     int groups, rows, M, N, K;  // M: kTN only; K: kNN and kNT
     float alpha, beta;
     uint32_t idesc;
-    int bf16, f32;  // element types: of the operands, of C
+    int bf16;       // element type of the operands, and of C unless that is f32
     int vec;        // rows of C start on 16-byte boundaries
 };
 
@@ -283,54 +292,35 @@ __device__ __forceinline__ void store_segment(uint8_t *c, int64_t pitch, const u
     }
 }
 
-// x += beta * (the row's old values).
+// x += beta * (the row's old 16-bit values).
 __device__ __forceinline__ void add_old(float (&x)[32], const uint8_t *row, int ncols, const TcArgs &p) {
-    if (p.f32) {
-        const float *c = reinterpret_cast<const float *>(row);
+    const uint16_t *c = reinterpret_cast<const uint16_t *>(row);
 #pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-            if (p.vec) {
-                if (e >= ncols) continue;
-                const float4 v = *reinterpret_cast<const float4 *>(c + e);
-                x[e] = fmaf(p.beta, v.x, x[e]);
-                x[e + 1] = fmaf(p.beta, v.y, x[e + 1]);
-                x[e + 2] = fmaf(p.beta, v.z, x[e + 2]);
-                x[e + 3] = fmaf(p.beta, v.w, x[e + 3]);
-            } else {
+    for (int e = 0; e < 32; e += 8) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        uint32_t *w = reinterpret_cast<uint32_t *>(&v);
+        if (p.vec) {
+            if (e < ncols) v = *reinterpret_cast<const uint4 *>(c + e);
+        } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (e + i < ncols) x[e + i] = fmaf(p.beta, c[e + i], x[e + i]);
-            }
+            for (int i = 0; i < 8; ++i)
+                if (e + i < ncols) w[i / 2] |= static_cast<uint32_t>(c[e + i]) << (i % 2 * 16);
         }
-    } else {
-        const uint16_t *c = reinterpret_cast<const uint16_t *>(row);
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            uint32_t *w = reinterpret_cast<uint32_t *>(&v);
-            if (p.vec) {
-                if (e < ncols) v = *reinterpret_cast<const uint4 *>(c + e);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (e + i < ncols) w[i / 2] |= static_cast<uint32_t>(c[e + i]) << (i % 2 * 16);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = p.bf16 ? b2b::Half16<true>::get2(w[i]) : b2b::Half16<false>::get2(w[i]);
-                x[e + 2 * i] = fmaf(p.beta, f.x, x[e + 2 * i]);
-                x[e + 2 * i + 1] = fmaf(p.beta, f.y, x[e + 2 * i + 1]);
-            }
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = p.bf16 ? b2b::Half16<true>::get2(w[i]) : b2b::Half16<false>::get2(w[i]);
+            x[e + 2 * i] = fmaf(p.beta, f.x, x[e + 2 * i]);
+            x[e + 2 * i + 1] = fmaf(p.beta, f.y, x[e + 2 * i + 1]);
         }
     }
 }
 
-template <int MODE, bool PAIR, int BN>
-__global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
+template <int MODE, bool PAIR, int BN, bool F32>
+__global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32>::THREADS), 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA16,
                       const __grid_constant__ CUtensorMap tmB, TcArgs p) {
     using namespace sm100;
-    using Cf = Cfg<MODE, PAIR, BN>;
+    using Cf = Cfg<MODE, PAIR, BN, F32>;
     constexpr int S = Cf::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -496,59 +486,62 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
                 int depth = p.K;
                 if constexpr (MODE == kTN) depth = tile_at<MODE, Cf>(p, start, off, t, g).depth;
                 const int kblocks = static_cast<int>(static_cast<uint32_t>(depth + 63) / 64);
-                if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x22,
-                               p.wait_ns)) {
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
-                for (int kb = 0; kb < kblocks; ++kb) {
-                    if (!mbar_wait(&full[stage], phase, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x23, p.wait_ns)) {
+                for (int kb0 = 0; ok && (kb0 == 0 || kb0 < kblocks); kb0 += Cf::PIECE) {
+                    if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x22,
+                                   p.wait_ns)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a = smem_u32(sA + stage * Cf::A_BYTES), b = smem_u32(sB + stage * Cf::B_BYTES);
-                    // K-major: 8-row atoms 1024 bytes apart, a k step of 16
-                    // moves 32 bytes inside the swizzled row.  MN-major:
-                    // 64-wide boxes, 8-row k groups 1024 bytes apart, a k
-                    // step moves 16 rows.
-                    auto k_step = [&](int kk) {
-                        const uint64_t ad = MODE == kTN ? sdesc_sw128(a + kk * 2048, kBoxBytes, 1024)
-                                                        : sdesc_sw128(a + kk * 32, 16, 1024);
-                        const uint64_t bd = MODE == kNT ? sdesc_sw128(b + kk * 32, 16, 1024)
-                                                        : sdesc_sw128(b + kk * 2048, kBoxBytes, 1024);
-                        if constexpr (PAIR)
-                            umma_f16_pair(d, ad, bd, p.idesc, (kb | kk) != 0 ? 1u : 0u);
-                        else
-                            umma_f16(d, ad, bd, p.idesc, (kb | kk) != 0 ? 1u : 0u);
-                    };
-                    const int left = depth - kb * 64;
-                    if (left >= 64) {
+                    const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
+                    const int kb_end = kblocks - kb0 < Cf::PIECE ? kblocks : kb0 + Cf::PIECE;
+                    for (int kb = kb0; kb < kb_end; ++kb) {
+                        if (!mbar_wait(&full[stage], phase, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x23, p.wait_ns)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                        const uint32_t a = smem_u32(sA + stage * Cf::A_BYTES), b = smem_u32(sB + stage * Cf::B_BYTES);
+                        // K-major: 8-row atoms 1024 bytes apart, a k step of 16
+                        // moves 32 bytes inside the swizzled row.  MN-major:
+                        // 64-wide boxes, 8-row k groups 1024 bytes apart, a k
+                        // step moves 16 rows.
+                        auto k_step = [&](int kk) {
+                            const uint64_t ad = MODE == kTN ? sdesc_sw128(a + kk * 2048, kBoxBytes, 1024)
+                                                            : sdesc_sw128(a + kk * 32, 16, 1024);
+                            const uint64_t bd = MODE == kNT ? sdesc_sw128(b + kk * 32, 16, 1024)
+                                                            : sdesc_sw128(b + kk * 2048, kBoxBytes, 1024);
+                            if constexpr (PAIR)
+                                umma_f16_pair(d, ad, bd, p.idesc, ((kb - kb0) | kk) != 0 ? 1u : 0u);
+                            else
+                                umma_f16(d, ad, bd, p.idesc, ((kb - kb0) | kk) != 0 ? 1u : 0u);
+                        };
+                        const int left = depth - kb * 64;
+                        if (left >= 64) {
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk) k_step(kk);
-                    } else {
-                        for (int kk = 0; kk * 16 < left; ++kk) k_step(kk);
+                            for (int kk = 0; kk < 4; ++kk) k_step(kk);
+                        } else {
+                            for (int kk = 0; kk * 16 < left; ++kk) k_step(kk);
+                        }
+                        if constexpr (PAIR)
+                            umma_commit_pair(&empty[stage], 0x3);
+                        else
+                            umma_commit(&empty[stage]);
+                        issued = true;
+                        if (++stage == S) {
+                            stage = 0;
+                            phase ^= 1u;
+                        }
                     }
+                    if (!ok) break;
                     if constexpr (PAIR)
-                        umma_commit_pair(&empty[stage], 0x3);
+                        umma_commit_pair(&tfull[acc], 0x3);
                     else
-                        umma_commit(&empty[stage]);
-                    issued = true;
-                    if (++stage == S) {
-                        stage = 0;
-                        phase ^= 1u;
+                        umma_commit(&tfull[acc]);
+                    if (++acc == 2) {
+                        acc = 0;
+                        acc_phase ^= 1u;
                     }
-                }
-                if (!ok) break;
-                if constexpr (PAIR)
-                    umma_commit_pair(&tfull[acc], 0x3);
-                else
-                    umma_commit(&tfull[acc]);
-                if (++acc == 2) {
-                    acc = 0;
-                    acc_phase ^= 1u;
                 }
             }
             if (!ok && issued) {
@@ -595,69 +588,112 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
         const int q = warp & 3;  // TMEM lanes 32q .. 32q + 31
         const int c_first = (warp - 2) / 4 * (BN / 2), c_end = c_first + BN / 2;  // the warp's columns
         uint8_t *buf = epi + (warp - 2) * 2048;
-        const int csize = p.f32 ? 4 : 2;
+        constexpr int csize = F32 ? 4 : 2;
         const int64_t pitch = static_cast<int64_t>(p.N) * csize;
         int acc = 0, g = 0;
         uint32_t acc_phase = 0;
-        for (uint32_t t = first; t < tiles; t += step) {
-            const Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
+        // the warp has read its share of the accumulator
+        auto release = [&] {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (leader)
+                    mbar_arrive(&tempty[acc]);
+                else
+                    mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
+            }
+        };
+        auto turn = [&] {  // to the other accumulator
+            if (++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1u;
+            }
+        };
+        auto wait_full = [&] {
             const bool ok = mbar_wait_sleepy(&tfull[acc], acc_phase, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x24,
                                              p.wait_ns);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            const bool all = __all_sync(0xffffffffu, ok);
             tc_fence_after();
-            // the warp has read its share of the accumulator
-            auto release = [&] {
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) {
-                    if (leader)
-                        mbar_arrive(&tempty[acc]);
-                    else
-                        mbar_arrive_cluster(mapa_shared(smem_u32(&tempty[acc]), 0));
-                }
-            };
+            return all;
+        };
+        const uint32_t tmem_warp = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+        bool ok = true;
+        for (uint32_t t = first; t < tiles && ok; t += step) {
+            const Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
             const int r0 = rank * 128 + q * 32;  // the warp's first row in the tile
             const int rows = min(32, o.valid - r0);
-            const bool empty_sum = MODE == kTN && o.kblocks == 0;
             uint8_t *C = static_cast<uint8_t *>(p.C) +
                          ((MODE == kTN ? static_cast<int64_t>(o.g) * p.M + o.m0 : static_cast<int64_t>(o.row0)) + r0) *
                              pitch;
             // the warp's columns that exist, in steps of 32; none where no row does
             const int left = p.N - o.n0 - c_first;
             const int c_stop = rows > 0 && left > 0 ? min(c_end, c_first + (left + 31) / 32 * 32) : c_first;
-            if (c_stop == c_first) release();
-#pragma unroll 1
-            for (int c = c_first; c < c_stop; c += 32) {
-                uint32_t r[32];
-                __syncwarp();
-                tmem_ld_32x32b_x32(tmem_base + (static_cast<uint32_t>(q * 32) << 16) +
-                                       static_cast<uint32_t>(acc * BN + c), r);
-                tmem_ld_wait();
-                if (c + 32 == c_stop) release();
-                const int col0 = o.n0 + c;
-                const int ncols = min(32, p.N - col0);
-                uint8_t *cbase = C + static_cast<int64_t>(col0) * csize;
-                float x[32];
+            if constexpr (F32) {
+                float x[BN / 2];
 #pragma unroll
-                for (int e = 0; e < 32; ++e) x[e] = p.alpha * __uint_as_float(r[e]);
-                if (empty_sum) {
+                for (int e = 0; e < BN / 2; ++e) x[e] = 0.0f;
+                for (int kb0 = 0; kb0 < o.kblocks || kb0 == 0; kb0 += Cf::PIECE) {
+                    ok = wait_full();
+                    if (!ok) break;
+                    if (o.kblocks > 0) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) x[e] = 0.0f;
-                }
-                if (p.beta != 0.0f && lane < rows) add_old(x, cbase + lane * pitch, ncols, p);
-                if (p.f32) {
-                    // two segments of 16 columns through the one buffer
+                        for (int c = 0; c < BN / 2; c += 16) {
+                            uint32_t r[16];
+                            tmem_ld_32x32b_x16(tmem_warp + static_cast<uint32_t>(acc * BN + c_first + c), r);
+                            tmem_ld_wait();
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        if (s) __syncwarp();
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            *reinterpret_cast<float4 *>(buf + seg_chunk(lane, j)) = make_float4(
-                                x[16 * s + 4 * j], x[16 * s + 4 * j + 1], x[16 * s + 4 * j + 2], x[16 * s + 4 * j + 3]);
-                        __syncwarp();
-                        store_segment<float>(cbase + s * 64, pitch, buf, rows, ncols - 16 * s, p.vec, lane);
+                            for (int e = 0; e < 16; ++e) x[c + e] += __uint_as_float(r[e]);
+                        }
                     }
-                } else {
+                    release();
+                    turn();
+                }
+                if (!ok) break;
+                // segments of 16 columns
+#pragma unroll
+                for (int c = 0; c < BN / 2; c += 16) {
+                    if (c_first + c >= c_stop) break;
+                    const int col0 = o.n0 + c_first + c, ncols = min(16, p.N - col0);
+                    if (ncols <= 0) break;
+                    uint8_t *cbase = C + static_cast<int64_t>(col0) * 4;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[c + e] = o.kblocks ? p.alpha * x[c + e] : 0.0f;
+                    if (p.beta != 0.0f && lane < rows) {
+                        const float *old = reinterpret_cast<const float *>(cbase + lane * pitch);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e)
+                            if (e < ncols) x[c + e] = fmaf(p.beta, old[e], x[c + e]);
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *reinterpret_cast<float4 *>(buf + seg_chunk(lane, j)) =
+                            make_float4(x[c + 4 * j], x[c + 4 * j + 1], x[c + 4 * j + 2], x[c + 4 * j + 3]);
+                    __syncwarp();
+                    store_segment<float>(cbase, pitch, buf, rows, ncols, p.vec, lane);
+                }
+            } else {
+                ok = wait_full();
+                if (!ok) break;
+                if (c_stop == c_first) release();
+#pragma unroll 1
+                for (int c = c_first; c < c_stop; c += 32) {
+                    uint32_t r[32];
+                    __syncwarp();
+                    tmem_ld_32x32b_x32(tmem_warp + static_cast<uint32_t>(acc * BN + c), r);
+                    tmem_ld_wait();
+                    if (c + 32 == c_stop) release();
+                    const int col0 = o.n0 + c;
+                    const int ncols = min(32, p.N - col0);
+                    uint8_t *cbase = C + static_cast<int64_t>(col0) * csize;
+                    float x[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[e] = p.alpha * __uint_as_float(r[e]);
+                    if (MODE == kTN && o.kblocks == 0) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) x[e] = 0.0f;
+                    }
+                    if (p.beta != 0.0f && lane < rows) add_old(x, cbase + lane * pitch, ncols, p);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         uint4 v;
@@ -676,10 +712,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN>::THREADS), 1)
                     __syncwarp();
                     store_segment<uint16_t>(cbase, pitch, buf, rows, ncols, p.vec, lane);
                 }
-            }
-            if (++acc == 2) {
-                acc = 0;
-                acc_phase ^= 1u;
+                turn();
             }
         }
     }
@@ -706,12 +739,12 @@ struct Launch {
 };
 std::mutex g_mu;
 
-template <int MODE, bool PAIR, int BN>
+template <int MODE, bool PAIR, int BN, bool F32 = false>
 int launch_tc(b2b_handle *h, const CUtensorMap &tmA, const CUtensorMap &tmA16, const CUtensorMap &tmB,
               const TcArgs &p, int64_t most_tiles) {
-    using Cf = Cfg<MODE, PAIR, BN>;
+    using Cf = Cfg<MODE, PAIR, BN, F32>;
     static Launch state;
-    auto kernel = grouped_tc_kernel<MODE, PAIR, BN>;
+    auto kernel = grouped_tc_kernel<MODE, PAIR, BN, F32>;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = PAIR ? 2 : 1;
@@ -746,6 +779,15 @@ int launch_tc(b2b_handle *h, const CUtensorMap &tmA, const CUtensorMap &tmA16, c
     cfg.gridDim = dim3((PAIR ? 2 : 1) * units);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmA, tmA16, tmB, p);
     return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, "grouped HGEMM tcgen05 launch");
+}
+
+template <bool F32>
+int launch_wgrad(b2b_handle *h, bool pair, int bn, const CUtensorMap &tmA, const CUtensorMap &tmB, const TcArgs &p,
+                 int64_t most) {
+    if (pair) return launch_tc<kTN, true, 256, F32>(h, tmA, tmA, tmB, p, most);
+    if (bn == 256) return launch_tc<kTN, false, 256, F32>(h, tmA, tmA, tmB, p, most);
+    if (bn == 128) return launch_tc<kTN, false, 128, F32>(h, tmA, tmA, tmB, p, most);
+    return launch_tc<kTN, false, 64, F32>(h, tmA, tmA, tmB, p, most);
 }
 
 // Tensor maps describe rows of a multiple of 16 bytes at 16-byte aligned
@@ -802,7 +844,7 @@ int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, si
         return rc;
     const uint32_t idesc = sm100::idesc_f32acc(bf16, 0, trans_b ? 0 : 1, pair ? 256 : 128, pair ? 256 : bn);
     const TcArgs p{C, offsets, h->d_status, h->wait_limit_ns, G, static_cast<int>(rows), 0, static_cast<int>(n),
-                   static_cast<int>(k), alpha, beta, idesc, bf16, 0, n % 8 == 0 && aligned16(C)};
+                   static_cast<int>(k), alpha, beta, idesc, bf16, n % 8 == 0 && aligned16(C)};
     const int bm = pair ? 256 : 128;
     const int64_t most = (R / bm + (R < G ? R : G)) * ((N + bn - 1) / bn);
     if (trans_b) {
@@ -836,13 +878,10 @@ int launch_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t group
     if (int rc = encode_tma_2d(&tmB, dt, 2, B, rows, n, 64, 64)) return rc;
     const uint32_t idesc = sm100::idesc_f32acc(bf16, 1, 1, pair ? 256 : 128, pair ? 256 : bn);
     const TcArgs p{C, offsets, h->d_status, h->wait_limit_ns, G, static_cast<int>(rows), static_cast<int>(m),
-                   static_cast<int>(n), 0, alpha, beta, idesc, bf16, f32, n % (f32 ? 4 : 8) == 0 && aligned16(C)};
+                   static_cast<int>(n), 0, alpha, beta, idesc, bf16, n % (f32 ? 4 : 8) == 0 && aligned16(C)};
     const int bm = pair ? 256 : 128;
     const int64_t most = G * ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
-    if (pair) return launch_tc<kTN, true, 256>(h, tmA, tmA, tmB, p, most);
-    if (bn == 256) return launch_tc<kTN, false, 256>(h, tmA, tmA, tmB, p, most);
-    if (bn == 128) return launch_tc<kTN, false, 128>(h, tmA, tmA, tmB, p, most);
-    return launch_tc<kTN, false, 64>(h, tmA, tmA, tmB, p, most);
+    return f32 ? launch_wgrad<true>(h, pair, bn, tmA, tmB, p, most) : launch_wgrad<false>(h, pair, bn, tmA, tmB, p, most);
 }
 
 }  // namespace b2b

@@ -211,17 +211,41 @@ def test_wgrad_alpha_beta(handle, f32, alpha, beta, m, n):
     check_wgrad(handle, "bf16", f32, [129, 0, 50], m, n, pad=2, alpha=alpha, beta=beta)
 
 
-@pytest.mark.parametrize("n", [72, 65])
-def test_wgrad_neighbours_nan_stays_out(handle, n):
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("m,n", [(136, 72), (264, 520), (65, 63)])
+def test_wgrad_long_groups(handle, t, f32, m, n):
+    check_wgrad(handle, t, f32, [513, 512, 0, 1500, 64], m, n, pad=7)
+    check_wgrad(handle, t, f32, [1027, 1, 600], m, n, alpha=-0.5, beta=2.0)
+
+
+@pytest.mark.parametrize("m,n", [(264, 264), (64, 72)])
+def test_wgrad_f32_keeps_f32_sums(handle, m, n):
+    """An addition in the accumulators may drop up to 2^-23 of the running sum;
+    sums are taken in pieces of 512 terms, 32 additions of 16.  On random terms
+    the running sum after i of 32 is about sqrt(i / 32) of the last, so the
+    pieces, and with them C, are off by at most 2^-23 * sum_i sqrt(i / 32) =
+    21.7 * 2^-23 of their size; the rounded additions of the pieces and inside
+    a step add a few 2^-24."""
+    rng = np.random.default_rng(12)
+    off = R.offsets_of([4096, 2000])
+    a, b = (R.value(R.bits(rng.standard_normal((off[-1], w)), "bf16"), "bf16") for w in (m, n))
+    c = np.zeros((2, m, n))
+    got, want = run_wgrad(handle, "bf16", True, a, b, off, c), R.wgrad(a, b, off, c)
+    assert np.linalg.norm(got - want) <= 25 * 2.0 ** -23 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("m,n", [(72, 72), (72, 65), (136, 136), (264, 264)])
+def test_wgrad_neighbours_nan_stays_out(handle, m, n):
     """Every count from 1 to 40 next to a group of NaN: the last k step of a
     group ends inside a block that holds the next group's rows."""
     rng = np.random.default_rng(8)
     counts = [x for i in range(1, 41) for x in (i, 1)]
     off = R.offsets_of(counts)
-    a, b = whole(rng, (off[-1], 72)), whole(rng, (off[-1], n))
+    a, b = whole(rng, (off[-1], m)), whole(rng, (off[-1], n))
     for g in range(1, len(counts), 2):
         a[off[g]], b[off[g]] = np.nan, np.inf
-    c = np.zeros((len(counts), 72, n))
+    c = np.zeros((len(counts), m, n))
     got = run_wgrad(handle, "f16", False, a, b, off, c)
     with np.errstate(invalid="ignore"):
         want = R.bits(R.wgrad(a, b, off, c), "f16")
