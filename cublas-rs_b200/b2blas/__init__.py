@@ -124,6 +124,11 @@ def _hp(a: np.ndarray) -> ctypes.c_void_p:
     return ctypes.c_void_p(a.ctypes.data)
 
 
+# np.dtype() of the element types that buffers commonly have.
+_DTYPE = {t: np.dtype(t) for t in (np.uint8, np.uint16, np.int32, np.uint32, np.uint64, np.float32, np.float64)}
+_U8, _U16, _I32, _F32 = (_DTYPE[t] for t in (np.uint8, np.uint16, np.int32, np.float32))
+
+
 class DeviceBuffer:
     """Typed device allocation, the stand-in for cuda_core::DeviceBuffer<T>
     (re-exported as cublas_rs::DeviceBuf, crates/cublas-rs/src/lib.rs:34).
@@ -135,7 +140,7 @@ class DeviceBuffer:
         self.handle = handle
         self.ptr = int(ptr)
         self._len = int(length)
-        self.dtype = np.dtype(dtype)
+        self.dtype = _DTYPE[dtype] if type(dtype) is type and dtype in _DTYPE else np.dtype(dtype)
         self._owner = owner
         self._owned = owned
 
@@ -164,7 +169,7 @@ class DeviceBuffer:
     @classmethod
     def from_ptr(cls, handle: "Handle", ptr: int, length: int, dtype, owner: Any = None) -> "DeviceBuffer":
         """Non-owning view of existing device memory (kept alive by `owner`)."""
-        return cls(handle, ptr, length, dtype, owner=owner, owned=False)
+        return cls(handle, ptr, length, dtype, owner, False)
 
     def to_host_vec(self) -> np.ndarray:
         return self.handle.download(self)
@@ -298,10 +303,10 @@ class Handle:
     # ---- helpers
     @staticmethod
     def _need(buf: DeviceBuffer, n: int, what: str, dtype) -> None:
-        if buf.dtype != np.dtype(dtype):
+        if buf.dtype is not dtype and buf.dtype != np.dtype(dtype):
             raise CublasError(3, f"{what} has dtype {buf.dtype}, expected {np.dtype(dtype)}")
-        if len(buf) < n:
-            raise CublasError(2, f"dimension mismatch in {what}: expected {n}, got {len(buf)}")
+        if buf._len < n:
+            raise CublasError(2, f"dimension mismatch in {what}: expected {n}, got {buf._len}")
 
     def _gemm_dev(self, fn, algo, cfg: GemmConfig, a, b, c, dtype):
         m, n, k = cfg.m, cfg.n, cfg.k
@@ -478,13 +483,13 @@ class Handle:
         DeviceBuffer of groups + 1 values.  a, b, c are uint16 bit patterns."""
         m, n, k = config.m, config.n, config.k
         if m and n and k and groups:
-            self._need(a, m * k, "A", np.uint16)
-            self._need(b, groups * k * n, "B", np.uint16)
-            self._need(offsets, groups + 1, "offsets", np.int32)
-            self._need(c, m * n, "C", np.uint16)
+            self._need(a, m * k, "A", _U16)
+            self._need(b, groups * k * n, "B", _U16)
+            self._need(offsets, groups + 1, "offsets", _I32)
+            self._need(c, m * n, "C", _U16)
         _check(self._lib.b2b_hgemm_grouped(
-            self._h, int(half), 1 if trans_b else 0, groups, m, n, k, config.alpha, ctypes.c_void_p(a.ptr),
-            ctypes.c_void_p(b.ptr), config.beta, ctypes.c_void_p(c.ptr), ctypes.c_void_p(offsets.ptr)))
+            self._h, int(half), 1 if trans_b else 0, groups, m, n, k, config.alpha, a.ptr,
+            b.ptr, config.beta, c.ptr, offsets.ptr))
 
     def hgemm_grouped_wgrad(self, config, groups, a, b, offsets, c, half=Half.F16):
         """C_g = alpha*A[rows of g]^T*B[rows of g] + beta*C_g
@@ -492,15 +497,15 @@ class Handle:
         B (k x n); c holds `groups` m x n matrices, in float32 or in the
         operands' type (uint16), by its dtype."""
         m, n, rows = config.m, config.n, config.k
-        f32 = c.dtype == np.dtype(np.float32)
+        f32 = c.dtype == _F32
         if m and n and groups:
-            self._need(a, rows * m, "A", np.uint16)
-            self._need(b, rows * n, "B", np.uint16)
-            self._need(offsets, groups + 1, "offsets", np.int32)
-            self._need(c, groups * m * n, "C", np.float32 if f32 else np.uint16)
+            self._need(a, rows * m, "A", _U16)
+            self._need(b, rows * n, "B", _U16)
+            self._need(offsets, groups + 1, "offsets", _I32)
+            self._need(c, groups * m * n, "C", _F32 if f32 else _U16)
         _check(self._lib.b2b_hgemm_grouped_wgrad(
-            self._h, int(half), 2 if f32 else int(half), groups, rows, m, n, config.alpha, ctypes.c_void_p(a.ptr),
-            ctypes.c_void_p(b.ptr), config.beta, ctypes.c_void_p(c.ptr), ctypes.c_void_p(offsets.ptr)))
+            self._h, int(half), 2 if f32 else int(half), groups, rows, m, n, config.alpha, a.ptr,
+            b.ptr, config.beta, c.ptr, offsets.ptr))
 
     # ---- Level 2: SGEMV (lib.rs:230-309)
     def sgemv(self, trans, m, n, alpha, a, x, beta, y, algo=Algo.Default):
@@ -559,58 +564,58 @@ class Handle:
     # ---- Level 2: 4-bit weights (no reference counterpart)
     def _need_w4(self, matrices, m, n, group, packed, scales, zeros):
         gs = -(-n // group) if group > 0 else 0  # the library refuses a group of 0
-        self._need(packed, matrices * m * ((n + 1) // 2), "packed", np.uint8)
-        self._need(scales, matrices * m * gs, "scales", np.uint16)
+        self._need(packed, matrices * m * ((n + 1) // 2), "packed", _U8)
+        self._need(scales, matrices * m * gs, "scales", _U16)
         if zeros is not None:
-            self._need(zeros, matrices * m * gs, "zeros", np.uint8)
-        return ctypes.c_void_p(zeros.ptr if zeros is not None else 0)
+            self._need(zeros, matrices * m * gs, "zeros", _U8)
+        return zeros.ptr if zeros is not None else 0
 
     def quantize_w4(self, m, n, group, w, packed, scales, zeros=None, half=Half.F16):
         """W (m x n, uint16 bit patterns) to 4-bit values with one scale, and
         with `zeros` one zero point, per group of columns (b2b_quantize_w4)."""
-        z = ctypes.c_void_p(zeros.ptr if zeros is not None else 0)
+        z = zeros.ptr if zeros is not None else 0
         if m and n:
             z = self._need_w4(1, m, n, group, packed, scales, zeros)
-            self._need(w, m * n, "W", np.uint16)
-        _check(self._lib.b2b_quantize_w4(self._h, int(half), m, n, group, ctypes.c_void_p(w.ptr),
-                                         ctypes.c_void_p(packed.ptr), ctypes.c_void_p(scales.ptr), z))
+            self._need(w, m * n, "W", _U16)
+        _check(self._lib.b2b_quantize_w4(self._h, int(half), m, n, group, w.ptr,
+                                         packed.ptr, scales.ptr, z))
 
     def dequantize_w4(self, m, n, group, packed, scales, zeros, w, half=Half.F16):
         """4-bit values back to the 16-bit W (b2b_dequantize_w4); zeros may be None."""
-        z = ctypes.c_void_p(zeros.ptr if zeros is not None else 0)
+        z = zeros.ptr if zeros is not None else 0
         if m and n:
             z = self._need_w4(1, m, n, group, packed, scales, zeros)
-            self._need(w, m * n, "W", np.uint16)
-        _check(self._lib.b2b_dequantize_w4(self._h, int(half), m, n, group, ctypes.c_void_p(packed.ptr),
-                                           ctypes.c_void_p(scales.ptr), z, ctypes.c_void_p(w.ptr)))
+            self._need(w, m * n, "W", _U16)
+        _check(self._lib.b2b_dequantize_w4(self._h, int(half), m, n, group, packed.ptr,
+                                           scales.ptr, z, w.ptr))
 
     def hgemv_w4(self, m, n, group, alpha, packed, scales, zeros, x, beta, y, count=1, half=Half.F16):
         """y_i = alpha*W*x_i + beta*y_i for `count` vectors with the 4-bit W
         (b2b_hgemv_w4); zeros may be None."""
-        z = ctypes.c_void_p(zeros.ptr if zeros is not None else 0)
+        z = zeros.ptr if zeros is not None else 0
         if m and n and count:
             z = self._need_w4(1, m, n, group, packed, scales, zeros)
-            self._need(x, count * n, "x", np.uint16)
-            self._need(y, count * m, "y", np.uint16)
-        _check(self._lib.b2b_hgemv_w4(self._h, int(half), m, n, group, alpha, ctypes.c_void_p(packed.ptr),
-                                      ctypes.c_void_p(scales.ptr), z, ctypes.c_void_p(x.ptr), count, beta,
-                                      ctypes.c_void_p(y.ptr)))
+            self._need(x, count * n, "x", _U16)
+            self._need(y, count * m, "y", _U16)
+        _check(self._lib.b2b_hgemv_w4(self._h, int(half), m, n, group, alpha, packed.ptr,
+                                      scales.ptr, z, x.ptr, count, beta,
+                                      y.ptr))
 
     def hgemv_w4_grouped(self, groups, m, n, group, alpha, packed, scales, zeros, x, index, beta, y, count, fan=1,
                          half=Half.F16):
         """y_i = alpha*W_e*x_{i // fan} + beta*y_i with e = index[i] of `groups`
         4-bit matrices (b2b_hgemv_w4_grouped); index is an int32 DeviceBuffer,
         and one outside [0, groups) names no expert."""
-        z = ctypes.c_void_p(zeros.ptr if zeros is not None else 0)
+        z = zeros.ptr if zeros is not None else 0
         if m and n and count and groups:
             z = self._need_w4(groups, m, n, group, packed, scales, zeros)
             if fan > 0:  # the library refuses a fan of 0
-                self._need(x, -(-count // fan) * n, "x", np.uint16)
-            self._need(index, count, "index", np.int32)
-            self._need(y, count * m, "y", np.uint16)
+                self._need(x, -(-count // fan) * n, "x", _U16)
+            self._need(index, count, "index", _I32)
+            self._need(y, count * m, "y", _U16)
         _check(self._lib.b2b_hgemv_w4_grouped(
-            self._h, int(half), groups, m, n, group, alpha, ctypes.c_void_p(packed.ptr), ctypes.c_void_p(scales.ptr),
-            z, ctypes.c_void_p(x.ptr), count, fan, ctypes.c_void_p(index.ptr), beta, ctypes.c_void_p(y.ptr)))
+            self._h, int(half), groups, m, n, group, alpha, packed.ptr, scales.ptr,
+            z, x.ptr, count, fan, index.ptr, beta, y.ptr))
 
     # ---- Level 1: SAXPY (lib.rs:110-129)
     def saxpy(self, n, alpha, x, y):
