@@ -21,26 +21,11 @@ namespace {
 
 constexpr int kMaxGroups = 1024;
 
-// One product of every group, addressed by strides: within group g, sum over
-// kk of A(i, kk) * B(kk, j) for M x N outputs.
-struct GroupedArgs {
-    const uint16_t *A, *B;
-    void *C;
-    const int32_t *offsets;
-    int *status;
-    int groups;
-    int64_t rows;    // rows of A (and of C, or of B in wgrad)
-    int64_t M, N, K; // M is the group's row count in forward, K in wgrad
-    int64_t a_i, a_k, b_k, b_j;
-    float alpha, beta;
-};
-
 // Tiles of `bm` rows that groups 0..g-1 hold, for g = 0..groups, in
-// start[0..groups], and the offsets themselves in off[0..groups] (when given);
-// false when the offsets do not ascend within [0, rows].
+// start[0..groups], and the offsets themselves in off[0..groups]; false when
+// the offsets do not ascend within [0, rows].
 // One warp; every lane returns the verdict.
-__device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, int bm, int *start,
-                            int *off = nullptr) {
+__device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, int bm, int *start, int *off) {
     const int lane = threadIdx.x & 31;
     bool ok = true;
     int carry = 0;
@@ -49,10 +34,8 @@ __device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, in
         int tiles = 0;
         if (g < groups) {
             const int64_t lo = offsets[g], hi = offsets[g + 1];
-            if (off) {
-                off[g] = static_cast<int>(lo);
-                if (g == groups - 1) off[groups] = static_cast<int>(hi);
-            }
+            off[g] = static_cast<int>(lo);
+            if (g == groups - 1) off[groups] = static_cast<int>(hi);
             if (lo < 0 || hi < lo || hi > rows)
                 ok = false;
             else
@@ -70,87 +53,6 @@ __device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, in
     if (lane == 0) start[0] = 0;
     return __all_sync(0xffffffffu, ok);
 }
-
-// 64 x 64 tiles, 4 x 4 outputs a thread, f32 sums: right for every size,
-// stride and alignment.
-template <bool BF16, bool WGRAD, bool F32>
-__global__ void __launch_bounds__(256) grouped_simt_kernel(GroupedArgs p) {
-    using H = b2b::Half16<BF16>;
-    __shared__ float As[16][64 + 4];
-    __shared__ float Bs[16][64 + 4];
-    __shared__ int start[kMaxGroups + 1];
-    __shared__ int valid;
-    const int tid = threadIdx.x;
-    if (tid < 32) {
-        const bool ok = scan_groups(p.offsets, p.groups, p.rows, 64, start);
-        if (tid == 0) {
-            valid = ok;
-            if (!ok) atomicCAS(p.status, 0, B2B_DEVSTAT_OFFSETS);
-        }
-    }
-    __syncthreads();
-    if (!valid) return;
-    const int tx = tid & 15, ty = tid >> 4;
-    const int64_t tiles_n = (p.N + 63) / 64;
-    const int64_t tiles_m = (p.M + 63) / 64;  // wgrad
-    const int64_t tiles = WGRAD ? p.groups * tiles_m * tiles_n : start[p.groups] * tiles_n;
-    int g = 0;
-    for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
-        int64_t m0;
-        const int64_t n0 = t % tiles_n * 64;
-        if (WGRAD) {
-            g = static_cast<int>(t / (tiles_m * tiles_n));
-            m0 = t / tiles_n % tiles_m * 64;
-        } else {
-            while (t / tiles_n >= start[g + 1]) ++g;
-            m0 = (t / tiles_n - start[g]) * 64;
-        }
-        const int64_t row0 = p.offsets[g], count = p.offsets[g + 1] - row0;
-        const int64_t M = WGRAD ? p.M : count, K = WGRAD ? count : p.K;
-        const uint16_t *A = p.A + (WGRAD ? row0 * p.a_k : row0 * p.a_i);
-        const uint16_t *B = p.B + (WGRAD ? row0 * p.b_k : g * p.N * p.K);
-        const int64_t c0 = WGRAD ? g * p.M * p.N : row0 * p.N;
-        float acc[4][4] = {};
-        for (int64_t k0 = 0; k0 < K; k0 += 16) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int idx = tid + i * 256;
-                const int r = idx & 63, kc = idx >> 6;
-                const int64_t kk = k0 + kc;
-                As[kc][r] = m0 + r < M && kk < K ? H::get(A[(m0 + r) * p.a_i + kk * p.a_k]) : 0.0f;
-                Bs[kc][r] = n0 + r < p.N && kk < K ? H::get(B[(n0 + r) * p.b_j + kk * p.b_k]) : 0.0f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int kk = 0; kk < 16; ++kk)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        acc[i][j] = fmaf(As[kk][ty * 4 + i], Bs[kk][tx * 4 + j], acc[i][j]);
-            __syncthreads();
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (m0 + ty * 4 + i >= M) continue;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (n0 + tx * 4 + j >= p.N) continue;
-                const int64_t at = c0 + (m0 + ty * 4 + i) * p.N + n0 + tx * 4 + j;
-                float v = K ? p.alpha * acc[i][j] : 0.0f;
-                if constexpr (F32) {
-                    float *C = static_cast<float *>(p.C);
-                    C[at] = p.beta != 0.0f ? fmaf(p.beta, C[at], v) : v;
-                } else {
-                    uint16_t *C = static_cast<uint16_t *>(p.C);
-                    if (p.beta != 0.0f) v = fmaf(p.beta, H::get(C[at]), v);
-                    C[at] = H::put(v);
-                }
-            }
-        }
-    }
-}
-
 
 // ---------------------------------------------------------------------------
 // Tensor-core kernel: tcgen05.mma on 128 x BN tiles of one CTA, or 256 x 256
@@ -177,15 +79,22 @@ __global__ void __launch_bounds__(256) grouped_simt_kernel(GroupedArgs p) {
 // rows past the end, in A and B both (0 times a neighbour's NaN is a NaN),
 // up to the next multiple of 16, and the MMA issues only those k steps.
 //
+// Operands that TMA cannot describe (rows of a length or at a base that is not
+// a multiple of 16 bytes) are loaded by the HAND form: six warps in pairs, one
+// for A and one for B of a k block, three blocks at a time, write the same
+// swizzled layouts with plain loads and fill ragged edges with zeros
+// themselves.
+//
 // Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer, 2..9 epilogue, 10
-// (kTN) the wiper.  Two accumulators: the epilogue of a tile runs under the
+// (kTN) the wiper; HAND: 10..15 load.  Two accumulators: the epilogue of a tile runs under the
 // MMAs of the next.  The epilogue goes through shared memory to 64-byte row
 // segments, since a TMA store would write past the group's last row; it is a
 // chain of short latencies, so two warps share each quarter of the TMEM lanes.
 enum Mode { kNN = 0, kNT = 1, kTN = 2 };
 
-template <int MODE, bool PAIR, int BN_, bool F32_>
+template <int MODE, bool PAIR, int BN_, bool F32_, bool HAND_>
 struct Cfg {
+    static constexpr bool HAND = HAND_;                // loads by warps
     static constexpr bool F32 = F32_;                  // C is f32 (kTN)
     static constexpr int PIECE = F32 ? 8 : 1 << 30;    // k blocks that an accumulator sums up
     static constexpr int BN = BN_;                     // columns of a tile
@@ -197,7 +106,7 @@ struct Cfg {
     static constexpr int STAGES = 196608 / STAGE_BYTES;
     static constexpr int EPI_BYTES = 8 * 2048;  // 32 rows of 64 bytes for each epilogue warp
     static constexpr int TMEM_COLS = 2 * BN;
-    static constexpr int THREADS = MODE == kTN ? 352 : 320;
+    static constexpr int THREADS = HAND ? 512 : MODE == kTN ? 352 : 320;
     static constexpr int TABLE_BYTES = 2 * 4224;  // tile starts and offsets: kMaxGroups + 1 ints each, rounded up
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + TABLE_BYTES + 1024 + 512;
     static_assert(SMEM_BYTES <= 232448 && TABLE_BYTES / 2 >= 4 * (kMaxGroups + 1), "shared memory per CTA");
@@ -206,6 +115,7 @@ constexpr int kBoxBytes = 64 * 64 * 2;  // 64 columns x 64 rows of an MN-major o
 constexpr int kGroupM = 16;             // raster: tile rows that sweep a group's columns together
 
 struct TcArgs {
+    const uint16_t *A, *B;  // HAND
     void *C;
     const int32_t *offsets;
     int *status;
@@ -315,12 +225,73 @@ __device__ __forceinline__ void add_old(float (&x)[32], const uint8_t *row, int 
     }
 }
 
-template <int MODE, bool PAIR, int BN, bool F32>
-__global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32>::THREADS), 1)
+// 8 values from p on, of which `have` exist, as a 16-byte piece.  p is 2-byte
+// aligned; nothing outside the values is read.
+struct Piece {
+    uint32_t w[4];
+    uint16_t first, last;
+    bool odd;
+    __device__ __forceinline__ void load(const uint16_t *p, int have) {
+        odd = false;
+        if (have >= 8) {
+            odd = (reinterpret_cast<uintptr_t>(p) & 2) != 0;
+            if (!odd) {
+                const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = __ldg(q + i);
+            } else {
+                first = __ldg(p);
+                last = __ldg(p + 7);
+                const uint32_t *q = reinterpret_cast<const uint32_t *>(p + 1);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) w[i] = __ldg(q + i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = 2 * i < have ? __ldg(p + 2 * i) : 0u;
+                if (2 * i + 1 < have) w[i] |= static_cast<uint32_t>(__ldg(p + 2 * i + 1)) << 16;
+            }
+        }
+    }
+    __device__ __forceinline__ uint4 get() const {
+        if (!odd) return make_uint4(w[0], w[1], w[2], w[3]);
+        return make_uint4(first | w[0] << 16, __funnelshift_r(w[0], w[1], 16), __funnelshift_r(w[1], w[2], 16),
+                          w[2] >> 16 | static_cast<uint32_t>(last) << 16);
+    }
+};
+
+// One warp writes an operand's 16 KiB of a stage: 128 rows of 64 k values
+// (K_MAJOR: `slow` rows exist and `fast` k values), or two boxes of 64 k rows
+// of 64 columns (`slow` k rows and `fast` columns exist), zeros elsewhere, in
+// the 128-byte swizzle.  8 pieces of a lane are in flight at once.
+template <bool K_MAJOR>
+__device__ __forceinline__ void fill_by_hand(uint8_t *to, const uint16_t *from, int ld, int slow, int fast, int lane) {
+#pragma unroll 1
+    for (int i0 = lane; i0 < 1024; i0 += 256) {
+        Piece piece[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + 32 * j, c = i & 7;
+            const int row = K_MAJOR ? i >> 3 : i >> 3 & 63, at = K_MAJOR ? c * 8 : (i >> 9) * 64 + c * 8;
+            piece[j].load(from + static_cast<int64_t>(row) * ld + at, row < slow ? fast - at : 0);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int i = i0 + 32 * j, c = i & 7;
+            const int row = K_MAJOR ? i >> 3 : i >> 3 & 63;
+            *reinterpret_cast<uint4 *>(to + (K_MAJOR ? 0 : (i >> 9) * kBoxBytes) + row * 128 + ((c ^ (row & 7)) << 4)) =
+                piece[j].get();
+        }
+    }
+}
+
+template <int MODE, bool PAIR, int BN, bool F32, bool HAND>
+__global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA16,
                       const __grid_constant__ CUtensorMap tmB, TcArgs p) {
     using namespace sm100;
-    using Cf = Cfg<MODE, PAIR, BN, F32>;
+    using Cf = Cfg<MODE, PAIR, BN, F32, HAND>;
     constexpr int S = Cf::STAGES;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -344,8 +315,9 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32>::THREADS), 1)
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
             // a pair's kTN stage is full when both CTAs say so: their
-            // producers, or for a group's last k block their wipers
-            mbar_init(&full[s], PAIR && MODE == kTN ? 2 : 1);
+            // producers, or for a group's last k block their wipers; HAND:
+            // when both its warps do
+            mbar_init(&full[s], HAND || (PAIR && MODE == kTN) ? 2 : 1);
             mbar_init(&empty[s], 1);
             mbar_init(&landed[s], 1);
         }
@@ -356,8 +328,10 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32>::THREADS), 1)
         mbar_init(drain, 1);
         *abort_flag = 0;
         fence_barrier_init();
-        prefetch_tensormap(&tmA);
-        prefetch_tensormap(&tmB);
+        if constexpr (!HAND) {
+            prefetch_tensormap(&tmA);
+            prefetch_tensormap(&tmB);
+        }
     }
     if (warp == 1) {
         if constexpr (PAIR) {
@@ -390,7 +364,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32>::THREADS), 1)
 
     if (warp == 0) {
         // ------------------------------------------------ TMA producer
-        if (lane == 0) {
+        if (!HAND && lane == 0) {
             int stage = 0, g = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -553,7 +527,46 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32>::THREADS), 1)
             }
         }
         __syncwarp();
-    } else if (MODE == kTN && warp == 10) {
+    } else if (HAND && warp >= 10) {
+        // ------------------------------------------------ loading warps (HAND)
+        const int pair = (warp - 10) >> 1;
+        const bool is_b = (warp - 10) & 1;
+        int g = 0;
+        uint32_t it = 0;  // k blocks of all tiles so far
+        bool ok = true;
+        for (uint32_t t = first; t < tiles && ok; t += step) {
+            const Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
+            for (int kb = 0; kb < o.kblocks; ++kb, ++it) {
+                if (static_cast<int>(it % 3u) != pair) continue;
+                const int s = static_cast<int>(it % S);
+                const uint32_t phase = it / S & 1u;
+                ok = mbar_wait(&empty[s], phase ^ 1u, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x21, p.wait_ns);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const int k0 = kb * 64, k_left = o.depth - k0;
+                if (!is_b) {
+                    if constexpr (MODE == kTN)
+                        fill_by_hand<false>(sA + s * Cf::A_BYTES, p.A + static_cast<int64_t>(o.row0 + k0) * p.M + o.m0, p.M,
+                                            k_left, p.M - o.m0, lane);
+                    else
+                        fill_by_hand<true>(sA + s * Cf::A_BYTES, p.A + static_cast<int64_t>(o.row0) * p.K + k0, p.K,
+                                           o.valid, k_left, lane);
+                } else {
+                    const int64_t matrix = MODE == kTN ? static_cast<int64_t>(o.row0) * p.N
+                                                       : static_cast<int64_t>(o.g) * p.N * p.K;
+                    if constexpr (MODE == kNT)
+                        fill_by_hand<true>(sB + s * Cf::B_BYTES, p.B + matrix + static_cast<int64_t>(o.n0) * p.K + k0, p.K,
+                                           p.N - o.n0, k_left, lane);
+                    else
+                        fill_by_hand<false>(sB + s * Cf::B_BYTES, p.B + matrix + static_cast<int64_t>(k0) * p.N + o.n0, p.N,
+                                            k_left, p.N - o.n0, lane);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&full[s]);
+            }
+        }
+    } else if (!HAND && MODE == kTN && warp == 10) {
         // ------------------------------------------------ wiper (kTN)
         int stage = 0, g = 0;
         uint32_t phases = 0;  // bit s: parity of landed[s]
@@ -739,12 +752,12 @@ struct Launch {
 };
 std::mutex g_mu;
 
-template <int MODE, bool PAIR, int BN, bool F32 = false>
+template <int MODE, bool PAIR, int BN, bool F32 = false, bool HAND = false>
 int launch_tc(b2b_handle *h, const CUtensorMap &tmA, const CUtensorMap &tmA16, const CUtensorMap &tmB,
               const TcArgs &p, int64_t most_tiles) {
-    using Cf = Cfg<MODE, PAIR, BN, F32>;
+    using Cf = Cfg<MODE, PAIR, BN, F32, HAND>;
     static Launch state;
-    auto kernel = grouped_tc_kernel<MODE, PAIR, BN, F32>;
+    auto kernel = grouped_tc_kernel<MODE, PAIR, BN, F32, HAND>;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = PAIR ? 2 : 1;
@@ -796,15 +809,6 @@ bool tma_can(const void *A, const void *B, int64_t ld_a, int64_t rows_b, int64_t
     return b2b::aligned16(A) && b2b::aligned16(B) && ld_a % 8 == 0 && ld_b % 8 == 0 && rows_b * ld_b < (1ll << 39);
 }
 
-template <bool WGRAD, bool F32>
-int launch_simt(b2b_handle *h, int type, const GroupedArgs &p) {
-    auto kernel = type == B2B_TYPE_BF16 ? grouped_simt_kernel<true, WGRAD, F32> : grouped_simt_kernel<false, WGRAD, F32>;
-    const int ctas = b2b::resident_ctas(h, reinterpret_cast<const void *>(kernel), 256, 0);
-    kernel<<<ctas, 256, 0, h->stream>>>(p);
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, "grouped HGEMM launch");
-}
-
 }  // namespace
 
 namespace b2b {
@@ -815,10 +819,17 @@ int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, si
     const int64_t N = static_cast<int64_t>(n), K = static_cast<int64_t>(k), R = static_cast<int64_t>(rows);
     const int G = static_cast<int>(groups);
     const bool bf16 = type == B2B_TYPE_BF16;
-    if (!tma_can(A, B, K, trans_b ? N : K, trans_b ? K : N) || (R / 128 + (R < G ? R : G)) * (N / 64 + 1) >= 1ll << 31) {
-        const GroupedArgs p{A, B, C, offsets, h->d_status, G, R, 0, N, K, K, 1, trans_b ? 1 : N, trans_b ? K : 1,
-                            alpha, beta};
-        return launch_simt<false, false>(h, type, p);
+    const bool tma = tma_can(A, B, K, trans_b ? N : K, trans_b ? K : N);
+    if ((R / 128 + (R < G ? R : G)) * (N / 64 + 1) >= 1ll << 31)
+        return fail(B2B_ERR_NOT_SUPPORTED, "grouped HGEMM: 2^31 tiles or more");
+    TcArgs p{A, B, C, offsets, h->d_status, h->wait_limit_ns, G, static_cast<int>(rows), 0, static_cast<int>(n),
+             static_cast<int>(k), alpha, beta, 0, bf16, n % 8 == 0 && aligned16(C)};
+    if (!tma) {
+        p.idesc = sm100::idesc_f32acc(bf16, 0, trans_b ? 0 : 1, 128, 128);
+        const int64_t most = (R / 128 + (R < G ? R : G)) * ((N + 127) / 128);
+        const CUtensorMap none{};
+        return trans_b ? launch_tc<kNT, false, 128, false, true>(h, none, none, none, p, most)
+                       : launch_tc<kNN, false, 128, false, true>(h, none, none, none, p, most);
     }
     // pairs where groups are long enough on average to fill their 256 rows
     const bool pair = R >= 192 * static_cast<int64_t>(G) && N > 128;
@@ -842,9 +853,7 @@ int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, si
     if (int rc = encode_tma_3d(&tmB, dt, 2, B, cols, brows, groups, cols * 2, cols * brows * 2, 64, trans_b ? ncta : 64,
                                CU_TENSOR_MAP_SWIZZLE_128B))
         return rc;
-    const uint32_t idesc = sm100::idesc_f32acc(bf16, 0, trans_b ? 0 : 1, pair ? 256 : 128, pair ? 256 : bn);
-    const TcArgs p{C, offsets, h->d_status, h->wait_limit_ns, G, static_cast<int>(rows), 0, static_cast<int>(n),
-                   static_cast<int>(k), alpha, beta, idesc, bf16, n % 8 == 0 && aligned16(C)};
+    p.idesc = sm100::idesc_f32acc(bf16, 0, trans_b ? 0 : 1, pair ? 256 : 128, pair ? 256 : bn);
     const int bm = pair ? 256 : 128;
     const int64_t most = (R / bm + (R < G ? R : G)) * ((N + bn - 1) / bn);
     if (trans_b) {
@@ -865,9 +874,16 @@ int launch_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t group
     const int64_t M = static_cast<int64_t>(m), N = static_cast<int64_t>(n), R = static_cast<int64_t>(rows);
     const int G = static_cast<int>(groups);
     const bool bf16 = type == B2B_TYPE_BF16, f32 = c_type == B2B_TYPE_F32;
-    if (rows == 0 || !tma_can(A, B, M, 1, N) || G * (M / 128 + 1) * (N / 64 + 1) >= 1ll << 31) {
-        const GroupedArgs p{A, B, C, offsets, h->d_status, G, R, M, N, 0, 1, M, N, 1, alpha, beta};
-        return f32 ? launch_simt<true, true>(h, type, p) : launch_simt<true, false>(h, type, p);
+    if (G * (M / 128 + 1) * (N / 64 + 1) >= 1ll << 31)
+        return fail(B2B_ERR_NOT_SUPPORTED, "grouped HGEMM: 2^31 tiles or more");
+    TcArgs p{A, B, C, offsets, h->d_status, h->wait_limit_ns, G, static_cast<int>(rows), static_cast<int>(m),
+             static_cast<int>(n), 0, alpha, beta, 0, bf16, n % (f32 ? 4 : 8) == 0 && aligned16(C)};
+    if (rows == 0 || !tma_can(A, B, M, 1, N)) {  // without rows nothing is loaded
+        p.idesc = sm100::idesc_f32acc(bf16, 1, 1, 128, 128);
+        const int64_t most = G * ((M + 127) / 128) * ((N + 127) / 128);
+        const CUtensorMap none{};
+        return f32 ? launch_tc<kTN, false, 128, true, true>(h, none, none, none, p, most)
+                   : launch_tc<kTN, false, 128, false, true>(h, none, none, none, p, most);
     }
     const bool pair = M > 128 && N > 128;
     int bn = 256;
@@ -876,9 +892,7 @@ int launch_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t group
     CUtensorMap tmA, tmB;
     if (int rc = encode_tma_2d(&tmA, dt, 2, A, rows, m, 64, 64)) return rc;
     if (int rc = encode_tma_2d(&tmB, dt, 2, B, rows, n, 64, 64)) return rc;
-    const uint32_t idesc = sm100::idesc_f32acc(bf16, 1, 1, pair ? 256 : 128, pair ? 256 : bn);
-    const TcArgs p{C, offsets, h->d_status, h->wait_limit_ns, G, static_cast<int>(rows), static_cast<int>(m),
-                   static_cast<int>(n), 0, alpha, beta, idesc, bf16, n % (f32 ? 4 : 8) == 0 && aligned16(C)};
+    p.idesc = sm100::idesc_f32acc(bf16, 1, 1, pair ? 256 : 128, pair ? 256 : bn);
     const int bm = pair ? 256 : 128;
     const int64_t most = G * ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
     return f32 ? launch_wgrad<true>(h, pair, bn, tmA, tmB, p, most) : launch_wgrad<false>(h, pair, bn, tmA, tmB, p, most);
