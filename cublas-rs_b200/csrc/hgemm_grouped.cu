@@ -225,63 +225,86 @@ __device__ __forceinline__ void add_old(float (&x)[32], const uint8_t *row, int 
     }
 }
 
-// 8 values from p on, of which `have` exist, as a 16-byte piece.  p is 2-byte
-// aligned; nothing outside the values is read.
-struct Piece {
-    uint32_t w[4];
-    uint16_t first, last;
-    bool odd;
-    __device__ __forceinline__ void load(const uint16_t *p, int have) {
-        odd = false;
-        if (have >= 8) {
-            odd = (reinterpret_cast<uintptr_t>(p) & 2) != 0;
-            if (!odd) {
-                const uint32_t *q = reinterpret_cast<const uint32_t *>(p);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = __ldg(q + i);
-            } else {
-                first = __ldg(p);
-                last = __ldg(p + 7);
-                const uint32_t *q = reinterpret_cast<const uint32_t *>(p + 1);
-#pragma unroll
-                for (int i = 0; i < 3; ++i) w[i] = __ldg(q + i);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = 2 * i < have ? __ldg(p + 2 * i) : 0u;
-                if (2 * i + 1 < have) w[i] |= static_cast<uint32_t>(__ldg(p + 2 * i + 1)) << 16;
-            }
-        }
-    }
-    __device__ __forceinline__ uint4 get() const {
-        if (!odd) return make_uint4(w[0], w[1], w[2], w[3]);
-        return make_uint4(first | w[0] << 16, __funnelshift_r(w[0], w[1], 16), __funnelshift_r(w[1], w[2], 16),
-                          w[2] >> 16 | static_cast<uint32_t>(last) << 16);
-    }
-};
+// The word (or the 16-bit value) at `a`, or 0 unless `take`: without a branch,
+// so that many are in flight.
+__device__ __forceinline__ uint32_t ldg16_if(uint64_t a, bool take) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .u16 h;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u16 h, 0;\n\t"
+                 "@p ld.global.nc.u16 h, [%1];\n\tcvt.u32.u16 %0, h;\n\t}"
+                 : "=r"(v) : "l"(a), "r"(static_cast<uint32_t>(take)));
+    return v;
+}
+__device__ __forceinline__ uint32_t ldg32_if(uint64_t a, bool take) {
+    uint32_t v;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\tmov.u32 %0, 0;\n\t@p ld.global.nc.u32 %0, [%1];\n\t}"
+                 : "=r"(v) : "l"(a), "r"(static_cast<uint32_t>(take)));
+    return v;
+}
 
 // One warp writes an operand's 16 KiB of a stage: 128 rows of 64 k values
 // (K_MAJOR: `slow` rows exist and `fast` k values), or two boxes of 64 k rows
 // of 64 columns (`slow` k rows and `fast` columns exist), zeros elsewhere, in
-// the 128-byte swizzle.  8 pieces of a lane are in flight at once.
+// the 128-byte swizzle.  A lane takes pieces of 8 values, by the aligned words
+// that hold them: four, or five where the row starts between two words.  Those
+// reach a value beyond the tile on either side, so where that may lie outside
+// the operand, [lo, hi), values are read one by one.  8 pieces of a lane are
+// in flight at once.
 template <bool K_MAJOR>
-__device__ __forceinline__ void fill_by_hand(uint8_t *to, const uint16_t *from, int ld, int slow, int fast, int lane) {
+__device__ __forceinline__ void fill_by_hand(uint8_t *to, const uint16_t *from, int ld, int slow, int fast,
+                                             const uint16_t *lo, const uint16_t *hi, int lane) {
+    constexpr int kPieces = 8, kSlow = K_MAJOR ? 128 : 64, kFast = K_MAJOR ? 64 : 128;
+    slow = min(slow, kSlow);
+    fast = min(fast, kFast);
+    if (from == lo || from + static_cast<int64_t>(slow - 1) * ld + (fast + 7) / 8 * 8 + 1 > hi) {
+        // a row of 64 values a turn, two to a lane, 16 rows in flight
+        uint8_t *out = to + (lane & 3) * 4;
 #pragma unroll 1
-    for (int i0 = lane; i0 < 1024; i0 += 256) {
-        Piece piece[8];
+        for (int i0 = 0; i0 < 128; i0 += 16) {
+            const int row0 = K_MAJOR ? i0 : i0 & 63, at = (K_MAJOR ? 0 : i0 >> 6 << 6) + 2 * lane;
+            const int left = fast - at;
+            const uint64_t p0 = reinterpret_cast<uint64_t>(from + static_cast<int64_t>(row0) * ld + at);
+            uint32_t a[16], b[16];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int i = i0 + 32 * j, c = i & 7;
-            const int row = K_MAJOR ? i >> 3 : i >> 3 & 63, at = K_MAJOR ? c * 8 : (i >> 9) * 64 + c * 8;
-            piece[j].load(from + static_cast<int64_t>(row) * ld + at, row < slow ? fast - at : 0);
+            for (int j = 0; j < 16; ++j) {
+                const uint64_t p = p0 + static_cast<uint64_t>(ld) * 2u * j;
+                a[j] = ldg16_if(p, row0 + j < slow && left > 0);
+                b[j] = ldg16_if(p + 2, row0 + j < slow && left > 1);
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+                *reinterpret_cast<uint32_t *>(out + (K_MAJOR ? 0 : i0 >> 6) * kBoxBytes + (row0 + j) * 128 +
+                                              (((lane >> 2) ^ (j & 7)) << 4)) = a[j] | b[j] << 16;
         }
+        return;
+    }
+    // piece j of a turn: chunk lane % 8 of the turn's row lane / 8 + 4 j
+    const int c = lane & 7, r = lane >> 3;
+    const uint64_t step = static_cast<uint64_t>(ld) * 8u;  // bytes of four rows
+#pragma unroll 1
+    for (int i0 = 0; i0 < 128; i0 += 4 * kPieces) {
+        const int row0 = (K_MAJOR ? i0 : i0 & 63) + r, at = (K_MAJOR ? 0 : i0 >> 6 << 6) + c * 8;
+        const int left = fast - at;  // values that exist
+        const uint64_t p0 = reinterpret_cast<uint64_t>(from + static_cast<int64_t>(row0) * ld + at);
+        uint32_t w[kPieces][5];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int i = i0 + 32 * j, c = i & 7;
-            const int row = K_MAJOR ? i >> 3 : i >> 3 & 63;
-            *reinterpret_cast<uint4 *>(to + (K_MAJOR ? 0 : (i >> 9) * kBoxBytes) + row * 128 + ((c ^ (row & 7)) << 4)) =
-                piece[j].get();
+        for (int j = 0; j < kPieces; ++j) {
+            const uint64_t p = p0 + step * j;
+            const bool have = row0 + 4 * j < slow && left > 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[j][i] = ldg32_if((p & ~3ull) + 4 * i, have);
+            w[j][4] = ldg32_if((p & ~3ull) + 16, have && (p & 2));
+        }
+        uint8_t *box = to + (K_MAJOR ? 0 : i0 >> 6) * kBoxBytes + row0 * 128;
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+            const uint32_t shift = (static_cast<uint32_t>(p0 + step * j) & 2u) << 3;
+            uint32_t v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = __funnelshift_r(w[j][i], w[j][i + 1], shift);
+                if (left < 8 && left < 2 * i + 2) v[i] = left < 2 * i + 1 ? 0u : v[i] & 0xffffu;
+            }
+            *reinterpret_cast<uint4 *>(box + j * 512 + ((c ^ ((row0 + 4 * j) & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
         }
     }
 }
@@ -531,6 +554,9 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
         // ------------------------------------------------ loading warps (HAND)
         const int pair = (warp - 10) >> 1;
         const bool is_b = (warp - 10) & 1;
+        const uint16_t *a_end = p.A + static_cast<int64_t>(p.rows) * (MODE == kTN ? p.M : p.K);
+        const uint16_t *b_end = p.B + (MODE == kTN ? static_cast<int64_t>(p.rows) * p.N
+                                                   : static_cast<int64_t>(p.groups) * p.N * p.K);
         int g = 0;
         uint32_t it = 0;  // k blocks of all tiles so far
         bool ok = true;
@@ -547,19 +573,19 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
                 if (!is_b) {
                     if constexpr (MODE == kTN)
                         fill_by_hand<false>(sA + s * Cf::A_BYTES, p.A + static_cast<int64_t>(o.row0 + k0) * p.M + o.m0, p.M,
-                                            k_left, p.M - o.m0, lane);
+                                            k_left, p.M - o.m0, p.A, a_end, lane);
                     else
                         fill_by_hand<true>(sA + s * Cf::A_BYTES, p.A + static_cast<int64_t>(o.row0) * p.K + k0, p.K,
-                                           o.valid, k_left, lane);
+                                           o.valid, k_left, p.A, a_end, lane);
                 } else {
                     const int64_t matrix = MODE == kTN ? static_cast<int64_t>(o.row0) * p.N
                                                        : static_cast<int64_t>(o.g) * p.N * p.K;
                     if constexpr (MODE == kNT)
                         fill_by_hand<true>(sB + s * Cf::B_BYTES, p.B + matrix + static_cast<int64_t>(o.n0) * p.K + k0, p.K,
-                                           p.N - o.n0, k_left, lane);
+                                           p.N - o.n0, k_left, p.B, b_end, lane);
                     else
                         fill_by_hand<false>(sB + s * Cf::B_BYTES, p.B + matrix + static_cast<int64_t>(k0) * p.N + o.n0, p.N,
-                                            k_left, p.N - o.n0, lane);
+                                            k_left, p.N - o.n0, p.B, b_end, lane);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
