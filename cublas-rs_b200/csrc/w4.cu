@@ -519,6 +519,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const Item *items = table->item;
 
     // ---- the sets of products
+    const int named = p.index && tid < p.count ? __ldg(p.index + p.first + tid) : 0;
+    if (TMA && tid == 0) prefetch_tensormap(&tmW);
     if (tid == 0) abort_flag = 0;
     if (tid < 4) reinterpret_cast<uint32_t *>(nothing)[tid] = 0;
     if (tid < 2 * kWarps) arrived[tid / kWarps][tid % kWarps] = finished[tid / kWarps][tid % kWarps] = 0;
@@ -527,8 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         fence_barrier_init();
     }
     if (p.index) {
-        const int mine = tid < p.count ? p.index[p.first + tid] : 0;
-        const int e = mine >= 0 && mine < p.matrices ? mine : -1;
+        const int e = named >= 0 && named < p.matrices ? named : -1;
         if (tid < p.count) table->index[tid] = e;
         __syncthreads();
         int seen = 0, lead = tid;  // products before this one of its matrix; the first of its set
@@ -582,13 +583,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         return p.index ? items[set].count
                        : static_cast<int>(min(static_cast<int64_t>(p.width), p.count - static_cast<int64_t>(set) * p.width));
     };
-    // Sum o (row o / nb, vector o % nb) of a tile leaves.
-    auto put = [&](uint32_t set, uint32_t tile, int nb, int o, float sum) {
-        const int64_t row = static_cast<int64_t>(tile) * kTileRows + o / nb;
+    // The sum of a tile's row r and its set's vector v leaves.
+    auto put = [&](uint32_t set, int e, uint32_t tile, int r, int v, float sum) {
+        const int64_t row = static_cast<int64_t>(tile) * kTileRows + r;
         if (row >= p.w.m) return;
-        const int64_t i = p.index ? p.first + items[set].member[o % nb] : static_cast<int64_t>(set) * p.width + o % nb;
+        const int64_t i = p.index ? p.first + items[set].member[v] : static_cast<int64_t>(set) * p.width + v;
         uint16_t *y = p.y + i * p.w.m + row;
-        float res = matrix_of(set) >= 0 ? p.alpha * sum : 0.0f;
+        float res = e >= 0 ? p.alpha * sum : 0.0f;
         if (p.beta != 0.0f) res = fmaf(p.beta, H::get(*y), res);
         *y = H::put(res);
     };
@@ -596,21 +597,25 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int spg = static_cast<int>(p.w.group / 32);
     const int nsteps = static_cast<int>(p.w.n / 32);
     int nb = 0;
-    uint32_t phase = 0, staged = 0xffffffffu;
+    uint32_t phase = 0;
 
     // The warp's next chunk, in this unit or a later one: as soon as a box of
     // the present chunk is used up, the next chunk's takes its place, and the
     // scales and zero points that belong to it are read, row `lane`'s by each
     // lane (the tile's last one by lanes whose row is not there).
     RowScales<SPG, ZEROS> scales[2];
-    uint32_t nu = u_begin;
+    uint32_t nset = u_begin / upers, nunit = u_begin % upers, nleft = u_end - u_begin;  // unit nunit of set nset; units to go
     int nc = 0, nchunk = 0, nrow = 0;
     const uint16_t *nscales = nullptr;
     const uint8_t *nzeros = nullptr;
     auto seek = [&] {
-        for (; nu < u_end; ++nu) {
-            const uint32_t set = nu / upers, tile = nu % upers * parts + part_no;
-            const int e = matrix_of(set);
+        for (; nleft; --nleft) {
+            const int e = matrix_of(nset);
+            const uint32_t tile = nunit * parts + part_no;
+            if (++nunit == upers) {
+                nunit = 0;
+                ++nset;
+            }
             if (own == 0 || e < 0 || tile >= tiles) continue;
             const int64_t row = e * p.w.m + static_cast<int64_t>(tile) * kTileRows;
             const int64_t left = p.w.m - 1 - static_cast<int64_t>(tile) * kTileRows;  // rows behind the tile's first
@@ -623,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     };
     auto load = [&](int b) {
-        if (nu >= u_end || dead) return;
+        if (!nleft || dead) return;
         if (lane == 0) {
             mbar_arrive_expect_tx(&full[b], kBoxBytes);
             tma_load_2d(ring + b * kBoxBytes, &tmW, &full[b], nchunk * (cols_of / 2) + b * (kBoxCols / 2), nrow);
@@ -638,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         nchunk += kw * KS;
         if (++nc == own) {
             nc = 0;
-            ++nu;
+            --nleft;
             seek();
         }
     };
@@ -649,45 +654,58 @@ __global__ void __launch_bounds__(kThreads, 1)
         advance();
     }
 
+    uint32_t set = u_begin / upers, unit = u_begin % upers;
+    int e = -1;          // the set's matrix
+    uint32_t over = 0;   // 2^16 / nb, rounded up: o * over >> 16 is o / nb for the sums of a tile
+    bool fresh = true;   // the set's vectors are not staged yet
+    const bool single = u_end - u_begin == 1;
     for (uint32_t u = u_begin; u < u_end; ++u) {
-        const uint32_t set = u / upers, tile = u % upers * parts + part_no;
-        const bool some = matrix_of(set) >= 0;
-        if (set != staged) {
-            staged = set;
+        if (fresh) {
+            fresh = false;
+            e = matrix_of(set);
             nb = vectors_of(set);
+            over = (65536u + nb - 1) / nb;
             __syncthreads();  // everyone is done with the old vectors
-            if (some) {
-                // 8 columns of one vector a turn; local chunk l is chunk l * KS + rank
-                const int octs = cols_of / 8, per = octs * nb;
-                for (int i = tid; i < local * per; i += kThreads) {
-                    const int l = i / per, r = i % per;
-                    const int b = r / octs, oct = r % octs;  // lanes along a vector
-                    const int64_t j = (static_cast<int64_t>(l) * KS + rank) * cols_of + oct * 8;
-                    const int64_t v = (p.index ? p.first + items[set].member[b]
-                                               : static_cast<int64_t>(set) * p.width + b) / p.fan;
-                    const uint16_t *src = p.x + v * p.w.n + j;
-                    uint16_t h[8];
-                    if (j + 8 <= p.w.n && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-                        *reinterpret_cast<uint4 *>(h) = __ldg(reinterpret_cast<const uint4 *>(src));
-                    } else {
+            if (e >= 0) {
+                // 8 columns of four vectors a turn; local chunk l is chunk l * KS + rank
+                const int shift = p.boxes == 2 ? 6 : 5, octs = 1 << shift;  // 8 columns of a chunk
+                for (int i = tid; i < local * octs; i += kThreads) {
+                    const int64_t j = (static_cast<int64_t>(i >> shift) * KS + rank) * cols_of + (i & octs - 1) * 8;
+                    for (int b0 = 0; b0 < nb; b0 += 4) {
+                        uint4 in[4];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) h[k] = j + k < p.w.n ? src[k] : uint16_t(0);
+                        for (int k = 0; k < 4; ++k) {
+                            if (b0 + k >= nb) continue;
+                            const int64_t v = p.index ? p.first + items[set].member[b0 + k]
+                                                      : static_cast<int64_t>(set) * p.width + b0 + k;
+                            const uint16_t *src = p.x + static_cast<int64_t>(static_cast<uint32_t>(v) / p.fan) * p.w.n + j;
+                            if (j + 8 <= p.w.n && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+                                in[k] = __ldg(reinterpret_cast<const uint4 *>(src));
+                            } else {
+                                uint16_t h[8];
+#pragma unroll
+                                for (int t = 0; t < 8; ++t) h[t] = j + t < p.w.n ? src[t] : uint16_t(0);
+                                in[k] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if (b0 + k >= nb) continue;
+                            // step i / 4 of the vectors' steps, vector, quarter i % 4
+                            *reinterpret_cast<uint4 *>(sx + ((i >> 2) * nb + b0 + k) * 64 + (i & 3) * 16) =
+                                make_uint4(__byte_perm(in[k].x, in[k].z, 0x5410), __byte_perm(in[k].x, in[k].z, 0x7632),
+                                           __byte_perm(in[k].y, in[k].w, 0x5410), __byte_perm(in[k].y, in[k].w, 0x7632));
+                        }
                     }
-                    uint4 o;
-                    o.x = h[0] | static_cast<uint32_t>(h[4]) << 16;
-                    o.y = h[1] | static_cast<uint32_t>(h[5]) << 16;
-                    o.z = h[2] | static_cast<uint32_t>(h[6]) << 16;
-                    o.w = h[3] | static_cast<uint32_t>(h[7]) << 16;
-                    // step (oct / 4), vector b, quarter oct % 4
-                    *reinterpret_cast<uint4 *>(sx + ((l * steps_of + (oct >> 2)) * nb + b) * 64 + (oct & 3) * 16) = o;
                 }
             }
             __syncthreads();
         }
+        const uint32_t tile = unit * parts + part_no;
 
         float total[2][4] = {};
-        if (some && tile < tiles) {
-            const int64_t row0 = matrix_of(set) * p.w.m + static_cast<int64_t>(tile) * kTileRows + g;
+        if (e >= 0 && tile < tiles) {
+            const int64_t row0 = e * p.w.m + static_cast<int64_t>(tile) * kTileRows + g;
             const int rows = static_cast<int>(p.w.m - static_cast<int64_t>(tile) * kTileRows) - g;  // > 8 i: row g + 8 i exists
             // lanes of vectors that the set does not have read zeros
             const int xstep = g < nb ? nb * 64 : 0;
@@ -770,37 +788,52 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
 
-        // ---- join: the last of a tile's warps to get here adds their sums up;
-        // none waits, but to reuse a buffer that is not joined yet
+        // ---- join.  A warp that has its tile to itself puts it out.  Else the
+        // last of a tile's warps to get here adds their sums up; none waits,
+        // but to reuse a buffer that is not joined yet.  A CTA of one unit has
+        // nothing to go on with: all its threads add up.
         const int v = static_cast<int>(u - u_begin), flip = v & 1;
-        if (v >= 2 && !wait_finished(&finished[flip][part_no], v >> 1, &abort_flag, p, lane)) dead = true;
-        float *mine = part + (flip * kWarps + warp) * sums;
+        if (kw == 1 && KS == 1) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {  // row g + 8 (i / 2), vector 2 q + i % 2
-            const int col = 2 * q + (i & 1);
-            if (col < nb) mine[(g + 8 * (i >> 1)) * nb + col] = total[i >> 2][i & 3];
-        }
-        __threadfence_block();
-        __syncwarp();
-        int last = 0;
-        if (lane == 0) last = atomicAdd(&arrived[flip][part_no], 1) == kw - 1;
-        if (__shfl_sync(0xffffffffu, last, 0)) {
-            __threadfence_block();
-            if (lane == 0) arrived[flip][part_no] = 0;
-            const float *from = part + (flip * kWarps + part_no * kw) * sums;
-            float *slot = slots + ((v / kBatch % 2 * kBatch + v % kBatch) * parts + part_no) * sums;
-            for (int o = lane; o < kTileRows * nb; o += 32) {
+            for (int i = 0; i < 8; ++i)  // row g + 8 (i / 2), vector 2 q + i % 2
+                if (2 * q + (i & 1) < nb) put(set, e, tile, g + 8 * (i >> 1), 2 * q + (i & 1), total[i >> 2][i & 3]);
+        } else {
+            if (v >= 2 && !wait_finished(&finished[flip][part_no], v >> 1, &abort_flag, p, lane)) dead = true;
+            float *mine = part + (flip * kWarps + warp) * sums;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int col = 2 * q + (i & 1);
+                if (col < nb) mine[(g + 8 * (i >> 1)) * nb + col] = total[i >> 2][i & 3];
+            }
+            auto add_up = [&](int t, int o) {  // sum o of the unit's tile t
+                const float *from = part + (flip * kWarps + t * kw) * sums + o;
                 float sum = 0.0f;
 #pragma unroll 4
-                for (int w = 0; w < kw; ++w) sum += from[w * sums + o];
+                for (int w = 0; w < kw; ++w) sum += from[w * sums];
+                const int r = static_cast<int>(o * over >> 16);
                 if (KS == 1)
-                    put(set, tile, nb, o, sum);
+                    put(set, e, unit * parts + t, r, o - r * nb, sum);
                 else
-                    slot[o] = sum;
+                    slots[((v / kBatch % 2 * kBatch + v % kBatch) * parts + t) * sums + o] = sum;
+            };
+            if (single) {
+                __syncthreads();
+                for (int i = tid; i < parts * 256; i += kThreads)
+                    if ((i & 255) < kTileRows * nb) add_up(i >> 8, i & 255);
+            } else {
+                __threadfence_block();
+                __syncwarp();
+                int last = 0;
+                if (lane == 0) last = atomicAdd(&arrived[flip][part_no], 1) == kw - 1;
+                if (__shfl_sync(0xffffffffu, last, 0)) {
+                    __threadfence_block();
+                    if (lane == 0) arrived[flip][part_no] = 0;
+                    for (int o = lane; o < kTileRows * nb; o += 32) add_up(part_no, o);
+                    __threadfence_block();
+                    __syncwarp();
+                    if (lane == 0) finished[flip][part_no] = (v >> 1) + 1;
+                }
             }
-            __threadfence_block();
-            __syncwarp();
-            if (lane == 0) finished[flip][part_no] = (v >> 1) + 1;
         }
         if (KS > 1 && (v % kBatch == kBatch - 1 || u + 1 == u_end)) {
             // the batch's sums are in the CTAs of the cluster: each adds up its
@@ -810,15 +843,21 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int v0 = v / kBatch * kBatch;
             for (int i = rank; i <= v - v0; i += KS) {
                 const uint32_t bu = u_begin + v0 + i, bset = bu / upers;
-                const int bnb = vectors_of(bset), per = kTileRows * bnb;
-                for (int o = tid; o < parts * per; o += kThreads) {
-                    const int t = o / per;
-                    const uint32_t at = smem_u32(slots + ((v / kBatch % 2 * kBatch + i) * parts + t) * sums + o % per);
+                const int bnb = vectors_of(bset), be = matrix_of(bset);
+                for (int k = tid; k < parts * 256; k += kThreads) {
+                    const int t = k >> 8, o = k & 255;
+                    if (o >= kTileRows * bnb) continue;
+                    const uint32_t at = smem_u32(slots + ((v / kBatch % 2 * kBatch + i) * parts + t) * sums + o);
                     float sum = 0.0f;
                     for (int r = 0; r < KS; ++r) sum += ld_shared_cluster(mapa_shared(at, r));
-                    put(bset, bu % upers * parts + t, bnb, o % per, sum);
+                    put(bset, be, bu % upers * parts + t, o / bnb, o % bnb, sum);
                 }
             }
+        }
+        if (++unit == upers) {
+            unit = 0;
+            ++set;
+            fresh = true;
         }
     }
     if (KS > 1) {  // no CTA leaves while another reads its sums
@@ -946,7 +985,7 @@ int launched(const char *what) {
 }
 
 constexpr int kMaxSmem = 227 * 1024 - 1024;  // dynamic shared memory of the GEMV kernel, static beside it
-constexpr int64_t kMaxXBytes = 40 * 1024;    // of its staged vectors
+constexpr int64_t kMaxXBytes = 40 * 1024;    // of its staged vectors where 8 CTAs share a tile; fewer may have more
 
 // Its shared memory for KS CTAs and kw warps of each a tile; sets the
 // vectors' bytes.
@@ -956,27 +995,31 @@ size_t gemv_smem(GemvArgs &p, bool tma, int KS, int kw, int64_t local) {
            (p.index ? sizeof(Table) : 0) + 1024;
 }
 
-// Resident clusters of KS CTAs of a kernel with that much shared memory,
-// asked once for each device.
-int resident_clusters(b2b_handle *h, const void *kernel, cudaLaunchConfig_t &cfg, int KS) {
-    struct Entry {
-        const void *kernel;
-        int device, ks, clusters;
-        size_t smem;
-    };
+// Clusters of KS CTAs (1, 2, 4 or 8) of the GEMV kernel that are resident at
+// once, asked once for each device: a CTA has an SM to itself by its registers,
+// so neither its type nor its shared memory matters.
+int resident_clusters(b2b_handle *h, const void *kernel, int KS) {
     static std::mutex mu;
-    static std::vector<Entry> cache;
+    static int known[64][9];
     std::lock_guard<std::mutex> lock(mu);
-    for (const Entry &e : cache)
-        if (e.kernel == kernel && e.device == h->device && e.ks == KS && e.smem == cfg.dynamicSmemBytes)
-            return e.clusters;
-    int clusters = 0;
-    cfg.gridDim = dim3(KS);
-    if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
-        cudaGetLastError();
-        clusters = h->sm_count / KS;
+    int &clusters = known[h->device & 63][KS];
+    if (clusters == 0) {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = KS;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(KS);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = kMaxSmem;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess || clusters < 1) {
+            cudaGetLastError();
+            clusters = h->sm_count / KS;
+        }
     }
-    cache.push_back(Entry{kernel, h->device, KS, clusters, cfg.dynamicSmemBytes});
     return clusters;
 }
 
@@ -1024,7 +1067,6 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
     cfg.blockDim = dim3(kThreads);
     cfg.stream = h->stream;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
     {
         static std::mutex mu;
         static bool ready[2][2][9][64];
@@ -1046,12 +1088,9 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
         const int64_t chunks = (cols + p.boxes - 1) / p.boxes;
         for (int KS = 1; KS <= 8 && (KS == 1 || KS < 2 * chunks); KS *= 2) {
             const int64_t local = (chunks + KS - 1) / KS;
-            if (local * p.boxes * kBoxCols * p.width * 2 > kMaxXBytes) continue;
+            const int64_t clusters = resident_clusters(h, fn, KS);
             for (int kw = kWarps; kw >= 1; kw /= 2) {
-                attr[0].val.clusterDim.x = KS;
-                cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, KS, kw, local);
-                if (cfg.dynamicSmemBytes > static_cast<size_t>(kMaxSmem)) continue;
-                const int64_t clusters = resident_clusters(h, fn, cfg, KS);
+                if (gemv_smem(p, spg != 0, KS, kw, local) > static_cast<size_t>(kMaxSmem)) continue;
                 const int64_t units = sets * ((tiles + kWarps / kw - 1) / (kWarps / kw));
                 const double time = static_cast<double>((units + clusters - 1) / clusters) *
                                     (static_cast<double>((local + kw - 1) / kw) * (p.boxes + 0.33) + 1.0);
@@ -1071,6 +1110,7 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
     const int64_t chunks = (cols + p.boxes - 1) / p.boxes, local = (chunks + best - 1) / best;
     attr[0].val.clusterDim.x = best;
     cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, best, best_kw, local);
+    cfg.numAttrs = best > 1;
     cfg.gridDim = dim3(best * best_grid);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmW, p);
     return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, "4-bit GEMV launch");
