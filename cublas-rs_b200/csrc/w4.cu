@@ -7,6 +7,7 @@
 //   y_i = alpha * W x_i + beta * y_i
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <mutex>
@@ -227,17 +228,19 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
 // bits.
 //
 //   * A tile is 32 rows of W for one set of vectors; its n columns are cut
-//     into chunks of 256 or 512 (a box or two), which the CTAs of a cluster
-//     and kw of a CTA's 16 warps take in turn; the 16 / kw parts of a CTA have
-//     a tile each.  A unit is those tiles.
+//     into chunks of 256 or 512 (a box or two), which the CTAs of a cluster and
+//     some of a CTA's 16 warps take in turn.  A cluster has an equal share of
+//     all tiles, next to each other, and takes them in rounds: of 16 tiles, a
+//     warp to each, while it has as many, then of 8, 4, 2 and 1 with 2, 4, 8
+//     and 16 warps to a tile, so that no warp idles while another has two.
 //   * Each warp holds one chunk (boxes of 32 rows x 128 bytes, 128-byte
 //     swizzle); TMA refills a box with the next chunk's as soon as it is used
-//     up, across units, so nothing drains at a unit's end.  16 warps hold
+//     up, across rounds, so nothing drains at a round's end.  16 warps hold
 //     128 KiB of W, in flight or in use.
 //   * The vectors are staged once for each set, each 8 columns reordered to
 //     the pairs (0,4) (1,5) (2,6) (3,7) that the words unpack to.
 //   * The last of a tile's warps to arrive adds their sums up while the others
-//     go on; the CTAs of a cluster read one another's sums once for 8 units.
+//     go on; the CTAs of a cluster read one another's sums once for 8 rounds.
 //     Both in a fixed order, whoever adds.
 // Rows that TMA cannot describe (n not a multiple of 32, packed not 16-byte
 // aligned) and groups that do not fit a chunk evenly are read by the same
@@ -248,7 +251,7 @@ constexpr int kTileRows = 32;
 constexpr int kBoxCols = 256;                     // 128 bytes of a row
 constexpr int kBoxSteps = kBoxCols / 32;          // of 32 columns
 constexpr int kBoxBytes = kTileRows * kBoxCols / 2;
-constexpr int kBatch = 8;                         // units that the CTAs of a cluster join at once
+constexpr int kBatch = 8;                         // rounds that the CTAs of a cluster join at once
 constexpr int kMaxIndexed = 256;                  // products of one launch that choose their matrix
 
 struct GemvArgs {
@@ -260,7 +263,7 @@ struct GemvArgs {
     uint64_t wait_ns;
     int matrices, count, fan, first;  // first: number of this launch's first product
     int width;    // vectors of a set: 8, or fewer where longer rows leave room for fewer
-    int kw;       // warps that share a tile
+    int parts;    // most tiles of a round, a power of two
     int boxes;    // of a chunk: 1 or 2
     int x_bytes;  // of the staged vectors
     int vec;      // a box's scales and zero points of a row are one aligned word each
@@ -500,19 +503,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr bool TMA = SPG != 0;
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag;
-    __shared__ int arrived[2][kWarps];            // warps whose sums of a tile are in `part`
-    __shared__ volatile int finished[2][kWarps];  // tiles joined from there so far
+    __shared__ int arrived[2][5][kWarps];         // warps of a tile (by log2 of their number) whose sums are in `part`
+    __shared__ volatile int finished[2][kWarps];  // rounds whose sums of this warp are joined
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, q = lane & 3;
     const int KS = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-    const int kw = p.kw, parts = kWarps / kw, part_no = warp / kw, kwarp = warp % kw;
     uint8_t *ring = smem + (TMA ? warp * 2 * kBoxBytes : 0);
     uint8_t *sx = smem + (TMA ? kWarps * 2 * kBoxBytes : 0);
     const int sums = kTileRows * p.width;                     // of a tile
     float *part = reinterpret_cast<float *>(sx + p.x_bytes);  // [2][kWarps][32 rows][width]
-    float *slots = part + 2 * kWarps * sums;                  // KS > 1: [2][kBatch][parts][32 rows][width]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(slots + (KS > 1 ? 2 * kBatch * parts * sums : 0));
+    float *slots = part + 2 * kWarps * sums;                  // KS > 1: [2][kBatch][p.parts][32 rows][width]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(slots + (KS > 1 ? 2 * kBatch * p.parts * sums : 0));
     uint64_t *full = bars + warp * 2;  // of its chunk's two boxes
     uint8_t *nothing = reinterpret_cast<uint8_t *>(bars + kWarps * 2);  // 16 bytes of 0
     Table *table = reinterpret_cast<Table *>(nothing + 16);
@@ -523,7 +525,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (TMA && tid == 0) prefetch_tensormap(&tmW);
     if (tid == 0) abort_flag = 0;
     if (tid < 4) reinterpret_cast<uint32_t *>(nothing)[tid] = 0;
-    if (tid < 2 * kWarps) arrived[tid / kWarps][tid % kWarps] = finished[tid / kWarps][tid % kWarps] = 0;
+    if (tid < 2 * 5 * kWarps) (&arrived[0][0][0])[tid] = 0;
+    if (tid < 2 * kWarps) finished[tid / kWarps][tid % kWarps] = 0;
     if (TMA && lane == 0) {
         for (int b = 0; b < 2; ++b) mbar_init(&full[b], 1);
         fence_barrier_init();
@@ -564,17 +567,35 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncthreads();
     const uint32_t tiles = static_cast<uint32_t>((p.w.m + kTileRows - 1) / kTileRows);
-    const uint32_t upers = (tiles + parts - 1) / parts;  // units of a set
     const uint32_t sets = p.index ? table->items : (p.count + p.width - 1) / p.width;
     const int steps_of = p.boxes * kBoxSteps, cols_of = p.boxes * kBoxCols;  // of a chunk
     const int chunks = static_cast<int>((p.w.n + cols_of - 1) / cols_of);
-    const int local = chunks > rank ? (chunks - rank + KS - 1) / KS : 0;   // this CTA's chunks of a tile
-    const int own = local > kwarp ? (local - kwarp + kw - 1) / kw : 0;     // this warp's
+    const int local = chunks > rank ? (chunks - rank + KS - 1) / KS : 0;  // this CTA's chunks of a tile
     const uint32_t clusters = gridDim.x / KS, cluster = blockIdx.x / KS;
-    // consecutive units to a cluster, so that it changes its vectors rarely
-    const uint64_t units = static_cast<uint64_t>(sets) * upers;
-    const uint32_t u_begin = static_cast<uint32_t>(units * cluster / clusters);
-    const uint32_t u_end = static_cast<uint32_t>(units * (cluster + 1) / clusters);
+    // next to each other, so that a cluster changes its vectors rarely
+    const uint64_t all = static_cast<uint64_t>(sets) * tiles;
+    const uint64_t t_begin = all * cluster / clusters, t_end = all * (cluster + 1) / clusters;
+
+    // A place in the cluster's sequence of rounds.
+    struct Place {
+        uint32_t set, tile, left;  // next tile, and how many are left
+        // Takes the next round: 2^result tiles from `tile` on.
+        __device__ __forceinline__ int take(uint32_t tiles, uint32_t most) {
+            const int lp = 31 - __clz(static_cast<int>(min(min(left, tiles - tile), most)));
+            left -= 1u << lp;
+            tile += 1u << lp;
+            return lp;
+        }
+        // ... after which a set may be done.
+        __device__ __forceinline__ void settle(uint32_t tiles) {
+            if (tile == tiles) {
+                tile = 0;
+                ++set;
+            }
+        }
+    };
+    Place here{static_cast<uint32_t>(t_begin / tiles), static_cast<uint32_t>(t_begin % tiles),
+               static_cast<uint32_t>(t_end - t_begin)};
 
     auto matrix_of = [&](uint32_t set) { return p.index ? items[set].matrix : 0; };
 
@@ -604,31 +625,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     // scales and zero points that belong to it are read, row `lane`'s by each
     // lane (the tile's last one by lanes whose row is not there).
     RowScales<SPG, ZEROS> scales[2];
-    uint32_t nset = u_begin / upers, nunit = u_begin % upers, nleft = u_end - u_begin;  // unit nunit of set nset; units to go
-    int nc = 0, nchunk = 0, nrow = 0;
+    Place ahead = here;
+    bool more = true;  // there is a next chunk
+    int nc = 0, nstep = 0, nchunk = 0, nrow = 0;  // chunks left of its tile, and how far apart they are
     const uint16_t *nscales = nullptr;
     const uint8_t *nzeros = nullptr;
     auto seek = [&] {
-        for (; nleft; --nleft) {
-            const int e = matrix_of(nset);
-            const uint32_t tile = nunit * parts + part_no;
-            if (++nunit == upers) {
-                nunit = 0;
-                ++nset;
-            }
-            if (own == 0 || e < 0 || tile >= tiles) continue;
-            const int64_t row = e * p.w.m + static_cast<int64_t>(tile) * kTileRows;
-            const int64_t left = p.w.m - 1 - static_cast<int64_t>(tile) * kTileRows;  // rows behind the tile's first
+        while (ahead.left) {
+            const int e = matrix_of(ahead.set);
+            const uint32_t first = ahead.tile;
+            const int lk = 4 - ahead.take(tiles, p.parts), kwarp = warp & ((1 << lk) - 1);
+            ahead.settle(tiles);
+            if (e < 0 || kwarp >= local) continue;
+            const int64_t tile = first + (warp >> lk), row = e * p.w.m + tile * kTileRows;
+            const int64_t left = p.w.m - 1 - tile * kTileRows;  // rows behind the tile's first
             const int64_t at = (row + min(left, static_cast<int64_t>(lane))) * p.w.gs;
             nrow = static_cast<int>(row);
             nscales = p.w.scales + at;
             if (ZEROS) nzeros = p.w.zeros + at;
             nchunk = kwarp * KS + rank;
+            nstep = KS << lk;
+            nc = (local - kwarp + (1 << lk) - 1) >> lk;
             return;
         }
+        more = false;
     };
     auto load = [&](int b) {
-        if (!nleft || dead) return;
+        if (!more || dead) return;
         if (lane == 0) {
             mbar_arrive_expect_tx(&full[b], kBoxBytes);
             tma_load_2d(ring + b * kBoxBytes, &tmW, &full[b], nchunk * (cols_of / 2) + b * (kBoxCols / 2), nrow);
@@ -640,12 +663,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         scales[b].load(nscales + grp, nzeros + grp, static_cast<int>(p.w.gs) - grp, p.vec);
     };
     auto advance = [&] {
-        nchunk += kw * KS;
-        if (++nc == own) {
-            nc = 0;
-            --nleft;
-            seek();
-        }
+        nchunk += nstep;
+        if (--nc == 0) seek();
     };
     if constexpr (TMA) {
         seek();
@@ -654,14 +673,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         advance();
     }
 
-    uint32_t set = u_begin / upers, unit = u_begin % upers;
     int e = -1;          // the set's matrix
     uint32_t over = 0;   // 2^16 / nb, rounded up: o * over >> 16 is o / nb for the sums of a tile
-    bool fresh = true;   // the set's vectors are not staged yet
-    const bool single = u_end - u_begin == 1;
-    for (uint32_t u = u_begin; u < u_end; ++u) {
-        if (fresh) {
-            fresh = false;
+    uint32_t staged = 0xffffffffu;  // the set whose vectors are staged
+    Place batch = here;  // where the batch of rounds began
+    bool single = true;  // the cluster has one round: nothing to go on with at its end
+    for (int v = 0; here.left; ++v) {
+        const uint32_t set = here.set, first = here.tile;
+        const int lp = here.take(tiles, p.parts), lk = 4 - lp, kw = 1 << lk;
+        here.settle(tiles);
+        single = single && here.left == 0;
+        const int part_no = warp >> lk, kwarp = warp & (kw - 1);
+        const int own = local > kwarp ? (local - kwarp + kw - 1) >> lk : 0;
+        const uint32_t tile = first + part_no;
+        if (set != staged) {
+            staged = set;
             e = matrix_of(set);
             nb = vectors_of(set);
             over = (65536u + nb - 1) / nb;
@@ -701,17 +727,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             __syncthreads();
         }
-        const uint32_t tile = unit * parts + part_no;
-
         float total[2][4] = {};
-        if (e >= 0 && tile < tiles) {
+        if (e >= 0) {
             const int64_t row0 = e * p.w.m + static_cast<int64_t>(tile) * kTileRows + g;
             const int rows = static_cast<int>(p.w.m - static_cast<int64_t>(tile) * kTileRows) - g;  // > 8 i: row g + 8 i exists
             // lanes of vectors that the set does not have read zeros
             const int xstep = g < nb ? nb * 64 : 0;
             if constexpr (TMA) {
                 for (int c = 0; c < own; ++c) {
-                    const int l = kwarp + c * kw, chunk = l * KS + rank;
+                    const int l = kwarp + (c << lk), chunk = l * KS + rank;
 #pragma unroll
                     for (int b = 0; b < 2; ++b) {
                         if (b && p.boxes == 1) break;
@@ -749,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // a row of this lane, or the last one for one that is not there
                 auto row_at = [&](int i) { return row0 + min(i, rows - 1); };
                 for (int c = 0; c < own; ++c) {
-                    const int l = kwarp + c * kw, chunk = l * KS + rank;
+                    const int l = kwarp + (c << lk), chunk = l * KS + rank;
                     const int steps = min(steps_of, static_cast<int>((p.w.n + 31) / 32) - chunk * steps_of);
                     const uint8_t *xs = g < nb ? sx + l * steps_of * nb * 64 + lane * 16 : nothing;
                     // all loads of 8 steps before their use
@@ -790,74 +814,72 @@ __global__ void __launch_bounds__(kThreads, 1)
 
         // ---- join.  A warp that has its tile to itself puts it out.  Else the
         // last of a tile's warps to get here adds their sums up; none waits,
-        // but to reuse a buffer that is not joined yet.  A CTA of one unit has
+        // but to reuse a buffer that is not joined yet.  A CTA of one round has
         // nothing to go on with: all its threads add up.
-        const int v = static_cast<int>(u - u_begin), flip = v & 1;
+        const int flip = v & 1;
         if (kw == 1 && KS == 1) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)  // row g + 8 (i / 2), vector 2 q + i % 2
                 if (2 * q + (i & 1) < nb) put(set, e, tile, g + 8 * (i >> 1), 2 * q + (i & 1), total[i >> 2][i & 3]);
+            if (lane == 0) finished[flip][warp] = (v >> 1) + 1;
         } else {
-            if (v >= 2 && !wait_finished(&finished[flip][part_no], v >> 1, &abort_flag, p, lane)) dead = true;
+            if (v >= 2 && !wait_finished(&finished[flip][warp], v >> 1, &abort_flag, p, lane)) dead = true;
             float *mine = part + (flip * kWarps + warp) * sums;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int col = 2 * q + (i & 1);
                 if (col < nb) mine[(g + 8 * (i >> 1)) * nb + col] = total[i >> 2][i & 3];
             }
-            auto add_up = [&](int t, int o) {  // sum o of the unit's tile t
-                const float *from = part + (flip * kWarps + t * kw) * sums + o;
+            auto add_up = [&](int t, int o) {  // sum o of the round's tile t
+                const float *from = part + (flip * kWarps + (t << lk)) * sums + o;
                 float sum = 0.0f;
 #pragma unroll 4
                 for (int w = 0; w < kw; ++w) sum += from[w * sums];
                 const int r = static_cast<int>(o * over >> 16);
                 if (KS == 1)
-                    put(set, e, unit * parts + t, r, o - r * nb, sum);
+                    put(set, e, first + t, r, o - r * nb, sum);
                 else
-                    slots[((v / kBatch % 2 * kBatch + v % kBatch) * parts + t) * sums + o] = sum;
+                    slots[((v / kBatch % 2 * kBatch + v % kBatch) * p.parts + t) * sums + o] = sum;
             };
             if (single) {
                 __syncthreads();
-                for (int i = tid; i < parts * 256; i += kThreads)
+                for (int i = tid; i < 256 << lp; i += kThreads)
                     if ((i & 255) < kTileRows * nb) add_up(i >> 8, i & 255);
             } else {
                 __threadfence_block();
                 __syncwarp();
                 int last = 0;
-                if (lane == 0) last = atomicAdd(&arrived[flip][part_no], 1) == kw - 1;
+                if (lane == 0) last = atomicAdd(&arrived[flip][lk][part_no], 1) == kw - 1;
                 if (__shfl_sync(0xffffffffu, last, 0)) {
                     __threadfence_block();
-                    if (lane == 0) arrived[flip][part_no] = 0;
+                    if (lane == 0) arrived[flip][lk][part_no] = 0;
                     for (int o = lane; o < kTileRows * nb; o += 32) add_up(part_no, o);
                     __threadfence_block();
                     __syncwarp();
-                    if (lane == 0) finished[flip][part_no] = (v >> 1) + 1;
+                    if (lane < kw) finished[flip][(part_no << lk) + lane] = (v >> 1) + 1;
                 }
             }
         }
-        if (KS > 1 && (v % kBatch == kBatch - 1 || u + 1 == u_end)) {
+        if (KS > 1 && (v % kBatch == kBatch - 1 || here.left == 0)) {
             // the batch's sums are in the CTAs of the cluster: each adds up its
-            // share of the units, and the next batch goes to the other slots
+            // share of the rounds, and the next batch goes to the other slots
             __syncwarp();
             cluster_sync();
-            const int v0 = v / kBatch * kBatch;
-            for (int i = rank; i <= v - v0; i += KS) {
-                const uint32_t bu = u_begin + v0 + i, bset = bu / upers;
+            for (int i = 0; i <= v % kBatch; ++i) {
+                const uint32_t bset = batch.set, bfirst = batch.tile;
+                const int blp = batch.take(tiles, p.parts);
+                batch.settle(tiles);
+                if (i % KS != rank) continue;
                 const int bnb = vectors_of(bset), be = matrix_of(bset);
-                for (int k = tid; k < parts * 256; k += kThreads) {
+                for (int k = tid; k < 256 << blp; k += kThreads) {
                     const int t = k >> 8, o = k & 255;
                     if (o >= kTileRows * bnb) continue;
-                    const uint32_t at = smem_u32(slots + ((v / kBatch % 2 * kBatch + i) * parts + t) * sums + o);
+                    const uint32_t at = smem_u32(slots + ((v / kBatch % 2 * kBatch + i) * p.parts + t) * sums + o);
                     float sum = 0.0f;
                     for (int r = 0; r < KS; ++r) sum += ld_shared_cluster(mapa_shared(at, r));
-                    put(bset, be, bu % upers * parts + t, o / bnb, o % bnb, sum);
+                    put(bset, be, bfirst + t, o / bnb, o % bnb, sum);
                 }
             }
-        }
-        if (++unit == upers) {
-            unit = 0;
-            ++set;
-            fresh = true;
         }
     }
     if (KS > 1) {  // no CTA leaves while another reads its sums
@@ -987,12 +1009,11 @@ int launched(const char *what) {
 constexpr int kMaxSmem = 227 * 1024 - 1024;  // dynamic shared memory of the GEMV kernel, static beside it
 constexpr int64_t kMaxXBytes = 40 * 1024;    // of its staged vectors where 8 CTAs share a tile; fewer may have more
 
-// Its shared memory for KS CTAs and kw warps of each a tile; sets the
-// vectors' bytes.
-size_t gemv_smem(GemvArgs &p, bool tma, int KS, int kw, int64_t local) {
+// Its shared memory for KS CTAs a tile; sets the vectors' bytes.
+size_t gemv_smem(GemvArgs &p, bool tma, int KS, int64_t local) {
     p.x_bytes = static_cast<int>(local * p.boxes * kBoxCols * p.width * 2);
-    return p.x_bytes + 2 * (kWarps + (KS > 1 ? kBatch * (kWarps / kw) : 0)) * kTileRows * p.width * 4 + kWarps * ((tma ? 2 * kBoxBytes : 0) + 16) + 16 +
-           (p.index ? sizeof(Table) : 0) + 1024;
+    return p.x_bytes + 2 * (kWarps + (KS > 1 ? kBatch * p.parts : 0)) * kTileRows * p.width * 4 +
+           kWarps * ((tma ? 2 * kBoxBytes : 0) + 16) + 16 + (p.index ? sizeof(Table) : 0) + 1024;
 }
 
 // Clusters of KS CTAs (1, 2, 4 or 8) of the GEMV kernel that are resident at
@@ -1056,9 +1077,14 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
     const int64_t cols = (p.w.n + kBoxCols - 1) / kBoxCols, tiles = (p.w.m + kTileRows - 1) / kTileRows;
     p.width = p.count < 8 ? p.count : 8;
     while (p.width > 1 && (cols + 7) / 8 * kBoxCols * p.width * 2 > kMaxXBytes) --p.width;
-    // with an index: the sets that it makes where it names each matrix equally often
-    const int64_t each = p.index ? (p.count + p.matrices - 1) / p.matrices : p.count;
-    const int64_t sets = (p.count + each - 1) / each * ((each + p.width - 1) / p.width);
+    // with an index: the matrices that it names, if it names them at random,
+    // and their sets
+    double sets = static_cast<double>((p.count + p.width - 1) / p.width);
+    if (p.index) {
+        const double named = p.matrices * (1.0 - pow(1.0 - 1.0 / p.matrices, p.count));
+        sets = named * ceil(p.count / named / p.width);
+    }
+    const int64_t all = static_cast<int64_t>(ceil(sets * static_cast<double>(tiles)));
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.y = 1;
@@ -1078,40 +1104,48 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
             done = true;
         }
     }
-    // Share a tile's columns among KS CTAs of a cluster and kw warps of each, in
-    // chunks of one box or two, so that the turns take least: the boxes that a
-    // warp computes one after another, a third of one for each chunk's
-    // bookkeeping and one for each tile's joining.
-    int best = 0, best_grid = 0, best_kw = 0, best_boxes = 0;
+    // Share a tile's columns among KS CTAs of a cluster, in chunks of one box or
+    // two, so that a cluster's rounds take least: the boxes that a warp computes
+    // one after another, a third of one for each chunk's bookkeeping and one for
+    // each round's joining.
+    int best = 0, best_boxes = 0, best_parts = 0;
     double best_time = 0;
     for (p.boxes = 1; p.boxes <= 2; ++p.boxes) {
         const int64_t chunks = (cols + p.boxes - 1) / p.boxes;
         for (int KS = 1; KS <= 8 && (KS == 1 || KS < 2 * chunks); KS *= 2) {
             const int64_t local = (chunks + KS - 1) / KS;
+            p.parts = kWarps;
+            while (p.parts > 1 && gemv_smem(p, spg != 0, KS, local) > static_cast<size_t>(kMaxSmem)) p.parts /= 2;
+            if (gemv_smem(p, spg != 0, KS, local) > static_cast<size_t>(kMaxSmem)) continue;
             const int64_t clusters = resident_clusters(h, fn, KS);
-            for (int kw = kWarps; kw >= 1; kw /= 2) {
-                if (gemv_smem(p, spg != 0, KS, kw, local) > static_cast<size_t>(kMaxSmem)) continue;
-                const int64_t units = sets * ((tiles + kWarps / kw - 1) / (kWarps / kw));
-                const double time = static_cast<double>((units + clusters - 1) / clusters) *
-                                    (static_cast<double>((local + kw - 1) / kw) * (p.boxes + 0.33) + 1.0);
-                if (!best || time < best_time) {
-                    best = KS;
-                    best_kw = kw;
-                    best_boxes = p.boxes;
-                    best_time = time;
-                    best_grid = static_cast<int>(units < clusters ? units : clusters);
-                }
+            int64_t left = (all + clusters - 1) / clusters;
+            auto round = [&](int parts) {
+                const int64_t kw = kWarps / parts;
+                return static_cast<double>((local + kw - 1) / kw) * (p.boxes + 0.33) + 1.0;
+            };
+            double time = static_cast<double>(left / p.parts) * round(p.parts);
+            left %= p.parts;
+            for (int parts = p.parts / 2; parts >= 1; parts /= 2)
+                if (left & parts) time += round(parts);
+            if (!best || time < best_time) {
+                best = KS;
+                best_boxes = p.boxes;
+                best_parts = p.parts;
+                best_time = time;
             }
         }
     }
     if (!best) return b2b::fail(B2B_ERR_NOT_SUPPORTED, "4-bit GEMV: rows longer than 163840 columns");
     p.boxes = best_boxes;
-    p.kw = best_kw;
+    p.parts = best_parts;
     const int64_t chunks = (cols + p.boxes - 1) / p.boxes, local = (chunks + best - 1) / best;
+    const int64_t clusters = resident_clusters(h, fn, best);
+    // an index may name more matrices than expected, but not more tiles than this
+    const int64_t most = (p.index ? p.count : (p.count + p.width - 1) / p.width) * tiles;
     attr[0].val.clusterDim.x = best;
-    cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, best, best_kw, local);
+    cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, best, local);
     cfg.numAttrs = best > 1;
-    cfg.gridDim = dim3(best * best_grid);
+    cfg.gridDim = dim3(static_cast<unsigned>(best * (most < clusters ? most : clusters)));
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmW, p);
     return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, "4-bit GEMV launch");
 }
