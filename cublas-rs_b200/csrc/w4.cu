@@ -438,10 +438,12 @@ struct RowScales {
     __device__ __forceinline__ uint32_t zero(int i) const { return ZEROS ? z[i / 4] >> (8 * (i & 3)) & 15u : 8u; }
 };
 
-// A box's products: this lane's words of its steps, the vectors' pieces of its
-// first step at shared address x.  FULL: it has all its steps.
-template <bool BF16, bool ZEROS, int SPG, bool FULL>
-__device__ __forceinline__ void box_products(float (&total)[2][4], const uint32_t (&words)[kBoxSteps][4], uint32_t x, int xstep,
+// A box's products: this lane's words of its steps, in registers (EARLY) or at
+// shared address w, the vectors' pieces of its first step at shared address x.
+// FULL: it has all its steps.
+template <bool BF16, bool ZEROS, int SPG, bool EARLY, bool FULL>
+__device__ __forceinline__ void box_products(float (&total)[2][4], const uint32_t (&words)[EARLY ? kBoxSteps : 1][4],
+                                             uint32_t w, uint32_t x, int xstep,
                                              const RowScales<SPG, ZEROS> &row, int g, int steps) {
     using H = b2b::Half16<BF16>;
     uint32_t sw[4], zw[4];  // of rows g, g + 8, g + 16, g + 24: two groups' scales, four groups' zero points
@@ -465,10 +467,13 @@ __device__ __forceinline__ void box_products(float (&total)[2][4], const uint32_
             if (!FULL && si > 0 && st >= steps) break;
             const uint4 xv = lds128(x);
             x += xstep;
+            uint32_t own[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) own[i] = EARLY ? words[EARLY ? st : 0][i] : lds32((w ^ (st << 4)) + i * 1024);
             if (si == 0)
-                step32<BF16, true>(sum, words[st], un, xv);
+                step32<BF16, true>(sum, own, un, xv);
             else
-                step32<BF16, false>(sum, words[st], un, xv);
+                step32<BF16, false>(sum, own, un, xv);
         }
         add_scaled(total, sum, scale);
     }
@@ -493,6 +498,25 @@ __device__ __forceinline__ bool wait_finished(const volatile int *count, int wan
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
+// A place in a cluster's sequence of rounds.
+struct Place {
+    uint32_t set, tile, left;  // next tile, and how many are left
+    // Takes the next round: 2^result tiles from `tile` on.
+    __device__ __forceinline__ int take(uint32_t tiles, uint32_t most) {
+        const int lp = 31 - __clz(static_cast<int>(min(min(left, tiles - tile), most)));
+        left -= 1u << lp;
+        tile += 1u << lp;
+        return lp;
+    }
+    // ... after which a set may be done.
+    __device__ __forceinline__ void settle(uint32_t tiles) {
+        if (tile == tiles) {
+            tile = 0;
+            ++set;
+        }
+    }
+};
+
 // SPG: steps of 32 columns in a group, 8 standing for its multiples; 0: plain
 // loads, any group.
 template <bool BF16, bool ZEROS, int SPG>
@@ -503,6 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr bool TMA = SPG != 0;
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag;
+    __shared__ Place batch_begin;                 // KS > 1: where the batch of rounds began
     __shared__ int arrived[2][5][kWarps];         // warps of a tile (by log2 of their number) whose sums are in `part`
     __shared__ volatile int finished[2][kWarps];  // rounds whose sums of this warp are joined
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -576,26 +601,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t all = static_cast<uint64_t>(sets) * tiles;
     const uint64_t t_begin = all * cluster / clusters, t_end = all * (cluster + 1) / clusters;
 
-    // A place in the cluster's sequence of rounds.
-    struct Place {
-        uint32_t set, tile, left;  // next tile, and how many are left
-        // Takes the next round: 2^result tiles from `tile` on.
-        __device__ __forceinline__ int take(uint32_t tiles, uint32_t most) {
-            const int lp = 31 - __clz(static_cast<int>(min(min(left, tiles - tile), most)));
-            left -= 1u << lp;
-            tile += 1u << lp;
-            return lp;
-        }
-        // ... after which a set may be done.
-        __device__ __forceinline__ void settle(uint32_t tiles) {
-            if (tile == tiles) {
-                tile = 0;
-                ++set;
-            }
-        }
-    };
     Place here{static_cast<uint32_t>(t_begin / tiles), static_cast<uint32_t>(t_begin % tiles),
                static_cast<uint32_t>(t_end - t_begin)};
+    if (tid == 0) batch_begin = here;
 
     auto matrix_of = [&](uint32_t set) { return p.index ? items[set].matrix : 0; };
 
@@ -676,7 +684,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     int e = -1;          // the set's matrix
     uint32_t over = 0;   // 2^16 / nb, rounded up: o * over >> 16 is o / nb for the sums of a tile
     uint32_t staged = 0xffffffffu;  // the set whose vectors are staged
-    Place batch = here;  // where the batch of rounds began
     bool single = true;  // the cluster has one round: nothing to go on with at its end
     for (int v = 0; here.left; ++v) {
         const uint32_t set = here.set, first = here.tile;
@@ -745,26 +752,35 @@ __global__ void __launch_bounds__(kThreads, 1)
                                                       p.wait_ns);
                             dead = !__all_sync(0xffffffffu, ok);
                         }
-                        // The words go to registers at once, so that the box is in
-                        // flight again while they are multiplied.
-                        // 16-byte piece st of row r sits at piece st ^ (r % 8).
+                        // 16-byte piece st of row r sits at piece st ^ (r % 8)
                         const uint32_t w = smem_u32(ring) + b * kBoxBytes + g * 128 + (g << 4) + q * 4;
-                        uint32_t words[kBoxSteps][4];
-#pragma unroll
-                        for (int st = 0; st < kBoxSteps; ++st)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) words[st][i] = lds32((w ^ (st << 4)) + i * 1024);
-                        const RowScales<SPG, ZEROS> here = scales[b];
-                        // every lane's reads come before the box's next contents
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        load(b);
                         const uint32_t xs = g < nb ? smem_u32(sx) + (l * steps_of + b * kBoxSteps) * nb * 64 + lane * 16
                                                    : smem_u32(nothing);
+                        // EARLY: the words go to registers at once, so that the box is in
+                        // flight again while they are multiplied.  Groups of 32 and 64
+                        // columns, whose scales and zero points take most of the time
+                        // and of the registers, leave them where they are.
+                        constexpr bool EARLY = SPG >= 4;
+                        uint32_t words[EARLY ? kBoxSteps : 1][4];
+                        const RowScales<SPG, ZEROS> mine = scales[b];
+                        auto refill = [&] {
+                            // every lane's reads come before the box's next contents
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            load(b);
+                        };
+                        if constexpr (EARLY) {
+#pragma unroll
+                            for (int st = 0; st < kBoxSteps; ++st)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) words[st][i] = lds32((w ^ (st << 4)) + i * 1024);
+                            refill();
+                        }
                         if (steps >= kBoxSteps)
-                            box_products<BF16, ZEROS, SPG, true>(total, words, xs, xstep, here, g, steps);
+                            box_products<BF16, ZEROS, SPG, EARLY, true>(total, words, w, xs, xstep, mine, g, steps);
                         else if (steps > 0)
-                            box_products<BF16, ZEROS, SPG, false>(total, words, xs, xstep, here, g, steps);
+                            box_products<BF16, ZEROS, SPG, EARLY, false>(total, words, w, xs, xstep, mine, g, steps);
+                        if constexpr (!EARLY) refill();
                     }
                     phase ^= 1u;
                     advance();
@@ -865,6 +881,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             // share of the rounds, and the next batch goes to the other slots
             __syncwarp();
             cluster_sync();
+            Place batch = batch_begin;
             for (int i = 0; i <= v % kBatch; ++i) {
                 const uint32_t bset = batch.set, bfirst = batch.tile;
                 const int blp = batch.take(tiles, p.parts);
@@ -880,6 +897,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     put(bset, be, bfirst + t, o / bnb, o % bnb, sum);
                 }
             }
+            __syncthreads();
+            if (tid == 0) batch_begin = here;
         }
     }
     if (KS > 1) {  // no CTA leaves while another reads its sums
