@@ -786,36 +786,56 @@ __global__ void __launch_bounds__(kThreads, 1)
                     advance();
                 }
             } else {
-                // a row of this lane, or the last one for one that is not there
-                auto row_at = [&](int i) { return row0 + min(i, rows - 1); };
+                // this lane's rows, or the last one for those that are not there
+                int64_t row[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) row[i] = row0 + min(8 * i, rows - 1);
+                int held = -1;  // the group whose scales and zero points are held
+                float scale[4];
+                Unpack<BF16> un[4] = {Unpack<BF16>(8), Unpack<BF16>(8), Unpack<BF16>(8), Unpack<BF16>(8)};
                 for (int c = 0; c < own; ++c) {
                     const int l = kwarp + (c << lk), chunk = l * KS + rank;
                     const int steps = min(steps_of, static_cast<int>((p.w.n + 31) / 32) - chunk * steps_of);
                     const uint8_t *xs = g < nb ? sx + l * steps_of * nb * 64 + lane * 16 : nothing;
                     // all loads of 8 steps before their use
                     for (int s0 = 0; s0 < steps; s0 += 8) {
+                        const int64_t byte0 = static_cast<int64_t>(chunk) * (cols_of / 2) + s0 * 16 + q * 4;
                         uint32_t words[8][4];
+                        // words and the ones behind them that lie in `packed` whatever the alignment
+                        const bool inside = (row0 - g + kTileRows) * p.w.pitch + byte0 + 8 * 16 + 8 <= p.total &&
+                                            byte0 + row0 * p.w.pitch >= 4;
+                        if (__all_sync(0xffffffffu, inside)) {
 #pragma unroll
-                        for (int st = 0; st < 8; ++st)
+                            for (int i = 0; i < 4; ++i) {
+                                const uint8_t *from = p.w.packed + row[i] * p.w.pitch + byte0;
+                                const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from) & 3);
+                                const uint32_t *at = reinterpret_cast<const uint32_t *>(from - shift);
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                words[st][i] = s0 + st < steps && 8 * i < rows
-                                                   ? word_at(p, (row0 + 8 * i) * p.w.pitch + static_cast<int64_t>(chunk) * (cols_of / 2) +
-                                                                    (s0 + st) * 16 + q * 4)
-                                                   : 0u;
+                                for (int st = 0; st < 8; ++st) words[st][i] = __ldg(at + st * 4);
+                                if (__any_sync(0xffffffffu, shift != 0)) {
+#pragma unroll
+                                    for (int st = 0; st < 8; ++st)
+                                        words[st][i] = __funnelshift_r(words[st][i], __ldg(at + st * 4 + 1), 8 * shift);
+                                }
+                            }
+                        } else {
+#pragma unroll
+                            for (int st = 0; st < 8; ++st)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) words[st][i] = word_at(p, row[i] * p.w.pitch + byte0 + st * 16);
+                        }
 #pragma unroll
                         for (int st = 0; st < 8; ++st) {
                             if (s0 + st < steps) {
                                 const int grp = (chunk * steps_of + s0 + st) / spg;
-                                RowScales<0, ZEROS> here[4];
+                                if (grp != held) {
+                                    held = grp;
 #pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    here[i].load(p.w.scales + row_at(8 * i) * p.w.gs + grp,
-                                                 p.w.zeros + row_at(8 * i) * p.w.gs + grp, 1, 0);
-                                const Unpack<BF16> un[4] = {Unpack<BF16>(here[0].zero(0)), Unpack<BF16>(here[1].zero(0)),
-                                                            Unpack<BF16>(here[2].zero(0)), Unpack<BF16>(here[3].zero(0))};
-                                const float scale[4] = {H::get(here[0].scale(0)), H::get(here[1].scale(0)),
-                                                        H::get(here[2].scale(0)), H::get(here[3].scale(0))};
+                                    for (int i = 0; i < 4; ++i) {
+                                        scale[i] = H::get(__ldg(p.w.scales + row[i] * p.w.gs + grp));
+                                        if (ZEROS) un[i] = Unpack<BF16>(__ldg(p.w.zeros + row[i] * p.w.gs + grp) & 15u);
+                                    }
+                                }
                                 const uint4 x = *reinterpret_cast<const uint4 *>(xs);
                                 xs += xstep;
                                 float sum[2][4];
