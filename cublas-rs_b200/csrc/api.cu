@@ -37,6 +37,12 @@ int check_algo(int algo, const char *fn, bool allow_3xtf32) {
     return B2B_OK;
 }
 
+bool aligned_to(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+int misaligned(const char *fn) {
+    return fail(B2B_ERR_INVALID_ARG, std::string(fn) + ": an operand is not aligned to its element type");
+}
+
 int check_half(int type, const char *fn) {
     if (type != B2B_TYPE_F16 && type != B2B_TYPE_BF16)
         return fail(B2B_ERR_INVALID_ARG, std::string(fn) + ": type must be B2B_TYPE_F16 or B2B_TYPE_BF16");
@@ -175,6 +181,8 @@ int b2b_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, size_
         return fail(B2B_ERR_INVALID_ARG, "b2b_hgemm_grouped: trans_b must be B2B_OP_N or B2B_OP_T");
     if (groups == 0 || rows == 0 || n == 0 || k == 0) return B2B_OK;
     if (!A || !B || !C || !offsets) return fail(B2B_ERR_INVALID_ARG, "b2b_hgemm_grouped: NULL operand");
+    if (!aligned_to(A, 2) || !aligned_to(B, 2) || !aligned_to(C, 2) || !aligned_to(offsets, 4))
+        return misaligned("b2b_hgemm_grouped");
     if (int rc = check_grouped("b2b_hgemm_grouped", groups, rows, n, k)) return rc;
     DeviceGuard g(h);
     return launch_hgemm_grouped(h, type, trans_b, groups, rows, n, k, alpha, A, B, beta, C, offsets);
@@ -190,6 +198,9 @@ int b2b_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t groups, 
     if (groups == 0 || m == 0 || n == 0) return B2B_OK;
     if ((rows != 0 && (!A || !B)) || !C || !offsets)
         return fail(B2B_ERR_INVALID_ARG, "b2b_hgemm_grouped_wgrad: NULL operand");
+    if (!aligned_to(A, 2) || !aligned_to(B, 2) || !aligned_to(C, c_type == B2B_TYPE_F32 ? 4 : 2) ||
+        !aligned_to(offsets, 4))
+        return misaligned("b2b_hgemm_grouped_wgrad");
     if (int rc = check_grouped("b2b_hgemm_grouped_wgrad", groups, rows, m, n)) return rc;
     DeviceGuard g(h);
     return launch_hgemm_grouped_wgrad(h, type, c_type, groups, rows, m, n, alpha, A, B, beta, C, offsets);
@@ -201,6 +212,7 @@ int b2b_quantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, c
     if (int rc = check_w4("b2b_quantize_w4", type, 1, m, n, group)) return rc;
     if (m == 0 || n == 0) return B2B_OK;
     if (!W || !packed || !scales) return fail(B2B_ERR_INVALID_ARG, "b2b_quantize_w4: NULL operand");
+    if (!aligned_to(W, 2) || !aligned_to(scales, 2)) return misaligned("b2b_quantize_w4");
     DeviceGuard g(h);
     return launch_quantize_w4(h, type, m, n, group, W, packed, scales, zeros);
 }
@@ -211,6 +223,7 @@ int b2b_dequantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group,
     if (int rc = check_w4("b2b_dequantize_w4", type, 1, m, n, group)) return rc;
     if (m == 0 || n == 0) return B2B_OK;
     if (!W || !packed || !scales) return fail(B2B_ERR_INVALID_ARG, "b2b_dequantize_w4: NULL operand");
+    if (!aligned_to(W, 2) || !aligned_to(scales, 2)) return misaligned("b2b_dequantize_w4");
     DeviceGuard g(h);
     return launch_dequantize_w4(h, type, m, n, group, packed, scales, zeros, W);
 }
@@ -222,6 +235,7 @@ int b2b_hgemv_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, floa
     if (int rc = check_w4("b2b_hgemv_w4", type, 1, m, n, group)) return rc;
     if (m == 0 || n == 0 || count == 0) return B2B_OK;
     if (!packed || !scales || !x || !y) return fail(B2B_ERR_INVALID_ARG, "b2b_hgemv_w4: NULL operand");
+    if (!aligned_to(scales, 2) || !aligned_to(x, 2) || !aligned_to(y, 2)) return misaligned("b2b_hgemv_w4");
     if (int rc = check_w4_vectors("b2b_hgemv_w4", count, n, count, m)) return rc;
     DeviceGuard g(h);
     return launch_hgemv_w4(h, type, 1, m, n, group, alpha, packed, scales, zeros, x, count, 1, nullptr, beta, y);
@@ -236,6 +250,8 @@ int b2b_hgemv_w4_grouped(b2b_handle *h, int type, size_t groups, size_t m, size_
     if (groups == 0 || m == 0 || n == 0 || count == 0) return B2B_OK;
     if (!packed || !scales || !x || !y || !index)
         return fail(B2B_ERR_INVALID_ARG, "b2b_hgemv_w4_grouped: NULL operand");
+    if (!aligned_to(scales, 2) || !aligned_to(x, 2) || !aligned_to(y, 2) || !aligned_to(index, 4))
+        return misaligned("b2b_hgemv_w4_grouped");
     if (int rc = check_w4_vectors("b2b_hgemv_w4_grouped", count / fan + (count % fan != 0), n, count, m)) return rc;
     DeviceGuard g(h);
     return launch_hgemv_w4(h, type, groups, m, n, group, alpha, packed, scales, zeros, x, count,

@@ -167,6 +167,12 @@ __device__ __forceinline__ Tile tile_at(const TcArgs &p, const int *start, const
     return o;
 }
 
+// The limit of a wait for a whole tile: the bound of any wait, and 2 us for
+// each of its k blocks (they take under 1), so that no sum is too long.
+__device__ __forceinline__ uint64_t tile_wait_ns(const TcArgs &p, const Tile &o) {
+    return p.wait_ns + 2000ull * static_cast<uint64_t>(o.kblocks);
+}
+
 // Rows of A that CTA `rank` of a kNN / kNT tile loads: all 128 in one box, or
 // boxes of 16 when half of them or fewer exist (a decoding step has a few
 // rows an expert: 16 of 128 loaded rows leave the L2 to the weights).
@@ -603,7 +609,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
             stage = (stage + o.kblocks) % S;
             if (o.klast == 64) continue;
             const bool ok = mbar_wait_sleepy(&landed[s], phases >> s & 1u, abort_flag, p.status,
-                                             B2B_DEVSTAT_TIMEOUT | 0x25, p.wait_ns);
+                                             B2B_DEVSTAT_TIMEOUT | 0x25, tile_wait_ns(p, o));
             if (!__all_sync(0xffffffffu, ok)) break;
             phases ^= 1u << s;
             // row r of a box is its 128 bytes at r * 128, whatever the swizzle
@@ -648,9 +654,9 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
                 acc_phase ^= 1u;
             }
         };
-        auto wait_full = [&] {
+        auto wait_full = [&](const Tile &o) {
             const bool ok = mbar_wait_sleepy(&tfull[acc], acc_phase, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x24,
-                                             p.wait_ns);
+                                             tile_wait_ns(p, o));
             const bool all = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             return all;
@@ -672,7 +678,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
 #pragma unroll
                 for (int e = 0; e < BN / 2; ++e) x[e] = 0.0f;
                 for (int kb0 = 0; kb0 < o.kblocks || kb0 == 0; kb0 += Cf::PIECE) {
-                    ok = wait_full();
+                    ok = wait_full(o);
                     if (!ok) break;
                     if (o.kblocks > 0) {
 #pragma unroll
@@ -712,7 +718,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
                     store_segment<float>(cbase, pitch, buf, rows, ncols, p.vec, lane);
                 }
             } else {
-                ok = wait_full();
+                ok = wait_full(o);
                 if (!ok) break;
                 if (c_stop == c_first) release();
 #pragma unroll 1
@@ -897,7 +903,7 @@ int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, si
 int launch_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t groups, size_t rows, size_t m, size_t n,
                                float alpha, const uint16_t *A, const uint16_t *B, float beta, void *C,
                                const int32_t *offsets) {
-    const int64_t M = static_cast<int64_t>(m), N = static_cast<int64_t>(n), R = static_cast<int64_t>(rows);
+    const int64_t M = static_cast<int64_t>(m), N = static_cast<int64_t>(n);
     const int G = static_cast<int>(groups);
     const bool bf16 = type == B2B_TYPE_BF16, f32 = c_type == B2B_TYPE_F32;
     if (G * (M / 128 + 1) * (N / 64 + 1) >= 1ll << 31)

@@ -12,7 +12,6 @@
 
 #include <mutex>
 #include <type_traits>
-#include <vector>
 
 #include "half_types.cuh"
 #include "internal.h"

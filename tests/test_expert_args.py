@@ -63,6 +63,17 @@ def test_null_operands(lib, fake, call, names):
         assert call(lib, fake, **{name: NULL}) == INVALID and b"NULL operand" in lib.b2b_last_error()
 
 
+@pytest.mark.parametrize("call,names", [(forward, ("a", "b", "c")), (wgrad, ("a", "b")), (quant, ("w", "s")),
+                                        (dequant, ("w", "s")), (gemv, ("s", "x", "y")), (gemvg, ("s", "x", "y"))])
+def test_misaligned_operands(lib, fake, call, names):
+    for name in names:
+        assert call(lib, fake, **{name: ctypes.c_void_p(257)}) == INVALID and b"aligned" in lib.b2b_last_error()
+    for four in {forward: ("off",), wgrad: ("off", "c"), gemvg: ("index",)}.get(call, ()):
+        assert call(lib, fake, **{four: ctypes.c_void_p(258)}) == INVALID and b"aligned" in lib.b2b_last_error()
+    if call is wgrad:
+        assert wgrad(lib, fake, c_type=0, c=ctypes.c_void_p(257)) == INVALID
+
+
 @pytest.mark.parametrize("call,names", [(forward, ("groups", "rows", "n", "k")), (wgrad, ("groups", "m", "n")),
                                         (quant, ("m", "n")), (dequant, ("m", "n")), (gemv, ("m", "n", "count")),
                                         (gemvg, ("groups", "m", "n", "count"))])
