@@ -14,6 +14,7 @@ struct Half16;
 template <>
 struct Half16<false> {
     static constexpr float kMax = 65504.0f;
+    static constexpr float kNormal = 6.103515625e-05f;  // 2^-14
     __device__ __forceinline__ static float get(uint16_t v) { return __half2float(__ushort_as_half(v)); }
     __device__ __forceinline__ static uint16_t put(float v) { return __half_as_ushort(__float2half_rn(v)); }
     // Two values to one word, the first in the low half.
@@ -29,6 +30,7 @@ struct Half16<false> {
 template <>
 struct Half16<true> {
     static constexpr float kMax = 3.38953138925153547590e38f;
+    static constexpr float kNormal = 1.17549435082228750797e-38f;  // 2^-126
     __device__ __forceinline__ static float get(uint16_t v) { return __uint_as_float(static_cast<uint32_t>(v) << 16); }
     __device__ __forceinline__ static uint16_t put(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
     __device__ __forceinline__ static uint32_t put2(float a, float b) {

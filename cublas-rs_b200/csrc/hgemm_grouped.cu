@@ -80,13 +80,13 @@ __device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, in
 // up to the next multiple of 16, and the MMA issues only those k steps.
 //
 // Operands that TMA cannot describe (rows of a length or at a base that is not
-// a multiple of 16 bytes) are loaded by the HAND form: six warps in pairs, one
-// for A and one for B of a k block, three blocks at a time, write the same
+// a multiple of 16 bytes) are loaded by the HAND form: ten warps in pairs, one
+// for A and one for B of a k block, five blocks at a time, write the same
 // swizzled layouts with plain loads and fill ragged edges with zeros
 // themselves.
 //
 // Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer, 2..9 epilogue, 10
-// (kTN) the wiper; HAND: 10..15 load.  Two accumulators: the epilogue of a tile runs under the
+// (kTN) the wiper; HAND: 10..19 load.  Two accumulators: the epilogue of a tile runs under the
 // MMAs of the next.  The epilogue goes through shared memory to 64-byte row
 // segments, since a TMA store would write past the group's last row; it is a
 // chain of short latencies, so two warps share each quarter of the TMEM lanes.
@@ -106,7 +106,7 @@ struct Cfg {
     static constexpr int STAGES = 196608 / STAGE_BYTES;
     static constexpr int EPI_BYTES = 8 * 2048;  // 32 rows of 64 bytes for each epilogue warp
     static constexpr int TMEM_COLS = 2 * BN;
-    static constexpr int THREADS = HAND ? 512 : MODE == kTN ? 352 : 320;
+    static constexpr int THREADS = HAND ? 640 : MODE == kTN ? 352 : 320;
     static constexpr int TABLE_BYTES = 2 * 4224;  // tile starts and offsets: kMaxGroups + 1 ints each, rounded up
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + TABLE_BYTES + 1024 + 512;
     static_assert(SMEM_BYTES <= 232448 && TABLE_BYTES / 2 >= 4 * (kMaxGroups + 1), "shared memory per CTA");
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
         for (uint32_t t = first; t < tiles && ok; t += step) {
             const Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
             for (int kb = 0; kb < o.kblocks; ++kb, ++it) {
-                if (static_cast<int>(it % 3u) != pair) continue;
+                if (static_cast<int>(it % 5u) != pair) continue;
                 const int s = static_cast<int>(it % S);
                 const uint32_t phase = it / S & 1u;
                 ok = mbar_wait(&empty[s], phase ^ 1u, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x21, p.wait_ns);

@@ -50,22 +50,25 @@ struct Quantizer {
     static constexpr float kBorder = 0.499996185302734375f;  // 1/2 - 2^-18
     bool live;    // s > 0: false for a zero and a NaN scale, whose groups hold their zero point
     bool divide;  // the reciprocal overflows
-    __device__ __forceinline__ Quantizer(float scale, float lo, bool zeros) : s(scale) {
+    bool clamps;  // values may pass 0..15: with zero points, or where the scale was rounded by more than 1 / 100
+    // `normal`: the least normal number of the scale's type
+    __device__ __forceinline__ Quantizer(float scale, float lo, bool zeros, float normal) : s(scale) {
         live = s > 0.0f;
         inverse = __fdividef(1.0f, s);
         divide = !(inverse < 1e38f);
+        clamps = zeros || !(s >= normal);
         zero = 8.0f;
         if (zeros) zero = live ? fminf(rintf(__fdiv_rn(-lo, s)), 15.0f) : 0.0f;
     }
     __device__ __forceinline__ float clamp(float r) const { return fminf(fmaxf(r + zero, 0.0f), 15.0f); }
     __device__ __forceinline__ float exact(float w) const { return live ? clamp(rintf(__fdiv_rn(w, s))) : zero; }
-    // N values 0..15, as floats.
+    // N values 0..15, as floats, less `zero` where that is returned; else 0.
     template <int N>
-    __device__ __forceinline__ void operator()(const float (&w)[N], float (&out)[N]) const {
+    __device__ __forceinline__ float operator()(const float (&w)[N], float (&out)[N]) const {
         if (divide) {
 #pragma unroll
             for (int i = 0; i < N; ++i) out[i] = exact(w[i]);
-            return;
+            return 0.0f;
         }
         float far = 0.0f;
 #pragma unroll
@@ -81,17 +84,43 @@ struct Quantizer {
                 if (fabsf(off) > kBorder && odd) out[i] += copysignf(1.0f, off);
             }
         }
+        if (!clamps) return zero;
 #pragma unroll
         for (int i = 0; i < N; ++i) out[i] = clamp(out[i]);
+        return 0.0f;
     }
 };
 
-// Eight values to a word: the nibbles of two halves are added up in f32, where
-// they are exact.
-__device__ __forceinline__ uint32_t pack8(const float *q) {
-    const float low = fmaf(4096.0f, q[3], fmaf(256.0f, q[2], fmaf(16.0f, q[1], q[0])));
-    const float high = fmaf(4096.0f, q[7], fmaf(256.0f, q[6], fmaf(16.0f, q[5], q[4])));
+// Eight values, `less` added to each, to a word: the nibbles of two halves are
+// added up in f32, where they are exact.
+__device__ __forceinline__ uint32_t pack8(const float *q, float less) {
+    const float all = 4369.0f * less;  // 0x1111
+    const float low = fmaf(4096.0f, q[3], fmaf(256.0f, q[2], fmaf(16.0f, q[1], q[0] + all)));
+    const float high = fmaf(4096.0f, q[7], fmaf(256.0f, q[6], fmaf(16.0f, q[5], q[4] + all)));
     return static_cast<uint32_t>(low) | static_cast<uint32_t>(high) << 16;
+}
+
+// Least and largest of 0 and 16 values, two at a time; false where one of them
+// is an infinity or a NaN.
+template <bool BF16>
+__device__ __forceinline__ bool extremes(const uint32_t (&words)[8], float &lo, float &hi) {
+    using T = typename std::conditional<BF16, __nv_bfloat162, __half2>::type;
+    const T *v = reinterpret_cast<const T *>(words);
+    uint32_t none = 0;
+    const T zero = *reinterpret_cast<const T *>(&none);
+    T a = zero, b = zero, nan = zero;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        a = __hmin2(a, v[i]);
+        b = __hmax2(b, v[i]);
+        nan = __hfma2(v[i], zero, nan);  // 0, or a NaN once an infinity or a NaN is met
+    }
+    const float2 fa = b2b::Half16<BF16>::get2(*reinterpret_cast<const uint32_t *>(&a));
+    const float2 fb = b2b::Half16<BF16>::get2(*reinterpret_cast<const uint32_t *>(&b));
+    const float2 fn = b2b::Half16<BF16>::get2(*reinterpret_cast<const uint32_t *>(&nan));
+    lo = fminf(fa.x, fa.y);
+    hi = fmaxf(fb.x, fb.y);
+    return fn.x == 0.0f && fn.y == 0.0f;
 }
 
 // Groups of 16 LANES columns, 16 of them to a lane, which reads them once.
@@ -110,42 +139,39 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const uint16_t *W, uin
         const int64_t row = task / per;
         const int64_t unit = task % per * 32 + lane, j0 = unit * 16;
         const uint16_t *w = W + row * n + j0;
-        float v[16];
-        if constexpr (WHOLE) {
+        uint32_t words[8];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h) {
+            if constexpr (WHOLE) {
                 uint4 in = make_uint4(0, 0, 0, 0);
                 if (j0 + 8 * h < n) in = __ldg(reinterpret_cast<const uint4 *>(w) + h);
-                const uint32_t words[4] = {in.x, in.y, in.z, in.w};
+                words[4 * h] = in.x, words[4 * h + 1] = in.y, words[4 * h + 2] = in.z, words[4 * h + 3] = in.w;
+            } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = H::get2(words[i]);
-                    v[8 * h + 2 * i] = f.x;
-                    v[8 * h + 2 * i + 1] = f.y;
+                for (int i = 4 * h; i < 4 * h + 4; ++i) {
+                    words[i] = j0 + 2 * i < n ? __ldg(w + 2 * i) : 0u;
+                    if (j0 + 2 * i + 1 < n) words[i] |= static_cast<uint32_t>(__ldg(w + 2 * i + 1)) << 16;
                 }
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = j0 + i < n ? H::get(w[i]) : 0.0f;
         }
-        float lo = 0.0f, hi = 0.0f, nan = 0.0f;  // nan: 0, or a NaN once an infinity or a NaN is met
+        float v[16], lo, hi;
+        if (!extremes<BF16>(words, lo, hi)) hi = __int_as_float(0x7f800000);  // reaches the group's other lanes as an infinity
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            nan = fmaf(v[i], 0.0f, nan);
-            lo = fminf(lo, v[i]);
-            hi = fmaxf(hi, v[i]);
+        for (int i = 0; i < 8; ++i) {
+            const float2 f = H::get2(words[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
         }
-        if (nan != 0.0f) hi = __int_as_float(0x7f800000);  // reaches the group's other lanes as an infinity
 #pragma unroll
         for (int d = LANES / 2; d; d >>= 1) {
             lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
             hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, d));
         }
         const uint16_t s16 = w4_scale<BF16>(lo, hi, hi < __int_as_float(0x7f800000), zeros != nullptr);
-        const Quantizer q(H::get(s16), lo, zeros != nullptr);
+        const Quantizer q(H::get(s16), lo, zeros != nullptr, H::kNormal);
         float out[16];
-        q(v, out);
-        const uint32_t word0 = pack8(out), word1 = pack8(out + 8);
+        const float less = q(v, out);
+        const uint32_t word0 = pack8(out, less), word1 = pack8(out + 8, less);
         uint8_t *to = packed + row * pitch + unit * 8;
         if constexpr (WHOLE) {
             if (j0 + 8 < n) {
@@ -201,7 +227,7 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
         }
         const bool finite = __all_sync(0xffffffffu, nan == 0.0f);
         const uint16_t s16 = w4_scale<BF16>(lo, hi, finite, zeros != nullptr);
-        const Quantizer q(H::get(s16), lo, zeros != nullptr);
+        const Quantizer q(H::get(s16), lo, zeros != nullptr, H::kNormal);
         if (lane == 0) {
             scales[at] = s16;
             if (zeros) zeros[at] = static_cast<uint8_t>(q.zero);
