@@ -305,9 +305,8 @@ struct Item {
 // What a launch that chooses matrices keeps of its products.
 struct Table {
     Item item[kMaxIndexed];
-    int index[kMaxIndexed];
-    uint8_t lead[kMaxIndexed];
-    int items;
+    int4 index[kMaxIndexed / 4];      // the matrix that each product names, -1 where none
+    uint32_t leads[kMaxIndexed / 32];  // the products that are their sets' first, a bit each
 };
 
 // The 4 bytes at packed + at, wherever that is aligned; bytes past the end
@@ -581,43 +580,48 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int b = 0; b < 2; ++b) mbar_init(&full[b], 1);
         fence_barrier_init();
     }
+    int sets_named = 0;
     if (p.index) {
         const int e = named >= 0 && named < p.matrices ? named : -1;
-        if (tid < p.count) table->index[tid] = e;
+        if (tid < kMaxIndexed) reinterpret_cast<int *>(table->index)[tid] = tid < p.count ? e : -2;
         __syncthreads();
-        int seen = 0, lead = tid;  // products before this one of its matrix; the first of its set
-        if (tid < p.count) {
-            for (int i = 0; i < tid; ++i)
-                if (table->index[i] == e) {
-                    if (seen % p.width == 0) lead = i;
-                    ++seen;
-                }
-            if (seen % p.width == 0) lead = tid;
-            table->lead[tid] = lead == tid;
+        int place = 0, lead = tid;  // in the set; the set's first product
+        if (tid < kMaxIndexed) {
+            for (int i = 0; i < tid && tid < p.count; i += 4) {  // products before this one of its matrix
+                const int4 four = table->index[i >> 2];
+                const int other[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (other[k] == e && i + k < tid) {
+                        if (place == 0) lead = i + k;
+                        if (++place == p.width) place = 0;
+                    }
+            }
+            if (place == 0) lead = tid;
+            const uint32_t leads = __ballot_sync(0xffffffffu, tid < p.count && lead == tid);
+            if (lane == 0) table->leads[warp] = leads;
         }
         __syncthreads();
         int number = 0;  // of this product's set
-        if (tid < p.count) {
-            for (int i = 0; i < lead; ++i) number += table->lead[i];
-            if (lead == tid) {
-                table->item[number].matrix = e;
-                table->item[number].count = 0;
-            }
-            if (tid == p.count - 1) {
-                int all = 0;
-                for (int i = 0; i < p.count; ++i) all += table->lead[i];
-                table->items = all;
-            }
+        for (int w = 0; w < kMaxIndexed / 32; ++w) {
+            const uint32_t leads = table->leads[w];
+            sets_named += __popc(leads);
+            if (w < lead >> 5) number += __popc(leads);
+            if (w == lead >> 5) number += __popc(leads & ((1u << (lead & 31)) - 1));
+        }
+        if (tid < p.count && lead == tid) {
+            table->item[number].matrix = e;
+            table->item[number].count = 0;
         }
         __syncthreads();
         if (tid < p.count) {
-            table->item[number].member[seen % p.width] = static_cast<uint8_t>(tid);
-            atomicAdd(&table->item[number].count, 1);
+            table->item[number].member[place] = static_cast<uint8_t>(tid);
+            atomicMax(&table->item[number].count, place + 1);
         }
     }
     __syncthreads();
     const uint32_t tiles = static_cast<uint32_t>((p.w.m + kTileRows - 1) / kTileRows);
-    const uint32_t sets = p.index ? table->items : (p.count + p.width - 1) / p.width;
+    const uint32_t sets = p.index ? sets_named : (p.count + p.width - 1) / p.width;
     const int steps_of = p.boxes * kBoxSteps, cols_of = p.boxes * kBoxCols;  // of a chunk
     const int chunks = static_cast<int>((p.w.n + cols_of - 1) / cols_of);
     const int local = chunks > rank ? (chunks - rank + KS - 1) / KS : 0;  // this CTA's chunks of a tile
