@@ -284,6 +284,9 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t remote_addr
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Its two halves: a warp may go on between them.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // Load from shared memory of a CTA of the cluster (address from mapa).
 __device__ __forceinline__ float ld_shared_cluster(uint32_t addr) {

@@ -253,22 +253,26 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
 // bits.
 //
 //   * A tile is 32 rows of W for one set of vectors; its n columns are cut
-//     into chunks of 256 or 512 (a box or two), which the CTAs of a cluster and
-//     some of a CTA's 16 warps take in turn.  A cluster has an equal share of
-//     all tiles, next to each other, and takes them in rounds: of 16 tiles, a
-//     warp to each, while it has as many, then of 8, 4, 2 and 1 with 2, 4, 8
-//     and 16 warps to a tile, so that no warp idles while another has two.
-//   * Each warp holds one chunk (boxes of 32 rows x 128 bytes, 128-byte
-//     swizzle); TMA refills a box with the next chunk's as soon as it is used
-//     up, across rounds, so nothing drains at a round's end.  16 warps hold
-//     128 KiB of W, in flight or in use.
+//     into boxes of 256, which the CTAs of a cluster and some of a CTA's 16
+//     warps take in turn.  A cluster has an equal share of all tiles, next to
+//     each other, and takes them in rounds: of 16 tiles, a warp to each, while
+//     it has as many, then of 8, 4, 2 and 1 with 2, 4, 8 and 16 warps to a
+//     tile, so that no warp idles while another has two.
+//   * Each warp holds one box (32 rows x 128 bytes, 128-byte swizzle), copies
+//     it to registers, and TMA refills it, across rounds, so nothing drains at
+//     a round's end: 64 KiB of an SM in flight.  Two boxes to a warp took 38 us
+//     where one takes 35 (18944 x 16384), and the room is the vectors'.
 //   * The vectors are staged once for each set, each 8 columns reordered to
-//     the pairs (0,4) (1,5) (2,6) (3,7) that the words unpack to.
+//     the pairs (0,4) (1,5) (2,6) (3,7) that the words unpack to.  Only where
+//     they do not fit one SM, or where there are fewer tiles than SMs, is a
+//     tile shared by a cluster: its joining costs most of what it saves.
 //   * The last of a tile's warps to arrive adds their sums up while the others
-//     go on; the CTAs of a cluster read one another's sums once for 8 rounds.
-//     Both in a fixed order, whoever adds.
+//     go on; the CTAs of a cluster join the sums of up to 8 rounds at once,
+//     when those of the next ones are ready (18944 x 16384 by 8 vectors: 104
+//     us where all waited for all after each batch, 47 now).  Both in a fixed
+//     order, whoever adds.
 // Rows that TMA cannot describe (n not a multiple of 32, packed not 16-byte
-// aligned) and groups that do not fit a chunk evenly are read by the same
+// aligned) and groups that do not fit a box evenly are read by the same
 // kernel with plain loads (SPG = 0).
 constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
@@ -276,7 +280,7 @@ constexpr int kTileRows = 32;
 constexpr int kBoxCols = 256;                     // 128 bytes of a row
 constexpr int kBoxSteps = kBoxCols / 32;          // of 32 columns
 constexpr int kBoxBytes = kTileRows * kBoxCols / 2;
-constexpr int kBatch = 8;                         // rounds that the CTAs of a cluster join at once
+constexpr int kMaxBatch = 8;                      // rounds that the CTAs of a cluster join at once
 constexpr int kMaxIndexed = 256;                  // products of one launch that choose their matrix
 
 struct GemvArgs {
@@ -289,7 +293,7 @@ struct GemvArgs {
     int matrices, count, fan, first;  // first: number of this launch's first product
     int width;    // vectors of a set: 8, or fewer where longer rows leave room for fewer
     int parts;    // most tiles of a round, a power of two
-    int boxes;    // of a chunk: 1 or 2
+    int batch;    // rounds that the CTAs of a cluster join at once, a power of two
     int x_bytes;  // of the staged vectors
     int vec;      // a box's scales and zero points of a row are one aligned word each
     float alpha, beta;
@@ -551,21 +555,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr bool TMA = SPG != 0;
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag;
-    __shared__ Place batch_begin;                 // KS > 1: where the batch of rounds began
     __shared__ int arrived[2][5][kWarps];         // warps of a tile (by log2 of their number) whose sums are in `part`
     __shared__ volatile int finished[2][kWarps];  // rounds whose sums of this warp are joined
+    __shared__ Place begin[2][kWarps];            // KS > 1: where the last two batches of rounds began, for each warp
     uint8_t *smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, q = lane & 3;
     const int KS = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-    uint8_t *ring = smem + (TMA ? warp * 2 * kBoxBytes : 0);
-    uint8_t *sx = smem + (TMA ? kWarps * 2 * kBoxBytes : 0);
+    uint8_t *box = smem + (TMA ? warp * kBoxBytes : 0);
+    uint8_t *sx = smem + (TMA ? kWarps * kBoxBytes : 0);
     const int sums = kTileRows * p.width;                     // of a tile
     float *part = reinterpret_cast<float *>(sx + p.x_bytes);  // [2][kWarps][32 rows][width]
-    float *slots = part + 2 * kWarps * sums;                  // KS > 1: [2][kBatch][p.parts][32 rows][width]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(slots + (KS > 1 ? 2 * kBatch * p.parts * sums : 0));
-    uint64_t *full = bars + warp * 2;  // of its chunk's two boxes
-    uint8_t *nothing = reinterpret_cast<uint8_t *>(bars + kWarps * 2);  // 16 bytes of 0
+    float *slots = part + 2 * kWarps * sums;                  // KS > 1: [2][p.batch][p.parts][32 rows][width]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(slots + (KS > 1 ? 2 * p.batch * p.parts * sums : 0));
+    uint64_t *full = bars + warp;
+    uint8_t *nothing = reinterpret_cast<uint8_t *>(bars + kWarps);  // 16 bytes of 0
     Table *table = reinterpret_cast<Table *>(nothing + 16);
     const Item *items = table->item;
 
@@ -577,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid < 2 * 5 * kWarps) (&arrived[0][0][0])[tid] = 0;
     if (tid < 2 * kWarps) finished[tid / kWarps][tid % kWarps] = 0;
     if (TMA && lane == 0) {
-        for (int b = 0; b < 2; ++b) mbar_init(&full[b], 1);
+        mbar_init(full, 1);
         fence_barrier_init();
     }
     int sets_named = 0;
@@ -622,9 +626,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     const uint32_t tiles = static_cast<uint32_t>((p.w.m + kTileRows - 1) / kTileRows);
     const uint32_t sets = p.index ? sets_named : (p.count + p.width - 1) / p.width;
-    const int steps_of = p.boxes * kBoxSteps, cols_of = p.boxes * kBoxCols;  // of a chunk
-    const int chunks = static_cast<int>((p.w.n + cols_of - 1) / cols_of);
-    const int local = chunks > rank ? (chunks - rank + KS - 1) / KS : 0;  // this CTA's chunks of a tile
+    const int boxes = static_cast<int>((p.w.n + kBoxCols - 1) / kBoxCols);
+    const int local = boxes > rank ? (boxes - rank + KS - 1) / KS : 0;  // this CTA's boxes of a tile
     const uint32_t clusters = gridDim.x / KS, cluster = blockIdx.x / KS;
     // next to each other, so that a cluster changes its vectors rarely
     const uint64_t all = static_cast<uint64_t>(sets) * tiles;
@@ -632,8 +635,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     Place here{static_cast<uint32_t>(t_begin / tiles), static_cast<uint32_t>(t_begin % tiles),
                static_cast<uint32_t>(t_end - t_begin)};
-    if (tid == 0) batch_begin = here;
-
     auto matrix_of = [&](uint32_t set) { return p.index ? items[set].matrix : 0; };
 
     bool dead = false;
@@ -657,14 +658,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     int nb = 0;
     uint32_t phase = 0;
 
-    // The warp's next chunk, in this unit or a later one: as soon as a box of
-    // the present chunk is used up, the next chunk's takes its place, and the
-    // scales and zero points that belong to it are read, row `lane`'s by each
-    // lane (the tile's last one by lanes whose row is not there).
-    RowScales<SPG, ZEROS> scales[2];
+    // The warp's next box, of this round or a later one: it takes the present
+    // one's place as soon as that is used up, and the scales and zero points
+    // that belong to it are read, row `lane`'s by each lane (the tile's last
+    // one by lanes whose row is not there).
+    RowScales<SPG, ZEROS> scales;
     Place ahead = here;
-    bool more = true;  // there is a next chunk
-    int nc = 0, nstep = 0, nchunk = 0, nrow = 0;  // chunks left of its tile, and how far apart they are
+    bool more = true;  // there is a next box
+    int nc = 0, nstep = 0, nbox = 0, nrow = 0;  // boxes left of its tile, and how far apart they are
     const uint16_t *nscales = nullptr;
     const uint8_t *nzeros = nullptr;
     auto seek = [&] {
@@ -680,42 +681,72 @@ __global__ void __launch_bounds__(kThreads, 1)
             nrow = static_cast<int>(row);
             nscales = p.w.scales + at;
             if (ZEROS) nzeros = p.w.zeros + at;
-            nchunk = kwarp * KS + rank;
+            nbox = kwarp * KS + rank;
             nstep = KS << lk;
             nc = (local - kwarp + (1 << lk) - 1) >> lk;
             return;
         }
         more = false;
     };
-    auto load = [&](int b) {
+    auto load = [&] {
         if (!more || dead) return;
         if (lane == 0) {
-            mbar_arrive_expect_tx(&full[b], kBoxBytes);
-            tma_load_2d(ring + b * kBoxBytes, &tmW, &full[b], nchunk * (cols_of / 2) + b * (kBoxCols / 2), nrow);
+            mbar_arrive_expect_tx(full, kBoxBytes);
+            tma_load_2d(box, &tmW, full, nbox * (kBoxCols / 2), nrow);
         }
-        // a box behind the row's end loads zeros and has no groups
-        const int step = nchunk * steps_of + b * kBoxSteps;
-        if (step >= nsteps) return;
+        const int step = nbox * kBoxSteps;
         const int grp = SPG == kBoxSteps ? step / spg : step / (SPG ? SPG : 1);
-        scales[b].load(nscales + grp, nzeros + grp, static_cast<int>(p.w.gs) - grp, p.vec);
-    };
-    auto advance = [&] {
-        nchunk += nstep;
+        scales.load(nscales + grp, nzeros + grp, static_cast<int>(p.w.gs) - grp, p.vec);
+        nbox += nstep;
         if (--nc == 0) seek();
     };
     if constexpr (TMA) {
         seek();
-        load(0);
-        if (p.boxes == 2) load(1);
-        advance();
+        load();
     }
 
     int e = -1;          // the set's matrix
     uint32_t over = 0;   // 2^16 / nb, rounded up: o * over >> 16 is o / nb for the sums of a tile
     uint32_t staged = 0xffffffffu;  // the set whose vectors are staged
+    // KS > 1: the CTAs' sums of a batch of rounds are joined when those of the
+    // next one are ready, so that no warp waits for the others' last boxes.  A
+    // CTA adds up its share; a batch's slots are free again when all have
+    // arrived with the next batch's sums.
+    auto slots_of = [&](int v) { return slots + (v & p.batch ? p.batch : 0) * p.parts * sums; };  // of round v's batch
+    auto join_cluster = [&](int v) {  // v: the batch's last round
+        __syncwarp();
+        cluster_wait();
+        const float *joins = slots_of(v);
+        const int rounds = (v & (p.batch - 1)) + 1;
+        Place at = begin[v & p.batch ? 1 : 0][warp];
+        int share = 0;  // 512 sums each
+        for (int i = 0; i < rounds; ++i) {
+            const uint32_t set = at.set, first = at.tile;
+            const int lp = at.take(tiles, p.parts);
+            at.settle(tiles);
+            const int nb = vectors_of(set), e = matrix_of(set);
+            for (int k = tid; k - tid < 256 << lp; k += kThreads) {
+                if ((share++ & (KS - 1)) != rank) continue;
+                const int t = k >> 8, o = k & 255;
+                if (t >> lp || o >= kTileRows * nb) continue;
+                const uint32_t from = smem_u32(joins + (i * p.parts + t) * sums + o);
+                float of[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < KS) of[r] = ld_shared_cluster(mapa_shared(from, r));
+                float sum = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < KS) sum += of[r];
+                put(set, e, first + t, o / nb, o % nb, sum);
+            }
+        }
+    };
     bool single = true;  // the cluster has one round: nothing to go on with at its end
-    for (int v = 0; here.left; ++v) {
+    int v = 0;
+    for (; here.left; ++v) {
         const uint32_t set = here.set, first = here.tile;
+        if (KS > 1 && (v & (p.batch - 1)) == 0 && lane == 0) begin[v & p.batch ? 1 : 0][warp] = here;
         const int lp = here.take(tiles, p.parts), lk = 4 - lp, kw = 1 << lk;
         here.settle(tiles);
         single = single && here.left == 0;
@@ -729,35 +760,47 @@ __global__ void __launch_bounds__(kThreads, 1)
             over = (65536u + nb - 1) / nb;
             __syncthreads();  // everyone is done with the old vectors
             if (e >= 0) {
-                // 8 columns of four vectors a turn; local chunk l is chunk l * KS + rank
-                const int shift = p.boxes == 2 ? 6 : 5, octs = 1 << shift;  // 8 columns of a chunk
-                for (int i = tid; i < local * octs; i += kThreads) {
-                    const int64_t j = (static_cast<int64_t>(i >> shift) * KS + rank) * cols_of + (i & octs - 1) * 8;
-                    for (int b0 = 0; b0 < nb; b0 += 4) {
-                        uint4 in[4];
+                // 8 columns of a vector a piece, four pieces of a thread at
+                // once; local box l is box l * KS + rank
+                constexpr int kOcts = kBoxCols / 8;
+                const int pieces = local * kOcts;
+                int i = tid, b = 0;  // the next piece, of vector b
+                auto settle = [&] {
+                    while (i >= pieces && b < nb) {
+                        i -= pieces;
+                        ++b;
+                    }
+                };
+                settle();
+                while (b < nb) {
+                    uint4 in[4];
+                    int to[4];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if (b0 + k >= nb) continue;
-                            const int64_t v = p.index ? p.first + items[set].member[b0 + k]
-                                                      : static_cast<int64_t>(set) * p.width + b0 + k;
-                            const uint16_t *src = p.x + static_cast<int64_t>(static_cast<uint32_t>(v) / p.fan) * p.w.n + j;
-                            if (j + 8 <= p.w.n && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-                                in[k] = __ldg(reinterpret_cast<const uint4 *>(src));
-                            } else {
-                                uint16_t h[8];
+                    for (int k = 0; k < 4; ++k) {
+                        to[k] = -1;
+                        if (b >= nb) continue;
+                        // step i / 4 of the vectors' steps, vector, quarter i % 4
+                        to[k] = ((i >> 2) * nb + b) * 64 + (i & 3) * 16;
+                        const int64_t j = (static_cast<int64_t>(i / kOcts) * KS + rank) * kBoxCols + i % kOcts * 8;
+                        const int64_t v = p.index ? p.first + items[set].member[b] : static_cast<int64_t>(set) * p.width + b;
+                        const uint16_t *src = p.x + (p.fan == 1 ? v : static_cast<uint32_t>(v) / static_cast<uint32_t>(p.fan)) * p.w.n + j;
+                        if (j + 8 <= p.w.n && (reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+                            in[k] = __ldg(reinterpret_cast<const uint4 *>(src));
+                        } else {
+                            uint16_t h[8];
 #pragma unroll
-                                for (int t = 0; t < 8; ++t) h[t] = j + t < p.w.n ? src[t] : uint16_t(0);
-                                in[k] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
-                            }
+                            for (int t = 0; t < 8; ++t) h[t] = j + t < p.w.n ? src[t] : uint16_t(0);
+                            in[k] = make_uint4(h[0] | h[1] << 16, h[2] | h[3] << 16, h[4] | h[5] << 16, h[6] | h[7] << 16);
                         }
+                        i += kThreads;
+                        settle();
+                    }
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if (b0 + k >= nb) continue;
-                            // step i / 4 of the vectors' steps, vector, quarter i % 4
-                            *reinterpret_cast<uint4 *>(sx + ((i >> 2) * nb + b0 + k) * 64 + (i & 3) * 16) =
-                                make_uint4(__byte_perm(in[k].x, in[k].z, 0x5410), __byte_perm(in[k].x, in[k].z, 0x7632),
-                                           __byte_perm(in[k].y, in[k].w, 0x5410), __byte_perm(in[k].y, in[k].w, 0x7632));
-                        }
+                    for (int k = 0; k < 4; ++k) {
+                        if (to[k] < 0) continue;
+                        *reinterpret_cast<uint4 *>(sx + to[k]) =
+                            make_uint4(__byte_perm(in[k].x, in[k].z, 0x5410), __byte_perm(in[k].x, in[k].z, 0x7632),
+                                       __byte_perm(in[k].y, in[k].w, 0x5410), __byte_perm(in[k].y, in[k].w, 0x7632));
                     }
                 }
             }
@@ -771,48 +814,42 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int xstep = g < nb ? nb * 64 : 0;
             if constexpr (TMA) {
                 for (int c = 0; c < own; ++c) {
-                    const int l = kwarp + (c << lk), chunk = l * KS + rank;
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        if (b && p.boxes == 1) break;
-                        const int steps = nsteps - chunk * steps_of - b * kBoxSteps;
-                        if (!dead) {
-                            const bool ok = mbar_wait(&full[b], phase, &abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x31,
-                                                      p.wait_ns);
-                            dead = !__all_sync(0xffffffffu, ok);
-                        }
-                        // 16-byte piece st of row r sits at piece st ^ (r % 8)
-                        const uint32_t w = smem_u32(ring) + b * kBoxBytes + g * 128 + (g << 4) + q * 4;
-                        const uint32_t xs = g < nb ? smem_u32(sx) + (l * steps_of + b * kBoxSteps) * nb * 64 + lane * 16
-                                                   : smem_u32(nothing);
-                        // EARLY: the words go to registers at once, so that the box is in
-                        // flight again while they are multiplied.  Groups of 32 and 64
-                        // columns, whose scales and zero points take most of the time
-                        // and of the registers, leave them where they are.
-                        constexpr bool EARLY = SPG >= 4;
-                        uint32_t words[EARLY ? kBoxSteps : 1][4];
-                        const RowScales<SPG, ZEROS> mine = scales[b];
-                        auto refill = [&] {
-                            // every lane's reads come before the box's next contents
-                            fence_proxy_async_smem();
-                            __syncwarp();
-                            load(b);
-                        };
-                        if constexpr (EARLY) {
-#pragma unroll
-                            for (int st = 0; st < kBoxSteps; ++st)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) words[st][i] = lds32((w ^ (st << 4)) + i * 1024);
-                            refill();
-                        }
-                        if (steps >= kBoxSteps)
-                            box_products<BF16, ZEROS, SPG, EARLY, true>(total, words, w, xs, xstep, mine, g, steps);
-                        else if (steps > 0)
-                            box_products<BF16, ZEROS, SPG, EARLY, false>(total, words, w, xs, xstep, mine, g, steps);
-                        if constexpr (!EARLY) refill();
+                    const int l = kwarp + (c << lk), steps = nsteps - (l * KS + rank) * kBoxSteps;
+                    if (!dead) {
+                        const bool ok = mbar_wait(full, phase, &abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x31, p.wait_ns);
+                        dead = !__all_sync(0xffffffffu, ok);
                     }
                     phase ^= 1u;
-                    advance();
+                    // 16-byte piece st of row r sits at piece st ^ (r % 8)
+                    const uint32_t w = smem_u32(box) + g * 128 + (g << 4) + q * 4;
+                    const uint32_t xs = g < nb ? smem_u32(sx) + l * kBoxSteps * nb * 64 + lane * 16 : smem_u32(nothing);
+                    // EARLY: the words go to registers at once, so that the box is in
+                    // flight again while they are multiplied.  Groups of 32 columns,
+                    // and of 64 with zero points, need the registers for their scales
+                    // and leave the words where they are (4096 x 4096 by 8 vectors,
+                    // groups of 32: 8.7 us, early 9.4; 18944 x 16384 by 8, groups of
+                    // 64: 67 and 69 us, without zero points 52 and 50).
+                    constexpr bool EARLY = SPG >= 4 || (SPG == 2 && !ZEROS);
+                    uint32_t words[EARLY ? kBoxSteps : 1][4];
+                    const RowScales<SPG, ZEROS> mine = scales;
+                    auto refill = [&] {
+                        // every lane's reads come before the box's next contents
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        load();
+                    };
+                    if constexpr (EARLY) {
+#pragma unroll
+                        for (int st = 0; st < kBoxSteps; ++st)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) words[st][i] = lds32((w ^ (st << 4)) + i * 1024);
+                        refill();
+                    }
+                    if (steps >= kBoxSteps)
+                        box_products<BF16, ZEROS, SPG, EARLY, true>(total, words, w, xs, xstep, mine, g, steps);
+                    else
+                        box_products<BF16, ZEROS, SPG, EARLY, false>(total, words, w, xs, xstep, mine, g, steps);
+                    if constexpr (!EARLY) refill();
                 }
             } else {
                 // this lane's rows, or the last one for those that are not there
@@ -823,54 +860,52 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float scale[4];
                 Unpack<BF16> un[4] = {Unpack<BF16>(8), Unpack<BF16>(8), Unpack<BF16>(8), Unpack<BF16>(8)};
                 for (int c = 0; c < own; ++c) {
-                    const int l = kwarp + (c << lk), chunk = l * KS + rank;
-                    const int steps = min(steps_of, static_cast<int>((p.w.n + 31) / 32) - chunk * steps_of);
-                    const uint8_t *xs = g < nb ? sx + l * steps_of * nb * 64 + lane * 16 : nothing;
-                    // all loads of 8 steps before their use
-                    for (int s0 = 0; s0 < steps; s0 += 8) {
-                        const int64_t byte0 = static_cast<int64_t>(chunk) * (cols_of / 2) + s0 * 16 + q * 4;
-                        uint32_t words[8][4];
-                        // words and the ones behind them that lie in `packed` whatever the alignment
-                        const bool inside = (row0 - g + kTileRows) * p.w.pitch + byte0 + 8 * 16 + 8 <= p.total &&
-                                            byte0 + row0 * p.w.pitch >= 4;
-                        if (__all_sync(0xffffffffu, inside)) {
+                    const int l = kwarp + (c << lk), step0 = (l * KS + rank) * kBoxSteps;
+                    const int steps = min(kBoxSteps, static_cast<int>((p.w.n + 31) / 32) - step0);
+                    const uint8_t *xs = g < nb ? sx + l * kBoxSteps * nb * 64 + lane * 16 : nothing;
+                    const int64_t byte0 = static_cast<int64_t>(step0) * 16 + q * 4;
+                    // all loads before their use
+                    uint32_t words[8][4];
+                    // words and the ones behind them that lie in `packed` whatever the alignment
+                    const bool inside = (row0 - g + kTileRows) * p.w.pitch + byte0 + 8 * 16 + 8 <= p.total &&
+                                        byte0 + row0 * p.w.pitch >= 4;
+                    if (__all_sync(0xffffffffu, inside)) {
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint8_t *from = p.w.packed + row[i] * p.w.pitch + byte0;
-                                const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from) & 3);
-                                const uint32_t *at = reinterpret_cast<const uint32_t *>(from - shift);
+                        for (int i = 0; i < 4; ++i) {
+                            const uint8_t *from = p.w.packed + row[i] * p.w.pitch + byte0;
+                            const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from) & 3);
+                            const uint32_t *at = reinterpret_cast<const uint32_t *>(from - shift);
 #pragma unroll
-                                for (int st = 0; st < 8; ++st) words[st][i] = __ldg(at + st * 4);
-                                if (__any_sync(0xffffffffu, shift != 0)) {
+                            for (int st = 0; st < 8; ++st) words[st][i] = __ldg(at + st * 4);
+                            if (__any_sync(0xffffffffu, shift != 0)) {
 #pragma unroll
-                                    for (int st = 0; st < 8; ++st)
-                                        words[st][i] = __funnelshift_r(words[st][i], __ldg(at + st * 4 + 1), 8 * shift);
-                                }
+                                for (int st = 0; st < 8; ++st)
+                                    words[st][i] = __funnelshift_r(words[st][i], __ldg(at + st * 4 + 1), 8 * shift);
                             }
-                        } else {
-#pragma unroll
-                            for (int st = 0; st < 8; ++st)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) words[st][i] = word_at(p, row[i] * p.w.pitch + byte0 + st * 16);
                         }
+                    } else {
 #pragma unroll
-                        for (int st = 0; st < 8; ++st) {
-                            if (s0 + st < steps) {
-                                const int grp = (chunk * steps_of + s0 + st) / spg;
-                                if (grp != held) {
-                                    held = grp;
+                        for (int st = 0; st < 8; ++st)
 #pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        scale[i] = H::get(__ldg(p.w.scales + row[i] * p.w.gs + grp));
-                                        if (ZEROS) un[i] = Unpack<BF16>(__ldg(p.w.zeros + row[i] * p.w.gs + grp) & 15u);
-                                    }
+                            for (int i = 0; i < 4; ++i) words[st][i] = word_at(p, row[i] * p.w.pitch + byte0 + st * 16);
+                    }
+#pragma unroll
+                    for (int st = 0; st < 8; ++st) {
+                        if (st < steps) {
+                            const int grp = (step0 + st) / spg;
+                            if (grp != held) {
+                                held = grp;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    scale[i] = H::get(__ldg(p.w.scales + row[i] * p.w.gs + grp));
+                                    if (ZEROS) un[i] = Unpack<BF16>(__ldg(p.w.zeros + row[i] * p.w.gs + grp) & 15u);
                                 }
-                                const uint4 x = *reinterpret_cast<const uint4 *>(xs);
-                                xs += xstep;
-                                float sum[2][4];
-                                step32<BF16, true>(sum, words[st], un, x);
-                                add_scaled(total, sum, scale);
                             }
+                            const uint4 x = *reinterpret_cast<const uint4 *>(xs);
+                            xs += xstep;
+                            float sum[2][4];
+                            step32<BF16, true>(sum, words[st], un, x);
+                            add_scaled(total, sum, scale);
                         }
                     }
                 }
@@ -881,11 +916,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         // last of a tile's warps to get here adds their sums up; none waits,
         // but to reuse a buffer that is not joined yet.  A CTA of one round has
         // nothing to go on with: all its threads add up.
-        const int flip = v & 1;
-        if (kw == 1 && KS == 1) {
+        const int flip = v & 1, turn = v & (p.batch - 1);
+        if (KS > 1 && turn == 0 && v > 0) join_cluster(v - 1);
+        if (kw == 1) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)  // row g + 8 (i / 2), vector 2 q + i % 2
-                if (2 * q + (i & 1) < nb) put(set, e, tile, g + 8 * (i >> 1), 2 * q + (i & 1), total[i >> 2][i & 3]);
+            for (int i = 0; i < 8; ++i) {
+                const int r = g + 8 * (i >> 1), b = 2 * q + (i & 1);
+                if (b >= nb) continue;
+                if (KS == 1)
+                    put(set, e, tile, r, b, total[i >> 2][i & 3]);
+                else
+                    slots_of(v)[(turn * p.parts + part_no) * sums + r * nb + b] = total[i >> 2][i & 3];
+            }
             if (lane == 0) finished[flip][warp] = (v >> 1) + 1;
         } else {
             if (v >= 2 && !wait_finished(&finished[flip][warp], v >> 1, &abort_flag, p, lane)) dead = true;
@@ -904,7 +946,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (KS == 1)
                     put(set, e, first + t, r, o - r * nb, sum);
                 else
-                    slots[((v / kBatch % 2 * kBatch + v % kBatch) * p.parts + t) * sums + o] = sum;
+                    slots_of(v)[(turn * p.parts + t) * sums + o] = sum;
             };
             if (single) {
                 __syncthreads();
@@ -925,33 +967,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         }
-        if (KS > 1 && (v % kBatch == kBatch - 1 || here.left == 0)) {
-            // the batch's sums are in the CTAs of the cluster: each adds up its
-            // share of the rounds, and the next batch goes to the other slots
+        if (KS > 1 && (turn == p.batch - 1 || here.left == 0)) {
             __syncwarp();
-            cluster_sync();
-            Place batch = batch_begin;
-            for (int i = 0; i <= v % kBatch; ++i) {
-                const uint32_t bset = batch.set, bfirst = batch.tile;
-                const int blp = batch.take(tiles, p.parts);
-                batch.settle(tiles);
-                if (i % KS != rank) continue;
-                const int bnb = vectors_of(bset), be = matrix_of(bset);
-                for (int k = tid; k < 256 << blp; k += kThreads) {
-                    const int t = k >> 8, o = k & 255;
-                    if (o >= kTileRows * bnb) continue;
-                    const uint32_t at = smem_u32(slots + ((v / kBatch % 2 * kBatch + i) * p.parts + t) * sums + o);
-                    float sum = 0.0f;
-                    for (int r = 0; r < KS; ++r) sum += ld_shared_cluster(mapa_shared(at, r));
-                    put(bset, be, bfirst + t, o / bnb, o % bnb, sum);
-                }
-            }
-            __syncthreads();
-            if (tid == 0) batch_begin = here;
+            cluster_arrive();
         }
     }
-    if (KS > 1) {  // no CTA leaves while another reads its sums
-        __syncwarp();
+    if (KS > 1) {
+        if (v > 0) join_cluster(v - 1);
+        __syncwarp();  // no CTA leaves while another reads its sums
         cluster_sync();
     }
     if (TMA && dead && lane == 0) {  // loads in flight land before the CTA leaves
@@ -1074,14 +1097,14 @@ int launched(const char *what) {
     return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, what);
 }
 
-constexpr int kMaxSmem = 227 * 1024 - 1024;  // dynamic shared memory of the GEMV kernel, static beside it
-constexpr int64_t kMaxXBytes = 40 * 1024;    // of its staged vectors where 8 CTAs share a tile; fewer may have more
+constexpr int kMaxSmem = 227 * 1024 - 1536;  // dynamic shared memory of the GEMV kernel, static beside it
+constexpr int64_t kMaxXBytes = 80 * 1024;    // of its staged vectors where 8 CTAs share a tile; fewer may have more
 
 // Its shared memory for KS CTAs a tile; sets the vectors' bytes.
 size_t gemv_smem(GemvArgs &p, bool tma, int KS, int64_t local) {
-    p.x_bytes = static_cast<int>(local * p.boxes * kBoxCols * p.width * 2);
-    return p.x_bytes + 2 * (kWarps + (KS > 1 ? kBatch * p.parts : 0)) * kTileRows * p.width * 4 +
-           kWarps * ((tma ? 2 * kBoxBytes : 0) + 16) + 16 + (p.index ? sizeof(Table) : 0) + 1024;
+    p.x_bytes = static_cast<int>(local * kBoxCols * p.width * 2);
+    return p.x_bytes + 2 * (kWarps + (KS > 1 ? p.batch * p.parts : 0)) * kTileRows * p.width * 4 +
+           kWarps * ((tma ? kBoxBytes : 0) + 8) + 16 + (p.index ? sizeof(Table) : 0) + 1024;
 }
 
 // Clusters of KS CTAs (1, 2, 4 or 8) of the GEMV kernel that are resident at
@@ -1145,6 +1168,8 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
     const int64_t cols = (p.w.n + kBoxCols - 1) / kBoxCols, tiles = (p.w.m + kTileRows - 1) / kTileRows;
     p.width = p.count < 8 ? p.count : 8;
     while (p.width > 1 && (cols + 7) / 8 * kBoxCols * p.width * 2 > kMaxXBytes) --p.width;
+    if ((cols + 7) / 8 * kBoxCols * p.width * 2 > kMaxXBytes)
+        return b2b::fail(B2B_ERR_NOT_SUPPORTED, "4-bit GEMV: rows longer than 327680 columns");
     // with an index: the matrices that it names, if it names them at random,
     // and their sets
     double sets = static_cast<double>((p.count + p.width - 1) / p.width);
@@ -1172,48 +1197,45 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
             done = true;
         }
     }
-    // Share a tile's columns among KS CTAs of a cluster, in chunks of one box or
-    // two, so that a cluster's rounds take least: the boxes that a warp computes
-    // one after another, a third of one for each chunk's bookkeeping and one for
-    // each round's joining.
-    int best = 0, best_boxes = 0, best_parts = 0;
+    // Share a tile's columns among KS CTAs of a cluster so that it takes least, in
+    // boxes that a warp computes one after another (1.5 to 2 us): with its share of
+    // the vectors to stage, a fifth of a box for 16 KB, and where KS > 1 a quarter
+    // of one for the cluster and a fifth for each tile's joining.  It picks the
+    // fastest KS of 1, 2, 4 and 8 or comes within 1 % of it for 12 measured
+    // shapes: 16384 x 1024 takes 12.5 us by 1 and 22 by 4, 300 x 16384 13 and 7.7.
+    GemvArgs best = p;
+    int best_ks = 0;
     double best_time = 0;
-    for (p.boxes = 1; p.boxes <= 2; ++p.boxes) {
-        const int64_t chunks = (cols + p.boxes - 1) / p.boxes;
-        for (int KS = 1; KS <= 8 && (KS == 1 || KS < 2 * chunks); KS *= 2) {
-            const int64_t local = (chunks + KS - 1) / KS;
-            p.parts = kWarps;
-            while (p.parts > 1 && gemv_smem(p, spg != 0, KS, local) > static_cast<size_t>(kMaxSmem)) p.parts /= 2;
-            if (gemv_smem(p, spg != 0, KS, local) > static_cast<size_t>(kMaxSmem)) continue;
-            const int64_t clusters = resident_clusters(h, fn, KS);
-            int64_t left = (all + clusters - 1) / clusters;
-            auto round = [&](int parts) {
-                const int64_t kw = kWarps / parts;
-                return static_cast<double>((local + kw - 1) / kw) * (p.boxes + 0.33) + 1.0;
-            };
-            double time = static_cast<double>(left / p.parts) * round(p.parts);
-            left %= p.parts;
-            for (int parts = p.parts / 2; parts >= 1; parts /= 2)
-                if (left & parts) time += round(parts);
-            if (!best || time < best_time) {
-                best = KS;
-                best_boxes = p.boxes;
-                best_parts = p.parts;
-                best_time = time;
-            }
+    for (int KS = 1; KS <= 8 && (KS == 1 || KS < 2 * cols); KS *= 2) {
+        const int64_t local = (cols + KS - 1) / KS, clusters = resident_clusters(h, fn, KS);
+        auto fits = [&] { return gemv_smem(p, spg != 0, KS, local) <= static_cast<size_t>(kMaxSmem); };
+        p.parts = kWarps;
+        p.batch = KS > 1 ? kMaxBatch : 1;
+        while (p.batch > 1 && !fits()) p.batch /= 2;
+        while (p.parts > 1 && !fits()) p.parts /= 2;
+        if (!fits()) continue;
+        int64_t left = (all + clusters - 1) / clusters;  // tiles of a cluster
+        double time = 0.2 * static_cast<double>(local * p.width) / 32.0;
+        if (KS > 1) time += 0.25 + 0.2 * static_cast<double>(left);
+        for (int parts = p.parts; parts >= 1; parts /= 2) {  // rounds of as many tiles
+            const int64_t kw = kWarps / parts;
+            time += static_cast<double>(left / parts * ((local + kw - 1) / kw));
+            left %= parts;
+        }
+        if (!best_ks || time < best_time) {
+            best = p;
+            best_ks = KS;
+            best_time = time;
         }
     }
-    if (!best) return b2b::fail(B2B_ERR_NOT_SUPPORTED, "4-bit GEMV: rows longer than 163840 columns");
-    p.boxes = best_boxes;
-    p.parts = best_parts;
-    const int64_t chunks = (cols + p.boxes - 1) / p.boxes, local = (chunks + best - 1) / best;
-    const int64_t clusters = resident_clusters(h, fn, best);
+    p = best;
+    const int64_t local = (cols + best_ks - 1) / best_ks, clusters = resident_clusters(h, fn, best_ks);
     // an index may name more matrices than expected, but not more tiles than this
     const int64_t most = (p.index ? p.count : (p.count + p.width - 1) / p.width) * tiles;
-    attr[0].val.clusterDim.x = best;
-    cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, best, local);
-    cfg.numAttrs = best > 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(best * (most < clusters ? most : clusters)));
+    attr[0].val.clusterDim.x = best_ks;
+    cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, best_ks, local);
+    cfg.numAttrs = best_ks > 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(best_ks * (most < clusters ? most : clusters)));
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmW, p);
     return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, "4-bit GEMV launch");
 }

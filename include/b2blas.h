@@ -341,7 +341,7 @@ B2B_API int b2b_dequantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_
 /* y_i <- alpha*W*x_i + beta*y_i for `count` vectors: x is count x n, y is
  * count x m.  Products are exact, sums f32, y is rounded to nearest even
  * once.  The weights are read once for every 8 vectors (fewer where n is
- * beyond 20480).  y must not overlap the other operands.  n above 163840
+ * beyond 40960).  y must not overlap the other operands.  n above 327680
  * returns B2B_ERR_NOT_SUPPORTED, here and below. */
 B2B_API int b2b_hgemv_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, float alpha,
                          const uint8_t *packed, const uint16_t *scales, const uint8_t *zeros, const uint16_t *x,

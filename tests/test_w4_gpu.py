@@ -205,6 +205,19 @@ def test_gemv_random_values(handle, t, with_zeros, group):
     assert (np.abs(got - want) <= R.UNIT[t] * np.abs(want) * 1.001 + R.TINY[t] + (n + 2) * 2 * R.U32 * size).all()
 
 
+@pytest.mark.parametrize("n", [49152, 163840, 327680])
+def test_gemv_of_wide_rows(handle, n):
+    check(handle, "f16", 37, n, 128, False, 9 if n < 163840 else 3)
+
+
+def test_gemv_refuses_rows_that_are_too_wide(handle):
+    import b2blas
+
+    with pytest.raises(b2blas.CublasError) as e:
+        check(handle, "f16", 2, 327681, 128, False, 1)
+    assert e.value.status == 5 and "327680" in str(e.value)  # B2B_ERR_NOT_SUPPORTED
+
+
 def test_gemv_nan_scale_stays_in_its_row(handle):
     rng = np.random.default_rng(4)
     m, n = 40, 256
@@ -352,7 +365,10 @@ def test_graph_and_other_stream():
 
 @pytest.mark.parametrize("e,m,n,group,count,t,with_zeros", [
     (1, 16384, 16384, 128, 1, "f16", False), (1, 8192, 16384, 32, 8, "bf16", True), (5, 4096, 2048, 64, 40, "f16", True),
-    (1, 4096, 4104, 64, 3, "f16", True), (2, 20000, 20480, 256, 3, "bf16", False)])
+    (1, 4096, 4104, 64, 3, "f16", True), (2, 20000, 20480, 256, 3, "bf16", False),
+    # vectors that several SMs share: many joins, and rounds of every size
+    (1, 18944, 16384, 128, 8, "f16", True), (1, 30000, 40960, 64, 8, "bf16", False), (1, 40, 200000, 128, 2, "f16", False),
+    (8, 2048, 16384, 128, 32, "f16", True), (3, 6000, 8200, 64, 21, "bf16", True), (1, 64, 8192, 128, 1, "bf16", False)])
 def test_gemv_gives_the_same_exact_bits_each_time(handle, e, m, n, group, count, t, with_zeros):
     """Many rounds of every warp's buffers, 20 times over, against exact sums
     of whole numbers."""
