@@ -9,6 +9,7 @@
 // 16-bit operands (f16 or bf16), f32 sums.
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include <mutex>
@@ -80,16 +81,19 @@ __device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, in
 // up to the next multiple of 16, and the MMA issues only those k steps.
 //
 // Operands that TMA cannot describe (rows of a length or at a base that is not
-// a multiple of 16 bytes) are loaded by the HAND form: ten warps in pairs, one
-// for A and one for B of a k block, five blocks at a time, write the same
+// a multiple of 16 bytes) are loaded by the HAND form: 16 warps in fours, two
+// for A and two for B of a k block, four blocks at a time, write the same
 // swizzled layouts with plain loads and fill ragged edges with zeros
-// themselves.
+// themselves.  Their loads keep L1 busy two thirds of the time and wait for it
+// in the rest; a pair, whose CTAs load half of what a result needs, is
+// 1.6 times as fast where its tiles fill the machine.
 //
 // Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer, 2..9 epilogue, 10
-// (kTN) the wiper; HAND: 10..19 load.  Two accumulators: the epilogue of a tile runs under the
-// MMAs of the next.  The epilogue goes through shared memory to 64-byte row
-// segments, since a TMA store would write past the group's last row; it is a
-// chain of short latencies, so two warps share each quarter of the TMEM lanes.
+// (kTN) the wiper; HAND: 10.. load.  Two accumulators: the epilogue of a tile
+// runs under the MMAs of the next.  The epilogue goes through shared memory to
+// 64-byte row segments, since a TMA store would write past the group's last
+// row; it is a chain of short latencies, so two warps share each quarter of the
+// TMEM lanes.
 enum Mode { kNN = 0, kNT = 1, kTN = 2 };
 
 template <int MODE, bool PAIR, int BN_, bool F32_, bool HAND_>
@@ -106,7 +110,8 @@ struct Cfg {
     static constexpr int STAGES = 196608 / STAGE_BYTES;
     static constexpr int EPI_BYTES = 8 * 2048;  // 32 rows of 64 bytes for each epilogue warp
     static constexpr int TMEM_COLS = 2 * BN;
-    static constexpr int THREADS = HAND ? 640 : MODE == kTN ? 352 : 320;
+    static constexpr int LOADERS = F32 ? 12 : 16;  // HAND: loading warps, in fours; F32 needs the registers
+    static constexpr int THREADS = 320 + (HAND ? 32 * LOADERS : MODE == kTN ? 32 : 0);
     static constexpr int TABLE_BYTES = 2 * 4224;  // tile starts and offsets: kMaxGroups + 1 ints each, rounded up
     static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_BYTES + TABLE_BYTES + 1024 + 512;
     static_assert(SMEM_BYTES <= 232448 && TABLE_BYTES / 2 >= 4 * (kMaxGroups + 1), "shared memory per CTA");
@@ -247,50 +252,49 @@ __device__ __forceinline__ uint32_t ldg32_if(uint64_t a, bool take) {
     return v;
 }
 
-// One warp writes an operand's 16 KiB of a stage: 128 rows of 64 k values
-// (K_MAJOR: `slow` rows exist and `fast` k values), or two boxes of 64 k rows
-// of 64 columns (`slow` k rows and `fast` columns exist), zeros elsewhere, in
-// the 128-byte swizzle.  A lane takes pieces of 8 values, by the aligned words
-// that hold them: four, or five where the row starts between two words.  Those
-// reach a value beyond the tile on either side, so where that may lie outside
-// the operand, [lo, hi), values are read one by one.  8 pieces of a lane are
-// in flight at once.
-template <bool K_MAJOR>
+// One warp writes a box of an operand, 64 rows of 64 values in the 128-byte
+// swizzle: rows of A or B and their k values (K-major), or k rows and columns.
+// `slow` rows and `fast` values exist; zeros take the others' places up to the
+// next 16 rows, and what lies behind meets no result.  A lane takes pieces of 8
+// values, by the aligned words that hold them: four, or five where the row
+// starts between two words.  Those reach a value beyond the box on either side,
+// so where that may lie outside the operand, [lo, hi), values are read one by
+// one.  8 pieces of a lane are in flight at once.
 __device__ __forceinline__ void fill_by_hand(uint8_t *to, const uint16_t *from, int ld, int slow, int fast,
                                              const uint16_t *lo, const uint16_t *hi, int lane) {
-    constexpr int kPieces = 8, kSlow = K_MAJOR ? 128 : 64, kFast = K_MAJOR ? 64 : 128;
-    slow = min(slow, kSlow);
-    fast = min(fast, kFast);
+    constexpr int kPieces = 8;
+    slow = min(slow, 64);
+    fast = min(fast, 64);
+    if (slow <= 0 || fast <= 0) return;
+    const int rows = (slow + 15) & ~15;
     if (from == lo || from + static_cast<int64_t>(slow - 1) * ld + (fast + 7) / 8 * 8 + 1 > hi) {
-        // a row of 64 values a turn, two to a lane, 16 rows in flight
+        // a row a turn, two values to a lane, 16 rows in flight
         uint8_t *out = to + (lane & 3) * 4;
+        const int left = fast - 2 * lane;
 #pragma unroll 1
-        for (int i0 = 0; i0 < 128; i0 += 16) {
-            const int row0 = K_MAJOR ? i0 : i0 & 63, at = (K_MAJOR ? 0 : i0 >> 6 << 6) + 2 * lane;
-            const int left = fast - at;
-            const uint64_t p0 = reinterpret_cast<uint64_t>(from + static_cast<int64_t>(row0) * ld + at);
+        for (int i0 = 0; i0 < rows; i0 += 16) {
+            const uint64_t p0 = reinterpret_cast<uint64_t>(from + static_cast<int64_t>(i0) * ld + 2 * lane);
             uint32_t a[16], b[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const uint64_t p = p0 + static_cast<uint64_t>(ld) * 2u * j;
-                a[j] = ldg16_if(p, row0 + j < slow && left > 0);
-                b[j] = ldg16_if(p + 2, row0 + j < slow && left > 1);
+                a[j] = ldg16_if(p, i0 + j < slow && left > 0);
+                b[j] = ldg16_if(p + 2, i0 + j < slow && left > 1);
             }
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-                *reinterpret_cast<uint32_t *>(out + (K_MAJOR ? 0 : i0 >> 6) * kBoxBytes + (row0 + j) * 128 +
-                                              (((lane >> 2) ^ (j & 7)) << 4)) = a[j] | b[j] << 16;
+                *reinterpret_cast<uint32_t *>(out + (i0 + j) * 128 + (((lane >> 2) ^ (j & 7)) << 4)) = a[j] | b[j] << 16;
         }
         return;
     }
     // piece j of a turn: chunk lane % 8 of the turn's row lane / 8 + 4 j
     const int c = lane & 7, r = lane >> 3;
+    const int left = fast - c * 8;                         // values that exist
     const uint64_t step = static_cast<uint64_t>(ld) * 8u;  // bytes of four rows
 #pragma unroll 1
-    for (int i0 = 0; i0 < 128; i0 += 4 * kPieces) {
-        const int row0 = (K_MAJOR ? i0 : i0 & 63) + r, at = (K_MAJOR ? 0 : i0 >> 6 << 6) + c * 8;
-        const int left = fast - at;  // values that exist
-        const uint64_t p0 = reinterpret_cast<uint64_t>(from + static_cast<int64_t>(row0) * ld + at);
+    for (int i0 = 0; i0 < rows; i0 += 4 * kPieces) {
+        const int row0 = i0 + r;
+        const uint64_t p0 = reinterpret_cast<uint64_t>(from + static_cast<int64_t>(row0) * ld + c * 8);
         uint32_t w[kPieces][5];
 #pragma unroll
         for (int j = 0; j < kPieces; ++j) {
@@ -300,7 +304,7 @@ __device__ __forceinline__ void fill_by_hand(uint8_t *to, const uint16_t *from, 
             for (int i = 0; i < 4; ++i) w[j][i] = ldg32_if((p & ~3ull) + 4 * i, have);
             w[j][4] = ldg32_if((p & ~3ull) + 16, have && (p & 2));
         }
-        uint8_t *box = to + (K_MAJOR ? 0 : i0 >> 6) * kBoxBytes + row0 * 128;
+        uint8_t *out = to + row0 * 128;
 #pragma unroll
         for (int j = 0; j < kPieces; ++j) {
             const uint32_t shift = (static_cast<uint32_t>(p0 + step * j) & 2u) << 3;
@@ -310,7 +314,7 @@ __device__ __forceinline__ void fill_by_hand(uint8_t *to, const uint16_t *from, 
                 v[i] = __funnelshift_r(w[j][i], w[j][i + 1], shift);
                 if (left < 8 && left < 2 * i + 2) v[i] = left < 2 * i + 1 ? 0u : v[i] & 0xffffu;
             }
-            *reinterpret_cast<uint4 *>(box + j * 512 + ((c ^ ((row0 + 4 * j) & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4 *>(out + j * 512 + ((c ^ ((row0 + 4 * j) & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
         }
     }
 }
@@ -346,7 +350,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
             // a pair's kTN stage is full when both CTAs say so: their
             // producers, or for a group's last k block their wipers; HAND:
             // when both its warps do
-            mbar_init(&full[s], HAND || (PAIR && MODE == kTN) ? 2 : 1);
+            mbar_init(&full[s], HAND ? (PAIR ? 8 : 4) : PAIR && MODE == kTN ? 2 : 1);
             mbar_init(&empty[s], 1);
             mbar_init(&landed[s], 1);
         }
@@ -558,8 +562,9 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
         __syncwarp();
     } else if (HAND && warp >= 10) {
         // ------------------------------------------------ loading warps (HAND)
-        const int pair = (warp - 10) >> 1;
-        const bool is_b = (warp - 10) & 1;
+        const int turn = (warp - 10) >> 2;  // of the k blocks that are in flight
+        const int h = (warp - 10) & 1;      // box of the operand
+        const bool is_b = (warp - 10) & 2;
         const uint16_t *a_end = p.A + static_cast<int64_t>(p.rows) * (MODE == kTN ? p.M : p.K);
         const uint16_t *b_end = p.B + (MODE == kTN ? static_cast<int64_t>(p.rows) * p.N
                                                    : static_cast<int64_t>(p.groups) * p.N * p.K);
@@ -568,8 +573,9 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
         bool ok = true;
         for (uint32_t t = first; t < tiles && ok; t += step) {
             const Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
+            const int am = rank * 128 + 64 * h, bn = o.n0 + rank * Cf::BN_CTA + 64 * h;
             for (int kb = 0; kb < o.kblocks; ++kb, ++it) {
-                if (static_cast<int>(it % 5u) != pair) continue;
+                if (static_cast<int>(it % (Cf::LOADERS / 4u)) != turn) continue;
                 const int s = static_cast<int>(it % S);
                 const uint32_t phase = it / S & 1u;
                 ok = mbar_wait(&empty[s], phase ^ 1u, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x21, p.wait_ns);
@@ -577,25 +583,30 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
                 if (!ok) break;
                 const int k0 = kb * 64, k_left = o.depth - k0;
                 if (!is_b) {
+                    uint8_t *to = sA + s * Cf::A_BYTES + h * kBoxBytes;
                     if constexpr (MODE == kTN)
-                        fill_by_hand<false>(sA + s * Cf::A_BYTES, p.A + static_cast<int64_t>(o.row0 + k0) * p.M + o.m0, p.M,
-                                            k_left, p.M - o.m0, p.A, a_end, lane);
+                        fill_by_hand(to, p.A + static_cast<int64_t>(o.row0 + k0) * p.M + o.m0 + am, p.M, k_left,
+                                     p.M - o.m0 - am, p.A, a_end, lane);
                     else
-                        fill_by_hand<true>(sA + s * Cf::A_BYTES, p.A + static_cast<int64_t>(o.row0) * p.K + k0, p.K,
-                                           o.valid, k_left, p.A, a_end, lane);
+                        fill_by_hand(to, p.A + static_cast<int64_t>(o.row0 + am) * p.K + k0, p.K, o.valid - am, k_left, p.A,
+                                     a_end, lane);
                 } else {
-                    const int64_t matrix = MODE == kTN ? static_cast<int64_t>(o.row0) * p.N
-                                                       : static_cast<int64_t>(o.g) * p.N * p.K;
+                    uint8_t *to = sB + s * Cf::B_BYTES + h * kBoxBytes;
+                    const uint16_t *matrix = p.B + (MODE == kTN ? static_cast<int64_t>(o.row0) * p.N
+                                                                : static_cast<int64_t>(o.g) * p.N * p.K);
                     if constexpr (MODE == kNT)
-                        fill_by_hand<true>(sB + s * Cf::B_BYTES, p.B + matrix + static_cast<int64_t>(o.n0) * p.K + k0, p.K,
-                                           p.N - o.n0, k_left, p.B, b_end, lane);
+                        fill_by_hand(to, matrix + static_cast<int64_t>(bn) * p.K + k0, p.K, p.N - bn, k_left, p.B, b_end, lane);
                     else
-                        fill_by_hand<false>(sB + s * Cf::B_BYTES, p.B + matrix + static_cast<int64_t>(k0) * p.N + o.n0, p.N,
-                                            k_left, p.N - o.n0, p.B, b_end, lane);
+                        fill_by_hand(to, matrix + static_cast<int64_t>(k0) * p.N + bn, p.N, k_left, p.N - bn, p.B, b_end, lane);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&full[s]);
+                if (lane == 0) {
+                    if (leader)
+                        mbar_arrive(&full[s]);
+                    else
+                        mbar_arrive_cluster(mapa_shared(smem_u32(&full[s]), 0));
+                }
             }
         }
     } else if (!HAND && MODE == kTN && warp == 10) {
@@ -841,6 +852,16 @@ bool tma_can(const void *A, const void *B, int64_t ld_a, int64_t rows_b, int64_t
     return b2b::aligned16(A) && b2b::aligned16(B) && ld_a % 8 == 0 && ld_b % 8 == 0 && rows_b * ld_b < (1ll << 39);
 }
 
+// HAND: whether pairs' turns, over that many tile rows of 128 and of 256, take
+// less.  A k block costs a pair 1.1 us and a CTA 0.92 us for half the rows and
+// columns (16384 x 2049 x 2047: 283 and 442 us), but pairs have half as many turns
+// to fill (1000 x 515 x 1001: 27 and 21 us).
+bool by_hand_in_pairs(const b2b_handle *h, double rows128, double rows256, int64_t N) {
+    const double one = ceil(rows128 * static_cast<double>((N + 127) / 128) / h->sm_count);
+    const double two = ceil(rows256 * static_cast<double>((N + 255) / 256) / (h->sm_count / 2));
+    return 1.2 * two < one;
+}
+
 }  // namespace
 
 namespace b2b {
@@ -856,15 +877,20 @@ int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, si
         return fail(B2B_ERR_NOT_SUPPORTED, "grouped HGEMM: 2^31 tiles or more");
     TcArgs p{A, B, C, offsets, h->d_status, h->wait_limit_ns, G, static_cast<int>(rows), 0, static_cast<int>(n),
              static_cast<int>(k), alpha, beta, 0, bf16, n % 8 == 0 && aligned16(C)};
+    // pairs where groups are long enough on average to fill their 256 rows
+    bool pair = R >= 192 * static_cast<int64_t>(G) && N > 128;
     if (!tma) {
-        p.idesc = sm100::idesc_f32acc(bf16, 0, trans_b ? 0 : 1, 128, 128);
-        const int64_t most = (R / 128 + (R < G ? R : G)) * ((N + 127) / 128);
+        pair = pair && by_hand_in_pairs(h, static_cast<double>(R) / 128 + 0.5 * G, static_cast<double>(R) / 256 + 0.5 * G, N);
+        const int bm = pair ? 256 : 128;
+        p.idesc = sm100::idesc_f32acc(bf16, 0, trans_b ? 0 : 1, bm, bm);
+        const int64_t most = (R / bm + (R < G ? R : G)) * ((N + bm - 1) / bm);
         const CUtensorMap none{};
+        if (pair)
+            return trans_b ? launch_tc<kNT, true, 256, false, true>(h, none, none, none, p, most)
+                           : launch_tc<kNN, true, 256, false, true>(h, none, none, none, p, most);
         return trans_b ? launch_tc<kNT, false, 128, false, true>(h, none, none, none, p, most)
                        : launch_tc<kNN, false, 128, false, true>(h, none, none, none, p, most);
     }
-    // pairs where groups are long enough on average to fill their 256 rows
-    const bool pair = R >= 192 * static_cast<int64_t>(G) && N > 128;
     int bn = 256;
     if (!pair) {
         // The width whose turns of CTAs take least.  A k block of 64 costs a
@@ -910,14 +936,17 @@ int launch_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t group
         return fail(B2B_ERR_NOT_SUPPORTED, "grouped HGEMM: 2^31 tiles or more");
     TcArgs p{A, B, C, offsets, h->d_status, h->wait_limit_ns, G, static_cast<int>(rows), static_cast<int>(m),
              static_cast<int>(n), 0, alpha, beta, 0, bf16, n % (f32 ? 4 : 8) == 0 && aligned16(C)};
-    if (rows == 0 || !tma_can(A, B, M, 1, N)) {  // without rows nothing is loaded
-        p.idesc = sm100::idesc_f32acc(bf16, 1, 1, 128, 128);
-        const int64_t most = G * ((M + 127) / 128) * ((N + 127) / 128);
-        const CUtensorMap none{};
-        return f32 ? launch_tc<kTN, false, 128, true, true>(h, none, none, none, p, most)
-                   : launch_tc<kTN, false, 128, false, true>(h, none, none, none, p, most);
-    }
     const bool pair = M > 128 && N > 128;
+    if (rows == 0 || !tma_can(A, B, M, 1, N)) {  // without rows nothing is loaded
+        const bool two = pair && !f32 && by_hand_in_pairs(h, G * ((M + 127) / 128), G * ((M + 255) / 256), N);
+        const int bm = two ? 256 : 128;
+        p.idesc = sm100::idesc_f32acc(bf16, 1, 1, bm, bm);
+        const int64_t most = G * ((M + bm - 1) / bm) * ((N + bm - 1) / bm);
+        const CUtensorMap none{};
+        if (f32) return launch_tc<kTN, false, 128, true, true>(h, none, none, none, p, most);
+        return two ? launch_tc<kTN, true, 256, false, true>(h, none, none, none, p, most)
+                    : launch_tc<kTN, false, 128, false, true>(h, none, none, none, p, most);
+    }
     int bn = 256;
     while (!pair && bn > 64 && (G * ((M + 127) / 128) * ((N + bn - 1) / bn) < h->sm_count || N <= bn / 2)) bn /= 2;
     const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
