@@ -132,6 +132,19 @@ def test_forward_many_tiles(handle, counts, n, k):
 
 @pytest.mark.parametrize("t", ["f16", "bf16"])
 @pytest.mark.parametrize("trans", [False, True])
+def test_forward_odd_sizes_of_many_tiles(handle, t, trans):
+    check_forward(handle, t, [1400, 0, 900, 1], 1001, 131, trans, first=1, pad=3)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("counts", [[70, 0, 200, 1], [1, 33, 64, 129]])
+def test_wgrad_odd_sizes_of_many_tiles(handle, t, f32, counts):
+    check_wgrad(handle, t, f32, counts, 1001, 1003, first=1, pad=3)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("trans", [False, True])
 def test_forward_random_values(handle, t, trans):
     rng = np.random.default_rng(5)
     counts, n, k = [150, 0, 260, 33], 320, 1096
@@ -235,7 +248,7 @@ def test_wgrad_f32_keeps_f32_sums(handle, m, n):
     assert np.linalg.norm(got - want) <= 25 * 2.0 ** -23 * np.linalg.norm(want)
 
 
-@pytest.mark.parametrize("m,n", [(72, 72), (72, 65), (136, 136), (264, 264)])
+@pytest.mark.parametrize("m,n", [(72, 72), (72, 65), (136, 136), (264, 264), (1025, 1027)])
 def test_wgrad_neighbours_nan_stays_out(handle, m, n):
     """Every count from 1 to 40 next to a group of NaN: the last k step of a
     group ends inside a block that holds the next group's rows."""
