@@ -127,7 +127,8 @@ __device__ __forceinline__ bool extremes(const uint32_t (&words)[8], float &lo, 
 // WHOLE: n is a multiple of 8 and W and packed allow 16-byte loads and 4-byte
 // stores; else values and bytes one at a time.  HBM-bound where WHOLE: about
 // 250 instructions for the 40 bytes that a lane moves, most of them the
-// rounding and clamping of its values.
+// rounding and clamping of its values: 4096 x 4096 takes 14.5 us (2.9 TB/s),
+// 8192 x 8192 55 us with its schedulers 72 % busy.
 template <bool BF16, int LANES, bool WHOLE>
 __global__ void __launch_bounds__(256) w4_quantize_kernel(const uint16_t *W, uint8_t *packed, uint16_t *scales,
                                                           uint8_t *zeros, int64_t m, int64_t n, int64_t pitch, int64_t gs) {
@@ -201,8 +202,10 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const uint16_t *W, uin
     }
 }
 
-// Other groups: one warp a group, two neighbouring values a lane.
-template <bool BF16>
+// Other groups: one warp a group, which it reads twice, the second time out of
+// L1 or L2 unless it is very long.  WHOLE as above: 8 neighbouring values a
+// lane, else two.
+template <bool BF16, bool WHOLE>
 __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W, uint8_t *packed, uint16_t *scales,
                                                               uint8_t *zeros, int64_t m, int64_t n, int64_t group,
                                                               int64_t pitch, int64_t gs) {
@@ -214,11 +217,31 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
         const int64_t j1 = j0 + group < n ? j0 + group : n;
         const uint16_t *w = W + row * n;
         float lo = 0.0f, hi = 0.0f, nan = 0.0f;
-        for (int64_t j = j0 + lane; j < j1; j += 32) {
-            const float v = H::get(w[j]);
+        auto take = [&](float v) {
             nan = fmaf(v, 0.0f, nan);
             lo = fminf(lo, v);
             hi = fmaxf(hi, v);
+        };
+        auto eight = [&](int64_t j, float (&v)[8]) {
+            const uint4 in = __ldg(reinterpret_cast<const uint4 *>(w + j));
+            const uint32_t words[4] = {in.x, in.y, in.z, in.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = H::get2(words[i]);
+                v[2 * i] = f.x;
+                v[2 * i + 1] = f.y;
+            }
+        };
+        if constexpr (WHOLE) {
+#pragma unroll 2
+            for (int64_t j = j0 + 8 * lane; j < j1; j += 256) {
+                float v[8];
+                eight(j, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) take(v[i]);
+            }
+        } else {
+            for (int64_t j = j0 + lane; j < j1; j += 32) take(H::get(w[j]));
         }
 #pragma unroll
         for (int d = 16; d; d >>= 1) {
@@ -231,6 +254,16 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
         if (lane == 0) {
             scales[at] = s16;
             if (zeros) zeros[at] = static_cast<uint8_t>(q.zero);
+        }
+        if constexpr (WHOLE) {
+#pragma unroll 2
+            for (int64_t j = j0 + 8 * lane; j < j1; j += 256) {
+                float v[8], out[8];
+                eight(j, v);
+                const float less = q(v, out);
+                *reinterpret_cast<uint32_t *>(packed + row * pitch + j / 2) = pack8(out, less);
+            }
+            continue;
         }
         for (int64_t j = j0 + 2 * lane; j < j1; j += 64) {
             uint32_t byte = static_cast<uint32_t>(q.exact(H::get(w[j])));
@@ -271,6 +304,10 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
 //     when those of the next ones are ready (18944 x 16384 by 8 vectors: 104
 //     us where all waited for all after each batch, 47 now).  Both in a fixed
 //     order, whoever adds.
+// It streams 5.6 TB/s (packed bytes) where rows are long, 4.9 where they have
+// 2048 columns, after 7 us that any call takes: 16384 x 16384 by one vector
+// 35 us, by 8 47 us; what it lacks to HBM's 6.4 is instructions, 20 for each
+// word of a warp, half a cycle each on the pipes that most of them need.
 // Rows that TMA cannot describe (n not a multiple of 32, packed not 16-byte
 // aligned) and groups that do not fit a box evenly are read by the same
 // kernel with plain loads (SPG = 0).
@@ -1256,7 +1293,8 @@ int launch_quantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group
         const unsigned ctas = ctas_for(h, reinterpret_cast<const void *>(kernel), (tasks + 7) / 8);
         kernel<<<ctas, 256, 0, h->stream>>>(W, packed, scales, zeros, p.m, p.n, p.pitch, p.gs);
     } else {
-        auto kernel = bf16 ? w4_quantize_any_kernel<true> : w4_quantize_any_kernel<false>;
+        auto kernel = whole ? (bf16 ? w4_quantize_any_kernel<true, true> : w4_quantize_any_kernel<false, true>)
+                            : (bf16 ? w4_quantize_any_kernel<true, false> : w4_quantize_any_kernel<false, false>);
         const unsigned ctas = ctas_for(h, reinterpret_cast<const void *>(kernel), (p.m * p.gs + 7) / 8);
         kernel<<<ctas, 256, 0, h->stream>>>(W, packed, scales, zeros, p.m, p.n, p.group, p.pitch, p.gs);
     }

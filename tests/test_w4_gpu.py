@@ -63,6 +63,14 @@ def test_quantize_and_back(handle, t, with_zeros, group, m, n, shift):
 
 @pytest.mark.parametrize("t", ["f16", "bf16"])
 @pytest.mark.parametrize("with_zeros", [False, True])
+@pytest.mark.parametrize("m,n,group,shift", [(3, 4096, 512, 0), (2, 5000, 1024, 0), (5, 2056, 2080, 0), (3, 4096, 512, 2),
+                                             (2, 5000, 96, 8), (2, 1001, 320, 0)])
+def test_quantize_long_groups(handle, t, with_zeros, m, n, group, shift):
+    test_quantize_and_back(handle, t, with_zeros, group, m, n, shift)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("with_zeros", [False, True])
 def test_quantize_extremes(handle, t, with_zeros):
     """Groups of zeros, subnormals, the largest values, one sign only, and
     infinities and NaN, which make the group's scale NaN and no other's."""
