@@ -516,10 +516,13 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
                     const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
                     const int kb_end = kblocks - kb0 < Cf::PIECE ? kblocks : kb0 + Cf::PIECE;
                     for (int kb = kb0; kb < kb_end; ++kb) {
-                        if (!mbar_wait(&full[stage], phase, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x23, p.wait_ns)) {
-                            ok = false;
-                            break;
-                        }
+                        // the other CTA's loading warps or its wiper may have written its half
+                        if (PAIR && (HAND || (MODE == kTN && depth - kb * 64 < 64)))
+                            ok = mbar_wait<true>(&full[stage], phase, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x23,
+                                                 p.wait_ns);
+                        else
+                            ok = mbar_wait(&full[stage], phase, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x23, p.wait_ns);
+                        if (!ok) break;
                         tc_fence_after();
                         const uint32_t a = smem_u32(sA + stage * Cf::A_BYTES), b = smem_u32(sB + stage * Cf::B_BYTES);
                         // K-major: 8-row atoms 1024 bytes apart, a k step of 16

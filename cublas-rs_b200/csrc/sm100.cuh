@@ -61,16 +61,31 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar_addr, uint32_t parity
 // Upper bound on polls of a single wait, independent of the timer.
 constexpr uint32_t kMaxPolls = 1u << 30;
 
+// The same for what other CTAs of the cluster wrote before they arrived.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar_addr, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(ok)
+        : "r"(bar_addr), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // Waits for phase `parity` of `bar` to complete.  Returns false (and raises
 // *abort, and records `code` in *status) if it did not complete within
 // limit_ns, or returns false at once if another role already raised *abort.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *status,
                                           int code, uint64_t limit_ns) {
     const uint32_t a = smem_u32(bar);
-    if (mbar_try_wait(a, parity)) return true;
+    auto done = [&] { return CLUSTER ? mbar_try_wait_cluster(a, parity) : mbar_try_wait(a, parity); };
+    if (done()) return true;
     const uint64_t t0 = globaltimer_ns();
     for (uint32_t it = 1; it < kMaxPolls; ++it) {
-        if (mbar_try_wait(a, parity)) return true;
+        if (done()) return true;
         if ((it & 31u) == 0u) {
             if (*abort) return false;
             if (globaltimer_ns() - t0 > limit_ns) break;
