@@ -101,6 +101,12 @@ __device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, in
 // in the rest; a pair, whose CTAs load half of what a result needs, is
 // 1.6 times as fast where its tiles fill the machine.
 //
+// SPLIT: where there are fewer tiles than SMs, a cluster of 2, 4 or 8 CTAs shares
+// each tile's k blocks.  Their f32 sums meet in shared memory, where the stages
+// were, and every CTA adds up some of the rows, always in the order of the k
+// blocks.  One row of 4 groups, 512 x 4096: 25 -> 11 us; 7 rows of 4 groups, 1052 x
+// 3770: 50 -> 30; the gradient of 16000 rows of 2 groups, 65 x 129: 124 -> 24.
+//
 // Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer, 2..9 epilogue, 10
 // (kTN) the wiper; HAND: 10.. load.  Two accumulators: the epilogue of a tile
 // runs under the MMAs of the next.  The epilogue goes through shared memory to
@@ -130,6 +136,7 @@ struct Cfg {
     static_assert(SMEM_BYTES <= 232448 && TABLE_BYTES / 2 >= 4 * (kMaxGroups + 1), "shared memory per CTA");
 };
 constexpr int kBoxBytes = 64 * 64 * 2;  // 64 columns x 64 rows of an MN-major operand
+constexpr int kSumPitch = 132;          // SPLIT: floats of a row of sums, 128 of them in use
 constexpr int kGroupM = 16;             // raster: tile rows that sweep a group's columns together
 
 struct TcArgs {
@@ -152,6 +159,7 @@ struct Tile {
     int valid;      // rows of the tile that exist
     int depth;           // of the sum
     int kblocks, klast;  // k blocks of 64, and what the last one holds
+    int kfirst, kend;    // the k blocks of this CTA: all but where SPLIT
 };
 
 // The t-th tile, t ascending from call to call (g is kept between them).
@@ -182,6 +190,8 @@ __device__ __forceinline__ Tile tile_at(const TcArgs &p, const int *start, const
     o.valid = min(Cf::BM, (MODE == kTN ? p.M : hi - lo) - o.m0);
     o.kblocks = static_cast<int>(static_cast<uint32_t>(depth + 63) / 64);
     o.klast = depth - (o.kblocks - 1) * 64;
+    o.kfirst = 0;
+    o.kend = o.kblocks;
     return o;
 }
 
@@ -332,7 +342,7 @@ __device__ __forceinline__ void fill_by_hand(uint8_t *to, const uint16_t *from, 
     }
 }
 
-template <int MODE, bool PAIR, int BN, bool F32, bool HAND>
+template <int MODE, bool PAIR, int BN, bool F32, bool HAND, bool SPLIT>  // SPLIT: a tile at most to each cluster
 __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
     grouped_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA16,
                       const __grid_constant__ CUtensorMap tmB, TcArgs p) {
@@ -356,7 +366,18 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;
     const bool leader = rank == 0;
-    const uint32_t first = PAIR ? blockIdx.x >> 1 : blockIdx.x, step = PAIR ? gridDim.x >> 1 : gridDim.x;
+    // SPLIT: the CTAs of a cluster share one tile's k blocks
+    const int part = SPLIT ? static_cast<int>(cluster_ctarank()) : 0, parts = SPLIT ? static_cast<int>(cluster_nctarank()) : 1;
+    const uint32_t first = PAIR ? blockIdx.x >> 1 : SPLIT ? blockIdx.x / parts : blockIdx.x;
+    const uint32_t step = PAIR ? gridDim.x >> 1 : SPLIT ? gridDim.x / parts : gridDim.x;
+    auto tile_of = [&](uint32_t t, int &g) {
+        Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
+        if constexpr (SPLIT) {
+            o.kfirst = static_cast<int>(static_cast<int64_t>(o.kblocks) * part / parts);
+            o.kend = static_cast<int>(static_cast<int64_t>(o.kblocks) * (part + 1) / parts);
+        }
+        return o;
+    };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S; ++s) {
@@ -415,10 +436,10 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
             uint32_t phase = 0;
             bool ok = true;
             for (uint32_t t = first; t < tiles && ok; t += step) {
-                const Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
+                const Tile o = tile_of(t, g);
                 const int mine = MODE == kTN ? 8 : a_boxes16(o.valid, rank);
                 const int both = !PAIR ? mine : MODE == kTN ? 16 : a_boxes16(o.valid, 0) + a_boxes16(o.valid, 1);
-                for (int kb = 0; kb < o.kblocks; ++kb) {
+                for (int kb = o.kfirst; kb < o.kend; ++kb) {
                     if (!mbar_wait(&empty[stage], phase ^ 1u, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x21,
                                    p.wait_ns)) {
                         ok = false;
@@ -503,10 +524,14 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
             uint32_t phase = 0, acc_phase = 0;
             bool ok = true, issued = false;
             for (uint32_t t = first; t < tiles && ok; t += step) {
-                int depth = p.K;
-                if constexpr (MODE == kTN) depth = tile_at<MODE, Cf>(p, start, off, t, g).depth;
-                const int kblocks = static_cast<int>(static_cast<uint32_t>(depth + 63) / 64);
-                for (int kb0 = 0; ok && (kb0 == 0 || kb0 < kblocks); kb0 += Cf::PIECE) {
+                int depth = p.K, kfirst = 0, kend = static_cast<int>(static_cast<uint32_t>(depth + 63) / 64);
+                if constexpr (MODE == kTN || SPLIT) {
+                    const Tile o = tile_of(t, g);
+                    depth = o.depth;
+                    kfirst = o.kfirst;
+                    kend = o.kend;
+                }
+                for (int kb0 = kfirst; ok && (kb0 == kfirst || kb0 < kend); kb0 += Cf::PIECE) {
                     if (!mbar_wait(&tempty[acc], acc_phase ^ 1u, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x22,
                                    p.wait_ns)) {
                         ok = false;
@@ -514,7 +539,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
                     }
                     tc_fence_after();
                     const uint32_t d = tmem_base + static_cast<uint32_t>(acc * BN);
-                    const int kb_end = kblocks - kb0 < Cf::PIECE ? kblocks : kb0 + Cf::PIECE;
+                    const int kb_end = kend - kb0 < Cf::PIECE ? kend : kb0 + Cf::PIECE;
                     for (int kb = kb0; kb < kb_end; ++kb) {
                         // the other CTA's loading warps or its wiper may have written its half
                         if (PAIR && (HAND || (MODE == kTN && depth - kb * 64 < 64)))
@@ -588,9 +613,9 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
         uint32_t it = 0;  // k blocks of all tiles so far
         bool ok = true;
         for (uint32_t t = first; t < tiles && ok; t += step) {
-            const Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
+            const Tile o = tile_of(t, g);
             const int am = rank * 128 + 64 * h, bn = o.n0 + rank * Cf::BN_CTA + 64 * h;
-            for (int kb = 0; kb < o.kblocks; ++kb, ++it) {
+            for (int kb = o.kfirst; kb < o.kend; ++kb, ++it) {
                 if (static_cast<int>(it % (Cf::LOADERS / 4u)) != turn) continue;
                 const int s = static_cast<int>(it % S);
                 const uint32_t phase = it / S & 1u;
@@ -630,11 +655,12 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
         int stage = 0, g = 0;
         uint32_t phases = 0;  // bit s: parity of landed[s]
         for (uint32_t t = first; t < tiles; t += step) {
-            const Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
-            if (o.kblocks == 0) continue;
-            const int s = (stage + o.kblocks - 1) % S;
-            stage = (stage + o.kblocks) % S;
-            if (o.klast == 64) continue;
+            const Tile o = tile_of(t, g);
+            const int count = o.kend - o.kfirst;
+            if (count == 0) continue;
+            const int s = (stage + count - 1) % S;
+            stage = (stage + count) % S;
+            if (o.klast == 64 || o.kend < o.kblocks) continue;
             const bool ok = mbar_wait_sleepy(&landed[s], phases >> s & 1u, abort_flag, p.status,
                                              B2B_DEVSTAT_TIMEOUT | 0x25, tile_wait_ns(p, o));
             if (!__all_sync(0xffffffffu, ok)) break;
@@ -662,6 +688,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
         uint8_t *buf = epi + (warp - 2) * 2048;
         constexpr int csize = F32 ? 4 : 2;
         const int64_t pitch = static_cast<int64_t>(p.N) * csize;
+        float *sums = reinterpret_cast<float *>(smem) + (q * 32 + lane) * kSumPitch;  // SPLIT: this thread's row
         int acc = 0, g = 0;
         uint32_t acc_phase = 0;
         // the warp has read its share of the accumulator
@@ -691,7 +718,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
         const uint32_t tmem_warp = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
         bool ok = true;
         for (uint32_t t = first; t < tiles && ok; t += step) {
-            const Tile o = tile_at<MODE, Cf>(p, start, off, t, g);
+            const Tile o = tile_of(t, g);
             const int r0 = rank * 128 + q * 32;  // the warp's first row in the tile
             const int rows = min(32, o.valid - r0);
             uint8_t *C = static_cast<uint8_t *>(p.C) +
@@ -704,10 +731,10 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
                 float x[BN / 2];
 #pragma unroll
                 for (int e = 0; e < BN / 2; ++e) x[e] = 0.0f;
-                for (int kb0 = 0; kb0 < o.kblocks || kb0 == 0; kb0 += Cf::PIECE) {
+                for (int kb0 = o.kfirst; kb0 < o.kend || kb0 == o.kfirst; kb0 += Cf::PIECE) {
                     ok = wait_full(o);
                     if (!ok) break;
-                    if (o.kblocks > 0) {
+                    if (o.kend > o.kfirst) {
 #pragma unroll
                         for (int c = 0; c < BN / 2; c += 16) {
                             uint32_t r[16];
@@ -721,6 +748,12 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
                     turn();
                 }
                 if (!ok) break;
+                if constexpr (SPLIT) {
+#pragma unroll
+                    for (int c = 0; c < BN / 2; c += 4)
+                        *reinterpret_cast<float4 *>(sums + c_first + c) = make_float4(x[c], x[c + 1], x[c + 2], x[c + 3]);
+                    continue;
+                }
                 // segments of 16 columns
 #pragma unroll
                 for (int c = 0; c < BN / 2; c += 16) {
@@ -755,6 +788,16 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
                     tmem_ld_32x32b_x32(tmem_warp + static_cast<uint32_t>(acc * BN + c), r);
                     tmem_ld_wait();
                     if (c + 32 == c_stop) release();
+                    if constexpr (SPLIT) {
+                        // no k block: nothing was summed
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4)
+                            *reinterpret_cast<float4 *>(sums + c + e) =
+                                o.kend > o.kfirst ? make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]),
+                                                                __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]))
+                                                  : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        continue;
+                    }
                     const int col0 = o.n0 + c;
                     const int ncols = min(32, p.N - col0);
                     uint8_t *cbase = C + static_cast<int64_t>(col0) * csize;
@@ -790,10 +833,55 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
     }
 
     tc_fence_before();
-    if constexpr (PAIR)
+    if constexpr (SPLIT) {
+        // the tile's sums are in the CTAs of the cluster: each adds up its
+        // share of the rows, in the order of their k blocks
+        __syncwarp();
         cluster_sync();
-    else
+        if (first < tiles) {
+            int g = 0;
+            const Tile o = tile_of(first, g);
+            const int col = lane * 4, ncols = min(4, p.N - o.n0 - col);
+            for (int row = warp * parts + part; row < o.valid; row += Cf::THREADS / 32 * parts) {
+                if (ncols <= 0) continue;
+                const uint32_t at = smem_u32(smem) + (row * kSumPitch + col) * 4;
+                float4 of[8];
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < parts) of[r] = ld_shared_cluster_v4(mapa_shared(at, r));
+                float x[4] = {};
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (r < parts) x[0] += of[r].x, x[1] += of[r].y, x[2] += of[r].z, x[3] += of[r].w;
+                const int64_t i = ((MODE == kTN ? static_cast<int64_t>(o.g) * p.M + o.m0 : static_cast<int64_t>(o.row0)) + row) * p.N +
+                                  o.n0 + col;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = o.kblocks ? p.alpha * x[e] : 0.0f;
+                if constexpr (F32) {
+                    float *c = static_cast<float *>(p.C) + i;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e < ncols) c[e] = p.beta != 0.0f ? fmaf(p.beta, c[e], x[e]) : x[e];
+                } else {
+                    uint16_t *c = static_cast<uint16_t *>(p.C) + i;
+                    using B = b2b::Half16<true>;
+                    using H = b2b::Half16<false>;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        if (e >= ncols) continue;
+                        if (p.beta != 0.0f) x[e] = fmaf(p.beta, p.bf16 ? B::get(c[e]) : H::get(c[e]), x[e]);
+                        c[e] = p.bf16 ? B::put(x[e]) : H::put(x[e]);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync();  // no CTA leaves while another reads its sums
+    } else if constexpr (PAIR) {
+        cluster_sync();
+    } else {
         __syncthreads();
+    }
     if (warp == 1) {
         tc_fence_after();
         if constexpr (PAIR)
@@ -811,15 +899,16 @@ struct Launch {
 };
 std::mutex g_mu;
 
-template <int MODE, bool PAIR, int BN, bool F32 = false, bool HAND = false>
+template <int MODE, bool PAIR, int BN, bool F32 = false, bool HAND = false, bool SPLIT = false>
 int launch_tc(b2b_handle *h, const CUtensorMap &tmA, const CUtensorMap &tmA16, const CUtensorMap &tmB,
-              const TcArgs &p, int64_t most_tiles) {
+              const TcArgs &p, int64_t most_tiles, int parts = 1) {
     using Cf = Cfg<MODE, PAIR, BN, F32, HAND>;
+    static_assert(!SPLIT || (!PAIR && BN == 128 && 128 * kSumPitch * 4 <= Cf::STAGES * Cf::STAGE_BYTES), "SPLIT");
     static Launch state;
-    auto kernel = grouped_tc_kernel<MODE, PAIR, BN, F32, HAND>;
+    auto kernel = grouped_tc_kernel<MODE, PAIR, BN, F32, HAND, SPLIT>;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = PAIR ? 2 : 1;
+    attr[0].val.clusterDim.x = PAIR ? 2 : parts;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg = {};
@@ -847,8 +936,9 @@ int launch_tc(b2b_handle *h, const CUtensorMap &tmA, const CUtensorMap &tmA16, c
         }
         resident = state.resident[dev];
     }
-    const int units = static_cast<int>(most_tiles < resident ? most_tiles : resident);
-    cfg.gridDim = dim3((PAIR ? 2 : 1) * units);
+    // SPLIT: a cluster to every tile
+    const int units = static_cast<int>(SPLIT || most_tiles < resident ? most_tiles : resident);
+    cfg.gridDim = dim3((PAIR ? 2 : parts) * units);
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmA, tmA16, tmB, p);
     return e == cudaSuccess ? B2B_OK : b2b::fail_cuda(e, "grouped HGEMM tcgen05 launch");
 }
@@ -866,6 +956,21 @@ int launch_wgrad(b2b_handle *h, bool pair, int bn, const CUtensorMap &tmA, const
 // bases, and matrices less than 2^40 bytes apart.
 bool tma_can(const void *A, const void *B, int64_t ld_a, int64_t rows_b, int64_t ld_b) {
     return b2b::aligned16(A) && b2b::aligned16(B) && ld_a % 8 == 0 && ld_b % 8 == 0 && rows_b * ld_b < (1ll << 39);
+}
+
+// SPLIT: into how many parts to cut the k blocks of each of `tiles` 128 x 128
+// tiles, 1 where the machine has no SMs left for more (7 of 8 where clusters of
+// 4 leave some out, 3 of 4 with 8) or `us` that it takes otherwise is less: a k
+// block takes a CTA `per` us, and the parts' joining about 2.5.
+int k_parts(const b2b_handle *h, int64_t tiles, int64_t kblocks, double per, double us) {
+    int best = 1;
+    for (int parts = 2, eighths = 8; parts <= 8; parts *= 2, --eighths) {
+        const double t = 2.5 + per * static_cast<double>((kblocks + parts - 1) / parts);
+        if (tiles * parts * 8 > static_cast<int64_t>(h->sm_count) * eighths || t > 0.95 * us) continue;
+        best = parts;
+        us = t;
+    }
+    return best;
 }
 
 // HAND: whether pairs' turns, over that many tile rows of 128 and of 256, take
@@ -895,8 +1000,16 @@ int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, si
              static_cast<int>(k), alpha, beta, 0, bf16, n % 8 == 0 && aligned16(C)};
     // pairs where groups are long enough on average to fill their 256 rows
     bool pair = R >= 192 * static_cast<int64_t>(G) && N > 128;
+    const int64_t kb = (K + 63) / 64, tiles128 = (R / 128 + (R < G ? R : G)) * ((N + 127) / 128);
     if (!tma) {
         pair = pair && by_hand_in_pairs(h, static_cast<double>(R) / 128 + 0.5 * G, static_cast<double>(R) / 256 + 0.5 * G, N);
+        const int parts = pair ? 1 : k_parts(h, tiles128, kb, 1.1, 1.1 * static_cast<double>(kb));
+        if (parts > 1) {
+            p.idesc = sm100::idesc_f32acc(bf16, 0, trans_b ? 0 : 1, 128, 128);
+            const CUtensorMap none{};
+            return trans_b ? launch_tc<kNT, false, 128, false, true, true>(h, none, none, none, p, tiles128, parts)
+                           : launch_tc<kNN, false, 128, false, true, true>(h, none, none, none, p, tiles128, parts);
+        }
         const int bm = pair ? 256 : 128;
         p.idesc = sm100::idesc_f32acc(bf16, 0, trans_b ? 0 : 1, bm, bm);
         const int64_t most = (R / bm + (R < G ? R : G)) * ((N + bm - 1) / bm);
@@ -907,8 +1020,11 @@ int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, si
         return trans_b ? launch_tc<kNT, false, 128, false, true>(h, none, none, none, p, most)
                        : launch_tc<kNN, false, 128, false, true>(h, none, none, none, p, most);
     }
-    int bn = 256;
-    if (!pair) {
+    int bn = 256, parts = 1;
+    if (pair) {  // a pair's k block takes 0.4 us; two CTAs a tile leave none idle where there are few
+        if (tiles128 < h->sm_count / 2) parts = k_parts(h, tiles128, kb, 0.375, 0.4 * static_cast<double>(kb));
+        if (parts > 1) pair = false, bn = 128;
+    } else {
         // The width whose turns of CTAs take least.  A k block of 64 costs a
         // CTA about 340 ns at 64 columns, 375 at 128 and 680 at 256 (its MMAs
         // take as long at any width, its share of HBM does not).
@@ -917,6 +1033,8 @@ int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, si
         const double t256 = 2.0 * turns(256), t128 = 1.1 * turns(128), t64 = 1.0 * turns(64);
         if (t128 < t256 || N <= 128) bn = 128;
         if (t64 < (bn == 128 ? t128 : t256) || N <= 64) bn = 64;
+        parts = k_parts(h, tiles128, kb, 0.375, 0.34 * static_cast<double>(kb) * (bn == 64 ? t64 : bn == 128 ? t128 : t256));
+        if (parts > 1) bn = 128;
     }
     const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap tmA, tmA16, tmB;
@@ -930,6 +1048,9 @@ int launch_hgemm_grouped(b2b_handle *h, int type, int trans_b, size_t groups, si
     p.idesc = sm100::idesc_f32acc(bf16, 0, trans_b ? 0 : 1, pair ? 256 : 128, pair ? 256 : bn);
     const int bm = pair ? 256 : 128;
     const int64_t most = (R / bm + (R < G ? R : G)) * ((N + bn - 1) / bn);
+    if (parts > 1)
+        return trans_b ? launch_tc<kNT, false, 128, false, false, true>(h, tmA, tmA16, tmB, p, tiles128, parts)
+                       : launch_tc<kNN, false, 128, false, false, true>(h, tmA, tmA16, tmB, p, tiles128, parts);
     if (trans_b) {
         if (pair) return launch_tc<kNT, true, 256>(h, tmA, tmA16, tmB, p, most);
         if (bn == 256) return launch_tc<kNT, false, 256>(h, tmA, tmA16, tmB, p, most);
@@ -952,19 +1073,27 @@ int launch_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t group
         return fail(B2B_ERR_NOT_SUPPORTED, "grouped HGEMM: 2^31 tiles or more");
     TcArgs p{A, B, C, offsets, h->d_status, h->wait_limit_ns, G, static_cast<int>(rows), static_cast<int>(m),
              static_cast<int>(n), 0, alpha, beta, 0, bf16, n % (f32 ? 4 : 8) == 0 && aligned16(C)};
-    const bool pair = M > 128 && N > 128;
+    bool pair = M > 128 && N > 128;
+    // k blocks of a group as long as the average
+    const int64_t kb = (static_cast<int64_t>(rows) + 64 * G - 1) / (64 * G), tiles128 = G * ((M + 127) / 128) * ((N + 127) / 128);
     if (rows == 0 || !tma_can(A, B, M, 1, N)) {  // without rows nothing is loaded
         const bool two = pair && !f32 && by_hand_in_pairs(h, G * ((M + 127) / 128), G * ((M + 255) / 256), N);
+        const int parts = two ? 1 : k_parts(h, tiles128, kb, 1.1, 1.1 * static_cast<double>(kb));
         const int bm = two ? 256 : 128;
         p.idesc = sm100::idesc_f32acc(bf16, 1, 1, bm, bm);
         const int64_t most = G * ((M + bm - 1) / bm) * ((N + bm - 1) / bm);
         const CUtensorMap none{};
+        if (parts > 1)
+            return f32 ? launch_tc<kTN, false, 128, true, true, true>(h, none, none, none, p, most, parts)
+                       : launch_tc<kTN, false, 128, false, true, true>(h, none, none, none, p, most, parts);
         if (f32) return launch_tc<kTN, false, 128, true, true>(h, none, none, none, p, most);
         return two ? launch_tc<kTN, true, 256, false, true>(h, none, none, none, p, most)
                     : launch_tc<kTN, false, 128, false, true>(h, none, none, none, p, most);
     }
     int bn = 256;
-    while (!pair && bn > 64 && (G * ((M + 127) / 128) * ((N + bn - 1) / bn) < h->sm_count || N <= bn / 2)) bn /= 2;
+    const int parts = tiles128 < h->sm_count / 2 ? k_parts(h, tiles128, kb, 0.375, (pair ? 0.4 : 0.34) * static_cast<double>(kb)) : 1;
+    if (parts > 1) pair = false, bn = 128;
+    while (!pair && parts == 1 && bn > 64 && (G * ((M + 127) / 128) * ((N + bn - 1) / bn) < h->sm_count || N <= bn / 2)) bn /= 2;
     const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     CUtensorMap tmA, tmB;
     if (int rc = encode_tma_2d(&tmA, dt, 2, A, rows, m, 64, 64)) return rc;
@@ -972,6 +1101,9 @@ int launch_hgemm_grouped_wgrad(b2b_handle *h, int type, int c_type, size_t group
     p.idesc = sm100::idesc_f32acc(bf16, 1, 1, pair ? 256 : 128, pair ? 256 : bn);
     const int bm = pair ? 256 : 128;
     const int64_t most = G * ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+    if (parts > 1)
+        return f32 ? launch_tc<kTN, false, 128, true, false, true>(h, tmA, tmA, tmB, p, most, parts)
+                   : launch_tc<kTN, false, 128, false, false, true>(h, tmA, tmA, tmB, p, most, parts);
     return f32 ? launch_wgrad<true>(h, pair, bn, tmA, tmB, p, most) : launch_wgrad<false>(h, pair, bn, tmA, tmB, p, most);
 }
 

@@ -143,6 +143,23 @@ def test_wgrad_odd_sizes_of_many_tiles(handle, t, f32, counts):
     check_wgrad(handle, t, f32, counts, 1001, 1003, first=1, pad=3)
 
 
+@pytest.mark.parametrize("t,alpha,beta", [("f16", 1.0, 0.0), ("bf16", -0.5, 2.0)])
+@pytest.mark.parametrize("trans", [False, True])
+@pytest.mark.parametrize("counts", [[1], [2, 0, 5], [130, 1], [0, 0]])
+@pytest.mark.parametrize("n,k", [(8, 4096), (300, 2051), (264, 1032), (1000, 1096)])
+def test_forward_few_tiles_of_long_sums(handle, t, alpha, beta, trans, counts, n, k):
+    """Few enough tiles that several SMs share the sum of each."""
+    check_forward(handle, t, counts, n, k, trans, first=1, pad=2, alpha=alpha, beta=beta)
+
+
+@pytest.mark.parametrize("t,alpha,beta", [("f16", 1.0, 0.0), ("bf16", -0.5, 2.0)])
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("counts", [[3000], [700, 0, 1501], [1, 2000], [0, 4096, 0, 7]])
+@pytest.mark.parametrize("m,n", [(8, 8), (136, 264), (65, 63), (129, 200)])
+def test_wgrad_few_tiles_of_long_sums(handle, t, alpha, beta, f32, counts, m, n):
+    check_wgrad(handle, t, f32, counts, m, n, first=1, pad=2, alpha=alpha, beta=beta)
+
+
 @pytest.mark.parametrize("t", ["f16", "bf16"])
 @pytest.mark.parametrize("trans", [False, True])
 def test_forward_random_values(handle, t, trans):
