@@ -309,14 +309,17 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
 // 35 us, by 8 47 us; what it lacks to HBM's 6.4 is instructions, 20 for each
 // word of a warp, half a cycle each on the pipes that most of them need.
 // Rows that TMA cannot describe (n not a multiple of 32, packed not 16-byte
-// aligned) and groups that do not fit a box evenly are read by the same
-// kernel with plain loads (SPG = 0).
+// aligned) come by cp.async (HAND): the aligned words that hold a box's rows, 33
+// of each, which are shifted into place on their way to registers.  Groups
+// that do not fit a box evenly (SPG = 0) read their scales when they begin.
 constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTileRows = 32;
 constexpr int kBoxCols = 256;                     // 128 bytes of a row
 constexpr int kBoxSteps = kBoxCols / 32;          // of 32 columns
 constexpr int kBoxBytes = kTileRows * kBoxCols / 2;
+constexpr int kHandPitch = 144;                   // HAND: bytes of a row's 33 words, so that 8 rows meet every bank once
+constexpr int kHandBytes = kTileRows * kHandPitch;
 constexpr int kMaxBatch = 8;                      // rounds that the CTAs of a cluster join at once
 constexpr int kMaxIndexed = 256;                  // products of one launch that choose their matrix
 
@@ -350,19 +353,9 @@ struct Table {
     uint32_t leads[kMaxIndexed / 32];  // the products that are their sets' first, a bit each
 };
 
-// The 4 bytes at packed + at, wherever that is aligned; bytes past the end
-// are 0 (they meet zeros of x).
-__device__ __forceinline__ uint32_t word_at(const GemvArgs &p, int64_t at) {
-    const uint8_t *src = p.w.packed + at;
-    const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(src) & 3);
-    if (at - shift >= 0 && at - shift + 8 <= p.total) {
-        const uint32_t *word = reinterpret_cast<const uint32_t *>(src - shift);
-        return shift ? __funnelshift_r(__ldg(word), __ldg(word + 1), 8 * shift) : __ldg(word);
-    }
-    uint32_t v = 0;
-    for (int i = 0; i < 4; ++i)
-        if (at + i < p.total) v |= static_cast<uint32_t>(src[i]) << (8 * i);
-    return v;
+// `bytes` of the aligned word at `src` to shared memory, and zeros for the rest.
+__device__ __forceinline__ void copy_word(uint32_t to, const uint8_t *src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(src), "r"(bytes) : "memory");
 }
 
 // c += a b, or c = a b where FRESH.
@@ -582,14 +575,15 @@ struct Place {
     }
 };
 
-// SPG: steps of 32 columns in a group, 8 standing for its multiples; 0: plain
-// loads, any group.
-template <bool BF16, bool ZEROS, int SPG>
+// SPG: steps of 32 columns in a group, 8 standing for its multiples; 0: any
+// group (HAND).
+template <bool BF16, bool ZEROS, int SPG, bool HAND>
 __global__ void __launch_bounds__(kThreads, 1)
     w4_gemv_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ GemvArgs p) {
     using namespace sm100;
     using H = b2b::Half16<BF16>;
-    constexpr bool TMA = SPG != 0;
+    static_assert(HAND || SPG != 0, "any group: HAND");
+    constexpr bool TMA = !HAND;
     extern __shared__ uint8_t smem_raw[];
     __shared__ int abort_flag;
     __shared__ int arrived[2][5][kWarps];         // warps of a tile (by log2 of their number) whose sums are in `part`
@@ -599,8 +593,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g = lane >> 2, q = lane & 3;
     const int KS = static_cast<int>(cluster_nctarank()), rank = static_cast<int>(cluster_ctarank());
-    uint8_t *box = smem + (TMA ? warp * kBoxBytes : 0);
-    uint8_t *sx = smem + (TMA ? kWarps * kBoxBytes : 0);
+    uint8_t *box = smem + warp * (TMA ? kBoxBytes : kHandBytes);
+    uint8_t *sx = smem + kWarps * (TMA ? kBoxBytes : kHandBytes);
     const int sums = kTileRows * p.width;                     // of a tile
     float *part = reinterpret_cast<float *>(sx + p.x_bytes);  // [2][kWarps][32 rows][width]
     float *slots = part + 2 * kWarps * sums;                  // KS > 1: [2][p.batch][p.parts][32 rows][width]
@@ -691,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     const int spg = static_cast<int>(p.w.group / 32);
-    const int nsteps = static_cast<int>(p.w.n / 32);
+    const int nsteps = static_cast<int>((p.w.n + 31) / 32);
     int nb = 0;
     uint32_t phase = 0;
 
@@ -702,7 +696,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     RowScales<SPG, ZEROS> scales;
     Place ahead = here;
     bool more = true;  // there is a next box
-    int nc = 0, nstep = 0, nbox = 0, nrow = 0;  // boxes left of its tile, and how far apart they are
+    int nc = 0, nstep = 0, nbox = 0;  // boxes left of its tile, and how far apart they are
+    int64_t nrow = 0, nleft = 0;      // the tile's first row, and how many are behind it
     const uint16_t *nscales = nullptr;
     const uint8_t *nzeros = nullptr;
     auto seek = [&] {
@@ -715,7 +710,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int64_t tile = first + (warp >> lk), row = e * p.w.m + tile * kTileRows;
             const int64_t left = p.w.m - 1 - tile * kTileRows;  // rows behind the tile's first
             const int64_t at = (row + min(left, static_cast<int64_t>(lane))) * p.w.gs;
-            nrow = static_cast<int>(row);
+            nrow = row;
+            nleft = left;
             nscales = p.w.scales + at;
             if (ZEROS) nzeros = p.w.zeros + at;
             nbox = kwarp * KS + rank;
@@ -727,20 +723,54 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto load = [&] {
         if (!more || dead) return;
-        if (lane == 0) {
-            mbar_arrive_expect_tx(full, kBoxBytes);
-            tma_load_2d(box, &tmW, full, nbox * (kBoxCols / 2), nrow);
+        if constexpr (TMA) {
+            if (lane == 0) {
+                mbar_arrive_expect_tx(full, kBoxBytes);
+                tma_load_2d(box, &tmW, full, nbox * (kBoxCols / 2), static_cast<int>(nrow));
+            }
+        } else {
+            // a lane copies word `lane` of each row, and the last one of row `lane`;
+            // words behind a row's end stay what they are (they meet zeros of x)
+            const int64_t at = nrow * p.w.pitch + static_cast<int64_t>(nbox) * (kBoxCols / 2);
+            const uint8_t *src = p.w.packed + at;
+            const uint32_t to = smem_u32(box) + lane * 4, last = smem_u32(box) + lane * kHandPitch + 128;
+            auto word = [](const uint8_t *q) { return reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(q) & ~uintptr_t(3)); };
+            const int have = static_cast<int>(min(static_cast<int64_t>(33), (p.w.n - static_cast<int64_t>(nbox) * kBoxCols + 7) / 8 + 1));
+            if (nleft >= kTileRows - 1 && at >= 4 && at + (kTileRows - 1) * p.w.pitch + 136 <= p.total) {
+                if (have == 33) copy_word(last, word(src + lane * p.w.pitch) + 128, 4);
+                if (lane < have) {
+#pragma unroll 8
+                    for (int r = 0; r < kTileRows; ++r, src += p.w.pitch) copy_word(to + r * kHandPitch, word(src) + lane * 4, 4);
+                }
+            } else {
+                // rows that do not exist repeat the last one, and bytes outside
+                // `packed` are 0
+                auto careful = [&](uint32_t dst, const uint8_t *q) {
+                    const int64_t have = p.w.packed + p.total - q;
+                    if (q >= p.w.packed) {
+                        copy_word(dst, have > 0 ? q : word(p.w.packed + 3), have > 4 ? 4 : have > 0 ? static_cast<int>(have) : 0);
+                        return;
+                    }
+                    uint32_t v = 0;  // the word that `packed` begins in
+                    for (int i = 0; i < 4; ++i)
+                        if (q + i >= p.w.packed && i < have) v |= static_cast<uint32_t>(q[i]) << (8 * i);
+                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(v) : "memory");
+                };
+                careful(last, word(src + min(static_cast<int64_t>(lane), nleft) * p.w.pitch) + 128);
+#pragma unroll 1
+                for (int r = 0; r < kTileRows; ++r)
+                    careful(to + r * kHandPitch, word(src + min(static_cast<int64_t>(r), nleft) * p.w.pitch) + lane * 4);
+            }
         }
-        const int step = nbox * kBoxSteps;
-        const int grp = SPG == kBoxSteps ? step / spg : step / (SPG ? SPG : 1);
-        scales.load(nscales + grp, nzeros + grp, static_cast<int>(p.w.gs) - grp, p.vec);
+        if constexpr (SPG != 0) {
+            const int step = nbox * kBoxSteps, grp = SPG == kBoxSteps ? step / spg : step / SPG;
+            scales.load(nscales + grp, nzeros + grp, static_cast<int>(p.w.gs) - grp, p.vec);
+        }
         nbox += nstep;
         if (--nc == 0) seek();
     };
-    if constexpr (TMA) {
-        seek();
-        load();
-    }
+    seek();
+    load();
 
     int e = -1;          // the set's matrix
     uint32_t over = 0;   // 2^16 / nb, rounded up: o * over >> 16 is o / nb for the sums of a tile
@@ -849,103 +879,94 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int rows = static_cast<int>(p.w.m - static_cast<int64_t>(tile) * kTileRows) - g;  // > 8 i: row g + 8 i exists
             // lanes of vectors that the set does not have read zeros
             const int xstep = g < nb ? nb * 64 : 0;
-            if constexpr (TMA) {
-                for (int c = 0; c < own; ++c) {
-                    const int l = kwarp + (c << lk), steps = nsteps - (l * KS + rank) * kBoxSteps;
+            // SPG = 0: the rows whose scales this lane reads, its own or the last
+            // one for those that are not there, and the group that they are of
+            int64_t row[SPG ? 1 : 4];
+            int held = -1;
+            float scale[4];
+            Unpack<BF16> un[4] = {Unpack<BF16>(8), Unpack<BF16>(8), Unpack<BF16>(8), Unpack<BF16>(8)};
+            if constexpr (SPG == 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) row[i] = row0 + min(8 * i, rows - 1);
+            }
+            uint32_t shift[HAND ? 4 : 1];  // bits that rows g + 8 i begin behind a word
+            if constexpr (HAND) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    shift[i] = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p.w.packed) + (row0 + min(8 * i, rows - 1)) * p.w.pitch & 3) * 8;
+            }
+            const bool shifts = HAND && ((reinterpret_cast<uintptr_t>(p.w.packed) | static_cast<uint64_t>(p.w.pitch)) & 3) != 0;
+            for (int c = 0; c < own; ++c) {
+                const int l = kwarp + (c << lk), step0 = (l * KS + rank) * kBoxSteps, steps = nsteps - step0;
+                if constexpr (TMA) {
                     if (!dead) {
                         const bool ok = mbar_wait(full, phase, &abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x31, p.wait_ns);
                         dead = !__all_sync(0xffffffffu, ok);
                     }
                     phase ^= 1u;
-                    // 16-byte piece st of row r sits at piece st ^ (r % 8)
-                    const uint32_t w = smem_u32(box) + g * 128 + (g << 4) + q * 4;
-                    const uint32_t xs = g < nb ? smem_u32(sx) + l * kBoxSteps * nb * 64 + lane * 16 : smem_u32(nothing);
-                    // EARLY: the words go to registers at once, so that the box is in
-                    // flight again while they are multiplied.  Groups of 32 columns,
-                    // and of 64 with zero points, need the registers for their scales
-                    // and leave the words where they are (4096 x 4096 by 8 vectors,
-                    // groups of 32: 8.7 us, early 9.4; 18944 x 16384 by 8, groups of
-                    // 64: 67 and 69 us, without zero points 52 and 50).
-                    constexpr bool EARLY = SPG >= 4 || (SPG == 2 && !ZEROS);
-                    uint32_t words[EARLY ? kBoxSteps : 1][4];
-                    const RowScales<SPG, ZEROS> mine = scales;
-                    auto refill = [&] {
-                        // every lane's reads come before the box's next contents
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        load();
-                    };
-                    if constexpr (EARLY) {
+                } else {
+                    asm volatile("cp.async.wait_all;" ::: "memory");
+                    __syncwarp();
+                }
+                // 16-byte piece st of row r sits at piece st ^ (r % 8)
+                const uint32_t w = smem_u32(box) + (TMA ? g * 128 + (g << 4) : g * kHandPitch) + q * 4;
+                const uint32_t xs = g < nb ? smem_u32(sx) + l * kBoxSteps * nb * 64 + lane * 16 : smem_u32(nothing);
+                // EARLY: the words go to registers at once, so that the box is in
+                // flight again while they are multiplied.  Groups of 32 columns,
+                // and of 64 with zero points, need the registers for their scales
+                // and leave the words where they are (4096 x 4096 by 8 vectors,
+                // groups of 32: 8.7 us, early 9.4; 18944 x 16384 by 8, groups of
+                // 64: 67 and 69 us, without zero points 52 and 50).
+                constexpr bool EARLY = HAND || SPG >= 4 || (SPG == 2 && !ZEROS);
+                uint32_t words[EARLY ? kBoxSteps : 1][4];
+                const RowScales<SPG, ZEROS> mine = scales;
+                auto refill = [&] {
+                    // every lane's reads come before the box's next contents
+                    if constexpr (TMA) fence_proxy_async_smem();
+                    __syncwarp();
+                    load();
+                };
+                if constexpr (EARLY) {
 #pragma unroll
-                        for (int st = 0; st < kBoxSteps; ++st)
+                    for (int st = 0; st < kBoxSteps; ++st)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) words[st][i] = lds32((w ^ (st << 4)) + i * 1024);
-                        refill();
+                        for (int i = 0; i < 4; ++i)
+                            words[st][i] = lds32(TMA ? (w ^ (st << 4)) + i * 1024 : w + st * 16 + i * 8 * kHandPitch);
+                    if constexpr (HAND) {
+                        if (shifts) {
+#pragma unroll
+                            for (int st = 0; st < kBoxSteps; ++st)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    words[st][i] = __funnelshift_r(words[st][i], lds32(w + st * 16 + i * 8 * kHandPitch + 4), shift[i]);
+                        }
                     }
+                    refill();
+                }
+                if constexpr (SPG != 0) {
                     if (steps >= kBoxSteps)
                         box_products<BF16, ZEROS, SPG, EARLY, true>(total, words, w, xs, xstep, mine, g, steps);
                     else
                         box_products<BF16, ZEROS, SPG, EARLY, false>(total, words, w, xs, xstep, mine, g, steps);
-                    if constexpr (!EARLY) refill();
-                }
-            } else {
-                // this lane's rows, or the last one for those that are not there
-                int64_t row[4];
+                } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) row[i] = row0 + min(8 * i, rows - 1);
-                int held = -1;  // the group whose scales and zero points are held
-                float scale[4];
-                Unpack<BF16> un[4] = {Unpack<BF16>(8), Unpack<BF16>(8), Unpack<BF16>(8), Unpack<BF16>(8)};
-                for (int c = 0; c < own; ++c) {
-                    const int l = kwarp + (c << lk), step0 = (l * KS + rank) * kBoxSteps;
-                    const int steps = min(kBoxSteps, static_cast<int>((p.w.n + 31) / 32) - step0);
-                    const uint8_t *xs = g < nb ? sx + l * kBoxSteps * nb * 64 + lane * 16 : nothing;
-                    const int64_t byte0 = static_cast<int64_t>(step0) * 16 + q * 4;
-                    // all loads before their use
-                    uint32_t words[8][4];
-                    // words and the ones behind them that lie in `packed` whatever the alignment
-                    const bool inside = (row0 - g + kTileRows) * p.w.pitch + byte0 + 8 * 16 + 8 <= p.total &&
-                                        byte0 + row0 * p.w.pitch >= 4;
-                    if (__all_sync(0xffffffffu, inside)) {
+                    for (int st = 0; st < kBoxSteps; ++st) {
+                        if (st >= steps) break;
+                        const int grp = (step0 + st) / spg;
+                        if (grp != held) {
+                            held = grp;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint8_t *from = p.w.packed + row[i] * p.w.pitch + byte0;
-                            const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(from) & 3);
-                            const uint32_t *at = reinterpret_cast<const uint32_t *>(from - shift);
-#pragma unroll
-                            for (int st = 0; st < 8; ++st) words[st][i] = __ldg(at + st * 4);
-                            if (__any_sync(0xffffffffu, shift != 0)) {
-#pragma unroll
-                                for (int st = 0; st < 8; ++st)
-                                    words[st][i] = __funnelshift_r(words[st][i], __ldg(at + st * 4 + 1), 8 * shift);
+                            for (int i = 0; i < 4; ++i) {
+                                scale[i] = H::get(__ldg(p.w.scales + row[i] * p.w.gs + grp));
+                                if (ZEROS) un[i] = Unpack<BF16>(__ldg(p.w.zeros + row[i] * p.w.gs + grp) & 15u);
                             }
                         }
-                    } else {
-#pragma unroll
-                        for (int st = 0; st < 8; ++st)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) words[st][i] = word_at(p, row[i] * p.w.pitch + byte0 + st * 16);
-                    }
-#pragma unroll
-                    for (int st = 0; st < 8; ++st) {
-                        if (st < steps) {
-                            const int grp = (step0 + st) / spg;
-                            if (grp != held) {
-                                held = grp;
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    scale[i] = H::get(__ldg(p.w.scales + row[i] * p.w.gs + grp));
-                                    if (ZEROS) un[i] = Unpack<BF16>(__ldg(p.w.zeros + row[i] * p.w.gs + grp) & 15u);
-                                }
-                            }
-                            const uint4 x = *reinterpret_cast<const uint4 *>(xs);
-                            xs += xstep;
-                            float sum[2][4];
-                            step32<BF16, true>(sum, words[st], un, x);
-                            add_scaled(total, sum, scale);
-                        }
+                        float sum[2][4];
+                        step32<BF16, true>(sum, words[st], un, lds128(xs + st * xstep));
+                        add_scaled(total, sum, scale);
                     }
                 }
+                if constexpr (!EARLY) refill();
             }
         }
 
@@ -1141,7 +1162,7 @@ constexpr int64_t kMaxXBytes = 80 * 1024;    // of its staged vectors where 8 CT
 size_t gemv_smem(GemvArgs &p, bool tma, int KS, int64_t local) {
     p.x_bytes = static_cast<int>(local * kBoxCols * p.width * 2);
     return p.x_bytes + 2 * (kWarps + (KS > 1 ? p.batch * p.parts : 0)) * kTileRows * p.width * 4 +
-           kWarps * ((tma ? kBoxBytes : 0) + 8) + 16 + (p.index ? sizeof(Table) : 0) + 1024;
+           kWarps * ((tma ? kBoxBytes : kHandBytes) + 8) + 16 + (p.index ? sizeof(Table) : 0) + 1024;
 }
 
 // Clusters of KS CTAs (1, 2, 4 or 8) of the GEMV kernel that are resident at
@@ -1186,21 +1207,25 @@ QuantizeKernel quantize_kernel(size_t group) {
 
 using GemvKernel = void (*)(CUtensorMap, GemvArgs);
 
-template <bool BF16, bool ZEROS>
+template <bool BF16, bool ZEROS, bool HAND>
 GemvKernel gemv_kernel(int spg) {
     switch (spg) {
-        case 1: return w4_gemv_kernel<BF16, ZEROS, 1>;
-        case 2: return w4_gemv_kernel<BF16, ZEROS, 2>;
-        case 4: return w4_gemv_kernel<BF16, ZEROS, 4>;
-        case 8: return w4_gemv_kernel<BF16, ZEROS, 8>;
-        default: return w4_gemv_kernel<BF16, ZEROS, 0>;
+        case 1: return w4_gemv_kernel<BF16, ZEROS, 1, HAND>;
+        case 2: return w4_gemv_kernel<BF16, ZEROS, 2, HAND>;
+        case 4: return w4_gemv_kernel<BF16, ZEROS, 4, HAND>;
+        case 8: return w4_gemv_kernel<BF16, ZEROS, 8, HAND>;
+        default: return w4_gemv_kernel<BF16, ZEROS, 0, true>;
     }
 }
 
-int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvArgs &p) {
+int launch_gemv(b2b_handle *h, bool bf16, int spg, bool tma, const CUtensorMap &tmW, GemvArgs &p) {
     const bool zeros = p.w.zeros != nullptr;
-    const GemvKernel kernel = bf16 ? (zeros ? gemv_kernel<true, true>(spg) : gemv_kernel<true, false>(spg))
-                                   : (zeros ? gemv_kernel<false, true>(spg) : gemv_kernel<false, false>(spg));
+    auto pick = [&](auto hand) {
+        constexpr bool HAND = decltype(hand)::value;
+        return bf16 ? (zeros ? gemv_kernel<true, true, HAND>(spg) : gemv_kernel<true, false, HAND>(spg))
+                    : (zeros ? gemv_kernel<false, true, HAND>(spg) : gemv_kernel<false, false, HAND>(spg));
+    };
+    const GemvKernel kernel = tma ? pick(std::false_type{}) : pick(std::true_type{});
     const void *fn = reinterpret_cast<const void *>(kernel);
     const int64_t cols = (p.w.n + kBoxCols - 1) / kBoxCols, tiles = (p.w.m + kTileRows - 1) / kTileRows;
     p.width = p.count < 8 ? p.count : 8;
@@ -1225,9 +1250,9 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
     cfg.attrs = attr;
     {
         static std::mutex mu;
-        static bool ready[2][2][9][64];
+        static bool ready[2][2][2][9][64];
         std::lock_guard<std::mutex> lock(mu);
-        bool &done = ready[bf16][zeros][spg][h->device & 63];
+        bool &done = ready[tma][bf16][zeros][spg][h->device & 63];
         if (!done) {
             const cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem);
             if (e != cudaSuccess) return b2b::fail_cuda(e, "4-bit GEMV shared memory");
@@ -1245,7 +1270,7 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
     double best_time = 0;
     for (int KS = 1; KS <= 8 && (KS == 1 || KS < 2 * cols); KS *= 2) {
         const int64_t local = (cols + KS - 1) / KS, clusters = resident_clusters(h, fn, KS);
-        auto fits = [&] { return gemv_smem(p, spg != 0, KS, local) <= static_cast<size_t>(kMaxSmem); };
+        auto fits = [&] { return gemv_smem(p, tma, KS, local) <= static_cast<size_t>(kMaxSmem); };
         p.parts = kWarps;
         p.batch = KS > 1 ? kMaxBatch : 1;
         while (p.batch > 1 && !fits()) p.batch /= 2;
@@ -1270,7 +1295,7 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, const CUtensorMap &tmW, GemvA
     // an index may name more matrices than expected, but not more tiles than this
     const int64_t most = (p.index ? p.count : (p.count + p.width - 1) / p.width) * tiles;
     attr[0].val.clusterDim.x = best_ks;
-    cfg.dynamicSmemBytes = gemv_smem(p, spg != 0, best_ks, local);
+    cfg.dynamicSmemBytes = gemv_smem(p, tma, best_ks, local);
     cfg.numAttrs = best_ks > 1;
     cfg.gridDim = dim3(static_cast<unsigned>(best_ks * (most < clusters ? most : clusters)));
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, tmW, p);
@@ -1330,16 +1355,18 @@ int launch_hgemv_w4(b2b_handle *h, int type, size_t groups, size_t m, size_t n, 
     const int64_t rows = static_cast<int64_t>(groups) * p.w.m;
     p.total = rows * p.w.pitch;
     const bool bf16 = type == B2B_TYPE_BF16;
-    // steps of a group that the TMA-fed kernel is made for
+    // steps of a group that divide a box's
     int spg = static_cast<int>(group / 32);
     if (spg % kBoxSteps == 0) spg = kBoxSteps;
-    const bool tma = n % 32 == 0 && aligned16(packed) && rows < (1ll << 31) && kBoxSteps % spg == 0;
-    if (!tma) spg = 0;
+    if (kBoxSteps % spg != 0) spg = 0;
+    const bool tma = n % 32 == 0 && aligned16(packed) && rows < (1ll << 31) && spg != 0;
     CUtensorMap tmW{};
     if (tma) {
         if (int rc = encode_tma_2d(&tmW, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, packed, rows, p.w.pitch, kBoxCols / 2,
                                    kTileRows))
             return rc;
+    }
+    if (spg != 0) {
         const int64_t per = kBoxSteps / spg;  // groups of a box
         p.vec = p.w.gs % per == 0 && aligned16(scales) && aligned16(zeros);
     }
@@ -1347,7 +1374,7 @@ int launch_hgemv_w4(b2b_handle *h, int type, size_t groups, size_t m, size_t n, 
     for (int64_t first = 0; first < all; first += index ? kMaxIndexed : all) {
         p.first = static_cast<int>(first);
         p.count = static_cast<int>(index && all - first > kMaxIndexed ? kMaxIndexed : all - first);
-        if (int rc = launch_gemv(h, bf16, spg, tmW, p)) return rc;
+        if (int rc = launch_gemv(h, bf16, spg, tma, tmW, p)) return rc;
     }
     return B2B_OK;
 }
