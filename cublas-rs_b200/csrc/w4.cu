@@ -290,7 +290,8 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
 //     warps take in turn.  A cluster has an equal share of all tiles, next to
 //     each other, and takes them in rounds: of 16 tiles, a warp to each, while
 //     it has as many, then of 8, 4, 2 and 1 with 2, 4, 8 and 16 warps to a
-//     tile, so that no warp idles while another has two.
+//     tile, so that no warp idles while another has two; what is left in one
+//     round as soon as there are warps for all its boxes.
 //   * Each warp holds one box (32 rows x 128 bytes, 128-byte swizzle), copies
 //     it to registers, and TMA refills it, across rounds, so nothing drains at
 //     a round's end: 64 KiB of an SM in flight.  Two boxes to a warp took 38 us
@@ -556,15 +557,25 @@ __device__ __forceinline__ bool wait_finished(const volatile int *count, int wan
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
+// A round: `count` tiles with 2^lk warps to each; the warps left over idle.
+struct Round {
+    int count, lk;
+};
 // A place in a cluster's sequence of rounds.
 struct Place {
     uint32_t set, tile, left;  // next tile, and how many are left
-    // Takes the next round: 2^result tiles from `tile` on.
-    __device__ __forceinline__ int take(uint32_t tiles, uint32_t most) {
-        const int lp = 31 - __clz(static_cast<int>(min(min(left, tiles - tile), most)));
-        left -= 1u << lp;
-        tile += 1u << lp;
-        return lp;
+    // Takes the next round, from `tile` on: all tiles that are left if there
+    // are warps for their boxes (2^lbox of them), else 2^i tiles.
+    __device__ __forceinline__ Round take(uint32_t tiles, uint32_t most, int lbox) {
+        const uint32_t have = min(left, tiles - tile);
+        Round r{static_cast<int>(have), lbox};
+        if (have > min(most, 16u >> lbox)) {
+            const int lp = 31 - __clz(static_cast<int>(min(have, most)));
+            r = Round{1 << lp, min(4 - lp, lbox)};
+        }
+        left -= r.count;
+        tile += r.count;
+        return r;
     }
     // ... after which a set may be done.
     __device__ __forceinline__ void settle(uint32_t tiles) {
@@ -659,6 +670,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t sets = p.index ? sets_named : (p.count + p.width - 1) / p.width;
     const int boxes = static_cast<int>((p.w.n + kBoxCols - 1) / kBoxCols);
     const int local = boxes > rank ? (boxes - rank + KS - 1) / KS : 0;  // this CTA's boxes of a tile
+    const int lbox = min(4, 32 - __clz((boxes + KS - 1) / KS - 1));  // log2 of the warps that a tile can use
     const uint32_t clusters = gridDim.x / KS, cluster = blockIdx.x / KS;
     // next to each other, so that a cluster changes its vectors rarely
     const uint64_t all = static_cast<uint64_t>(sets) * tiles;
@@ -704,9 +716,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         while (ahead.left) {
             const int e = matrix_of(ahead.set);
             const uint32_t first = ahead.tile;
-            const int lk = 4 - ahead.take(tiles, p.parts), kwarp = warp & ((1 << lk) - 1);
+            const Round round = ahead.take(tiles, p.parts, lbox);
+            const int lk = round.lk, kwarp = warp & ((1 << lk) - 1);
             ahead.settle(tiles);
-            if (e < 0 || kwarp >= local) continue;
+            if (e < 0 || kwarp >= local || warp >> lk >= round.count) continue;
             const int64_t tile = first + (warp >> lk), row = e * p.w.m + tile * kTileRows;
             const int64_t left = p.w.m - 1 - tile * kTileRows;  // rows behind the tile's first
             const int64_t at = (row + min(left, static_cast<int64_t>(lane))) * p.w.gs;
@@ -789,13 +802,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         int share = 0;  // 512 sums each
         for (int i = 0; i < rounds; ++i) {
             const uint32_t set = at.set, first = at.tile;
-            const int lp = at.take(tiles, p.parts);
+            const int count = at.take(tiles, p.parts, lbox).count;
             at.settle(tiles);
             const int nb = vectors_of(set), e = matrix_of(set);
-            for (int k = tid; k - tid < 256 << lp; k += kThreads) {
+            for (int k = tid; k - tid < 256 * count; k += kThreads) {
                 if ((share++ & (KS - 1)) != rank) continue;
                 const int t = k >> 8, o = k & 255;
-                if (t >> lp || o >= kTileRows * nb) continue;
+                if (t >= count || o >= kTileRows * nb) continue;
                 const uint32_t from = smem_u32(joins + (i * p.parts + t) * sums + o);
                 float of[8];
 #pragma unroll
@@ -814,11 +827,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (; here.left; ++v) {
         const uint32_t set = here.set, first = here.tile;
         if (KS > 1 && (v & (p.batch - 1)) == 0 && lane == 0) begin[v & p.batch ? 1 : 0][warp] = here;
-        const int lp = here.take(tiles, p.parts), lk = 4 - lp, kw = 1 << lk;
+        const Round round = here.take(tiles, p.parts, lbox);
+        const int lk = round.lk, kw = 1 << lk;
         here.settle(tiles);
         single = single && here.left == 0;
         const int part_no = warp >> lk, kwarp = warp & (kw - 1);
-        const int own = local > kwarp ? (local - kwarp + kw - 1) >> lk : 0;
+        const bool idle = part_no >= round.count;
+        const int own = local > kwarp && !idle ? (local - kwarp + kw - 1) >> lk : 0;
         const uint32_t tile = first + part_no;
         if (set != staged) {
             staged = set;
@@ -874,7 +889,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncthreads();
         }
         float total[2][4] = {};
-        if (e >= 0) {
+        if (e >= 0 && !idle) {
             const int64_t row0 = e * p.w.m + static_cast<int64_t>(tile) * kTileRows + g;
             const int rows = static_cast<int>(p.w.m - static_cast<int64_t>(tile) * kTileRows) - g;  // > 8 i: row g + 8 i exists
             // lanes of vectors that the set does not have read zeros
@@ -973,12 +988,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ---- join.  A warp that has its tile to itself puts it out.  Else the
         // last of a tile's warps to get here adds their sums up; none waits,
         // but to reuse a buffer that is not joined yet.  A CTA of one round has
-        // nothing to go on with: all its threads add up.
+        // nothing to go on with: all its threads add up and put out.
         const int flip = v & 1, turn = v & (p.batch - 1);
         if (KS > 1 && turn == 0 && v > 0) join_cluster(v - 1);
-        if (kw == 1) {
+        // A warp that had nothing to hand over may be here before its sums of two
+        // rounds ago are joined: the larger number stays.  It writes sums again
+        // in another set, after the barriers of its vectors.
+        auto joined = [&](int w) { atomicMax(const_cast<int *>(&finished[flip][w]), (v >> 1) + 1); };
+        if (idle && !single) {
+            if (lane == 0) joined(warp);
+        } else if (kw == 1 && !(single && round.count <= 4)) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < 8 && !idle; ++i) {
                 const int r = g + 8 * (i >> 1), b = 2 * q + (i & 1);
                 if (b >= nb) continue;
                 if (KS == 1)
@@ -986,14 +1007,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 else
                     slots_of(v)[(turn * p.parts + part_no) * sums + r * nb + b] = total[i >> 2][i & 3];
             }
-            if (lane == 0) finished[flip][warp] = (v >> 1) + 1;
+            if (lane == 0) joined(warp);
         } else {
-            if (v >= 2 && !wait_finished(&finished[flip][warp], v >> 1, &abort_flag, p, lane)) dead = true;
+            if (v >= 2 && !idle && !wait_finished(&finished[flip][warp], v >> 1, &abort_flag, p, lane)) dead = true;
             float *mine = part + (flip * kWarps + warp) * sums;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int col = 2 * q + (i & 1);
-                if (col < nb) mine[(g + 8 * (i >> 1)) * nb + col] = total[i >> 2][i & 3];
+                if (col < nb && !idle) mine[(g + 8 * (i >> 1)) * nb + col] = total[i >> 2][i & 3];
             }
             auto add_up = [&](int t, int o) {  // sum o of the round's tile t
                 const float *from = part + (flip * kWarps + (t << lk)) * sums + o;
@@ -1008,7 +1029,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             if (single) {
                 __syncthreads();
-                for (int i = tid; i < 256 << lp; i += kThreads)
+                for (int i = tid; i < 256 * round.count; i += kThreads)
                     if ((i & 255) < kTileRows * nb) add_up(i >> 8, i & 255);
             } else {
                 __threadfence_block();
@@ -1021,7 +1042,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     for (int o = lane; o < kTileRows * nb; o += 32) add_up(part_no, o);
                     __threadfence_block();
                     __syncwarp();
-                    if (lane < kw) finished[flip][(part_no << lk) + lane] = (v >> 1) + 1;
+                    if (lane < kw) joined((part_no << lk) + lane);
                 }
             }
         }
@@ -1283,6 +1304,10 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, bool tma, const CUtensorMap &
             const int64_t kw = kWarps / parts;
             time += static_cast<double>(left / parts * ((local + kw - 1) / kw));
             left %= parts;
+            if (left * local <= kWarps && left <= p.parts) {  // one round of what is left
+                time += left > 0;
+                break;
+            }
         }
         if (!best_ks || time < best_time) {
             best = p;

@@ -376,7 +376,12 @@ def test_graph_and_other_stream():
     (1, 4096, 4104, 64, 3, "f16", True), (2, 20000, 20480, 256, 3, "bf16", False),
     # vectors that several SMs share: many joins, and rounds of every size
     (1, 18944, 16384, 128, 8, "f16", True), (1, 30000, 40960, 64, 8, "bf16", False), (1, 40, 200000, 128, 2, "f16", False),
-    (8, 2048, 16384, 128, 32, "f16", True), (3, 6000, 8200, 64, 21, "bf16", True), (1, 64, 8192, 128, 1, "bf16", False)])
+    (8, 2048, 16384, 128, 32, "f16", True), (3, 6000, 8200, 64, 21, "bf16", True), (1, 64, 8192, 128, 1, "bf16", False),
+    # rounds whose warps are not all needed, in many sets
+    (2, 2500, 256, 64, 36, "f16", True), (3, 20000, 768, 32, 70, "bf16", False), (5, 9000, 1000, 128, 60, "f16", True),
+    (1, 12000, 1500, 96, 33, "bf16", True), (40, 700, 300, 128, 300, "f16", False),
+    # rows that begin at any byte
+    (1, 5000, 16388, 128, 1, "f16", False), (1, 3000, 4099, 64, 9, "bf16", True), (4, 2001, 2046, 32, 17, "f16", True)])
 def test_gemv_gives_the_same_exact_bits_each_time(handle, e, m, n, group, count, t, with_zeros):
     """Many rounds of every warp's buffers, 20 times over, against exact sums
     of whole numbers."""
