@@ -389,7 +389,8 @@ def test_offsets_past_32_bits(handle):
     torch.cuda.empty_cache()
 
 
-def test_two_graphs_of_one_handle_replay_at_once():
+@pytest.mark.parametrize("rows,k", [(900, 256), (130, 4096), (6000, 64)])
+def test_two_graphs_of_one_handle_replay_at_once(rows, k):
     """Captured calls keep no state in the handle: two graphs captured through
     it replay on two streams at once and give the eager bits."""
     import torch
@@ -404,7 +405,6 @@ def test_two_graphs_of_one_handle_replay_at_once():
         view = lambda t, d=np.uint16: b2blas.DeviceBuffer.from_ptr(h, t.data_ptr(), t.numel(), d, t)  # noqa: E731
         jobs = []
         for n in (520, 515):
-            rows, k = 900, 256
             a = torch.randn(rows, k, generator=gen, device="cuda").half()
             b = torch.randn(3, k, n, generator=gen, device="cuda").half()
             c, w = torch.zeros(rows, n, device="cuda").half(), torch.zeros(3, k, n, device="cuda")
