@@ -497,13 +497,20 @@ struct RowScales {
     __device__ __forceinline__ uint32_t zero(int i) const { return ZEROS ? z[i / 4] >> (8 * (i & 3)) & 15u : 8u; }
 };
 
+// Where row g + 8 i's word of step st is, from that of g's first step: 16-byte
+// piece st of row r sits at piece st ^ (r % 8), or in order (HAND).
+template <bool HAND>
+__device__ __forceinline__ uint32_t word_of(uint32_t w, int st, int i) {
+    return HAND ? w + st * 16 + i * 8 * kHandPitch : (w ^ (st << 4)) + i * 1024;
+}
+
 // A box's products: this lane's words of its steps, in registers (EARLY) or at
 // shared address w, the vectors' pieces of its first step at shared address x.
 // FULL: it has all its steps.
-template <bool BF16, bool ZEROS, int SPG, bool EARLY, bool FULL>
+template <bool BF16, bool ZEROS, int SPG, bool EARLY, bool HAND, bool FULL>
 __device__ __forceinline__ void box_products(float (&total)[2][4], const uint32_t (&words)[EARLY ? kBoxSteps : 1][4],
-                                             uint32_t w, uint32_t x, int xstep,
-                                             const RowScales<SPG, ZEROS> &row, int g, int steps) {
+                                             uint32_t w, const uint32_t (&shift)[HAND ? 4 : 1], bool shifts, uint32_t x,
+                                             int xstep, const RowScales<SPG, ZEROS> &row, int g, int steps) {
     using H = b2b::Half16<BF16>;
     uint32_t sw[4], zw[4];  // of rows g, g + 8, g + 16, g + 24: two groups' scales, four groups' zero points
 #pragma unroll
@@ -528,7 +535,13 @@ __device__ __forceinline__ void box_products(float (&total)[2][4], const uint32_
             x += xstep;
             uint32_t own[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) own[i] = EARLY ? words[EARLY ? st : 0][i] : lds32((w ^ (st << 4)) + i * 1024);
+            for (int i = 0; i < 4; ++i) own[i] = EARLY ? words[EARLY ? st : 0][i] : lds32(word_of<HAND>(w, st, i));
+            if constexpr (HAND && !EARLY) {
+                if (shifts) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) own[i] = __funnelshift_r(own[i], lds32(word_of<HAND>(w, st, i) + 4), shift[i]);
+                }
+            }
             if (si == 0)
                 step32<BF16, true>(sum, own, un, xv);
             else
@@ -923,7 +936,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                     asm volatile("cp.async.wait_all;" ::: "memory");
                     __syncwarp();
                 }
-                // 16-byte piece st of row r sits at piece st ^ (r % 8)
                 const uint32_t w = smem_u32(box) + (TMA ? g * 128 + (g << 4) : g * kHandPitch) + q * 4;
                 const uint32_t xs = g < nb ? smem_u32(sx) + l * kBoxSteps * nb * 64 + lane * 16 : smem_u32(nothing);
                 // EARLY: the words go to registers at once, so that the box is in
@@ -932,7 +944,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // and leave the words where they are (4096 x 4096 by 8 vectors,
                 // groups of 32: 8.7 us, early 9.4; 18944 x 16384 by 8, groups of
                 // 64: 67 and 69 us, without zero points 52 and 50).
-                constexpr bool EARLY = HAND || SPG >= 4 || (SPG == 2 && !ZEROS);
+                constexpr bool EARLY = SPG == 0 || SPG >= 4 || (SPG == 2 && !ZEROS);
                 uint32_t words[EARLY ? kBoxSteps : 1][4];
                 const RowScales<SPG, ZEROS> mine = scales;
                 auto refill = [&] {
@@ -945,24 +957,24 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                     for (int st = 0; st < kBoxSteps; ++st)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            words[st][i] = lds32(TMA ? (w ^ (st << 4)) + i * 1024 : w + st * 16 + i * 8 * kHandPitch);
+                        for (int i = 0; i < 4; ++i) words[st][i] = lds32(word_of<HAND>(w, st, i));
                     if constexpr (HAND) {
                         if (shifts) {
 #pragma unroll
                             for (int st = 0; st < kBoxSteps; ++st)
 #pragma unroll
                                 for (int i = 0; i < 4; ++i)
-                                    words[st][i] = __funnelshift_r(words[st][i], lds32(w + st * 16 + i * 8 * kHandPitch + 4), shift[i]);
+                                    words[st][i] = __funnelshift_r(words[st][i], lds32(word_of<HAND>(w, st, i) + 4), shift[i]);
                         }
                     }
                     refill();
                 }
                 if constexpr (SPG != 0) {
                     if (steps >= kBoxSteps)
-                        box_products<BF16, ZEROS, SPG, EARLY, true>(total, words, w, xs, xstep, mine, g, steps);
+                        box_products<BF16, ZEROS, SPG, EARLY, HAND, true>(total, words, w, shift, shifts, xs, xstep, mine, g, steps);
                     else
-                        box_products<BF16, ZEROS, SPG, EARLY, false>(total, words, w, xs, xstep, mine, g, steps);
+                        box_products<BF16, ZEROS, SPG, EARLY, HAND, false>(total, words, w, shift, shifts, xs, xstep, mine, g,
+                                                                            steps);
                 } else {
 #pragma unroll
                     for (int st = 0; st < kBoxSteps; ++st) {
