@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
 // word of a warp, half a cycle each on the pipes that most of them need.
 // Rows that TMA cannot describe (n not a multiple of 32, packed not 16-byte
 // aligned) come by cp.async (HAND): the aligned words that hold a box's rows, 33
-// of each, which are shifted into place on their way to registers.  Groups
+// of each, which are shifted into place on their way to registers: 16384 x
+// 16388 takes 61 us, 16384 x 16376, whose rows begin at words, 53.  Groups
 // that do not fit a box evenly (SPG = 0) read their scales when they begin.
 constexpr int kWarps = 16;
 constexpr int kThreads = kWarps * 32;
@@ -762,15 +763,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t to = smem_u32(box) + lane * 4, last = smem_u32(box) + lane * kHandPitch + 128;
             auto word = [](const uint8_t *q) { return reinterpret_cast<const uint8_t *>(reinterpret_cast<uintptr_t>(q) & ~uintptr_t(3)); };
             const int have = static_cast<int>(min(static_cast<int64_t>(33), (p.w.n - static_cast<int64_t>(nbox) * kBoxCols + 7) / 8 + 1));
-            if (nleft >= kTileRows - 1 && at >= 4 && at + (kTileRows - 1) * p.w.pitch + 136 <= p.total) {
-                if (have == 33) copy_word(last, word(src + lane * p.w.pitch) + 128, 4);
-                if (lane < have) {
+            // rows that do not exist repeat the last one
+            const int behind = static_cast<int>(min(nleft, static_cast<int64_t>(kTileRows - 1)));
+            if ((at >= 4 || (reinterpret_cast<uintptr_t>(p.w.packed) & 3) == 0) && at + behind * p.w.pitch + 136 <= p.total) {
+                if (have == 33) copy_word(last, word(src + min(lane, behind) * p.w.pitch) + 128, 4);
+                if (lane < have && behind == kTileRows - 1) {
 #pragma unroll 8
                     for (int r = 0; r < kTileRows; ++r, src += p.w.pitch) copy_word(to + r * kHandPitch, word(src) + lane * 4, 4);
+                } else if (lane < have) {
+#pragma unroll 4
+                    for (int r = 0; r < kTileRows; ++r) {
+                        copy_word(to + r * kHandPitch, word(src) + lane * 4, 4);
+                        if (r < behind) src += p.w.pitch;
+                    }
                 }
             } else {
-                // rows that do not exist repeat the last one, and bytes outside
-                // `packed` are 0
+                // bytes outside `packed` are 0
                 auto careful = [&](uint32_t dst, const uint8_t *q) {
                     const int64_t have = p.w.packed + p.total - q;
                     if (q >= p.w.packed) {
@@ -782,10 +790,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (q + i >= p.w.packed && i < have) v |= static_cast<uint32_t>(q[i]) << (8 * i);
                     asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(v) : "memory");
                 };
-                careful(last, word(src + min(static_cast<int64_t>(lane), nleft) * p.w.pitch) + 128);
+                careful(last, word(src + min(lane, behind) * p.w.pitch) + 128);
 #pragma unroll 1
                 for (int r = 0; r < kTileRows; ++r)
-                    careful(to + r * kHandPitch, word(src + min(static_cast<int64_t>(r), nleft) * p.w.pitch) + lane * 4);
+                    careful(to + r * kHandPitch, word(src + min(r, behind) * p.w.pitch) + lane * 4);
             }
         }
         if constexpr (SPG != 0) {
@@ -943,8 +951,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 // and of 64 with zero points, need the registers for their scales
                 // and leave the words where they are (4096 x 4096 by 8 vectors,
                 // groups of 32: 8.7 us, early 9.4; 18944 x 16384 by 8, groups of
-                // 64: 67 and 69 us, without zero points 52 and 50).
-                constexpr bool EARLY = SPG == 0 || SPG >= 4 || (SPG == 2 && !ZEROS);
+                // 64: 67 and 69 us, without zero points 52 and 50), and so do rows
+                // that are copied by words (16384 x 16388: early is 5 % slower).
+                constexpr bool EARLY = SPG == 0 || (TMA && (SPG >= 4 || (SPG == 2 && !ZEROS)));
                 uint32_t words[EARLY ? kBoxSteps : 1][4];
                 const RowScales<SPG, ZEROS> mine = scales;
                 auto refill = [&] {
