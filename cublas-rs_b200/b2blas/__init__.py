@@ -607,10 +607,11 @@ class Handle:
         4-bit matrices (b2b_hgemv_w4_grouped); index is an int32 DeviceBuffer,
         and one outside [0, groups) names no expert."""
         z = zeros.ptr if zeros is not None else 0
+        if fan < 1:  # the C ABI takes a size_t: a negative one would be huge there
+            raise CublasError(3, f"fan must be at least 1, got {fan}")
         if m and n and count and groups:
             z = self._need_w4(groups, m, n, group, packed, scales, zeros)
-            if fan > 0:  # the library refuses a fan of 0
-                self._need(x, -(-count // fan) * n, "x", _U16)
+            self._need(x, -(-count // fan) * n, "x", _U16)
             self._need(index, count, "index", _I32)
             self._need(y, count * m, "y", _U16)
         _check(self._lib.b2b_hgemv_w4_grouped(

@@ -1,0 +1,27 @@
+"""What the Python mirror of the expert-layer calls settles itself (CPU only)."""
+import numpy as np
+import pytest
+
+from test_expert_args import Fake, buf
+
+
+@pytest.fixture
+def h():
+    import b2blas
+
+    h = b2blas.Handle.__new__(b2blas.Handle)
+    h._h, h._lib = None, Fake._lib()
+    return h
+
+
+@pytest.mark.parametrize("fan", [0, -1, -3, -2 ** 63])
+@pytest.mark.parametrize("x", [0, 65, 130])
+def test_fan_below_one_is_refused(h, fan, x):
+    """A negative fan would reach the C ABI as a huge size_t, which stands for
+    "all products share one vector", with x of unchecked length."""
+    import b2blas
+
+    with pytest.raises(b2blas.CublasError, match="fan") as e:
+        h.hgemv_w4_grouped(2, 3, 65, 32, 1.0, buf(6 * 33, np.uint8), buf(18, np.uint16), None, buf(x, np.uint16),
+                           buf(4, np.int32), 0.0, buf(12, np.uint16), count=4, fan=fan)
+    assert e.value.kind == "InvalidArgument"
