@@ -305,8 +305,8 @@ class Handle:
     def _need(buf: DeviceBuffer, n: int, what: str, dtype) -> None:
         if buf.dtype is not dtype and buf.dtype != np.dtype(dtype):
             raise CublasError(3, f"{what} has dtype {buf.dtype}, expected {np.dtype(dtype)}")
-        if buf._len < n:
-            raise CublasError(2, f"dimension mismatch in {what}: expected {n}, got {buf._len}")
+        if len(buf) < n:
+            raise CublasError(2, f"dimension mismatch in {what}: expected {n}, got {len(buf)}")
 
     def _gemm_dev(self, fn, algo, cfg: GemmConfig, a, b, c, dtype):
         m, n, k = cfg.m, cfg.n, cfg.k
