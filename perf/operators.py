@@ -254,15 +254,21 @@ _kept = {}
 
 
 def _handle():
-    """The program's handle, on the stream that it runs on."""
-    if "h" not in _kept:
+    """The program's handle of the current device, on the current stream."""
+    if "m" not in _kept:
         import os
         import sys
         sys.path.insert(1, os.path.join(os.getcwd(), "cublas-rs_b200"))
         import b2blas
-        _kept["m"], _kept["h"] = b2blas, b2blas.Handle(torch.cuda.current_device())
-        _kept["h"].set_stream(torch.cuda.current_stream().cuda_stream)
-    return _kept["m"], _kept["h"]
+        _kept["m"] = b2blas
+    device, stream = torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream
+    if device not in _kept:
+        _kept[device] = [_kept["m"].Handle(device), None]
+    kept = _kept[device]
+    if kept[1] != stream:
+        kept[0].set_stream(stream)
+        kept[1] = stream
+    return _kept["m"], kept[0]
 
 
 _KIND = {torch.float16: np.uint16, torch.bfloat16: np.uint16, torch.float32: np.float32, torch.int32: np.int32, torch.uint8: np.uint8}
