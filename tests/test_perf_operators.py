@@ -22,6 +22,7 @@ def ops(monkeypatch):
     at = types.SimpleNamespace(device=0, stream=0)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: at.device)
     monkeypatch.setattr(torch.cuda, "current_stream", lambda *a: types.SimpleNamespace(cuda_stream=at.stream))
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: at.stream, raising=False)
     monkeypatch.setattr(module, "_kept", {})
     monkeypatch.setitem(__import__("sys").modules, "b2blas", types.SimpleNamespace(Handle=Handle))
     return module, at
