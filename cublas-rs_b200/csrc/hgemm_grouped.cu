@@ -76,12 +76,17 @@ __device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, in
 //   kNT  C[r] = A[r] B_g^T   A K-major, B (n x k rows) K-major
 //   kTN  C_g = A_g^T B_g     both MN-major; the ragged rows are the k axis
 //
-// The accumulators' f32 additions drop low bits instead of rounding them, about
-// 2^-24 of the sum for each 16 deep step and always toward zero: 2.9e-6 of a
-// sum of 2048 terms, where rounded f32 sums have 0.5e-6.  16-bit results do not
-// see it.  An f32 C_g is therefore summed in pieces of 512: the epilogue's
-// threads hold the tile in registers and add each piece, rounded, while the
-// MMAs fill the other accumulator.
+// The accumulators' f32 additions cut low bits, always toward zero: measured
+// 2.3 f32 steps of the running sum for each 16 deep step.  A sum of one sign
+// loses 2.4e-6 of itself over 512 terms, 2.5e-5 over 4096, 1.5e-3 over 2^18,
+// where one of rounded f32 additions stays below 1e-6.  So no accumulator sums
+// up more than a piece; the epilogue adds the pieces, rounded, while the MMAs
+// fill the other accumulator:
+//   f32 C_g    pieces of 512, added up in registers (random terms, 2048 rows:
+//              2.9e-6 off in one piece, 0.5e-6 in four)
+//   16-bit C   pieces of 4096, whose loss is a twentieth of the rounding to f16,
+//              added up in local memory, which only longer sums touch: 16384 rows
+//              of each of 4 groups, 1024 x 2048: 267 us in one piece, 285 in four
 //
 // No operand is transposed or copied: the three products differ in the shared
 // memory layouts that the MMA descriptors name.  B of kNN / kNT is a 3-D
@@ -119,7 +124,7 @@ template <int MODE, bool PAIR, int BN_, bool F32_, bool HAND_>
 struct Cfg {
     static constexpr bool HAND = HAND_;                // loads by warps
     static constexpr bool F32 = F32_;                  // C is f32 (kTN)
-    static constexpr int PIECE = F32 ? 8 : 1 << 30;    // k blocks that an accumulator sums up
+    static constexpr int PIECE = F32 ? 8 : 64;         // k blocks that an accumulator sums up
     static constexpr int BN = BN_;                     // columns of a tile
     static constexpr int BM = PAIR ? 256 : 128;        // rows of a tile, 128 to a CTA
     static constexpr int BN_CTA = PAIR ? BN / 2 : BN;  // columns of B that a CTA loads
@@ -778,7 +783,39 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
                     store_segment<float>(cbase, pitch, buf, rows, ncols, p.vec, lane);
                 }
             } else {
-                ok = wait_full(o);
+                // A sum of several pieces: the warp's columns of all but the last are added up
+                // here (in local memory: the columns are a loop), and then into the accumulator
+                // of the last, from where all sums go on.
+                float held[BN / 2];
+                for (int kb0 = o.kfirst;; kb0 += Cf::PIECE) {
+                    ok = wait_full(o);
+                    const bool last = o.kend - kb0 <= Cf::PIECE;
+                    if (!ok || (last && kb0 == o.kfirst)) break;
+#pragma unroll 1
+                    for (int c = 0; c < c_stop - c_first; c += 16) {
+                        const uint32_t at = tmem_warp + static_cast<uint32_t>(acc * BN + c_first + c);
+                        uint32_t r[16];
+                        __syncwarp();
+                        tmem_ld_32x32b_x16(at, r);
+                        tmem_ld_wait();
+                        if (kb0 != o.kfirst) {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(held[c + e] + __uint_as_float(r[e]));
+                        }
+                        if (last) {
+                            tmem_st_32x32b_x16(at, r);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) held[c + e] = __uint_as_float(r[e]);
+                        }
+                    }
+                    if (last) {
+                        tmem_st_wait();
+                        break;
+                    }
+                    release();
+                    turn();
+                }
                 if (!ok) break;
                 if (c_stop == c_first) release();
 #pragma unroll 1
