@@ -78,10 +78,9 @@ __device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, in
 //
 // The accumulators' f32 additions cut low bits, always toward zero: measured
 // 2.3 f32 steps of the running sum for each 16 deep step.  A sum of one sign
-// loses 2.4e-6 of itself over 512 terms, 2.5e-5 over 4096, 1.5e-3 over 2^18,
-// where one of rounded f32 additions stays below 1e-6.  So no accumulator sums
-// up more than a piece; the epilogue adds the pieces, rounded, while the MMAs
-// fill the other accumulator:
+// loses 2.4e-6 of itself over 512 terms, 2.5e-5 over 4096, 1.5e-3 over 2^18.
+// So no accumulator sums up more than a piece; the epilogue adds the pieces,
+// rounded, while the MMAs fill the other accumulator:
 //   f32 C_g    pieces of 512, added up in registers (random terms, 2048 rows:
 //              2.9e-6 off in one piece, 0.5e-6 in four)
 //   16-bit C   pieces of 4096, whose loss is a twentieth of the rounding to f16,

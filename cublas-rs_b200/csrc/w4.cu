@@ -1087,11 +1087,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 // Back to 16 bits.  scale * (q - zero) is 11 bits times 5: its product in 16
 // bits is the exact one rounded once.
+// Whether a finite scale may take values beyond the type, where they become its
+// largest finite one; infinities and NaN show in every value.
 template <bool BF16>
-__device__ __forceinline__ uint16_t w4_back(float scale, int q) {
+__device__ __forceinline__ bool w4_clamps(float scale) {
+    using H = b2b::Half16<BF16>;
+    return fabsf(scale) > H::kMax / 16.0f && fabsf(scale) <= H::kMax;
+}
+template <bool BF16>
+__device__ __forceinline__ uint16_t w4_back(float scale, bool clamps, int q) {
     using H = b2b::Half16<BF16>;
     const float v = scale * static_cast<float>(q);
-    return H::put(v > H::kMax ? H::kMax : v < -H::kMax ? -H::kMax : v);
+    return H::put(clamps ? fminf(fmaxf(v, -H::kMax), H::kMax) : v);
 }
 
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b, __half) { return as_word(__hmul2(as_half2(a), as_half2(b))); }
@@ -1138,12 +1145,13 @@ __global__ void __launch_bounds__(256) w4_dequantize_kernel(W4Args p, uint16_t *
                 o[1] = __byte_perm(v[2], v[3], 0x5410);
                 o[2] = __byte_perm(v[0], v[1], 0x7632);
                 o[3] = __byte_perm(v[2], v[3], 0x7632);
-            } else {  // a product may pass the largest value, or the scale is a NaN
+            } else {  // a product may pass the largest value, or the scale is not finite
+                const bool clamps = w4_clamps<BF16>(s);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int a = static_cast<int>(word[h] >> (8 * i) & 15u), b = static_cast<int>(word[h] >> (8 * i + 4) & 15u);
                     const int z = static_cast<int>(zero[h]);
-                    o[i] = w4_back<BF16>(s, a - z) | static_cast<uint32_t>(w4_back<BF16>(s, b - z)) << 16;
+                    o[i] = w4_back<BF16>(s, clamps, a - z) | static_cast<uint32_t>(w4_back<BF16>(s, clamps, b - z)) << 16;
                 }
             }
             *(reinterpret_cast<uint4 *>(W + row * p.n) + oct0 + 32 * h) = make_uint4(o[0], o[1], o[2], o[3]);
@@ -1176,8 +1184,9 @@ __global__ void __launch_bounds__(256) w4_dequantize_any_kernel(W4Args p, uint16
         for (int i = 0; i < 4; ++i) {
             const int64_t at = at0 + 32 * i;
             uint16_t *w = W + row * p.n + 2 * at;
-            if (2 * at < p.n) w[0] = w4_back<BF16>(s[i], (byte[i] & 15) - zero[i]);
-            if (2 * at + 1 < p.n) w[1] = w4_back<BF16>(s[i], (byte[i] >> 4) - zero[i]);
+            const bool clamps = w4_clamps<BF16>(s[i]);
+            if (2 * at < p.n) w[0] = w4_back<BF16>(s[i], clamps, (byte[i] & 15) - zero[i]);
+            if (2 * at + 1 < p.n) w[1] = w4_back<BF16>(s[i], clamps, (byte[i] >> 4) - zero[i]);
         }
     }
 }

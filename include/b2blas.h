@@ -339,7 +339,8 @@ B2B_API int b2b_quantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t 
                             uint8_t *packed, uint16_t *scales, uint8_t *zeros);
 /* packed, scales, zeros -> W in `type`, each value rounded once to nearest
  * even (one that a finite scale takes beyond the type becomes its largest
- * finite value): the 16-bit operand that the matrix products take. */
+ * finite value; an infinite or NaN scale shows in its values): the 16-bit
+ * operand that the matrix products take. */
 B2B_API int b2b_dequantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, const uint8_t *packed,
                               const uint16_t *scales, const uint8_t *zeros, uint16_t *W);
 /* y_i <- alpha*W*x_i + beta*y_i for `count` vectors: x is count x n, y is
