@@ -199,10 +199,10 @@ __device__ __forceinline__ Tile tile_at(const TcArgs &p, const int *start, const
     return o;
 }
 
-// The limit of a wait for a whole tile: the bound of any wait, and 2 us for
-// each of its k blocks (they take under 1), so that no sum is too long.
-__device__ __forceinline__ uint64_t tile_wait_ns(const TcArgs &p, const Tile &o) {
-    return p.wait_ns + 2000ull * static_cast<uint64_t>(o.kblocks);
+// The limit of a wait for tiles of `kblocks` k blocks in all: the bound of any
+// wait, and 2 us for each block (they take up to 1.1), so that no sum is too long.
+__device__ __forceinline__ uint64_t tile_wait_ns(const TcArgs &p, int64_t kblocks) {
+    return p.wait_ns + 2000ull * static_cast<uint64_t>(kblocks);
 }
 
 // Rows of A that CTA `rank` of a kNN / kNT tile loads: all 128 in one box, or
@@ -658,15 +658,18 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
         // ------------------------------------------------ wiper (kTN)
         int stage = 0, g = 0;
         uint32_t phases = 0;  // bit s: parity of landed[s]
+        int64_t behind = 0;   // k blocks since the last wait, and 16 for each tile's epilogue: all come before this one
         for (uint32_t t = first; t < tiles; t += step) {
             const Tile o = tile_of(t, g);
             const int count = o.kend - o.kfirst;
+            behind += count + 16;
             if (count == 0) continue;
             const int s = (stage + count - 1) % S;
             stage = (stage + count) % S;
             if (o.klast == 64 || o.kend < o.kblocks) continue;
             const bool ok = mbar_wait_sleepy(&landed[s], phases >> s & 1u, abort_flag, p.status,
-                                             B2B_DEVSTAT_TIMEOUT | 0x25, tile_wait_ns(p, o));
+                                             B2B_DEVSTAT_TIMEOUT | 0x25, tile_wait_ns(p, behind));
+            behind = 0;
             if (!__all_sync(0xffffffffu, ok)) break;
             phases ^= 1u << s;
             // row r of a box is its 128 bytes at r * 128, whatever the swizzle
@@ -714,7 +717,7 @@ __global__ void __launch_bounds__((Cfg<MODE, PAIR, BN, F32, HAND>::THREADS), 1)
         };
         auto wait_full = [&](const Tile &o) {
             const bool ok = mbar_wait_sleepy(&tfull[acc], acc_phase, abort_flag, p.status, B2B_DEVSTAT_TIMEOUT | 0x24,
-                                             tile_wait_ns(p, o));
+                                             tile_wait_ns(p, o.kblocks));
             const bool all = __all_sync(0xffffffffu, ok);
             tc_fence_after();
             return all;
