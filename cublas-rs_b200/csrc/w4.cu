@@ -681,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncthreads();
     const uint32_t tiles = static_cast<uint32_t>((p.w.m + kTileRows - 1) / kTileRows);
-    const uint32_t sets = p.index ? sets_named : (p.count + p.width - 1) / p.width;
+    const uint32_t sets = p.index ? sets_named : (static_cast<uint32_t>(p.count) + p.width - 1) / p.width;
     const int boxes = static_cast<int>((p.w.n + kBoxCols - 1) / kBoxCols);
     const int local = boxes > rank ? (boxes - rank + KS - 1) / KS : 0;  // this CTA's boxes of a tile
     const int lbox = min(4, 32 - __clz((boxes + KS - 1) / KS - 1));  // log2 of the warps that a tile can use
@@ -1285,7 +1285,8 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, bool tma, const CUtensorMap &
         return b2b::fail(B2B_ERR_NOT_SUPPORTED, "4-bit GEMV: rows longer than 327680 columns");
     // with an index: the matrices that it names, if it names them at random,
     // and their sets
-    double sets = static_cast<double>((p.count + p.width - 1) / p.width);
+    const int64_t count = p.count, full = (count + p.width - 1) / p.width;  // sets without an index
+    double sets = static_cast<double>(full);
     if (p.index) {
         const double named = p.matrices * (1.0 - pow(1.0 - 1.0 / p.matrices, p.count));
         sets = named * ceil(p.count / named / p.width);
@@ -1348,7 +1349,7 @@ int launch_gemv(b2b_handle *h, bool bf16, int spg, bool tma, const CUtensorMap &
     p = best;
     const int64_t local = (cols + best_ks - 1) / best_ks, clusters = resident_clusters(h, fn, best_ks);
     // an index may name more matrices than expected, but not more tiles than this
-    const int64_t most = (p.index ? p.count : (p.count + p.width - 1) / p.width) * tiles;
+    const int64_t most = (p.index ? count : full) * tiles;
     attr[0].val.clusterDim.x = best_ks;
     cfg.dynamicSmemBytes = gemv_smem(p, tma, best_ks, local);
     cfg.numAttrs = best_ks > 1;
