@@ -166,3 +166,39 @@ def test_long_wgrad_is_exact_on_whole_numbers(handle, t, alpha, beta, counts, m,
 @pytest.mark.parametrize("k", [4096, 4104, 8192, 12345, 20488])
 def test_long_forward_is_exact_on_whole_numbers(handle, t, alpha, beta, trans, counts, n, k):
     check_whole(handle, t, counts, n, k, trans, alpha, beta)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("counts,m,n", [
+    ([65536], 1160, 1160),                     # CTA pairs
+    ([65536] + [1] * 149, 120, 248),           # one CTA, 256 columns
+    ([65536] + [1] * 79, 120, 248),            # 128 columns
+    ([65536] + [1] * 149, 64, 56),             # 64 columns
+    ([65536], 1161, 1163),                     # loaded by warps
+    ([65536] + [1] * 149, 65, 63),
+    ([524288], 136, 136),                      # a cluster shares each sum
+    ([524288], 65, 63)])
+def test_f32_wgrad_of_one_sign(handle, t, counts, m, n):
+    """f32 C in pieces of 512: at most 32 steps x 17 x 2^-23 / 2 within them,
+    3.2e-5, and one rounding, 2^-24, for each that is added up.  One piece of
+    65536 terms loses ten times as much (3.8e-4 measured for f16, 2.4 of the 17
+    a step), and so would the eighth of a shared sum of 524288.  The f32 tests
+    on whole numbers cannot see that, and the one on random terms has so few
+    tiles that clusters share its sums, in parts not much longer than a piece."""
+    import torch
+
+    import b2blas
+
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(m)
+    depth = counts[0]
+    a, b, _ = inputs(t, counts, n, m, None, lambda s: (torch.rand(s, generator=gen, device="cuda") + 0.5).to(R.HALF[t]))
+    c = torch.zeros(len(counts), m, n, device="cuda")
+    torch.cuda.synchronize()
+    handle.hgemm_grouped_wgrad(b2blas.GemmConfig(m, n, sum(counts), 1.0 / depth, 0.0), len(counts), view(handle, a),
+                               view(handle, b), view(handle, offsets(counts), np.int32), view(handle, c, np.float32),
+                               half=half_of(t))
+    handle.synchronize()
+    want = exact(counts[:1], a, b)[0] / depth
+    off = float(((c[0].double() - want) / want).abs().max())
+    assert off <= 32 * 17 / 2 * 2.0 ** -23 * 1.01 + (depth / 512 + 2) * 2.0 ** -24
