@@ -345,9 +345,11 @@ B2B_API int b2b_dequantize_w4(b2b_handle *h, int type, size_t m, size_t n, size_
                               const uint16_t *scales, const uint8_t *zeros, uint16_t *W);
 /* y_i <- alpha*W*x_i + beta*y_i for `count` vectors: x is count x n, y is
  * count x m.  Products are exact, sums f32, y is rounded to nearest even
- * once.  The weights are read once for every 8 vectors (fewer where n is
- * beyond 40960).  y must not overlap the other operands.  n above 327680
- * returns B2B_ERR_NOT_SUPPORTED, here and below. */
+ * once.  A group's columns, at most 256 at a time, are summed before their
+ * scale comes in, which stays finite for |x| < 2^116 (bf16; f16 always).  The
+ * weights are read once for every 8 vectors (fewer where n is beyond 40960).
+ * y must not overlap the other operands.  n above 327680 returns
+ * B2B_ERR_NOT_SUPPORTED, here and below. */
 B2B_API int b2b_hgemv_w4(b2b_handle *h, int type, size_t m, size_t n, size_t group, float alpha,
                          const uint8_t *packed, const uint16_t *scales, const uint8_t *zeros, const uint16_t *x,
                          size_t count, float beta, uint16_t *y);
