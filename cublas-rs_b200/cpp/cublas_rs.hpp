@@ -89,6 +89,45 @@ struct f16 {
     }
 };
 
+// bfloat16 bits (no reference counterpart: its half type is f16 only);
+// from_f32 rounds to nearest even.
+struct bf16 {
+    uint16_t bits = 0;
+    static bf16 from_bits(uint16_t b) {
+        bf16 h;
+        h.bits = b;
+        return h;
+    }
+    static bf16 from_f32(float f) {
+        uint32_t x;
+        std::memcpy(&x, &f, 4);
+        if ((x & 0x7fffffffu) > 0x7f800000u) return from_bits(uint16_t(x >> 16 | 0x40u));  // NaN
+        return from_bits(uint16_t((x + 0x7fffu + (x >> 16 & 1u)) >> 16));
+    }
+    float to_f32() const {
+        const uint32_t x = uint32_t(bits) << 16;
+        float f;
+        std::memcpy(&f, &x, 4);
+        return f;
+    }
+};
+
+// b2b_type of the element types of the grouped and 4-bit-weight calls.
+template <typename T>
+struct element;
+template <>
+struct element<f16> {
+    static constexpr int type = B2B_TYPE_F16;
+};
+template <>
+struct element<bf16> {
+    static constexpr int type = B2B_TYPE_BF16;
+};
+template <>
+struct element<float> {
+    static constexpr int type = B2B_TYPE_F32;
+};
+
 class CublasError : public std::runtime_error {
    public:
     enum class Kind { Driver, EmbeddedModule, DimensionMismatch, InvalidArgument };
@@ -376,6 +415,89 @@ class Handle {
                                                batch_count));
     }
 
+    // ---- grouped HGEMM (no reference counterpart); H is f16 or bf16
+    // C[r] <- alpha A[r] op(B_g) + beta C[r] for the rows r of every group g:
+    // c.m counts all rows of A and C, offsets holds groups + 1 row numbers.
+    template <typename H>
+    void hgemm_grouped(const GemmConfig<float> &c, size_t groups, const DeviceBuffer<H> &a, const DeviceBuffer<H> &b,
+                       const DeviceBuffer<int32_t> &offsets, DeviceBuffer<H> &cc,
+                       Transpose trans_b = Transpose::NoTrans) const {
+        if (c.m && c.n && c.k && groups) {
+            need(a, c.m * c.k, "A");
+            need(b, groups * c.k * c.n, "B");
+            need(offsets, groups + 1, "offsets");
+            need(cc, c.m * c.n, "C");
+        }
+        check(b2b_hgemm_grouped(h_, element<H>::type, int(trans_b), groups, c.m, c.n, c.k, c.alpha, words(a), words(b),
+                                c.beta, words(cc), offsets.ptr()));
+    }
+    // C_g <- alpha A[rows of g]^T B[rows of g] + beta C_g: c.k counts all rows
+    // of A and B; C is of H or of float.
+    template <typename H, typename C>
+    void hgemm_grouped_wgrad(const GemmConfig<float> &c, size_t groups, const DeviceBuffer<H> &a,
+                             const DeviceBuffer<H> &b, const DeviceBuffer<int32_t> &offsets, DeviceBuffer<C> &cc) const {
+        if (c.m && c.n && groups) {
+            need(a, c.k * c.m, "A");
+            need(b, c.k * c.n, "B");
+            need(offsets, groups + 1, "offsets");
+            need(cc, groups * c.m * c.n, "C");
+        }
+        check(b2b_hgemm_grouped_wgrad(h_, element<H>::type, element<C>::type, groups, c.k, c.m, c.n, c.alpha, words(a),
+                                      words(b), c.beta, cc.ptr(), offsets.ptr()));
+    }
+
+    // ---- 4-bit weights (no reference counterpart); zeros == nullptr: 8 everywhere
+    template <typename H>
+    void quantize_w4(size_t m, size_t n, size_t group, const DeviceBuffer<H> &w, DeviceBuffer<uint8_t> &packed,
+                     DeviceBuffer<H> &scales, DeviceBuffer<uint8_t> *zeros = nullptr) const {
+        if (m && n) {
+            need_w4(1, m, n, group, packed, scales, zeros);
+            need(w, m * n, "W");
+        }
+        check(b2b_quantize_w4(h_, element<H>::type, m, n, group, words(w), packed.ptr(), words(scales),
+                              zeros ? zeros->ptr() : nullptr));
+    }
+    template <typename H>
+    void dequantize_w4(size_t m, size_t n, size_t group, const DeviceBuffer<uint8_t> &packed,
+                       const DeviceBuffer<H> &scales, const DeviceBuffer<uint8_t> *zeros, DeviceBuffer<H> &w) const {
+        if (m && n) {
+            need_w4(1, m, n, group, packed, scales, zeros);
+            need(w, m * n, "W");
+        }
+        check(b2b_dequantize_w4(h_, element<H>::type, m, n, group, packed.ptr(), words(scales),
+                                zeros ? zeros->ptr() : nullptr, words(w)));
+    }
+    // y_i <- alpha W x_i + beta y_i for `count` vectors
+    template <typename H>
+    void hgemv_w4(size_t m, size_t n, size_t group, float alpha, const DeviceBuffer<uint8_t> &packed,
+                  const DeviceBuffer<H> &scales, const DeviceBuffer<uint8_t> *zeros, const DeviceBuffer<H> &x,
+                  float beta, DeviceBuffer<H> &y, size_t count = 1) const {
+        if (m && n && count) {
+            need_w4(1, m, n, group, packed, scales, zeros);
+            need(x, count * n, "x");
+            need(y, count * m, "y");
+        }
+        check(b2b_hgemv_w4(h_, element<H>::type, m, n, group, alpha, packed.ptr(), words(scales),
+                           zeros ? zeros->ptr() : nullptr, words(x), count, beta, words(y)));
+    }
+    // y_i <- alpha W_e x_{i / fan} + beta y_i with e = index[i]; an index
+    // outside [0, groups) names no matrix
+    template <typename H>
+    void hgemv_w4_grouped(size_t groups, size_t m, size_t n, size_t group, float alpha,
+                          const DeviceBuffer<uint8_t> &packed, const DeviceBuffer<H> &scales,
+                          const DeviceBuffer<uint8_t> *zeros, const DeviceBuffer<H> &x,
+                          const DeviceBuffer<int32_t> &index, float beta, DeviceBuffer<H> &y, size_t count,
+                          size_t fan = 1) const {
+        if (m && n && count && groups && fan) {  // the library refuses a fan of 0
+            need_w4(groups, m, n, group, packed, scales, zeros);
+            need(x, (count / fan + (count % fan != 0)) * n, "x");
+            need(index, count, "index");
+            need(y, count * m, "y");
+        }
+        check(b2b_hgemv_w4_grouped(h_, element<H>::type, groups, m, n, group, alpha, packed.ptr(), words(scales),
+                                   zeros ? zeros->ptr() : nullptr, words(x), count, fan, index.ptr(), beta, words(y)));
+    }
+
    private:
     template <typename T>
     static void need(const DeviceBuffer<T> &d, size_t n, const char *what) {
@@ -391,6 +513,19 @@ class Handle {
             need(b, c.k * c.n, "B");
             need(cc, c.m * c.n, "C");
         }
+    }
+    template <typename H>
+    static void need_w4(size_t matrices, size_t m, size_t n, size_t group, const DeviceBuffer<uint8_t> &packed,
+                        const DeviceBuffer<H> &scales, const DeviceBuffer<uint8_t> *zeros) {
+        const size_t groups = group ? n / group + (n % group != 0) : 0;  // the library refuses a group of 0
+        need(packed, matrices * m * (n / 2 + n % 2), "packed");
+        need(scales, matrices * m * groups, "scales");
+        if (zeros) need(*zeros, matrices * m * groups, "zeros");
+    }
+    template <typename H>
+    static uint16_t *words(const DeviceBuffer<H> &d) {
+        static_assert(sizeof(H) == 2, "a 16-bit type");
+        return reinterpret_cast<uint16_t *>(d.ptr());
     }
     b2b_handle *h_ = nullptr;
 };

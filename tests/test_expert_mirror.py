@@ -49,3 +49,14 @@ def test_buffers_of_the_callers_own_are_taken(h):
     with pytest.raises(AssertionError, match="b2b_hgemm_grouped reached the library"):
         h.hgemm_grouped(b2blas.GemmConfig(10, 6, 4), 2, Own(40, np.uint16), Own(48, np.uint16), Own(3, np.int32),
                         Own(60, np.uint16))
+
+
+def test_every_expert_call_has_its_cpp_method():
+    import os
+    import re
+
+    from conftest import PKG
+
+    src = open(os.path.join(PKG, "cpp", "cublas_rs.hpp")).read()
+    for name in ("hgemm_grouped", "hgemm_grouped_wgrad", "quantize_w4", "dequantize_w4", "hgemv_w4", "hgemv_w4_grouped"):
+        assert re.search(rf"void {name}\(", src) and f"b2b_{name}(h_" in src
