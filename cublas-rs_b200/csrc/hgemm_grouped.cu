@@ -59,25 +59,28 @@ __device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, in
 // Tensor-core kernel: tcgen05.mma on 128 x BN tiles of one CTA, or 256 x 256
 // tiles of a CTA pair, persistent over the tiles of all groups.
 //
-// What bounds it, and what it reaches on a B200 (warm, one call):
-//   many rows a group    the tensor pipe under the power limit: 8 groups of 2048
-//                        rows, 4096 x 4096, 394 us = 1.40 PFLOP/s, where the
-//                        library's dense HGEMM of as many rows has 1.43 to 1.47;
-//                        ragged groups add their half-filled tiles (438 us)
+// What bounds it, and what it reaches on a B200 (warm; calls in turn with pauses
+// between them, at 1950 MHz, and without, where the power limit sets the clock):
+//   many rows a group    the tensor pipe: 8 groups of 2048 rows, 4096 x 4096, 405 us
+//                        = 1.36 PFLOP/s (470 at 1335 MHz), where the dense HGEMM of
+//                        as many rows, in tiles twice as wide, takes 374 (429).
+//                        Ragged groups: 68 to 70 tile rows of 256 for 64 make 15 or
+//                        16 turns of 14, 444 to 463 us (515 to 553)
 //   few rows a group     HBM, for the matrices: 16 groups of 2 rows, 4096 x 2048,
 //                        46 us = 5.8 TB/s; 64 of 128, 2048 x 1024, 59 us = 5.4 TB/s
 //   wgrad, short groups  writing C: 32 groups of 128 rows, 1024 x 1024, 29.5 us for
 //                        67 MB (pure writes reach 3.9 TB/s)
-//   wgrad, long groups   the tensor pipe: 8 groups of 2048 rows, 2048 x 4096, 198 us
-//                        = 1.39 PFLOP/s in 16 bits; f32 230 us, for its pieces
-//                        (below) and twice the bytes of C
+//   wgrad, long groups   the tensor pipe: 8 groups of 2048 rows, 2048 x 4096, 202 us
+//                        = 1.36 PFLOP/s in 16 bits (234 at 1480 MHz); f32 231 us
+//                        (273), for its pieces (below) and twice the bytes of C;
+//                        ragged groups 219 and 247 (252 and 300)
 //
 //   kNN  C[r] = A[r] B_g     A K-major, B (k x n rows) MN-major
 //   kNT  C[r] = A[r] B_g^T   A K-major, B (n x k rows) K-major
 //   kTN  C_g = A_g^T B_g     both MN-major; the ragged rows are the k axis
 //
 // The accumulators' f32 additions cut low bits, always toward zero: measured
-// 2.3 f32 steps of the running sum for each 16 deep step.  A sum of one sign
+// 2.4 f32 steps of the running sum for each 16 deep step.  A sum of one sign
 // loses 2.4e-6 of itself over 512 terms, 2.5e-5 over 4096, 1.5e-3 over 2^18.
 // So no accumulator sums up more than a piece; the epilogue adds the pieces,
 // rounded, while the MMAs fill the other accumulator:
@@ -114,9 +117,10 @@ __device__ bool scan_groups(const int32_t *offsets, int groups, int64_t rows, in
 // Warps: 0 TMA producer, 1 TMEM allocator and MMA issuer, 2..9 epilogue, 10
 // (kTN) the wiper; HAND: 10.. load.  Two accumulators: the epilogue of a tile
 // runs under the MMAs of the next.  The epilogue goes through shared memory to
-// 64-byte row segments, since a TMA store would write past the group's last
-// row; it is a chain of short latencies, so two warps share each quarter of the
-// TMEM lanes.
+// 64-byte row segments: in kNN and kNT a TMA store would write past a group's
+// last row.  In kTN every C_g has M rows and a 3-D map would clip there; its
+// results take the same way.  The epilogue is a chain of short latencies, so two
+// warps share each quarter of the TMEM lanes.
 enum Mode { kNN = 0, kNT = 1, kTN = 2 };
 
 template <int MODE, bool PAIR, int BN_, bool F32_, bool HAND_>

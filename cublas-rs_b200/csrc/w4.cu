@@ -125,10 +125,10 @@ __device__ __forceinline__ bool extremes(const uint32_t (&words)[8], float &lo, 
 
 // Groups of 16 LANES columns, 16 of them to a lane, which reads them once.
 // WHOLE: n is a multiple of 8 and W and packed allow 16-byte loads and 4-byte
-// stores; else values and bytes one at a time.  HBM-bound where WHOLE: about
-// 250 instructions for the 40 bytes that a lane moves, most of them the
-// rounding and clamping of its values: 4096 x 4096 takes 14.5 us (2.9 TB/s),
-// 8192 x 8192 55 us with its schedulers 72 % busy.
+// stores; else values and bytes one at a time.  Bound by its instructions where
+// WHOLE: about 250 for the 40 bytes that a lane moves, most of them the rounding
+// and clamping of its values: 4096 x 4096 takes 14.3 us (2.9 TB/s), 8192 x 8192
+// 50 to 55 us (3.1 to 3.4 TB/s) with its schedulers 72 % busy.
 template <bool BF16, int LANES, bool WHOLE>
 __global__ void __launch_bounds__(256) w4_quantize_kernel(const uint16_t *W, uint8_t *packed, uint16_t *scales,
                                                           uint8_t *zeros, int64_t m, int64_t n, int64_t pitch, int64_t gs) {
@@ -275,8 +275,8 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
 
 // ---------------------------------------------------------------------------
 // Products with vectors: y_i = alpha W x_i + beta y_i for up to 8 vectors that
-// share W.  HBM-bound: the packed values are read once, so the work for each
-// must stay well under the ~2.5 instructions that 148 SMs can issue in the
+// share W.  The packed values are read once, and to be bound by HBM the work for
+// each must stay well under the ~2.5 instructions that 148 SMs can issue in the
 // time a value takes to arrive.  Multiplying on the tensor cores with the 8
 // columns of mma.m16n8k16 does that for 1 vector as for 8: a word of 8 values
 // becomes four register pairs of exact (q - zero) in 9 instructions (f16: or
@@ -305,10 +305,12 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
 //     when those of the next ones are ready (18944 x 16384 by 8 vectors: 104
 //     us where all waited for all after each batch, 47 now).  Both in a fixed
 //     order, whoever adds.
-// It streams 5.6 TB/s (packed bytes) where rows are long, 4.9 where they have
-// 2048 columns, after 7 us that any call takes: 16384 x 16384 by one vector
-// 35 us, by 8 47 us; what it lacks to HBM's 6.4 is instructions, 20 for each
-// word of a warp, half a cycle each on the pipes that most of them need.
+// f16 by one vector, no zero points: 7.6 us, and 7.1 for each tile of an SM where
+// rows have 16384 columns (5.6 TB/s of packed bytes), 6.5 and 7.9 for 8 tiles of
+// 2048 (5.1).  Tiles are whole: 16384 rows, 3.46 tiles for each of 148 SMs, take
+// 35.7 us, 18944, 4 for each, 36.3 (by 8 vectors both 47).  Unpacking bfloat16 with
+// zero points adds a tenth.  What a tile lacks to HBM's 6.4 is instructions, 20
+// for each word of a warp, half a cycle each on the pipes that most of them need.
 // Rows that TMA cannot describe (n not a multiple of 32, packed not 16-byte
 // aligned) come by cp.async (HAND): the aligned words that hold a box's rows, 33
 // of each, which are shifted into place on their way to registers: 16384 x
@@ -1087,6 +1089,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // ---------------------------------------------------------------------------
 // Back to 16 bits.  scale * (q - zero) is 11 bits times 5: its product in 16
 // bits is the exact one rounded once.
+
 // Whether a finite scale may take values beyond the type, where they become its
 // largest finite one; infinities and NaN show in every value.
 template <bool BF16>
@@ -1106,8 +1109,9 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b, __nv_bfloat16) 
     return as_word(__hmul2(as_bf162(a), as_bf162(b)));
 }
 
-// Whole words and 16-byte stores: n a multiple of 8.  HBM-bound: about 25
-// instructions for the 20 bytes and more that a lane moves.
+// Whole words and 16-byte stores: n a multiple of 8.  About 25 instructions for the
+// 20 bytes and more that a lane moves: 4096 x 4096 takes 9.4 us, 8192 x 8192 35 to
+// 39 (4.3 to 4.8 TB/s, of which four fifths are writes).
 template <bool BF16>
 __global__ void __launch_bounds__(256) w4_dequantize_kernel(W4Args p, uint16_t *W) {
     using H = b2b::Half16<BF16>;
