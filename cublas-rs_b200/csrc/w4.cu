@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(256) w4_quantize_any_kernel(const uint16_t *W,
 //   * Each warp holds one box (32 rows x 128 bytes, 128-byte swizzle), copies
 //     it to registers, and TMA refills it, across rounds, so nothing drains at
 //     a round's end: 64 KiB of an SM in flight.  Two boxes to a warp took 38 us
-//     where one takes 35 (18944 x 16384), and the room is the vectors'.
+//     where one takes 36 (18944 x 16384), and the room is the vectors'.
 //   * The vectors are staged once for each set, each 8 columns reordered to
 //     the pairs (0,4) (1,5) (2,6) (3,7) that the words unpack to.  Only where
 //     they do not fit one SM, or where there are fewer tiles than SMs, is a

@@ -227,7 +227,7 @@ B2B_API int b2b_sgemm_batched_simple(b2b_handle *h, size_t m, size_t n, size_t k
  *   - Sums are f32.  The tensor cores cut low bits of a running sum where f32
  *     additions would round them, so sums are taken in pieces of 4096 terms
  *     (512 where C is f32) that are added up with rounding: of a sum of one
- *     sign a piece loses at most about 2.5e-5 (2.4e-6), whatever its length.
+ *     sign a piece loses about 2.5e-5 (2.4e-6), and so does the whole.
  *   - At most 1024 groups, and sizes below 2^31 (else B2B_ERR_NOT_SUPPORTED).
  *   - C must not overlap A, B or the offsets.
  *   - No workspace is used: calls through one handle may be captured in
